@@ -464,6 +464,74 @@ const char* bfp8_plan_kernel_name(void* plan, int stage);
 int bfp8_plan_quantize(void* plan, void* stream);
 void bfp8_plan_destroy(void* plan);
 
+/* Gated linear attention over device buffers: a text's tokens in one call, or
+ * one token for each of many sequences (gdn_recurrent_step is one token of one
+ * sequence on host pointers).  For value head h, reading key head
+ * h / (heads_v / heads_k), and a sequence's tokens in order:
+ *
+ *   S' = alpha S;  u = beta (v - S'^T k);  S = S' + k u^T;  out = scale S^T q
+ *
+ * (04/qwen_kernels_opt.c:664-813 with scale 1), or u = v where beta is NULL:
+ * linear attention with a decay for each head.  State layout: for each slot and
+ * value head dim_k x dim_v floats in gdn_recurrent_step's blocks, S[i][j] at
+ * ((j / 4 * (dim_k / 4) + i / 4) * 4 + j % 4) * 4 + i % 4.
+ *
+ * Rows: row r of q, k is at q + r * q_row elements and holds heads_k vectors
+ * of dim_k one after the other, v and out heads_v of dim_v, alpha and beta
+ * heads_v floats (gate_row between rows); the row strides let them be parts of
+ * one projection's row.  q, k, v and out are all float32 or all bf16 (dtype);
+ * sums, states and everything between two tokens are float32: in the prompt form
+ * matrix operands are sums of bf16 terms that hold a float32's 24 bits.
+ *
+ * gdn_dev_prompt: sequence s is rows starts[s] .. starts[s + 1] - 1 (device
+ * array of n_seq + 1 ascending values within 0 .. rows; NULL: n_seq is 1 and
+ * the sequence is every row), of any length, none included.  Chunks of 64
+ * tokens in two launches, whose work buffer is gdn_dev_prompt_work_bytes() of
+ * device memory, 16-byte aligned, the caller's (calls that may overlap need one
+ * each).  gdn_dev_step: sequence s is row s (rows == n_seq; starts and work are
+ * not used).
+ *
+ * Sequence s starts from the state in slot slots[s] of state_in (NULL: zeros)
+ * and leaves its last state in the same slot of state_out (may be state_in; other
+ * overlaps are not allowed).  slots NULL: slot s.  A sequence whose slot is
+ * outside 0 .. n_slots - 1 (an empty place of a padded batch: -1), or is the
+ * slot of an earlier sequence of the call, is skipped: its rows of out and its
+ * slot's state stay as they were but for the earlier sequence's work.  A sequence
+ * without tokens has its state copied.  Rows that no sequence holds are neither
+ * read nor written.
+ *
+ * dim_k, dim_v: multiples of 4 up to 256; heads_v a multiple of heads_k; alpha
+ * in [0, 1] (0 forgets the state), any beta.  state_in, state_out and work are
+ * 16-byte aligned, the others aligned to their elements.  A NaN or infinity in a
+ * token gives NaN or infinite values in that sequence and head from that
+ * chunk of 64 tokens on, and nowhere else.
+ *
+ * Nothing is allocated and nothing waits: the calls can be captured. */
+#define GDN_F32 0
+#define GDN_BF16 1
+typedef struct gdn_dev_args {
+    void* out;
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* alpha;
+    const float* beta;
+    const float* state_in;
+    float* state_out;
+    const int32_t* slots;
+    const int32_t* starts;
+    void* work;
+    size_t work_bytes;
+    int64_t q_row, k_row, v_row, out_row, gate_row;
+    int rows, n_seq, n_slots;
+    int heads_k, heads_v, dim_k, dim_v;
+    int dtype;
+    float scale;
+} gdn_dev_args;
+size_t gdn_dev_prompt_work_bytes(const gdn_dev_args* args); /* 0: invalid sizes */
+int gdn_dev_prompt(const gdn_dev_args* args, void* stream);
+int gdn_dev_step(const gdn_dev_args* args, void* stream);
+
 /* Synthetic reference-format planes on the device: mantissas uniform in
  * [-127, 127], exponents uniform in [e_lo, e_hi], from a counter-based hash
  * of (seed, index) -- bfp8_synth_planes_host gives the same bytes. */

@@ -13,9 +13,11 @@ Translation units:
   csrc/forward_chain.hip     a run of decode layers in one launch, f32 flush-to-zero
   csrc/sweep.hip             a whole plan in one launch (a tile queue, LDS-quantized activations, in-launch top-k)
   csrc/batch_mfma.hip        the batched GEMV (up to 16 vectors) on the matrix cores, f32 flush-to-zero
+  csrc/linear_attention.hip  gated linear attention over prompts and batches, IEEE
   csrc/qwen_kernels_api.cpp  C ABI host code (include/qwen_kernels.h)
   csrc/qwen_runtime_api.cpp  C ABI of the runtime kernels and the forward loop
   csrc/qwen_weights.cpp      manifest-driven weight-image loader
+  csrc/qwen_text_api.cpp     C ABI of the operators over a text's tokens
 
 Every device TU is built with -ffp-contract=off (no fused multiply-add: the
 reference rounds every product and sum) and without packed FP32 ops.
@@ -60,9 +62,11 @@ UNITS = {
     "bfp8_ieee.hip": [],
     "select.hip": [],
     "noalloc.hip": [],
+    "linear_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "qwen_kernels_api.cpp": [],
     "qwen_runtime_api.cpp": [],
     "qwen_weights.cpp": [],
+    "qwen_text_api.cpp": [],
 }
 
 

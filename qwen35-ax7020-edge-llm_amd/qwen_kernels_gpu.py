@@ -17,7 +17,7 @@ library raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_double, c_float, c_int, c_size_t, c_uint64, c_void_p
+from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 from typing import Optional, Sequence
 
@@ -71,6 +71,22 @@ class MlpPlan(ctypes.Structure):
         ("post_ln_w", c_void_p), ("mant_gate", c_void_p), ("exp_gate", c_void_p), ("M_gate", c_int),
         ("K_gate", c_int), ("mant_up", c_void_p), ("exp_up", c_void_p), ("M_up", c_int), ("K_up", c_int),
         ("mant_down", c_void_p), ("exp_down", c_void_p), ("M_down", c_int), ("K_down", c_int),
+    ]
+
+
+GDN_F32, GDN_BF16 = 0, 1
+
+
+class gdn_dev_args(ctypes.Structure):
+    """Mirror of ``gdn_dev_args`` (include/qwen_kernels.h)."""
+
+    _fields_ = [
+        ("out", c_void_p), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("alpha", c_void_p),
+        ("beta", c_void_p), ("state_in", c_void_p), ("state_out", c_void_p), ("slots", c_void_p),
+        ("starts", c_void_p), ("work", c_void_p), ("work_bytes", c_size_t),
+        ("q_row", c_int64), ("k_row", c_int64), ("v_row", c_int64), ("out_row", c_int64), ("gate_row", c_int64),
+        ("rows", c_int), ("n_seq", c_int), ("n_slots", c_int), ("heads_k", c_int), ("heads_v", c_int),
+        ("dim_k", c_int), ("dim_v", c_int), ("dtype", c_int), ("scale", c_float),
     ]
 
 
@@ -205,6 +221,11 @@ def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.bfp8_synth_normal.restype = None
     lib.bfp8_synth_swiglu.argtypes = [vp, i, c_uint64, c_double, c_float]
     lib.bfp8_synth_swiglu.restype = None
+    lib.gdn_dev_prompt_work_bytes.argtypes = [POINTER(gdn_dev_args)]
+    lib.gdn_dev_prompt_work_bytes.restype = c_size_t
+    for name in ("gdn_dev_prompt", "gdn_dev_step"):
+        getattr(lib, name).argtypes = [POINTER(gdn_dev_args), vp]
+        getattr(lib, name).restype = i
     lib.bfp8_stream.argtypes = []
     lib.bfp8_stream.restype = vp
     return lib
@@ -527,3 +548,137 @@ class SweepPlan:
             self.close()
         except Exception:
             pass
+
+
+# ---- a text's tokens -------------------------------------------------------------------
+def _same_device(first, **tensors):
+    """Every tensor on the device of `first`, a GPU; a context that makes it current."""
+    torch = _torch()
+    if not first.is_cuda:
+        raise ValueError("the tensors have to be on a GPU")
+    for name, t in tensors.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+    return torch.cuda.device(first.device)
+
+
+def _rows_of(t, name, shape, dtype):
+    """t of this shape and type, each of its rows contiguous -> the stride between rows."""
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{name} has to be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    step = 1
+    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n != 1 and s != step:
+            raise ValueError(f"{name}: a row's elements have to be contiguous")
+        step *= n
+    if t.shape[0] > 1 and t.stride(0) < step:
+        raise ValueError(f"{name}: its rows overlap")
+    return t.stride(0) if t.shape[0] > 1 else step
+
+
+def _flat(t, name, shape, dtype):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} has to be a contiguous {tuple(shape)} of {dtype}")
+
+
+def _gdn_args(q, k, v, alpha, beta, scale, states, slots, out):
+    """The arguments that both forms of the attention share."""
+    torch = _torch()
+    if q.dim() != 3 or v.dim() != 3 or q.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("q, k, v are [rows, heads, dim] in float32 or bfloat16")
+    rows, hk, dk = q.shape
+    hv, dv = v.shape[1:]
+    a = gdn_dev_args()
+    a.q_row = _rows_of(q, "q", (rows, hk, dk), q.dtype)
+    a.k_row = _rows_of(k, "k", (rows, hk, dk), q.dtype)
+    a.v_row = _rows_of(v, "v", (rows, hv, dv), q.dtype)
+    a.out_row = _rows_of(out, "out", (rows, hv, dv), q.dtype)
+    a.gate_row = _rows_of(alpha, "alpha", (rows, hv), torch.float32)
+    if beta is not None and _rows_of(beta, "beta", (rows, hv), torch.float32) != a.gate_row:
+        raise ValueError("alpha and beta have to have the same row stride")
+    n_slots = None
+    for name, t in states.items():
+        if t is not None:
+            n_slots = t.shape[0] if n_slots is None else n_slots
+            _flat(t, name, (n_slots, hv, dk * dv), torch.float32)
+            setattr(a, name, _dp(t))
+    if slots is not None:
+        a.slots = _dp(slots)
+    a.out, a.q, a.k, a.v, a.alpha = _dp(out), _dp(q), _dp(k), _dp(v), _dp(alpha)
+    a.beta = None if beta is None else _dp(beta)
+    a.rows, a.n_slots, a.heads_k, a.heads_v, a.dim_k, a.dim_v = rows, n_slots, hk, hv, dk, dv
+    a.dtype = GDN_F32 if q.dtype == torch.float32 else GDN_BF16
+    a.scale = scale
+    return a
+
+
+def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0, state_in=None, state_out=None,
+                            slots=None, out=None, work=None):
+    """Gated linear attention over the tokens of packed sequences -> (out, state_out).
+
+    q, k [rows, heads_k, dim_k], v [rows, heads_v, dim_v] (float32 or bfloat16;
+    parts of one projection's row are fine), alpha and beta float32 [rows,
+    heads_v]; beta None: no delta rule.  Sequence s is rows starts[s] to
+    starts[s + 1] (int32 on the device; None: one sequence).  States are float32
+    [slots, heads_v, dim_k * dim_v] in the decode runtime's blocks; a sequence
+    starts from its slot of state_in (None: zeros) and leaves its state in that
+    slot of state_out (None: a new tensor; it may be state_in).  slots: int32 on
+    the device, None: slot s for sequence s.  work: uint8 scratch of at least
+    linear_attention_prompt_work_bytes, for callers that keep one.  The rest is
+    gdn_dev_prompt's contract (include/qwen_kernels.h)."""
+    torch = _torch()
+    with _same_device(q, k=k, v=v, alpha=alpha, beta=beta, starts=starts, state_in=state_in, state_out=state_out,
+                      slots=slots, out=out, work=work):
+        n_seq = 1 if starts is None else starts.numel() - 1
+        if starts is not None:
+            _flat(starts, "starts", (max(n_seq, 0) + 1,), torch.int32)
+        if slots is not None:
+            _flat(slots, "slots", (n_seq,), torch.int32)
+        if out is None:
+            out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        if state_out is None:
+            if slots is not None:
+                raise ValueError("slots need a state_out that holds them")
+            state_out = torch.empty(n_seq, v.shape[1], q.shape[2] * v.shape[2], dtype=torch.float32, device=q.device)
+        a = _gdn_args(q, k, v, alpha, beta, scale, {"state_in": state_in, "state_out": state_out}, slots, out)
+        if slots is None and a.n_slots < n_seq:
+            raise ValueError("fewer states than sequences")
+        a.starts = None if starts is None else _dp(starts)
+        a.n_seq = n_seq
+        lib = load()
+        need = lib.gdn_dev_prompt_work_bytes(a)
+        if need and work is None:
+            work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        if work is not None:
+            a.work, a.work_bytes = _dp(work), work.numel() * work.element_size()
+        check(lib.gdn_dev_prompt(a, _stream()), "linear_attention_prompt")
+    return out, state_out
+
+
+def linear_attention_prompt_work_bytes(rows, n_seq, heads_k, heads_v, dim_k, dim_v, dtype) -> int:
+    """Bytes of linear_attention_prompt's work for these sizes (dtype: of q, k, v)."""
+    a = gdn_dev_args()
+    a.rows, a.n_seq, a.heads_k, a.heads_v, a.dim_k, a.dim_v = rows, n_seq, heads_k, heads_v, dim_k, dim_v
+    a.dtype = {_torch().float32: GDN_F32, _torch().bfloat16: GDN_BF16}[dtype]
+    n = load().gdn_dev_prompt_work_bytes(a)
+    if not n:
+        check(BFP8_EINVAL, "linear_attention_prompt_work_bytes")
+    return n
+
+
+def linear_attention_step(q, k, v, alpha, beta, state, *, scale=1.0, slots=None, out=None):
+    """One token for each sequence: row s of q, k, v updates the state in slot
+    slots[s] (None: s) of `state` in place -> out.  Types and layouts as in
+    linear_attention_prompt; gdn_dev_step (include/qwen_kernels.h)."""
+    torch = _torch()
+    with _same_device(q, k=k, v=v, alpha=alpha, beta=beta, state=state, slots=slots, out=out):
+        if slots is not None:
+            _flat(slots, "slots", (q.shape[0],), torch.int32)
+        if out is None:
+            out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        a = _gdn_args(q, k, v, alpha, beta, scale, {"state_in": state, "state_out": state}, slots, out)
+        if slots is None and a.n_slots < a.rows:
+            raise ValueError("fewer states than sequences")
+        a.n_seq = a.rows
+        check(load().gdn_dev_step(a, _stream()), "linear_attention_step")
+    return out
