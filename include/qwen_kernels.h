@@ -464,6 +464,10 @@ const char* bfp8_plan_kernel_name(void* plan, int stage);
 int bfp8_plan_quantize(void* plan, void* stream);
 void bfp8_plan_destroy(void* plan);
 
+/* Types of the operators below. */
+#define QWEN_F32 0
+#define QWEN_BF16 1
+
 /* Gated linear attention over device buffers: a text's tokens in one call, or
  * one token for each of many sequences (gdn_recurrent_step is one token of one
  * sequence on host pointers).  For value head h, reading key head
@@ -507,8 +511,6 @@ void bfp8_plan_destroy(void* plan);
  * chunk of 64 tokens on, and nowhere else.
  *
  * Nothing is allocated and nothing waits: the calls can be captured. */
-#define GDN_F32 0
-#define GDN_BF16 1
 typedef struct gdn_dev_args {
     void* out;
     const void* q;
@@ -531,6 +533,58 @@ typedef struct gdn_dev_args {
 size_t gdn_dev_prompt_work_bytes(const gdn_dev_args* args); /* 0: invalid sizes */
 int gdn_dev_prompt(const gdn_dev_args* args, void* stream);
 int gdn_dev_step(const gdn_dev_args* args, void* stream);
+
+/* The score of a text under the bf16 tied-embedding head, and its gradient.  For
+ * row n with hidden state h_n and target t_n, over table rows w_v:
+ *
+ *   z_nv = w_v . h_n;  lse_n = log sum_v exp z_nv;  loss_n = lse_n - z_n,t_n
+ *   D_nv = grad_loss_n (exp(z_nv - lse_n) - [v = t_n])
+ *   grad_h_n = sum_v D_nv w_v;  grad_table_v = sum_n D_nv h_n
+ *
+ * without keeping the logits: the loss goes over tiles of them, the gradient over
+ * pieces of the vocabulary whose D is held (at most 128 MiB, or 1024 columns of
+ * it) and whose logits are computed again.  No counterpart in the reference.
+ *
+ * h: rows x hidden, float32 or bf16 (dtype); table: vocab x hidden bf16; grad_h
+ * has h's type, grad_table is bf16 (gradients are overwritten, not added to);
+ * loss, lse, grad_loss: float32.  Row strides in elements.  The products of
+ * float32 hidden states keep their 24 bits (three bf16 terms); sums, lse and D are
+ * float32, D as an operand bf16 (dtype bf16) or 24 bits (float32).
+ *
+ * A row with a target below 0 is ignored, whatever h holds there: loss, lse and
+ * its row of grad_h are 0.  A target of vocab or more gives NaN in the three,
+ * and counts as ignored in grad_table.  A NaN or infinite logit gives its row a
+ * NaN loss.
+ *
+ * bf16_dev_lm_head_loss writes loss and lse (either may be NULL);
+ * bf16_dev_lm_head_loss_grad reads lse (of the same h, table and targets) and
+ * grad_loss and writes grad_h and grad_table (either may be NULL, and is then not
+ * computed).  work: device memory of the size that the matching
+ * .._work_bytes function gives for these arguments, 256-byte aligned, the
+ * caller's (calls that may overlap need one each).  Table rows that are 16-byte
+ * aligned (pointer, stride, and hidden a multiple of 8) are streamed through LDS;
+ * others are read through registers, more slowly.  hidden up to 65536, vocab up to
+ * 2^28, rows up to 2^20.  Nothing is allocated and nothing waits: the calls can
+ * be captured. */
+typedef struct lm_head_loss_args {
+    float* loss;
+    float* lse;
+    void* grad_h;
+    uint16_t* grad_table;
+    const void* h;
+    const uint16_t* table;
+    const int32_t* targets;
+    const float* grad_loss;
+    void* work;
+    size_t work_bytes;
+    int64_t h_row, table_row, grad_h_row, grad_table_row;
+    int rows, vocab, hidden;
+    int dtype;
+} lm_head_loss_args;
+size_t bf16_dev_lm_head_loss_work_bytes(const lm_head_loss_args* args); /* 0: invalid sizes */
+size_t bf16_dev_lm_head_loss_grad_work_bytes(const lm_head_loss_args* args);
+int bf16_dev_lm_head_loss(const lm_head_loss_args* args, void* stream);
+int bf16_dev_lm_head_loss_grad(const lm_head_loss_args* args, void* stream);
 
 /* Synthetic reference-format planes on the device: mantissas uniform in
  * [-127, 127], exponents uniform in [e_lo, e_hi], from a counter-based hash

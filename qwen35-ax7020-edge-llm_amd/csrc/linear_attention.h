@@ -27,8 +27,8 @@ struct GdnWork {
 inline GdnWork gdn_work(const gdn_dev_args& a) {
     GdnWork w{};
     w.ks = a.dim_k <= 32 ? 1 : a.dim_k <= 64 ? 2 : a.dim_k <= 128 ? 4 : 8;
-    w.nt = a.dtype == GDN_BF16 ? 1 : 3;
-    w.no = a.dtype == GDN_BF16 ? 2 : 3;
+    w.nt = a.dtype == QWEN_BF16 ? 1 : 3;
+    w.no = a.dtype == QWEN_BF16 ? 2 : 3;
     w.key_bytes = (size_t)3 * 4 * w.ks * w.nt * 1024;
     w.tri_bytes = (size_t)(6 * 3 + 6 * w.no) * 1024 + 1024;
     w.n_chunks = (size_t)(a.rows / GDN_CHUNK) + (size_t)a.n_seq;

@@ -14,93 +14,16 @@
 // side by side; gdn_scan_kernel takes the state from chunk to chunk, 16 of a
 // head's value columns in a workgroup (the columns do not mix).
 //
-// Arithmetic: every product runs on the bf16 matrix cores.  A float32 operand
-// goes in as the sum of three bf16 terms, cut (not rounded) from its 24 bits, so
-// that nothing is lost; a product of two such sums takes the six pairs of terms
-// above 2^-24.  What only a bf16 output sees (S0 in Q S0, P, U in P U) has two
+// Arithmetic: every product runs on the bf16 matrix cores, a float32 operand as
+// the sum of three bf16 terms (bf16_terms.h), a product of two such sums as the
+// six pairs of terms above 2^-24.  What only a bf16 output sees (S0 in Q S0, P, U in P U) has two
 // terms: 2^-16, against the output's own 2^-9.
-#include <hip/hip_bf16.h>
-
+#include "bf16_terms.h"
 #include "linear_attention.h"
 
 namespace {
 
-using f32x4 = __attribute__((ext_vector_type(4))) float;
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
-using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
-using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
-
 constexpr int C = GDN_CHUNK;
-
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                   0, 0);
-}
-
-// Term t of x: x's upper 16 bits, then those of what is left, and again.
-__device__ __forceinline__ uint32_t cut(float& x) {
-    const uint32_t u = __float_as_uint(x) & 0xffff0000u;
-    x -= __uint_as_float(u);
-    return u;
-}
-__device__ __forceinline__ uint32_t pack(uint32_t lo, uint32_t hi) { return (lo >> 16) | hi; }
-
-// Eight floats as N bf16 terms, in the order of an MFMA operand's eight values.
-template <int N>
-__device__ __forceinline__ void split8(float (&x)[8], u32x4 (&t)[N]) {
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = cut(x[2 * j]), hi = cut(x[2 * j + 1]);
-            t[n][j] = pack(lo, hi);
-        }
-}
-template <int N>
-__device__ __forceinline__ void split4(f32x4 x, u32x2 (&t)[N]) {
-    float y[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t lo = cut(y[2 * j]), hi = cut(y[2 * j + 1]);
-            t[n][j] = pack(lo, hi);
-        }
-}
-
-// sum over the pairs of terms with ta + tb < kMost of a[ta] x b[tb]
-template <int NA, int NB, int kMost>
-__device__ __forceinline__ f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c) {
-#pragma unroll
-    for (int s = NA + NB - 2; s >= 0; --s)  // the smallest first
-#pragma unroll
-        for (int ta = 0; ta < NA; ++ta) {
-            const int tb = s - ta;
-            if (tb >= 0 && tb < NB && s < kMost) c = mfma(a[ta], b[tb], c);
-        }
-    return c;
-}
-
-template <class T>
-__device__ __forceinline__ float to_float(T x);
-template <>
-__device__ __forceinline__ float to_float<float>(float x) {
-    return x;
-}
-template <>
-__device__ __forceinline__ float to_float<uint16_t>(uint16_t x) {
-    return __uint_as_float((uint32_t)x << 16);
-}
-template <class T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ float from_float<float>(float x) {
-    return x;
-}
-template <>
-__device__ __forceinline__ uint16_t from_float<uint16_t>(float x) {  // to nearest, ties to even
-    return __builtin_bit_cast(uint16_t, __float2bfloat16(x));
-}
 
 // Elements i .. i + 7 of a row as terms; those from dim on are zero.
 template <int NT>
@@ -673,7 +596,7 @@ hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s)
 
 template <int KS>
 hipError_t launch_prompt_of(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
-    if (a.dtype == GDN_BF16)
+    if (a.dtype == QWEN_BF16)
         return a.beta ? launch_prompt<KS, 1, true>(a, w, s) : launch_prompt<KS, 1, false>(a, w, s);
     return a.beta ? launch_prompt<KS, 3, true>(a, w, s) : launch_prompt<KS, 3, false>(a, w, s);
 }
@@ -683,7 +606,7 @@ hipError_t launch_step(const gdn_dev_args& a, hipStream_t s) {
     const int groups = a.dim_v / 4;
     const size_t units = (size_t)a.n_seq * a.heads_v * ((groups + G - 1) / G);
     const dim3 grid((unsigned)((units + 3) / 4));
-    if (a.dtype == GDN_BF16)
+    if (a.dtype == QWEN_BF16)
         gdn_step_kernel<NI, G, uint16_t><<<grid, 256, 0, s>>>(a, groups);
     else
         gdn_step_kernel<NI, G, float><<<grid, 256, 0, s>>>(a, groups);

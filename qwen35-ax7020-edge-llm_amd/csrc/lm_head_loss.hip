@@ -1,0 +1,609 @@
+// lm_head_loss.hip -- the score of a text under the bf16 tied-embedding head and
+// its gradient (bf16_dev_lm_head_loss, bf16_dev_lm_head_loss_grad).
+//
+//   z_nv = w_v . h_n;  lse_n = log sum_v exp z_nv;  loss_n = lse_n - z_n,t_n
+//   D_nv = g_n (exp(z_nv - lse_n) - [v = t_n]);  grad_h = D W;  grad_w = D^T h
+//
+// lhl_prepare_kernel gathers the rows that count (a text's own prompt often does
+// not), as bf16 terms.  The rest are tiled products on the matrix cores:
+//   lhl_logits_kernel    W h^T; its epilogue leaves a tile's maximum and sum of
+//                        exponentials for each row, or D for a piece of the vocabulary
+//   lhl_grad_h_kernel    W^T D^T, split over the vocabulary, float32 sums
+//   lhl_grad_table_kernel  h^T D
+// and lhl_loss_kernel / lhl_finish_kernel join the parts.  Every sum has one fixed
+// order: results repeat bit for bit.
+#include "bf16_terms.h"
+#include "lm_head_loss.h"
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- tiles ----------------------------------------------------------------------------
+// An operand in memory: rows x cols bf16 values, `term` elements from one term to the
+// next.  Its tiles are B (rows or columns of the result) x 64 (terms of the sum).
+struct Operand {
+    const uint16_t* p;
+    int64_t pitch, term;
+    int rows, cols;
+};
+
+// Brings an operand's tiles to LDS.  TR false: the sum runs along an operand's rows
+// (rows of the tile are rows in memory); LDS holds row r's eight 16-byte parts at
+// positions part ^ (r & 7), so that a column of 16 rows' parts spreads over the banks.
+// TR true: the sum runs down its columns; LDS holds 64 rows of B values, row k's
+// 32-byte blocks at positions block ^ swizzle(k), for ds_read_tr16_b64, whose 16 lanes
+// read 4 rows x 32 bytes and get a column of 4 each.  Each wave instruction copies 1 KiB
+// to consecutive LDS bytes: the permutations are in the global addresses.
+// VEC false: rows without 16-byte alignment, through registers.
+template <int B, bool TR, int N, int WAVES, bool VEC>
+struct Loader {
+    static constexpr int I = N * B / 8 / WAVES;
+    static_assert(N * B % (8 * WAVES) == 0, "every wavefront copies the same share");
+    static constexpr int kBytes = N * B * 128;
+    const char* at[I];
+    int kc, k_end;        // first element along the sum of this lane's part of a step; the sum's end
+    int col_left[I];      // VEC false, TR: columns from the part's first on
+    int64_t step;         // bytes from one step to the next
+
+    static __device__ int swizzle(int k) { return (k & 3) | (k >> 1 & 4); }
+    static __device__ int k_row(int q, int lane) { return 512 / B * (q % (B / 8)) + lane / (B / 8); }
+
+    // m0: first row or column of the result; the sum from element k0
+    __device__ void init(const Operand& op, int m0, int64_t k0, int wave, int lane) {
+        k_end = TR ? op.rows : op.cols;
+        step = TR ? (int64_t)LHL_STEP * op.pitch * 2 : LHL_STEP * 2;
+        kc = 8 * ((lane & 7) ^ (lane >> 3));
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int q = wave * I + i, term = q / (B / 8);
+            int64_t e;
+            if constexpr (TR) {
+                const int k = k_row(q, lane), pos = lane % (B / 8);
+                int col = m0 + 16 * ((pos >> 1) ^ swizzle(k)) + 8 * (pos & 1);
+                if (VEC) col = min(col, op.cols - 8);  // past the last column: values that nothing reads
+                col_left[i] = op.cols - col;
+                e = (k0 + k) * op.pitch + col;
+            } else {
+                const int row = min(m0 + 8 * (q % (B / 8)) + lane / 8, op.rows - 1);  // as above
+                e = row * op.pitch + k0 + kc;
+            }
+            at[i] = reinterpret_cast<const char*>(op.p + term * op.term + e);
+        }
+    }
+
+    // Starts the copy of the step whose sum begins at k (from 0) and moves on.
+    __device__ void issue(char* lds, int k, const char* zeros, int wave, int lane) {
+        const bool tail = k + LHL_STEP > k_end;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int q = wave * I + i;
+            const int mine = k + (TR ? k_row(q, lane) : kc);
+            if constexpr (VEC) {
+                const char* src = at[i];
+                if (tail && mine >= k_end) src = zeros;
+                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + q * 1024), 16, 0, 0);
+            } else {
+                const int n = TR ? (mine < k_end ? col_left[i] : 0) : k_end - mine;
+                u32x4 v = {0, 0, 0, 0};
+                if (n >= 8) {
+                    __builtin_memcpy(&v, at[i], 16);
+                } else {
+                    const uint16_t* p = reinterpret_cast<const uint16_t*>(at[i]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < n) v[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
+                }
+                *reinterpret_cast<u32x4*>(lds + q * 1024 + lane * 16) = v;
+            }
+            at[i] += step;
+        }
+    }
+};
+
+// A wavefront's MFMA operands from a tile: T 16-wide parts from column (row) first on.
+template <int B, bool TR, int N, int T>
+struct Reader {
+    int at[TR ? T : 2];
+    __device__ void init(int first, int lane) {
+        const int c = lane & 15, g = lane >> 4;
+        if constexpr (TR) {
+            const int f = (c >> 2) | (g & 1) << 2;
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                at[t] = (8 * g + (c >> 2)) * 2 * B + ((first / 16 + t) ^ f) * 32 + (c & 3) * 8;
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) at[s] = (first + c) * 128 + ((4 * s + g) ^ (c & 7)) * 16;
+        }
+    }
+    // part t, half-step s (32 terms of the sum)
+    __device__ void read(const char* lds, int t, int s, u32x4 (&x)[N]) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const char* p = lds + n * B * 128;
+            if constexpr (TR) {
+                using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + at[t] + 32 * s * 2 * B));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + at[t] + (32 * s + 4) * 2 * B));
+                const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+                x[n] = u32x4{a[0], a[1], b[0], b[1]};
+            } else {
+                x[n] = *reinterpret_cast<const u32x4*>(p + at[s] + t * 2048);
+            }
+        }
+    }
+};
+
+// BM x BN of a product by WM x WN wavefronts: acc[i][j] holds rows 16 i + 4 (lane / 16) .. + 3
+// and column 16 j + lane % 16 of the wavefront's part.  NA, NB: the operands' terms, the pairs
+// with ta + tb < MOST taken.  Two or more steps' tiles in LDS: while one is multiplied the next
+// are on their way; one barrier a step.
+template <int BM_, int BN_, int WM_, int WN_, bool TRA, bool TRB, int NA, int NB, int MOST, bool VEC, int STAGES>
+struct Product {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
+    using LA = Loader<BM, TRA, NA, kWaves, VEC>;
+    using LB = Loader<BN, TRB, NB, kWaves, true>;
+    static constexpr int kStage = LA::kBytes + LB::kBytes;
+    static constexpr int kLds = STAGES * kStage;
+
+    static __device__ void wait(bool all) {
+        constexpr int kLeft = VEC ? (STAGES - 2) * (LA::I + LB::I) : 0;
+        static_assert(kLeft < 64, "vmcnt has six bits");
+        // vmcnt(0 or kLeft) lgkmcnt(0): this wavefront's share of the step is in LDS, and its reads
+        // of the step before are done
+        if (all || kLeft == 0)
+            __builtin_amdgcn_s_waitcnt(0x0070);
+        else
+            __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | (kLeft >> 4) << 14);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    static __device__ void run(const Operand& a, const Operand& b, int m0, int n0, int k0, int steps, const char* zeros,
+                               char* lds, f32x4 (&acc)[MT][NT]) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        LA la;
+        LB lb;
+        la.init(a, m0, k0, wave, lane);
+        lb.init(b, n0, k0, wave, lane);
+        Reader<BM, TRA, NA, MT> ra;
+        Reader<BN, TRB, NB, NT> rb;
+        ra.init(wave / WN * (BM / WM), lane);
+        rb.init(wave % WN * (BN / WN), lane);
+        auto issue = [&](int s) {
+            char* p = lds + s % STAGES * kStage;
+            la.issue(p, k0 + s * LHL_STEP, zeros, wave, lane);
+            lb.issue(p + LA::kBytes, k0 + s * LHL_STEP, zeros, wave, lane);
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s)
+            if (s < steps) issue(s);
+        for (int s = 0; s < steps; ++s) {
+            wait(s + STAGES - 2 >= steps);
+            if (s + STAGES - 1 < steps) issue(s + STAGES - 1);
+            const char* p = lds + s % STAGES * kStage;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 fa[MT][NA], fb[NT][NB];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) ra.read(p, i, h, fa[i]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) rb.read(p + LA::kBytes, j, h, fb[j]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma_terms<NA, NB, MOST>(fa[i], fb[j], acc[i][j]);
+            }
+        }
+    }
+};
+
+template <int MT, int NT>
+__device__ __forceinline__ void clear(f32x4 (&acc)[MT][NT]) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+}
+
+// Tile t of tm x tn: workgroups go round the eight XCDs, so each XCD gets a run of tiles; in a run
+// 8 tiles of m take turns along n, so that the tiles at work in an XCD share their operands in its L2.
+__device__ __forceinline__ bool tile_of(int tm, int tn, int& m, int& n) {
+    const int total = tm * tn, each = (total + 7) / 8, t = blockIdx.x % 8 * each + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= each || t >= total) return false;
+    const int group = t / (8 * tn), first = group * 8, deep = min(8, tm - first), in = t - group * 8 * tn;
+    m = first + in % deep;
+    n = in / deep;
+    return true;
+}
+inline unsigned tile_grid(size_t tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
+
+struct Parts {
+    char* work;
+    LossWork w;
+    template <class T>
+    __device__ T* at(size_t offset) const {
+        return reinterpret_cast<T*>(work + offset);
+    }
+    __device__ int count() const { return *reinterpret_cast<const int*>(work); }
+    __device__ const char* zeros() const { return work + 256; }
+};
+
+// ---- the rows that count ---------------------------------------------------------------
+// 64 rows to a workgroup, which counts the rows before its own by itself: four bytes a row,
+// next to the 2 KiB and more of a row's state.
+template <int NT>
+__global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, bool grad) {
+    __shared__ int before_sh[4], local[64], kept_sh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * 64;
+    auto counts = [&](int r) {
+        const int t = a.targets[r];
+        return t >= 0 && t < a.vocab;
+    };
+    int before = 0;
+    for (int r = threadIdx.x; r < r0; r += 256) before += counts(r);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
+    if (lane == 0) before_sh[wave] = before;
+    if (blockIdx.x == 0 && threadIdx.x < 64) reinterpret_cast<uint32_t*>(p.work + 256)[threadIdx.x] = 0;
+    __syncthreads();
+    before = before_sh[0] + before_sh[1] + before_sh[2] + before_sh[3];
+    if (wave == 0) {
+        const int r = r0 + lane;
+        const bool in = r < a.rows, kept = in && counts(r);
+        const uint64_t all = __ballot(kept);
+        const int mine = __popcll(all & ((1ull << lane) - 1)), c = before + mine;
+        if (kept) {
+            local[mine] = r;
+            p.at<int>(p.w.rows_at)[c] = r;
+            p.at<int>(p.w.target_at)[c] = a.targets[r];
+            if (grad) {
+                p.at<float>(p.w.lse_at)[c] = a.lse[r];
+                p.at<float>(p.w.gl_at)[c] = a.grad_loss[r];
+            }
+        } else if (in && !grad) {
+            const float x = a.targets[r] < 0 ? 0.0f : __builtin_nanf("");
+            if (a.loss) a.loss[r] = x;
+            if (a.lse) a.lse[r] = x;
+        }
+        if (in) p.at<int>(p.w.place_at)[r] = kept ? c : a.targets[r] < 0 ? -1 : -2;
+        if (lane == 0) {
+            kept_sh = __popcll(all);
+            if (r0 + 64 >= a.rows) *reinterpret_cast<int*>(p.work) = before + __popcll(all);
+        }
+    }
+    __syncthreads();
+    const int kept = kept_sh;
+    uint16_t* out = p.at<uint16_t>(p.w.h_at);
+    const int parts = p.w.pitch / 8;
+    for (int u = threadIdx.x; u < kept * parts; u += 256) {
+        const int i = u / parts, e = 8 * (u % parts), c = before + i;
+        const int64_t src = (int64_t)local[i] * a.h_row + e;
+        float x[8];
+        u32x4 t[NT];
+        if constexpr (NT == 1) {
+            const uint16_t* h = static_cast<const uint16_t*>(a.h) + src;
+            if (e + 8 <= a.hidden) {
+                __builtin_memcpy(&t[0], h, 16);
+            } else {
+                t[0] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (e + j < a.hidden) t[0][j / 2] |= (uint32_t)h[j] << (j % 2 * 16);
+            }
+        } else {
+            const float* h = static_cast<const float*>(a.h) + src;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = e + j < a.hidden ? h[j] : 0.0f;
+            split8(x, t);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<u32x4*>(out + ((size_t)n * a.rows + c) * p.w.pitch + e) = t[n];
+    }
+}
+
+// ---- logits ---------------------------------------------------------------------------
+__device__ __forceinline__ Operand states_of(const lm_head_loss_args& a, const Parts& p, int count) {
+    return Operand{p.at<uint16_t>(p.w.h_at), p.w.pitch, (int64_t)a.rows * p.w.pitch, count, p.w.pitch};
+}
+
+// Tiles of vocabulary x counted rows.  kGrad false: for each row the tile's maximum and sum of
+// exponentials above it, and the target's logit; true: D for vocabulary rows v0 .. of a piece.
+template <class P, int NT, bool kGrad>
+__global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_args a, Parts p, int v0, int tm, int tn) {
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    int m, n;
+    if (!tile_of(tm, tn, m, n)) return;
+    const int count = p.count();
+    if (n * P::BN >= count) return;
+    const int vfirst = v0 + m * P::BM;
+    f32x4 acc[P::MT][P::NT];
+    clear(acc);
+    const Operand w{a.table, a.table_row, 0, a.vocab, a.hidden};
+    P::run(w, states_of(a, p, count), vfirst, n * P::BN, 0, p.w.pitch / LHL_STEP, p.zeros(), lds, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int vw = vfirst + wave / P::WN * (P::BM / P::WM) + 4 * g;
+    const int nw = n * P::BN + wave % P::WN * (P::BN / P::WN) + c;
+    if constexpr (kGrad) {
+#pragma unroll
+        for (int j = 0; j < P::NT; ++j) {
+            const int row = nw + 16 * j;
+            if (row >= count) continue;
+            const float lse = p.at<float>(p.w.lse_at)[row], gl = p.at<float>(p.w.gl_at)[row];
+            const int target = p.at<int>(p.w.target_at)[row];
+            uint16_t* out = p.at<uint16_t>(p.w.d_at) + (size_t)row * p.w.piece;
+#pragma unroll
+            for (int i = 0; i < P::MT; ++i) {
+                const int v = vw + 16 * i;
+                f32x4 d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = exp2f((acc[i][j][e] - lse) * kLog2e);
+                    d[e] = v + e < a.vocab ? gl * (v + e == target ? y - 1.0f : y) : 0.0f;
+                }
+                u32x2 t[NT];
+                if constexpr (NT == 1) {
+                    // D rounded to nearest: half a step of each term of the sums that read it, as
+                    // independent as the logits are, so less than their own bf16 result's
+                    t[0][0] = from_float<uint16_t>(d[0]) | (uint32_t)from_float<uint16_t>(d[1]) << 16;
+                    t[0][1] = from_float<uint16_t>(d[2]) | (uint32_t)from_float<uint16_t>(d[3]) << 16;
+                } else {
+                    split4(d, t);
+                }
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+                    *reinterpret_cast<u32x2*>(out + (size_t)x * a.rows * p.w.piece + (v - v0)) = t[x];
+            }
+        }
+    } else {
+        __syncthreads();  // the tiles in LDS have been read
+        float2* red = reinterpret_cast<float2*>(lds);
+#pragma unroll
+        for (int j = 0; j < P::NT; ++j) {
+            const int row = nw + 16 * j;
+            const int target = row < count ? p.at<int>(p.w.target_at)[row] : -1;
+            float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = vw + 16 * i + e;
+                    if (v >= a.vocab) acc[i][j][e] = -__builtin_inff();
+                    if (v == target) p.at<float>(p.w.logit_at)[row] = acc[i][j][e];
+                    top = fmaxf(top, acc[i][j][e]);
+                }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // (a part past the vocabulary has no maximum: its terms are 0)
+            const float ref = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+            for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += exp2f((acc[i][j][e] - ref) * kLog2e);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (g == 0) red[wave / P::WN * P::BN + wave % P::WN * (P::BN / P::WN) + 16 * j + c] = {top, sum};
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < P::BN; x += P::kThreads) {
+            const int row = n * P::BN + x;
+            if (row >= count) break;
+            float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < P::WM; ++y) top = fmaxf(top, red[y * P::BN + x].x);
+#pragma unroll
+            for (int y = 0; y < P::WM; ++y) {
+                const float2 r = red[y * P::BN + x];
+                sum += r.x == -__builtin_inff() ? r.y : r.y * exp2f((r.x - top) * kLog2e);
+            }
+            p.at<float2>(p.w.part_at)[(size_t)row * tm + m] = {top, sum};
+        }
+    }
+}
+
+// One wavefront a row: lse from the tiles' parts.
+__global__ __launch_bounds__(256) void lhl_loss_kernel(lm_head_loss_args a, Parts p, int tiles) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= p.count()) return;
+    const float2* part = p.at<float2>(p.w.part_at) + (size_t)row * tiles;
+    float top = -__builtin_inff(), sum = 0.0f;
+    for (int t = lane; t < tiles; t += 64) top = fmaxf(top, part[t].x);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    for (int t = lane; t < tiles; t += 64) sum += part[t].y * exp2f((part[t].x - top) * kLog2e);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) {
+        const float lse = top + logf(sum);
+        const int r = p.at<int>(p.w.rows_at)[row];
+        if (a.lse) a.lse[r] = lse;
+        if (a.loss) a.loss[r] = lse - p.at<float>(p.w.logit_at)[row];
+    }
+}
+
+// ---- gradients ------------------------------------------------------------------------
+// sum[split][row][h]: tiles of h x counted rows, the sum over a split of the piece's vocabulary
+// rows v0 .. v0 + width, on top of the pieces' before.
+template <class P>
+__global__ __launch_bounds__(P::kThreads) void lhl_grad_h_kernel(lm_head_loss_args a, Parts p, int v0, int width, int tm,
+                                                                  int tn) {
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    int m, n;
+    if (!tile_of(tm, tn * p.w.splits, m, n)) return;
+    const int split = n / tn;
+    n %= tn;
+    const int count = p.count();
+    if (n * P::BN >= count) return;
+    const int steps = (width + LHL_STEP - 1) / LHL_STEP, each = (steps + p.w.splits - 1) / p.w.splits;
+    const int s0 = min(split * each, steps), s1 = min(s0 + each, steps);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int hw = m * P::BM + wave / P::WN * (P::BM / P::WM) + 4 * g;
+    const int nw = n * P::BN + wave % P::WN * (P::BN / P::WN) + c;
+    float* sum = p.at<float>(p.w.sum_at) + (size_t)split * a.rows * p.w.pitch;
+    f32x4 acc[P::MT][P::NT];
+    clear(acc);
+    if (v0 > 0)
+#pragma unroll
+        for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < P::NT; ++j)
+                if (nw + 16 * j < count && hw + 16 * i < p.w.pitch)
+                    acc[i][j] = *reinterpret_cast<const f32x4*>(sum + (size_t)(nw + 16 * j) * p.w.pitch + hw + 16 * i);
+    const Operand w{a.table + (int64_t)v0 * a.table_row, a.table_row, 0, a.vocab - v0, a.hidden};
+    const Operand d{p.at<uint16_t>(p.w.d_at), p.w.piece, (int64_t)a.rows * p.w.piece, count, p.w.piece};
+    P::run(w, d, m * P::BM, n * P::BN, s0 * LHL_STEP, s1 - s0, p.zeros(), lds, acc);
+#pragma unroll
+    for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < P::NT; ++j)
+            if (nw + 16 * j < count && hw + 16 * i < p.w.pitch)
+                *reinterpret_cast<f32x4*>(sum + (size_t)(nw + 16 * j) * p.w.pitch + hw + 16 * i) = acc[i][j];
+}
+
+// grad_h's rows from the splits' sums; rows that do not count get 0 or NaN.
+template <class T>
+__global__ __launch_bounds__(256) void lhl_finish_kernel(lm_head_loss_args a, Parts p) {
+    const int row = blockIdx.x, at = p.at<int>(p.w.place_at)[row];
+    T* out = static_cast<T*>(a.grad_h) + (int64_t)row * a.grad_h_row;
+    const float* sum = p.at<float>(p.w.sum_at) + (size_t)max(at, 0) * p.w.pitch;
+    for (int h = threadIdx.x; h < a.hidden; h += 256) {
+        float x = at == -2 ? __builtin_nanf("") : 0.0f;
+        if (at >= 0)
+            for (int s = 0; s < p.w.splits; ++s) x += sum[(size_t)s * a.rows * p.w.pitch + h];
+        out[h] = from_float<T>(x);
+    }
+}
+
+// grad_table for vocabulary rows v0 .. v0 + width: tiles of h x vocabulary.
+template <class P>
+__global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_loss_args a, Parts p, int v0, int tm,
+                                                                      int tn, int wide) {
+    __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+    int m, n;
+    if (!tile_of(tm, tn, m, n)) return;
+    const int count = p.count();
+    f32x4 acc[P::MT][P::NT];
+    clear(acc);
+    const Operand d{p.at<uint16_t>(p.w.d_at), p.w.piece, (int64_t)a.rows * p.w.piece, count, p.w.piece};
+    P::run(states_of(a, p, count), d, m * P::BM, n * P::BN, 0, (count + LHL_STEP - 1) / LHL_STEP, p.zeros(), lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int hw = m * P::BM + wave / P::WN * (P::BM / P::WM) + 4 * g;
+    const int vw = v0 + n * P::BN + wave % P::WN * (P::BN / P::WN) + c;
+#pragma unroll
+    for (int j = 0; j < P::NT; ++j) {
+        const int v = vw + 16 * j;
+        if (v >= a.vocab) continue;
+        uint16_t* out = a.grad_table + (int64_t)v * a.grad_table_row;
+#pragma unroll
+        for (int i = 0; i < P::MT; ++i) {
+            const int h = hw + 16 * i;
+            uint16_t x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = from_float<uint16_t>(acc[i][j][e]);
+            if (wide && h + 4 <= a.hidden) {
+                *reinterpret_cast<u32x2*>(out + h) = u32x2{x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (h + e < a.hidden) out[h + e] = x[e];
+            }
+        }
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------
+template <int NT>
+hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStream_t s) {
+    lhl_prepare_kernel<NT><<<dim3((unsigned)std::max(1, (a.rows + 63) / 64)), 256, 0, s>>>(a, p, grad);
+    return hipGetLastError();
+}
+
+template <int BN, int NT, bool VEC, bool kGrad>
+hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
+    constexpr int WN = BN == 128 ? 2 : 1, WM = 4 / WN;
+    constexpr int kStages = BN == 128 || !VEC ? 2 : 3;
+    using P = Product<LHL_TILE, BN, WM, WN, false, false, 1, NT, 3, VEC, kStages>;
+    const int tm = (width + LHL_TILE - 1) / LHL_TILE, tn = (a.rows + BN - 1) / BN;
+    lhl_logits_kernel<P, NT, kGrad>
+        <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn);
+    return hipGetLastError();
+}
+
+template <int NT, bool VEC, bool kGrad>
+hipError_t logits_of(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
+    if (a.rows <= 32) return logits<32, NT, VEC, kGrad>(a, p, v0, width, s);
+    if (a.rows <= 64) return logits<64, NT, VEC, kGrad>(a, p, v0, width, s);
+    return logits<128, NT, VEC, kGrad>(a, p, v0, width, s);
+}
+
+template <int NT, bool VEC>
+hipError_t loss(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
+    hipError_t e = prepare<NT>(a, p, false, s);
+    if (e == hipSuccess) e = logits_of<NT, VEC, false>(a, p, 0, a.vocab, s);
+    if (e != hipSuccess) return e;
+    lhl_loss_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s>>>(a, p, p.w.vtiles);
+    return hipGetLastError();
+}
+
+template <int BN, int NT, bool VEC>
+hipError_t grad_h(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
+    using P = Product<128, BN, BN == 128 ? 2 : 4, BN == 128 ? 2 : 1, true, false, 1, NT, 3, VEC, 2>;
+    const int tm = (p.w.pitch + 127) / 128, tn = (a.rows + BN - 1) / BN;
+    lhl_grad_h_kernel<P>
+        <<<dim3(tile_grid((size_t)tm * tn * p.w.splits)), P::kThreads, 0, s>>>(a, p, v0, width, tm, tn);
+    return hipGetLastError();
+}
+
+template <int NT, bool VEC>
+hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
+    hipError_t e = prepare<NT>(a, p, true, s);
+    const bool wide = ((uintptr_t)a.grad_table | (uintptr_t)(a.grad_table_row * 2)) % 8 == 0;
+    for (int v0 = 0; v0 < a.vocab && e == hipSuccess; v0 += p.w.piece) {
+        const int width = std::min(p.w.piece, a.vocab - v0);
+        if (a.rows > 0) e = logits_of<NT, VEC, true>(a, p, v0, width, s);
+        if (e == hipSuccess && a.grad_h && a.rows > 0)
+            e = a.rows <= 64 ? grad_h<64, NT, VEC>(a, p, v0, width, s) : grad_h<128, NT, VEC>(a, p, v0, width, s);
+        if (e == hipSuccess && a.grad_table) {
+            constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 2^-16 of its terms
+            using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 2>;
+            const int tm = (p.w.pitch + 127) / 128, tn = (width + 127) / 128;
+            lhl_grad_table_kernel<P>
+                <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+            e = hipGetLastError();
+        }
+    }
+    if (e != hipSuccess || !a.grad_h || a.rows == 0) return e;
+    if (NT == 1)
+        lhl_finish_kernel<uint16_t><<<dim3((unsigned)a.rows), 256, 0, s>>>(a, p);
+    else
+        lhl_finish_kernel<float><<<dim3((unsigned)a.rows), 256, 0, s>>>(a, p);
+    return hipGetLastError();
+}
+
+bool rows_of_16(const lm_head_loss_args& a) {
+    return ((uintptr_t)a.table | (uintptr_t)(a.table_row * 2) | (uintptr_t)(a.hidden * 2)) % 16 == 0;
+}
+
+}  // namespace
+
+hipError_t lhl_launch_loss(const lm_head_loss_args& a, const LossWork& w, hipStream_t s) {
+    const Parts p{static_cast<char*>(a.work), w};
+    if (a.dtype == QWEN_BF16) return rows_of_16(a) ? loss<1, true>(a, p, s) : loss<1, false>(a, p, s);
+    return rows_of_16(a) ? loss<3, true>(a, p, s) : loss<3, false>(a, p, s);
+}
+
+hipError_t lhl_launch_grad(const lm_head_loss_args& a, const LossWork& w, hipStream_t s) {
+    const Parts p{static_cast<char*>(a.work), w};
+    if (a.dtype == QWEN_BF16) return rows_of_16(a) ? grad<1, true>(a, p, s) : grad<1, false>(a, p, s);
+    return rows_of_16(a) ? grad<3, true>(a, p, s) : grad<3, false>(a, p, s);
+}

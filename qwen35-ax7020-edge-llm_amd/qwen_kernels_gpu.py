@@ -74,7 +74,7 @@ class MlpPlan(ctypes.Structure):
     ]
 
 
-GDN_F32, GDN_BF16 = 0, 1
+QWEN_F32, QWEN_BF16 = 0, 1
 
 
 class gdn_dev_args(ctypes.Structure):
@@ -87,6 +87,17 @@ class gdn_dev_args(ctypes.Structure):
         ("q_row", c_int64), ("k_row", c_int64), ("v_row", c_int64), ("out_row", c_int64), ("gate_row", c_int64),
         ("rows", c_int), ("n_seq", c_int), ("n_slots", c_int), ("heads_k", c_int), ("heads_v", c_int),
         ("dim_k", c_int), ("dim_v", c_int), ("dtype", c_int), ("scale", c_float),
+    ]
+
+
+class lm_head_loss_args(ctypes.Structure):
+    """Mirror of ``lm_head_loss_args`` (include/qwen_kernels.h)."""
+
+    _fields_ = [
+        ("loss", c_void_p), ("lse", c_void_p), ("grad_h", c_void_p), ("grad_table", c_void_p), ("h", c_void_p),
+        ("table", c_void_p), ("targets", c_void_p), ("grad_loss", c_void_p), ("work", c_void_p),
+        ("work_bytes", c_size_t), ("h_row", c_int64), ("table_row", c_int64), ("grad_h_row", c_int64),
+        ("grad_table_row", c_int64), ("rows", c_int), ("vocab", c_int), ("hidden", c_int), ("dtype", c_int),
     ]
 
 
@@ -225,6 +236,11 @@ def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gdn_dev_prompt_work_bytes.restype = c_size_t
     for name in ("gdn_dev_prompt", "gdn_dev_step"):
         getattr(lib, name).argtypes = [POINTER(gdn_dev_args), vp]
+        getattr(lib, name).restype = i
+    for name in ("bf16_dev_lm_head_loss", "bf16_dev_lm_head_loss_grad"):
+        getattr(lib, name + "_work_bytes").argtypes = [POINTER(lm_head_loss_args)]
+        getattr(lib, name + "_work_bytes").restype = c_size_t
+        getattr(lib, name).argtypes = [POINTER(lm_head_loss_args), vp]
         getattr(lib, name).restype = i
     lib.bfp8_stream.argtypes = []
     lib.bfp8_stream.restype = vp
@@ -607,7 +623,7 @@ def _gdn_args(q, k, v, alpha, beta, scale, states, slots, out):
     a.out, a.q, a.k, a.v, a.alpha = _dp(out), _dp(q), _dp(k), _dp(v), _dp(alpha)
     a.beta = None if beta is None else _dp(beta)
     a.rows, a.n_slots, a.heads_k, a.heads_v, a.dim_k, a.dim_v = rows, n_slots, hk, hv, dk, dv
-    a.dtype = GDN_F32 if q.dtype == torch.float32 else GDN_BF16
+    a.dtype = QWEN_F32 if q.dtype == torch.float32 else QWEN_BF16
     a.scale = scale
     return a
 
@@ -659,7 +675,7 @@ def linear_attention_prompt_work_bytes(rows, n_seq, heads_k, heads_v, dim_k, dim
     """Bytes of linear_attention_prompt's work for these sizes (dtype: of q, k, v)."""
     a = gdn_dev_args()
     a.rows, a.n_seq, a.heads_k, a.heads_v, a.dim_k, a.dim_v = rows, n_seq, heads_k, heads_v, dim_k, dim_v
-    a.dtype = {_torch().float32: GDN_F32, _torch().bfloat16: GDN_BF16}[dtype]
+    a.dtype = {_torch().float32: QWEN_F32, _torch().bfloat16: QWEN_BF16}[dtype]
     n = load().gdn_dev_prompt_work_bytes(a)
     if not n:
         check(BFP8_EINVAL, "linear_attention_prompt_work_bytes")
@@ -682,3 +698,85 @@ def linear_attention_step(q, k, v, alpha, beta, state, *, scale=1.0, slots=None,
         a.n_seq = a.rows
         check(load().gdn_dev_step(a, _stream()), "linear_attention_step")
     return out
+
+
+def _loss_args(h, table, targets):
+    torch = _torch()
+    if h.dim() != 2 or table.dim() != 2 or h.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("h is [rows, hidden] in float32 or bfloat16, table [vocab, hidden] in bfloat16")
+    a = lm_head_loss_args()
+    a.rows, a.hidden = h.shape
+    a.vocab = table.shape[0]
+    a.h_row = _rows_of(h, "h", (a.rows, a.hidden), h.dtype)
+    a.table_row = _rows_of(table, "table", (a.vocab, a.hidden), torch.bfloat16)
+    _flat(targets, "targets", (a.rows,), torch.int32)
+    a.h, a.table, a.targets = _dp(h), _dp(table), _dp(targets)
+    a.dtype = QWEN_F32 if h.dtype == torch.float32 else QWEN_BF16
+    return a
+
+
+def _loss_call(name, a, work, device):
+    """Runs entry point `name` with the caller's work or a new one."""
+    torch = _torch()
+    lib = load()
+    need = getattr(lib, name + "_work_bytes")(a)
+    if need and work is None:
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+    if work is not None:
+        a.work, a.work_bytes = _dp(work), work.numel() * work.element_size()
+    check(getattr(lib, name)(a, _stream()), name)
+
+
+def lm_head_loss(h, table, targets, *, work=None):
+    """Negative log-likelihood of each row's target under the tied-embedding head
+    -> (loss, lse), float32 [rows]; the logits are not kept.
+
+    h [rows, hidden] float32 or bfloat16, table [vocab, hidden] bfloat16, targets
+    int32 [rows]: below 0 the row is ignored (loss and lse 0), vocab or more
+    gives NaN.  work: uint8 scratch of at least lm_head_loss_work_bytes.  The rest
+    is bf16_dev_lm_head_loss's contract (include/qwen_kernels.h)."""
+    torch = _torch()
+    with _same_device(h, table=table, targets=targets, work=work):
+        a = _loss_args(h, table, targets)
+        loss, lse = torch.empty(2, a.rows, dtype=torch.float32, device=h.device)
+        a.loss, a.lse = _dp(loss), _dp(lse)
+        _loss_call("bf16_dev_lm_head_loss", a, work, h.device)
+    return loss, lse
+
+
+def lm_head_loss_grad(h, table, targets, lse, grad_loss, *, need_h=True, need_table=True, grad_h=None,
+                      grad_table=None, work=None):
+    """The gradients of sum(grad_loss * loss) -> (grad_h, grad_table), in h's and the
+    table's type, overwritten where given; None for one that is not needed.
+    lse is lm_head_loss's; grad_loss float32 [rows]."""
+    torch = _torch()
+    with _same_device(h, table=table, targets=targets, lse=lse, grad_loss=grad_loss, grad_h=grad_h,
+                      grad_table=grad_table, work=work):
+        a = _loss_args(h, table, targets)
+        _flat(lse, "lse", (a.rows,), torch.float32)
+        _flat(grad_loss, "grad_loss", (a.rows,), torch.float32)
+        if need_h and grad_h is None:
+            grad_h = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        if need_table and grad_table is None:
+            grad_table = torch.empty(table.shape, dtype=table.dtype, device=h.device)
+        a.lse, a.grad_loss = _dp(lse), _dp(grad_loss)
+        if need_h:
+            a.grad_h, a.grad_h_row = _dp(grad_h), _rows_of(grad_h, "grad_h", h.shape, h.dtype)
+        if need_table:
+            a.grad_table = _dp(grad_table)
+            a.grad_table_row = _rows_of(grad_table, "grad_table", table.shape, table.dtype)
+        _loss_call("bf16_dev_lm_head_loss_grad", a, work, h.device)
+    return grad_h if need_h else None, grad_table if need_table else None
+
+
+def lm_head_loss_work_bytes(rows, vocab, hidden, dtype, *, grad=False, need_h=True) -> int:
+    """Bytes of lm_head_loss's work for these sizes (dtype: of h), or of lm_head_loss_grad's."""
+    a = lm_head_loss_args()
+    a.rows, a.vocab, a.hidden = rows, vocab, hidden
+    a.dtype = {_torch().float32: QWEN_F32, _torch().bfloat16: QWEN_BF16}[dtype]
+    a.grad_h = 1 if need_h else None  # only whether it is there
+    lib = load()
+    n = (lib.bf16_dev_lm_head_loss_grad_work_bytes if grad else lib.bf16_dev_lm_head_loss_work_bytes)(a)
+    if not n:
+        check(BFP8_EINVAL, "lm_head_loss_work_bytes")
+    return n
