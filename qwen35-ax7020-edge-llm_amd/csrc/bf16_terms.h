@@ -19,13 +19,10 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
                                                    0, 0);
 }
 
-// The next term of x: its upper 16 bits, which x then lacks.
-__device__ __forceinline__ uint32_t cut(float& x) {
-    const uint32_t u = __float_as_uint(x) & 0xffff0000u;
-    x -= __uint_as_float(u);
-    return u;
-}
-__device__ __forceinline__ uint32_t pack(uint32_t lo, uint32_t hi) { return (lo >> 16) | hi; }
+// Takes its first term, its upper 16 bits, from x.
+__device__ __forceinline__ void cut(float& x) { x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// The upper halves of two words in one.
+__device__ __forceinline__ uint32_t pack(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
 
 // Eight floats as N terms, in the order of an MFMA operand's eight values.
 template <int N>
@@ -34,8 +31,8 @@ __device__ __forceinline__ void split8(float (&x)[8], u32x4 (&t)[N]) {
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = cut(x[2 * j]), hi = cut(x[2 * j + 1]);
-            t[n][j] = pack(lo, hi);
+            t[n][j] = pack(__float_as_uint(x[2 * j]), __float_as_uint(x[2 * j + 1]));
+            if (n + 1 < N) cut(x[2 * j]), cut(x[2 * j + 1]);
         }
 }
 template <int N>
@@ -45,8 +42,8 @@ __device__ __forceinline__ void split4(f32x4 x, u32x2 (&t)[N]) {
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t lo = cut(y[2 * j]), hi = cut(y[2 * j + 1]);
-            t[n][j] = pack(lo, hi);
+            t[n][j] = pack(__float_as_uint(y[2 * j]), __float_as_uint(y[2 * j + 1]));
+            if (n + 1 < N) cut(y[2 * j]), cut(y[2 * j + 1]);
         }
 }
 

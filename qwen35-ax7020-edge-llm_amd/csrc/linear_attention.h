@@ -19,7 +19,7 @@ struct GdnWork {
     int ks;            // steps of 32 along dim_k (1, 2, 4 or 8: dim_k is padded to 32 ks)
     int nt;            // bf16 terms of an input (1: bf16, 3: float32)
     int no;            // bf16 terms of what only outputs need (2 or 3)
-    size_t key_bytes;  // per chunk and key head: K, K^T and Q fragments
+    size_t key_bytes;  // per chunk and key head: K and Q as operands
     size_t tri_bytes;  // per chunk and value head: T and P fragments, the decays
     size_t n_chunks, total;
 };
@@ -29,7 +29,7 @@ inline GdnWork gdn_work(const gdn_dev_args& a) {
     w.ks = a.dim_k <= 32 ? 1 : a.dim_k <= 64 ? 2 : a.dim_k <= 128 ? 4 : 8;
     w.nt = a.dtype == QWEN_BF16 ? 1 : 3;
     w.no = a.dtype == QWEN_BF16 ? 2 : 3;
-    w.key_bytes = (size_t)3 * 4 * w.ks * w.nt * 1024;
+    w.key_bytes = (size_t)2 * 4 * w.ks * w.nt * 1024;
     w.tri_bytes = (size_t)(6 * 3 + 6 * w.no) * 1024 + 1024;
     w.n_chunks = (size_t)(a.rows / GDN_CHUNK) + (size_t)a.n_seq;
     w.total = w.n_chunks * (w.key_bytes * a.heads_k + w.tri_bytes * a.heads_v);

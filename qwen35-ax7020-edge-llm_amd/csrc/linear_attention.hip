@@ -23,14 +23,17 @@
 
 namespace {
 
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+
 constexpr int C = GDN_CHUNK;
 
-// Elements i .. i + 7 of a row as terms; those from dim on are zero.
+// Elements i .. i + 7 of a row as terms, zeros for those from dim on.  full: the whole padded row is
+// there, 16-byte aligned.
 template <int NT>
-__device__ __forceinline__ void load_terms(const void* row, int i, int dim, bool vec, u32x4 (&t)[NT]) {
+__device__ __forceinline__ void load_terms(const void* row, int i, int dim, bool full, u32x4 (&t)[NT]) {
     if constexpr (NT == 1) {
         const uint16_t* p = static_cast<const uint16_t*>(row);
-        if (vec && i + 8 <= dim) {
+        if (full) {
             t[0] = *reinterpret_cast<const u32x4*>(p + i);
             return;
         }
@@ -42,7 +45,7 @@ __device__ __forceinline__ void load_terms(const void* row, int i, int dim, bool
     } else {
         const float* p = static_cast<const float*>(row);
         float x[8];
-        if (vec && i + 8 <= dim) {
+        if (full) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(p + i), b = *reinterpret_cast<const f32x4*>(p + i + 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
@@ -83,42 +86,105 @@ __device__ __forceinline__ int slot_of(const gdn_dev_args& a, int s) {
 
 // The byte offsets of the work buffer's parts for one chunk.
 struct Places {
-    char *k, *kt, *q;            // fragments of key head: [4 or 2 ks row tiles][ks or 2 steps][nt] KiB
+    char *k, *q;                 // key head: the image of a KTile, Q fragments [4 row tiles][ks][nt] KiB
     char *t, *p;                 // triangular fragments: tile(rt, ts) of 6, x 3 or no terms
     float *up, *down, *last;     // 2^g, 2^(g_C - g), 2^(g_C)
 };
 template <int KS, int NT, int NO>
-__device__ __forceinline__ Places places(const gdn_dev_args& a, size_t n_chunks, size_t chunk, int hk, int hv) {
-    constexpr size_t kKey = (size_t)3 * 4 * KS * NT * 1024, kTri = (size_t)(18 + 6 * NO) * 1024 + 1024;
-    char* base = static_cast<char*>(a.work);
-    Places w;
-    w.k = base + (chunk * a.heads_k + hk) * kKey;
-    w.kt = w.k + (size_t)4 * KS * NT * 1024;
-    w.q = w.kt + (size_t)4 * KS * NT * 1024;
-    char* tri = base + n_chunks * a.heads_k * kKey + (chunk * a.heads_v + hv) * kTri;
-    w.t = tri;
-    w.p = tri + 18 * 1024;
-    w.up = reinterpret_cast<float*>(tri + (18 + 6 * NO) * 1024);
-    w.down = w.up + C;
-    w.last = w.down + C;
-    return w;
-}
+struct Layout {
+    static constexpr size_t kKey = (size_t)2 * 4 * KS * NT * 1024, kTri = (size_t)(18 + 6 * NO) * 1024 + 1024;
+    static __device__ Places at(const gdn_dev_args& a, size_t n_chunks, size_t chunk, int hk, int hv) {
+        char* base = static_cast<char*>(a.work);
+        Places w;
+        w.k = base + (chunk * a.heads_k + hk) * kKey;
+        w.q = w.k + kKey / 2;
+        char* tri = base + n_chunks * a.heads_k * kKey + (chunk * a.heads_v + hv) * kTri;
+        w.t = tri;
+        w.p = tri + 18 * 1024;
+        w.up = reinterpret_cast<float*>(tri + (18 + 6 * NO) * 1024);
+        w.down = w.up + C;
+        w.last = w.down + C;
+        return w;
+    }
+    static __device__ void next(const gdn_dev_args& a, Places& w) {
+        const size_t key = a.heads_k * kKey, tri = a.heads_v * kTri;
+        w.k += key;
+        w.q += key;
+        w.t += tri;
+        w.p += tri;
+        w.up += tri / 4;
+        w.down += tri / 4;
+        w.last += tri / 4;
+    }
+};
+
+// A chunk's K in LDS: a row of 64 KS bytes a token, [term][token], its 16-byte parts at positions
+// part ^ mix(token), so that neither eight consecutive elements of 16 tokens (K as a left operand) nor
+// four of four tokens (ds_read_tr16_b64: K^T) meet in a bank.
+template <int KS, int NT>
+struct KTile {
+    static constexpr int kRow = 64 * KS, kTerm = C * kRow, kBytes = NT * kTerm;
+    static __device__ __forceinline__ int mix(int t) {
+        if (KS >= 4) return (t & 3) << 2 | (t >> 2 & 3);
+        if (KS == 2) return (t & 1) << 2 | (t >> 1 & 3);
+        return t >> 2 & 3;
+    }
+    static __device__ __forceinline__ int part(int t, int c) { return t * kRow + (c ^ mix(t)) * 16; }
+    // K of tokens 16 w .., step s
+    static __device__ __forceinline__ void rows(const char* k, int w, int s, int lane, u32x4 (&f)[NT]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            f[t] = *reinterpret_cast<const u32x4*>(k + t * kTerm + part(16 * w + (lane & 15), 4 * s + (lane >> 4)));
+    }
+    // K^T: the state's rows of `tile`, tokens 32 ts ..
+    static __device__ __forceinline__ void columns(const char* k, int tile, int ts, int lane, u32x4 (&f)[NT]) {
+        using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+        const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            u32x2 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                v[h] = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (lds_s16x4*)(k + t * kTerm + part(32 * ts + 16 * h + 4 * g + c / 4, 4 * (tile / 2) + c % 4) +
+                                            8 * (tile % 2))));
+            f[t] = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+        }
+    }
+};
 // Tiles of a lower triangle of 4 x 2 tiles of 16 x 32: row tiles 0 and 1 have only
 // step 0.
 __device__ __forceinline__ constexpr int tri_tile(int rt, int ts) { return rt < 2 ? rt : 2 + (rt - 2) * 2 + ts; }
 
+// A product's result has four consecutive rows of a column in a lane; as the next
+// product's right operand it stays in that lane, if the next product sums in this order:
+// place e of lane group g is row 4 g + e of the first tile of a pair (e < 4) or 4 g + e - 4
+// of the second.  Tokens are in tiles of 16 in order; a pair of the state's tiles holds
+// rows 32 s + 8 g + e of dim_k, so that K and Q are eight consecutive elements a lane.
+__device__ __forceinline__ int state_row(int tile, int g) { return 32 * (tile / 2) + 8 * g + 4 * (tile % 2); }
+
+__device__ __forceinline__ void sync_lds() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): loads from memory stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // ---- chunks -------------------------------------------------------------------------
-// One chunk of one value head; wavefront w has its 16-row tile w.  What it writes is
-// in the order in which gdn_scan_kernel's lanes load it.
+// One chunk of one value head; wavefront w has tokens 16 w .. 16 w + 15.  What it writes is
+// in the order in which gdn_scan_kernel loads it.  direct: that kernel takes K and Q from
+// the inputs.
 template <int KS, int NT, bool kDelta>
-__global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n_chunks, int vec_q, int vec_k) {
-    constexpr int NO = NT == 1 ? 2 : 3;
-    __shared__ u32x4 ksh[4 * KS * NT * 64];  // K fragments
-    __shared__ __attribute__((aligned(16))) float lsh[C][C + 4];
-    __shared__ __attribute__((aligned(16))) float psh[C][C + 4];
+__global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n_chunks, int full_q, int full_k,
+                                                        int direct) {
+    constexpr int NO = NT == 1 ? 2 : 3, KP = 32 * KS + 8;
+    __shared__ __attribute__((aligned(16))) uint16_t ksh[NT][C][KP];  // K, a row a token
+    __shared__ __attribute__((aligned(16))) float lsh[kDelta ? C : 1][C + 4];
     __shared__ double gsh[C];
     __shared__ float bsh[C];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15,
+              grp = lane >> 4;
     const size_t chunk = blockIdx.x / a.heads_v;
     const int hv = blockIdx.x % a.heads_v, reach = a.heads_v / a.heads_k, hk = hv / reach;
 
@@ -141,39 +207,28 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
     const long c = (long)chunk - (first / C + seq);
     if (c < 0 || c * C >= len) return;
     const int row0 = first + (int)c * C, n = min(C, len - (int)c * C);
-    const Places at = places<KS, NT, NO>(a, n_chunks, chunk, hk, hv);
+    const Places at = Layout<KS, NT, NO>::at(a, n_chunks, chunk, hk, hv);
     const bool keys = hv % reach == 0;  // this workgroup leaves the key head's fragments too
 
     // K and Q rows of tile w as operand fragments
     u32x4 kf[KS][NT], qf[KS][NT];
     const int r = 16 * w + col;
     const int es = NT == 1 ? 2 : 4;
-    const char* krow = static_cast<const char*>(a.k) + ((int64_t)(row0 + r) * a.k_row + (int64_t)hk * a.dim_k) * es;
-    const char* qrow = static_cast<const char*>(a.q) + ((int64_t)(row0 + r) * a.q_row + (int64_t)hk * a.dim_k) * es;
+    // (rows behind the end: the last one, then zeros)
+    const int64_t row = row0 + min(r, n - 1);
+    const char* krow = static_cast<const char*>(a.k) + (row * a.k_row + (int64_t)hk * a.dim_k) * es;
+    const char* qrow = static_cast<const char*>(a.q) + (row * a.q_row + (int64_t)hk * a.dim_k) * es;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        const int dim = r < n ? a.dim_k : 0;
-        load_terms(krow, 32 * s + 8 * grp, dim, vec_k, kf[s]);
-        load_terms(qrow, 32 * s + 8 * grp, dim, vec_q, qf[s]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int f = ((w * KS + s) * NT + t) * 64 + lane;
-            ksh[f] = kf[s][t];
-            if (keys) {
-                reinterpret_cast<u32x4*>(at.k)[f] = kf[s][t];
-                reinterpret_cast<u32x4*>(at.q)[f] = qf[s][t];
-            }
-        }
+        load_terms(krow, 32 * s + 8 * grp, a.dim_k, full_k, kf[s]);
+        load_terms(qrow, 32 * s + 8 * grp, a.dim_k, full_q, qf[s]);
     }
     if (w == 0) {
         // g in double: differences of large sums stay exact to a float32.  A decay of 0
         // counts as 2^-16384, which no product brings back.
-        const int64_t row = (int64_t)(row0 + lane) * a.gate_row + hv;
-        double g = 0.0;
-        if (lane < n) {
-            const float al = a.alpha[row];
-            g = al == 0.0f ? -16384.0 : log2((double)al);
-        }
+        const int64_t grow = (int64_t)(row0 + min(lane, n - 1)) * a.gate_row + hv;
+        const float al = a.alpha[grow], be = kDelta ? a.beta[grow] : 0.0f;
+        double g = lane >= n ? 0.0 : al == 0.0f ? -16384.0 : log2((double)al);
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const double o = __shfl_up(g, d);
@@ -181,124 +236,169 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
         }
         const double gc = __shfl(g, 63);
         gsh[lane] = g;
-        bsh[lane] = kDelta && lane < n ? a.beta[row] : 0.0f;
+        bsh[lane] = lane < n ? be : 0.0f;
         at.up[lane] = exp2_of(g);
         at.down[lane] = exp2_of(gc - g);
         if (lane == 0) at.last[0] = exp2_of(gc);
     }
-    __syncthreads();
-
-    // K K^T and Q K^T, the tiles on and below the diagonal
 #pragma unroll
-    for (int ct = 0; ct < 4; ++ct) {
-        if (ct > w) {
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) psh[16 * w + 4 * grp + e][16 * ct + col] = 0.0f;
-            continue;
+        for (int t = 0; t < NT; ++t) {
+            if (r >= n) kf[s][t] = qf[s][t] = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(&ksh[t][r][32 * s + 8 * grp]) = kf[s][t];
+            const int f = ((w * KS + s) * NT + t) * 64 + lane;
+            if (keys && !direct) {
+                using K = KTile<KS, NT>;
+                *reinterpret_cast<u32x4*>(at.k + t * K::kTerm + K::part(r, 4 * s + grp)) = kf[s][t];
+                reinterpret_cast<u32x4*>(at.q)[f] = qf[s][t];
+            }
         }
+    sync_lds();
+
+    // K K^T and K Q^T, the tiles that hold a j <= i: lane has token i = r, four tokens j
+    f32x4 pt[4];
+    const double gi = gsh[r];
+    const float bi = bsh[r];
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) {
+        pt[jt] = f32x4{0, 0, 0, 0};
+        if (jt > w) continue;
         f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             u32x4 b[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) b[t] = ksh[((ct * KS + s) * NT + t) * 64 + lane];
-            if (kDelta) kk = mfma_terms<NT, NT, 3>(kf[s], b, kk);
-            qk = mfma_terms<NT, NT, 3>(qf[s], b, qk);
+            for (int t = 0; t < NT; ++t)
+                b[t] = *reinterpret_cast<const u32x4*>(&ksh[t][16 * jt + col][32 * s + 8 * grp]);
+            if (kDelta) kk = mfma_terms<NT, NT, 3>(b, kf[s], kk);
+            qk = mfma_terms<NT, NT, 3>(b, qf[s], qk);
         }
-        const int j = 16 * ct + col;
-        const double gj = gsh[j];
+        f32x4 l;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = 16 * w + 4 * grp + e;
-            const float d = i >= j ? exp2_of(gsh[i] - gj) : 0.0f;
-            psh[i][j] = i >= j ? qk[e] * d : 0.0f;
-            if (kDelta) lsh[i][j] = i > j ? bsh[i] * d * kk[e] : 0.0f;
+            const int j = 16 * jt + 4 * grp + e;
+            const float d = r >= j ? exp2_of(gi - gsh[j]) : 0.0f;
+            pt[jt][e] = r >= j ? qk[e] * d : 0.0f;
+            l[e] = r > j ? bi * d * kk[e] : 0.0f;
         }
+        if constexpr (kDelta) *reinterpret_cast<f32x4*>(&lsh[r][16 * jt + 4 * grp]) = l;
     }
-    __syncthreads();
-
-    if (kDelta && w == 0) {
-        // lane j solves (I + L) x = b_j e_j from the first row down: column j of T
-        float x[C];
-        const float bj = bsh[lane];
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            float s0 = i == lane ? bj : 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-#pragma unroll
-            for (int j = 0; j < (i & ~3); j += 4) {
-                const f32x4 l = *reinterpret_cast<const f32x4*>(&lsh[i][j]);
-                s0 = __builtin_fmaf(-l[0], x[j], s0);
-                s1 = __builtin_fmaf(-l[1], x[j + 1], s1);
-                s2 = __builtin_fmaf(-l[2], x[j + 2], s2);
-                s3 = __builtin_fmaf(-l[3], x[j + 3], s3);
-            }
-#pragma unroll
-            for (int j = i & ~3; j < i; ++j) s0 = __builtin_fmaf(-lsh[i][j], x[j], s0);
-            x[i] = (s0 + s1) + (s2 + s3);
-        }
-#pragma unroll
-        for (int i = 0; i < C; ++i) lsh[i][lane] = x[i];
-    }
-    if (keys) {
-        // K^T: row i of the state, eight tokens to a lane
-        const uint16_t* kw = reinterpret_cast<const uint16_t*>(ksh);
-        for (int f = w; f < 2 * KS * 2 * NT; f += 4) {
-            const int t = f % NT, ts = f / NT % 2, it = f / NT / 2;
-            const int i = 16 * it + col, s = i / 32, sub = i % 32 / 8, e = i % 8;
-            u32x4 v;
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                uint32_t h[2];
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    const int tok = 32 * ts + 8 * grp + j + d;
-                    h[d] = kw[((((tok / 16) * KS + s) * NT + t) * 64 + sub * 16 + tok % 16) * 8 + e];
-                }
-                v[j / 2] = h[0] | h[1] << 16;
-            }
-            reinterpret_cast<u32x4*>(at.kt)[f * 64 + lane] = v;
-        }
-    }
-    if (kDelta) __syncthreads();
-
-    // T and P as operand fragments of row tile w
 #pragma unroll
     for (int ts = 0; ts < 2; ++ts) {
         if (ts == 1 && w < 2) break;
-        const int tile = tri_tile(w, ts);
         float x[8];
-        if (kDelta) {
-            u32x4 t[3];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = lsh[r][32 * ts + 8 * grp + j];
-            split8(x, t);
-#pragma unroll
-            for (int m = 0; m < 3; ++m) reinterpret_cast<u32x4*>(at.t)[(tile * 3 + m) * 64 + lane] = t[m];
-        }
         u32x4 p[NO];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = psh[r][32 * ts + 8 * grp + j];
+        for (int e = 0; e < 4; ++e) x[e] = pt[2 * ts][e], x[4 + e] = pt[2 * ts + 1][e];
         split8(x, p);
 #pragma unroll
-        for (int m = 0; m < NO; ++m) reinterpret_cast<u32x4*>(at.p)[(tile * NO + m) * 64 + lane] = p[m];
+        for (int m = 0; m < NO; ++m) reinterpret_cast<u32x4*>(at.p)[(tri_tile(w, ts) * NO + m) * 64 + lane] = p[m];
+    }
+    if constexpr (kDelta) {
+        // X = (I + L)^-1 in blocks of 16.  The blocks on the diagonal by substitution, a column a
+        // lane (each of the four lane groups does the same); X_ij = -X_ii sum_k L_ik X_kj below, in
+        // float32, column j's blocks by wavefront j.
+        sync_lds();
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s0 = i == col ? 1.0f : 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; j += 4) {
+                const f32x4 l = *reinterpret_cast<const f32x4*>(&lsh[16 * w + i][16 * w + j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j + e < i) (e % 2 ? s1 : s0) = __builtin_fmaf(-l[e], x[j + e], e % 2 ? s1 : s0);
+            }
+            x[i] = s0 + s1;
+        }
+        f32x4 X[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) X[k] = f32x4{0, 0, 0, 0};
+        f32x4 d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = grp == 0 ? x[e] : grp == 1 ? x[4 + e] : grp == 2 ? x[8 + e] : x[12 + e];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k == w) X[k] = d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lsh[16 * w + 4 * grp + e][16 * w + col] = d[e];
+        sync_lds();
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            if (i <= w) continue;
+            f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < i; ++k) {
+                if (k < w) continue;
+                const f32x4 l = *reinterpret_cast<const f32x4*>(&lsh[16 * i + col][16 * k + 4 * grp]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(-l[e], X[k][e], sum, 0, 0, 0);
+            }
+            const f32x4 inv = *reinterpret_cast<const f32x4*>(&lsh[16 * i + col][16 * i + 4 * grp]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) X[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[e], sum[e], X[i], 0, 0, 0);
+        }
+        sync_lds();
+        const float bj = bsh[16 * w + col];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lsh[16 * i + 4 * grp + e][16 * w + col] = X[i][e] * bj;
+        sync_lds();
+        // T = X diag(b)
+#pragma unroll
+        for (int ts = 0; ts < 2; ++ts) {
+            if (ts == 1 && w < 2) break;
+            u32x4 t[3];
+            float y[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&lsh[r][32 * ts + 16 * h + 4 * grp]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[4 * h + e] = v[e];
+            }
+            split8(y, t);
+#pragma unroll
+            for (int m = 0; m < 3; ++m)
+                reinterpret_cast<u32x4*>(at.t)[(tri_tile(w, ts) * 3 + m) * 64 + lane] = t[m];
+        }
     }
 }
 
 // ---- the state from chunk to chunk --------------------------------------------------
-// 16 value columns of one head of one sequence.  Wavefront w has rows 16 w .. of each
-// chunk, and TPW 16-row tiles of the state in its accumulators; the state, the right
-// side, and U pass between the wavefronts as bf16 terms in LDS, [term][column][row], a
-// row of padding of 16 bytes.
-template <int KS, int NT, bool kDelta, class T>
-__global__ __launch_bounds__(256, 1) void gdn_scan_kernel(gdn_dev_args a, size_t n_chunks, int slices) {
+// NC x 16 value columns of one head of one sequence in nine wavefronts.  The first four carry the
+// state: wavefront w has tokens 16 w .. of each chunk, and TPW tiles of 16 of the state's rows in its
+// accumulators.  The next four follow with the outputs, so that a chunk's chain of dependent steps is
+// K S0, T R, K^T U and three barriers.  The last brings the next chunk's K to LDS and, with inputs that
+// it can copy from as they are (kDirect), V, T and the decays: a load instruction in the chain costs
+// it some 30 cycles.  The state, the right side and U pass between wavefronts as bf16 terms in LDS, lane by
+// lane (see state_row).  Other fragments of the next chunk are loaded into each register as soon as it
+// is free.
+template <int KS, int NT, int NC, bool kDelta, bool kDirect, class T>
+__global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t n_chunks, int slices) {
     constexpr int NO = NT == 1 ? 2 : 3;
     constexpr int TPW = KS >= 2 ? KS / 2 : 1;
-    constexpr int SP = 32 * KS + 8, UP = C + 8;  // pitches, in bf16
-    __shared__ __attribute__((aligned(16))) uint16_t ssh[3][16][SP];
-    __shared__ __attribute__((aligned(16))) uint16_t rsh[kDelta ? 3 : 1][16][UP];
-    __shared__ __attribute__((aligned(16))) uint16_t ush[NO][16][UP];
-    __shared__ __attribute__((aligned(16))) uint16_t dsh[3][16][UP];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    // chunks in LDS: three where they fit (their copies are on the way for a whole chunk), one where two
+    // don't; T always two
+    constexpr int kBufs = kDirect && KS <= 4 ? 3 : KS * NT <= 12 ? 2 : 1;
+    using L = Layout<KS, NT, NO>;
+    using K = KTile<KS, NT>;
+    static_assert(!kDirect || kBufs >= 2, "kDirect copies a chunk ahead");
+    __shared__ __attribute__((aligned(1024))) char ksh[kBufs][K::kBytes];
+    constexpr int kVRow = 32 * NC;  // bytes of a token's V
+    __shared__ __attribute__((aligned(1024))) char vsh[kDirect ? kBufs : 1][kDirect ? C * kVRow : 16];
+    __shared__ __attribute__((aligned(1024))) char tsh[kDirect ? 2 : 1][kDirect && kDelta ? 18 * 1024 : 16];
+    __shared__ __attribute__((aligned(1024))) float gsh[kDirect ? kBufs : 1][kDirect ? 256 : 4];
+    // [columns][pair of tiles][term][lane][tile of the pair]: an operand is one 16-byte read
+    __shared__ u32x4 ssh[NC][KS][3][64];
+    __shared__ u32x4 rsh[kDelta ? NC : 1][kDelta ? 2 : 1][3][64];
+    __shared__ u32x4 ush[NC][2][NO][64];
+    __shared__ u32x4 dsh[NC][2][3][64];
+    __shared__ __attribute__((aligned(16))) T osh[4][16][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3,
+              col = lane & 15, grp = lane >> 4;
     // a head's slices a multiple of the heads apart: with 8 | heads on one XCD, whose
     // L2 then holds the fragments that they share
     const int heads = a.n_seq * a.heads_v;
@@ -308,183 +408,424 @@ __global__ __launch_bounds__(256, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
     if (slot < 0) return;
     int first, len;
     span(a, seq, first, len);
-    const int j = 16 * slice + col;  // value column
-    const bool jin = j < a.dim_v;
-
-    // the state: lane holds rows 16 tile + 4 grp .. + 3 of column j
-    const size_t head_state = ((size_t)slot * a.heads_v + hv) * a.dim_k * a.dim_v;
-    f32x4 S[TPW];
-    size_t s_at[TPW];
-    bool s_in[TPW];
-#pragma unroll
-    for (int t = 0; t < TPW; ++t) {
-        const int i = 16 * (w * TPW + t) + 4 * grp;
-        s_in[t] = jin && i < a.dim_k;
-        s_at[t] = head_state + (((size_t)(j / 4) * (a.dim_k / 4) + i / 4) * 4 + j % 4) * 4;
-        S[t] = f32x4{0, 0, 0, 0};
-        if (s_in[t] && a.state_in) S[t] = *reinterpret_cast<const f32x4*>(a.state_in + s_at[t]);
-    }
-    auto put_state = [&] {
-#pragma unroll
-        for (int t = 0; t < TPW; ++t) {
-            if (w * TPW + t >= 2 * KS) break;
-            u32x2 x[3];
-            split4(S[t], x);
-#pragma unroll
-            for (int m = 0; m < 3; ++m)
-                *reinterpret_cast<u32x2*>(&ssh[m][col][16 * (w * TPW + t) + 4 * grp]) = x[m];
-        }
-    };
-
+    const int j0 = 16 * NC * slice + col;  // first value column
     const int nc = (len + C - 1) / C;
-    const size_t chunk0 = (size_t)(first / C) + seq;
-    u32x4 kf[KS][NT], qf[KS][NT], tf[2][3], ktf[TPW][2][NT], pf[2][NO];
-    float v[4];
-    f32x4 up, down;
-    float last;
-    const T* vbase = static_cast<const T*>(a.v) + (int64_t)hv * a.dim_v + j;
-    auto load_kq = [&](const Places& at) {
+    Places at = L::at(a, n_chunks, (size_t)(first / C) + seq, hk, hv);
+    auto half = [&](u32x4(&x)[64], int tile) -> u32x2& { return reinterpret_cast<u32x2*>(&x[lane])[tile & 1]; };
+
+    using lds_void = __attribute__((address_space(3))) void;
+    using global_void = const __attribute__((address_space(1))) void;
+    if (wave == 8) {
+        // K, V and the decays of chunk c are kRest copies of 1 KiB, T kT
+        constexpr int kK = K::kBytes / 1024, kV = kDirect ? 2 * NC : 0, kRest = kK + (kDirect ? kV + 1 : 0);
+        constexpr int kT = kDirect && kDelta ? 18 : 0;
+        constexpr int kParts = K::kRow / 16, kKRows = 64 / kParts, kVRows = 32 / NC;  // rows that a copy holds
+        constexpr int kMixes = KS == 4 ? 4 : K::kBytes / 1024;  // copies whose rows are mixed differently
+        const uint16_t* kp = static_cast<const uint16_t*>(a.k) + first * a.k_row + (int64_t)hk * (32 * KS);
+        const uint16_t* vp = static_cast<const uint16_t*>(a.v) + first * a.v_row + (int64_t)hv * a.dim_v;
+        const int vcol = min(16 * NC * slice + 8 * (lane % (2 * NC)), a.dim_v - 8);
+        auto kcol = [&](int i) { return ((lane % kParts) ^ K::mix(i * kKRows + lane / kParts)) * 8; };
+        // a lane's offset from a copy's first row, in bytes: the rest of an address is the same for all lanes
+        uint32_t koff[kMixes];
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+        for (int i = 0; i < kMixes; ++i) koff[i] = (uint32_t)(lane / kParts * a.k_row + kcol(i)) * 2;
+        const uint32_t voff = (uint32_t)(lane / (2 * NC) * a.v_row + vcol) * 2;
+        // (where the chunk is not whole, the last token for those past the end: U is zero there)
+        auto copy_as = [&](int c, const Places& p, auto from, auto to, auto whole) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int f = ((w * KS + s) * NT + t) * 64 + lane;
-                if (kDelta) kf[s][t] = reinterpret_cast<const u32x4*>(at.k)[f];
-                qf[s][t] = reinterpret_cast<const u32x4*>(at.q)[f];
+            for (int i = decltype(from)::value; i < decltype(to)::value; ++i) {
+                const char* src;
+                char* dst = ksh[c % kBufs] + i * 1024;
+                if constexpr (kDirect) {
+                    const int v = i - kK;
+                    if (i < kK) {
+                        src = reinterpret_cast<const char*>(kp + (int64_t)(c * C + i * kKRows) * a.k_row) + koff[i % kMixes];
+                        if (!decltype(whole)::value)
+                            src = reinterpret_cast<const char*>(
+                                kp + min(c * C + i * kKRows + lane / kParts, len - 1) * a.k_row + kcol(i));
+                    } else if (i < kK + kV) {
+                        src = reinterpret_cast<const char*>(vp + (int64_t)(c * C + v * kVRows) * a.v_row) + voff;
+                        if (!decltype(whole)::value)
+                            src = reinterpret_cast<const char*>(
+                                vp + min(c * C + v * kVRows + lane / (2 * NC), len - 1) * a.v_row + vcol);
+                        dst = vsh[c % kBufs] + v * 1024;
+                    } else {
+                        src = reinterpret_cast<const char*>(p.up) + (uint32_t)lane * 16;
+                        dst = reinterpret_cast<char*>(gsh[c % kBufs]);
+                    }
+                } else {
+                    src = p.k + i * 1024 + (uint32_t)lane * 16;
+                }
+                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)dst, 16, 0, 0);
             }
-    };
-    auto load_vt = [&](const Places& at, int c) {
+        };
+        auto copy = [&](int c, const Places& p, auto from, auto to) {
+            if (c * C + C <= len || !kDirect)
+                copy_as(c, p, from, to, std::true_type());
+            else
+                copy_as(c, p, from, to, std::false_type());
+        };
+        auto copy_t = [&](int c, const Places& p) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int t = c * C + 16 * w + 4 * grp + e;
-            v[e] = t < len && jin ? to_float<T>(vbase[(int64_t)(first + t) * a.v_row]) : 0.0f;
+            for (int i = 0; i < kT; ++i)
+                __builtin_amdgcn_global_load_lds((global_void*)(p.t + i * 1024 + lane * 16),
+                                                 (lds_void*)(tsh[c % 2] + i * 1024), 16, 0, 0);
+        };
+        using Zero = std::integral_constant<int, 0>;
+        using Half = std::integral_constant<int, kBufs == 3 && kDelta ? kRest / 6 : 0>;
+        using All = std::integral_constant<int, kRest>;
+        static_assert(kBufs < 3 || kRest < 64, "vmcnt has six bits");
+        Places at2 = at;  // one chunk behind `at`
+        if (nc > 0) {
+            copy_t(0, at);
+            copy(0, at, Zero(), All());
+            L::next(a, at);
+            if (kBufs == 3 && nc > 1) copy(1, at, Zero(), All());
+            if (kBufs == 3) L::next(a, at);
+            L::next(a, at2);
         }
-        up = *reinterpret_cast<const f32x4*>(at.up + 16 * w + 4 * grp);
-        if (kDelta)
+        for (int c = 0; c < nc; ++c) {
+            // chunk c has to be there, T of it too; of the next one, copied while c - 1 was worked on, not all
+            if (kBufs == 3 && c + 1 < nc)
+                __builtin_amdgcn_s_waitcnt(0x0F70 | (kRest & 15) | (kRest >> 4) << 14);  // vmcnt(kRest)
+            else
+                __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+            sync_lds();
+            // spread over the chunk, as Q and P are: a load takes the compute unit some 40 cycles, and a
+            // wavefront that waits to issue one is late at the barrier
+            const bool more = kBufs >= 2 && c + kBufs - 1 < nc;
+            if (c + 1 < nc) copy_t(c + 1, at2);
+            if (kBufs == 2 && more) copy(c + 1, at, Zero(), All());
+            if (kDelta) {
+                sync_lds();
+                if (kBufs == 3 && more) copy(c + 2, at, Zero(), Half());
+            }
+            sync_lds();
+            if (kBufs == 3 && more) copy(c + 2, at, Half(), All());
+            if (kBufs == 1) {
+                sync_lds();
+                if (c + 1 < nc) copy(c + 1, at, Zero(), All());
+            }
+            L::next(a, at);
+            L::next(a, at2);
+        }
+        return;
+    }
+
+    if (wave >= 4) {
+        // O = scale (2^g Q S0 + P U), Q and P loaded two chunks ahead (float32: one, for the registers):
+        // nobody is to wait for these wavefronts at a barrier
+        constexpr int kSets = NT == 1 ? 2 : 1;
+        struct Ahead {
+            u32x4 q[KS][NT], p[2][NO];
+            f32x4 up;
+        } set[kSets];
+        const uint16_t* qp = nullptr;
+        int loaded = 0;
+        auto load_q = [&](Ahead& x) {
+            const int c = min(loaded, nc - 1);  // behind the last chunk its own again
+            if constexpr (kDirect) {
+                if (loaded == 0 || loaded >= nc - 1)
+                    qp = static_cast<const uint16_t*>(a.q) + (first + min(c * C + 16 * w + col, len - 1)) * a.q_row +
+                         (int64_t)hk * (32 * KS) + 8 * grp;
+                else
+                    qp += C * a.q_row;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) x.q[s][0] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
+            } else {
+                const u32x4* p = reinterpret_cast<const u32x4*>(at.q) + w * KS * NT * 64 + lane;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) x.q[s][t] = p[(s * NT + t) * 64];
+            }
+        };
+        auto load_p = [&](Ahead& x) {
+            const u32x4* p = reinterpret_cast<const u32x4*>(at.p) + tri_tile(w, 0) * NO * 64 + lane;
+#pragma unroll
+            for (int m = 0; m < NO; ++m) x.p[0][m] = p[m * 64];
+            if (w >= 2)
+#pragma unroll
+                for (int m = 0; m < NO; ++m) x.p[1][m] = p[(NO + m) * 64];
+            if (!kDirect) x.up = *reinterpret_cast<const f32x4*>(at.up + 16 * w + 4 * grp);
+            if (++loaded < nc) L::next(a, at);
+        };
+#pragma unroll
+        for (int h = 0; h < kSets; ++h) {
+#pragma unroll
+            for (int m = 0; m < NO; ++m) set[h].p[1][m] = u32x4{0, 0, 0, 0};
+            if (nc > 0) {
+                load_q(set[h]);
+                load_p(set[h]);
+            }
+        }
+        // a lane's part of a tile of 16 tokens x 16 columns as it is stored: EL elements of a token's row
+        constexpr int EL = 16 / (int)sizeof(T) / (NT == 1 ? 2 : 1), kLanes = 16 / EL;
+        static_assert(64 / kLanes == 16, "a tile is one store of a wavefront");
+        const int token = 16 * w + lane / kLanes, part = lane % kLanes * EL;
+        T* out = static_cast<T*>(a.out) + (first + token) * a.out_row + (int64_t)hv * a.dim_v + 16 * NC * slice + part;
+        const bool wide = ((uintptr_t)a.out | (uintptr_t)(a.out_row * sizeof(T)) | (uintptr_t)(a.dim_v * sizeof(T))) %
+                              (EL * sizeof(T)) == 0;
+        auto chunk = [&](int c, Ahead& x, Ahead& other) {
+            sync_lds();
+            if (kSets == 2 && c > 0) load_p(other);
+            f32x4 o[NC];
+#pragma unroll
+            for (int y = 0; y < NC; ++y) o[y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int y = 0; y < NC; ++y) {
+                    u32x4 b[NO];
+#pragma unroll
+                    for (int m = 0; m < NO; ++m) b[m] = ssh[y][s][m][lane];
+                    o[y] = mfma_terms<NT, NO, NO>(x.q[s], b, o[y]);
+                }
+            const f32x4 up = kDirect ? *reinterpret_cast<const f32x4*>(&gsh[c % kBufs][kDirect ? 16 * w + 4 * grp : 0]) : x.up;
+#pragma unroll
+            for (int y = 0; y < NC; ++y) o[y] *= up;
+            if (kDelta) sync_lds();
+            load_q(x);
+            sync_lds();
 #pragma unroll
             for (int ts = 0; ts < 2; ++ts)
-                if (ts == 0 || w >= 2)
 #pragma unroll
-                    for (int m = 0; m < 3; ++m)
-                        tf[ts][m] = reinterpret_cast<const u32x4*>(at.t)[(tri_tile(w, ts) * 3 + m) * 64 + lane];
+                for (int y = 0; y < NC; ++y) {
+                    u32x4 b[NO];
+#pragma unroll
+                    for (int m = 0; m < NO; ++m) b[m] = ush[y][ts][m][lane];
+                    o[y] = mfma_terms<NO, NO, NO>(x.p[ts], b, o[y]);
+                }
+            if (kSets == 1) load_p(x);
+#pragma unroll
+            for (int y = 0; y < NC; ++y) {
+                // the tile row by row (nobody else's part of LDS, and in order within a wavefront)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) osh[w][4 * grp + e][col] = from_float<T>(a.scale * o[y][e]);
+                struct alignas(EL * sizeof(T)) Part {
+                    T x[EL];
+                };
+                asm volatile("" ::: "memory");
+                const Part v = *reinterpret_cast<const Part*>(&osh[w][lane / kLanes][part]);
+                asm volatile("" ::: "memory");
+                T* to = out + 16 * y;
+                const int left = a.dim_v - (16 * NC * slice + 16 * y + part);
+                if (c * C + token < len) {
+                    if (wide && left >= EL) {
+                        *reinterpret_cast<Part*>(to) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < EL; ++e)
+                            if (e < left) to[e] = v.x[e];
+                    }
+                }
+            }
+            out += C * a.out_row;
+            if (kBufs == 1) sync_lds();
+        };
+        for (int c = 0; c < nc; c += kSets) {
+            chunk(c, set[0], set[kSets - 1]);
+            if (kSets == 2 && c + 1 < nc) chunk(c + 1, set[kSets - 1], set[0]);
+        }
+        return;
+    }
+
+    // the state: lane holds rows state_row(tile, grp) .. + 3 of column j0 + 16 x
+    const size_t head_state = ((size_t)slot * a.heads_v + hv) * a.dim_k * a.dim_v;
+    f32x4 S[NC][TPW];
+    auto each_state = [&](auto&& f) {
+#pragma unroll
+        for (int x = 0; x < NC; ++x)
+#pragma unroll
+            for (int t = 0; t < TPW; ++t) {
+                const int i = state_row(w * TPW + t, grp), j = j0 + 16 * x;
+                if (j < a.dim_v && i < a.dim_k && w * TPW + t < 2 * KS)
+                    f(S[x][t], head_state + (((size_t)(j / 4) * (a.dim_k / 4) + i / 4) * 4 + j % 4) * 4);
+            }
     };
-    auto load_down = [&](const Places& at) {
+#pragma unroll
+    for (int x = 0; x < NC; ++x)
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) S[x][t] = f32x4{0, 0, 0, 0};
+    if (a.state_in)
+        each_state([&](f32x4& s, size_t i) { s = *reinterpret_cast<const f32x4*>(a.state_in + i); });
+    u32x4 tf[2][3];
+    const T* vp[NC][4];
+    T v[NC][4];
+    f32x4 up, down;
+    float last;
+    const T* vbase = static_cast<const T*>(a.v) + first * a.v_row + (int64_t)hv * a.dim_v;
+    auto load_t = [&] {
+        if (!kDelta || kDirect) return;
+        const u32x4* p = reinterpret_cast<const u32x4*>(at.t) + tri_tile(w, 0) * 3 * 64 + lane;
+#pragma unroll
+        for (int m = 0; m < 3; ++m) tf[0][m] = p[m * 64];
+        if (w >= 2)
+#pragma unroll
+            for (int m = 0; m < 3; ++m) tf[1][m] = p[(3 + m) * 64];
+    };
+    auto load_v = [&](int c) {
+        if (kDirect) return;
+#pragma unroll
+        for (int x = 0; x < NC; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (c == 0 || c == nc - 1)
+                    vp[x][e] = vbase + min(c * C + 16 * w + 4 * grp + e, len - 1) * a.v_row +
+                               min(j0 + 16 * x, a.dim_v - 1);
+                else
+                    vp[x][e] += C * a.v_row;
+                v[x][e] = *vp[x][e];
+            }
+        if (kDelta) up = *reinterpret_cast<const f32x4*>(at.up + 16 * w + 4 * grp);
+    };
+    auto load_down = [&] {
+        if (kDirect) return;
         down = *reinterpret_cast<const f32x4*>(at.down + 16 * w + 4 * grp);
-    };
-    auto load_kt = [&](const Places& at) {
         last = at.last[0];
-#pragma unroll
-        for (int t = 0; t < TPW; ++t)
-            if (w * TPW + t < 2 * KS)
-#pragma unroll
-                for (int ts = 0; ts < 2; ++ts)
-#pragma unroll
-                    for (int m = 0; m < NT; ++m)
-                        ktf[t][ts][m] =
-                            reinterpret_cast<const u32x4*>(at.kt)[(((w * TPW + t) * 2 + ts) * NT + m) * 64 + lane];
     };
-    auto load_p = [&](const Places& at) {
+    auto put_state = [&] {
 #pragma unroll
-        for (int ts = 0; ts < 2; ++ts)
-            if (ts == 0 || w >= 2)
+        for (int x = 0; x < NC; ++x)
 #pragma unroll
-                for (int m = 0; m < NO; ++m)
-                    pf[ts][m] = reinterpret_cast<const u32x4*>(at.p)[(tri_tile(w, ts) * NO + m) * 64 + lane];
+            for (int t = 0; t < TPW; ++t)
+                if (w * TPW + t < 2 * KS) {
+                    u32x2 y[3];
+                    split4(S[x][t], y);
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) half(ssh[x][(w * TPW + t) / 2][m], w * TPW + t) = y[m];
+                }
     };
+#pragma unroll
+    for (int m = 0; m < 3; ++m) tf[1][m] = u32x4{0, 0, 0, 0};
     if (nc > 0) {
-        const Places at = places<KS, NT, NO>(a, n_chunks, chunk0, hk, hv);
-        load_kq(at);
-        load_vt(at, 0);
-        load_down(at);
-        load_kt(at);
-        load_p(at);
+        load_v(0);
+        load_t();
+        load_down();
     }
     put_state();
     for (int c = 0; c < nc; ++c) {
-        // the next chunk's fragments are loaded into each register as soon as it is free
-        const bool more = c + 1 < nc;
-        const Places next = places<KS, NT, NO>(a, n_chunks, chunk0 + c + 1, hk, hv);
-        __syncthreads();
-        // K S0 and Q S0
-        f32x4 ks = {0, 0, 0, 0}, o = {0, 0, 0, 0};
+        const int nx = min(c + 1, nc - 1);
+        if (c + 1 < nc) L::next(a, at);
+        const char* kt = ksh[c % kBufs];
+        sync_lds();
+        if constexpr (kDirect) {
+            const float* g = &gsh[c % kBufs][16 * w + 4 * grp];
+            up = *reinterpret_cast<const f32x4*>(g);
+            down = *reinterpret_cast<const f32x4*>(g + C);
+            last = gsh[c % kBufs][2 * C];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            u32x4 b[3], bo[NO];
+            for (int x = 0; x < NC; ++x)
 #pragma unroll
-            for (int m = 0; m < 3; ++m) b[m] = *reinterpret_cast<const u32x4*>(&ssh[m][col][32 * s + 8 * grp]);
-#pragma unroll
-            for (int m = 0; m < NO; ++m) bo[m] = b[m];
-            if (kDelta) ks = mfma_terms<NT, 3, 3>(kf[s], b, ks);
-            o = mfma_terms<NT, NO, NO>(qf[s], bo, o);
+                for (int e = 0; e < 4; ++e)
+                    v[x][e] = *reinterpret_cast<const T*>(vsh[c % kBufs] + (16 * w + 4 * grp + e) * kVRow + (16 * x + col) * 2);
         }
-        if (more) load_kq(next);
-        o *= up;
-        f32x4 u = {v[0], v[1], v[2], v[3]};
-        if (kDelta) {
-            u -= up * ks;
-            u32x2 x[3];
-            split4(u, x);
+        f32x4 u[NC];
+        if constexpr (kDelta) {
+            // R = V - 2^g K S0
+            f32x4 ks[NC][2];
 #pragma unroll
-            for (int m = 0; m < 3; ++m) *reinterpret_cast<u32x2*>(&rsh[m][col][16 * w + 4 * grp]) = x[m];
-            __syncthreads();
-            u = f32x4{0, 0, 0, 0};
+            for (int x = 0; x < NC; ++x) ks[x][0] = ks[x][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int ts = 0; ts < 2; ++ts)
-                if (ts == 0 || w >= 2) {
+            for (int s = 0; s < KS; ++s) {
+                u32x4 kf[NT];
+                K::rows(kt, w, s, lane, kf);
+#pragma unroll
+                for (int x = 0; x < NC; ++x) {
                     u32x4 b[3];
 #pragma unroll
-                    for (int m = 0; m < 3; ++m)
-                        b[m] = *reinterpret_cast<const u32x4*>(&rsh[m][col][32 * ts + 8 * grp]);
-                    u = mfma_terms<3, 3, 3>(tf[ts], b, u);
+                    for (int m = 0; m < 3; ++m) b[m] = ssh[x][s][m][lane];
+                    ks[x][s % 2] = mfma_terms<NT, 3, 3>(kf, b, ks[x][s % 2]);
                 }
+            }
+#pragma unroll
+            for (int x = 0; x < NC; ++x) {
+                f32x4 rhs;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    rhs[e] = __builtin_fmaf(-up[e], ks[x][0][e] + ks[x][1][e], to_float<T>(v[x][e]));
+                u32x2 y[3];
+                split4(rhs, y);
+#pragma unroll
+                for (int m = 0; m < 3; ++m) half(rsh[x][w / 2][m], w) = y[m];
+            }
+            load_v(nx);
+            sync_lds();
+            f32x4 u2[NC][2];
+            u32x4 b[NC][2][3];
+#pragma unroll
+            for (int x = 0; x < NC; ++x)
+#pragma unroll
+                for (int ts = 0; ts < 2; ++ts) {
+                    u2[x][ts] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) b[x][ts][m] = rsh[x][ts][m][lane];
+                }
+            if constexpr (kDirect) {
+                const u32x4* p = reinterpret_cast<const u32x4*>(tsh[c % 2]) + tri_tile(w, 0) * 3 * 64 + lane;
+#pragma unroll
+                for (int m = 0; m < 3; ++m) tf[0][m] = p[m * 64];
+                if (w >= 2)
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) tf[1][m] = p[(3 + m) * 64];
+            }
+#pragma unroll
+            for (int z = 2; z >= 0; --z)  // the pairs of terms, the chains side by side
+#pragma unroll
+                for (int y = 0; y <= z; ++y)
+#pragma unroll
+                    for (int ts = 0; ts < 2; ++ts)
+#pragma unroll
+                        for (int x = 0; x < NC; ++x) u2[x][ts] = mfma(tf[ts][y], b[x][ts][z - y], u2[x][ts]);
+            load_t();
+#pragma unroll
+            for (int x = 0; x < NC; ++x) u[x] = u2[x][0] + u2[x][1];
+        } else {
+#pragma unroll
+            for (int x = 0; x < NC; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    u[x][e] = c * C + 16 * w + 4 * grp + e < len ? to_float<T>(v[x][e]) : 0.0f;
+            load_v(nx);
         }
-        if (more) load_vt(next, c + 1);
-        {
-            u32x2 x[NO], d[3];
-            split4(u, x);
-            split4(u * down, d);
+        const float keep = last;
 #pragma unroll
-            for (int m = 0; m < NO; ++m) *reinterpret_cast<u32x2*>(&ush[m][col][16 * w + 4 * grp]) = x[m];
+        for (int x = 0; x < NC; ++x) {
+            u32x2 y[NO], d[3];
+            split4(u[x] * down, d);
 #pragma unroll
-            for (int m = 0; m < 3; ++m) *reinterpret_cast<u32x2*>(&dsh[m][col][16 * w + 4 * grp]) = d[m];
+            for (int m = 0; m < 3; ++m) half(dsh[x][w / 2][m], w) = d[m];
+            split4(u[x], y);
+#pragma unroll
+            for (int m = 0; m < NO; ++m) half(ush[x][w / 2][m], w) = y[m];
         }
-        if (more) load_down(next);
-        __syncthreads();
-        // S0 <- last S0 + K^T (down U)
+        load_down();
+        sync_lds();
+        // S0 <- 2^(g_C) S0 + K^T (2^(g_C - g) U)
 #pragma unroll
-        for (int t = 0; t < TPW; ++t) S[t] *= last;
+        for (int x = 0; x < NC; ++x)
+#pragma unroll
+            for (int t = 0; t < TPW; ++t) S[x][t] *= keep;
 #pragma unroll
         for (int ts = 0; ts < 2; ++ts) {
-            u32x4 b[3];
+            u32x4 b[NC][3];
 #pragma unroll
-            for (int m = 0; m < 3; ++m) b[m] = *reinterpret_cast<const u32x4*>(&dsh[m][col][32 * ts + 8 * grp]);
+            for (int x = 0; x < NC; ++x)
+#pragma unroll
+                for (int m = 0; m < 3; ++m) b[x][m] = dsh[x][ts][m][lane];
 #pragma unroll
             for (int t = 0; t < TPW; ++t)
-                if (w * TPW + t < 2 * KS) S[t] = mfma_terms<NT, 3, 3>(ktf[t][ts], b, S[t]);
+                if (w * TPW + t < 2 * KS) {
+                    u32x4 kf[NT];
+                    K::columns(kt, w * TPW + t, ts, lane, kf);
+#pragma unroll
+                    for (int x = 0; x < NC; ++x) S[x][t] = mfma_terms<NT, 3, 3>(kf, b[x], S[x][t]);
+                }
         }
-        if (more) load_kt(next);
         put_state();
-        // O = scale (up Q S0 + P U)
-#pragma unroll
-        for (int ts = 0; ts < 2; ++ts)
-            if (ts == 0 || w >= 2) {
-                u32x4 b[NO];
-#pragma unroll
-                for (int m = 0; m < NO; ++m) b[m] = *reinterpret_cast<const u32x4*>(&ush[m][col][32 * ts + 8 * grp]);
-                o = mfma_terms<NO, NO, NO>(pf[ts], b, o);
-            }
-        if (more) load_p(next);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int t = c * C + 16 * w + 4 * grp + e;
-            if (t < len && jin)
-                static_cast<T*>(a.out)[(int64_t)(first + t) * a.out_row + (int64_t)hv * a.dim_v + j] =
-                    from_float<T>(a.scale * o[e]);
-        }
+        if (kBufs == 1) sync_lds();
     }
-#pragma unroll
-    for (int t = 0; t < TPW; ++t)
-        if (s_in[t]) *reinterpret_cast<f32x4*>(a.state_out + s_at[t]) = S[t];
+    each_state([&](const f32x4& s, size_t i) { *reinterpret_cast<f32x4*>(a.state_out + i) = s; });
 }
 
 // ---- one token ------------------------------------------------------------------------
@@ -585,12 +926,31 @@ bool rows_of_16(const void* p, int64_t row, int dim, int es) {
 template <int KS, int NT, bool kDelta>
 hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
     using T = std::conditional_t<NT == 1, uint16_t, float>;
-    const int es = NT == 1 ? 2 : 4, slices = (a.dim_v + 15) / 16;
+    const int es = NT == 1 ? 2 : 4;
+    const bool full_q = a.dim_k == 32 * KS && rows_of_16(a.q, a.q_row, a.dim_k, es);
+    const bool full_k = a.dim_k == 32 * KS && rows_of_16(a.k, a.k_row, a.dim_k, es);
+    const bool direct = NT == 1 && full_q && full_k && rows_of_16(a.v, a.v_row, a.dim_v, es) &&
+                        a.k_row < 1 << 24 && a.v_row < 1 << 24;  // (offsets of 64 rows in 32 bits)
     if (a.rows > 0)
-        gdn_chunk_kernel<KS, NT, kDelta><<<dim3((unsigned)(w.n_chunks * a.heads_v)), 256, 0, s>>>(
-            a, w.n_chunks, rows_of_16(a.q, a.q_row, a.dim_k, es), rows_of_16(a.k, a.k_row, a.dim_k, es));
-    gdn_scan_kernel<KS, NT, kDelta, T>
-        <<<dim3((unsigned)((size_t)a.n_seq * a.heads_v * slices)), 256, 0, s>>>(a, w.n_chunks, slices);
+        gdn_chunk_kernel<KS, NT, kDelta>
+            <<<dim3((unsigned)(w.n_chunks * a.heads_v)), 256, 0, s>>>(a, w.n_chunks, full_q, full_k, direct);
+    auto scan = [&](auto nc, auto from_inputs) {
+        constexpr int NC = decltype(nc)::value;
+        const int slices = (a.dim_v + 16 * NC - 1) / (16 * NC);
+        gdn_scan_kernel<KS, NT, NC, kDelta, decltype(from_inputs)::value, T>
+            <<<dim3((unsigned)((size_t)a.n_seq * a.heads_v * slices)), 576, 0, s>>>(a, w.n_chunks, slices);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, KS <= 4 ? 2 : 1>;
+    using Direct = std::integral_constant<bool, NT == 1>;
+    // 16 columns a workgroup while the workgroups have a compute unit each (they hold most of its LDS):
+    // the shortest chain; else 32, which load K, T and P half as often.  Sequences of 1024 tokens, 16 heads
+    // of 128, bf16 with the delta rule, 16 | 32 columns: 2 sequences 44 | 56 us, 3 72 | 59, 16 486 | 284.
+    const bool two = (size_t)a.n_seq * a.heads_v * ((a.dim_v + 15) / 16) > 256;
+    if (direct)
+        two ? scan(Two(), Direct()) : scan(One(), Direct());
+    else
+        two ? scan(Two(), std::false_type()) : scan(One(), std::false_type());
     return hipGetLastError();
 }
 
