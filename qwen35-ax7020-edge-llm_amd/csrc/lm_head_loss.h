@@ -10,6 +10,7 @@
 #include "qwen_kernels.h"
 
 constexpr int LHL_TILE = 128;   // vocabulary rows of a tile of logits
+constexpr int LHL_WIDE = 256;   // of a large tile; pieces of the vocabulary are multiples of it
 constexpr int LHL_STEP = 64;    // terms of a sum that a tile takes in one step
 
 // The caller's work buffer: byte offsets of its parts.
@@ -55,7 +56,7 @@ inline LossWork loss_work(const lm_head_loss_args& a, bool grad, bool grad_h) {
     } else {
         // pieces whose gradients stay under 128 MiB: they and their part of the table fit the 256 MiB
         // last-level cache that they are read from again
-        const size_t whole = (size_t)w.vtiles * LHL_TILE;
+        const size_t whole = ((size_t)a.vocab + LHL_WIDE - 1) / LHL_WIDE * LHL_WIDE;
         const size_t fit = ((size_t)128 << 20) / (2 * std::max<size_t>(n, 1) * w.terms) / 1024 * 1024;
         w.piece = (int)std::min(whole, std::max<size_t>(fit, 1024));
         w.d_at = put(2 * n * w.terms * w.piece);

@@ -21,7 +21,10 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 
-constexpr float kLog2e = 1.4426950408889634f;
+// Exponentials in base 2: exp z = 2^(z log2 e), the product and the difference to a tile's maximum in
+// one rounding; the maximum is kept in base 2 too, so that its own rounding cancels.
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: 0
 
 // ---- tiles ----------------------------------------------------------------------------
 // An operand in memory: rows x cols bf16 values, `term` elements from one term to the
@@ -45,7 +48,8 @@ struct Loader {
     static constexpr int I = N * B / 8 / WAVES;
     static_assert(N * B % (8 * WAVES) == 0, "every wavefront copies the same share");
     static constexpr int kBytes = N * B * 128;
-    const char* at[I];
+    const char* base[I];  // the same for all lanes, moved on step by step
+    uint32_t off[I];      // a lane's own part of an address
     int kc, k_end;        // first element along the sum of this lane's part of a step; the sum's end
     int col_left[I];      // VEC false, TR: columns from the part's first on
     int64_t step;         // bytes from one step to the next
@@ -61,47 +65,53 @@ struct Loader {
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const int q = wave * I + i, term = q / (B / 8);
-            int64_t e;
+            base[i] = reinterpret_cast<const char*>(op.p + term * op.term + (TR ? k0 * op.pitch : m0 * op.pitch + k0));
             if constexpr (TR) {
                 const int k = k_row(q, lane), pos = lane % (B / 8);
                 int col = m0 + 16 * ((pos >> 1) ^ swizzle(k)) + 8 * (pos & 1);
                 if (VEC) col = min(col, op.cols - 8);  // past the last column: values that nothing reads
                 col_left[i] = op.cols - col;
-                e = (k0 + k) * op.pitch + col;
+                off[i] = (uint32_t)(k * op.pitch + col) * 2;
             } else {
-                const int row = min(m0 + 8 * (q % (B / 8)) + lane / 8, op.rows - 1);  // as above
-                e = row * op.pitch + k0 + kc;
+                const int row = min(8 * (q % (B / 8)) + lane / 8, op.rows - 1 - m0);  // as above
+                off[i] = (uint32_t)(row * op.pitch + kc) * 2;
             }
-            at[i] = reinterpret_cast<const char*>(op.p + term * op.term + e);
         }
     }
 
     // Starts the copy of the step whose sum begins at k (from 0) and moves on.
     __device__ void issue(char* lds, int k, const char* zeros, int wave, int lane) {
-        const bool tail = k + LHL_STEP > k_end;
+        if (!VEC) {
 #pragma unroll
-        for (int i = 0; i < I; ++i) {
-            const int q = wave * I + i;
-            const int mine = k + (TR ? k_row(q, lane) : kc);
-            if constexpr (VEC) {
-                const char* src = at[i];
-                if (tail && mine >= k_end) src = zeros;
-                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + q * 1024), 16, 0, 0);
-            } else {
+            for (int i = 0; i < I; ++i) {
+                const int q = wave * I + i, mine = k + (TR ? k_row(q, lane) : kc);
                 const int n = TR ? (mine < k_end ? col_left[i] : 0) : k_end - mine;
                 u32x4 v = {0, 0, 0, 0};
                 if (n >= 8) {
-                    __builtin_memcpy(&v, at[i], 16);
+                    __builtin_memcpy(&v, base[i] + off[i], 16);
                 } else {
-                    const uint16_t* p = reinterpret_cast<const uint16_t*>(at[i]);
+                    const uint16_t* p = reinterpret_cast<const uint16_t*>(base[i] + off[i]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (j < n) v[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
                 }
                 *reinterpret_cast<u32x4*>(lds + q * 1024 + lane * 16) = v;
             }
-            at[i] += step;
+        } else if (k + LHL_STEP <= k_end) {
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+                __builtin_amdgcn_global_load_lds((global_void*)(base[i] + off[i]),
+                                                 (lds_void*)(lds + (wave * I + i) * 1024), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int q = wave * I + i;
+                const char* src = k + (TR ? k_row(q, lane) : kc) < k_end ? base[i] + off[i] : zeros;
+                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + q * 1024), 16, 0, 0);
+            }
         }
+#pragma unroll
+        for (int i = 0; i < I; ++i) base[i] += step;
     }
 };
 
@@ -141,8 +151,9 @@ struct Reader {
 
 // BM x BN of a product by WM x WN wavefronts: acc[i][j] holds rows 16 i + 4 (lane / 16) .. + 3
 // and column 16 j + lane % 16 of the wavefront's part.  NA, NB: the operands' terms, the pairs
-// with ta + tb < MOST taken.  Two or more steps' tiles in LDS: while one is multiplied the next
-// are on their way; one barrier a step.
+// with ta + tb < MOST taken.  STAGES steps' tiles in LDS, copied that far ahead.  A step is two halves: the
+// second half's operands are read before the first is multiplied, and the next step's first half's before
+// the second, with the step's one barrier between, so that the matrix cores work through both waits.
 template <int BM_, int BN_, int WM_, int WN_, bool TRA, bool TRB, int NA, int NB, int MOST, bool VEC, int STAGES>
 struct Product {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
@@ -153,22 +164,21 @@ struct Product {
     static constexpr int kStage = LA::kBytes + LB::kBytes;
     static constexpr int kLds = STAGES * kStage;
 
-    static __device__ void wait(bool all) {
-        constexpr int kLeft = VEC ? (STAGES - 2) * (LA::I + LB::I) : 0;
+    // This wavefront's share of the oldest step is in LDS, but for kSteps newer ones; its own reads are done.
+    template <int kSteps>
+    static __device__ void wait() {
+        constexpr int kLeft = VEC ? kSteps * (LA::I + LB::I) : 0;
         static_assert(kLeft < 64, "vmcnt has six bits");
-        // vmcnt(0 or kLeft) lgkmcnt(0): this wavefront's share of the step is in LDS, and its reads
-        // of the step before are done
-        if (all || kLeft == 0)
-            __builtin_amdgcn_s_waitcnt(0x0070);
-        else
-            __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | (kLeft >> 4) << 14);
+        __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | (kLeft >> 4) << 14);  // vmcnt(kLeft) lgkmcnt(0)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
 
+    // STAGES 1: sums of one step only.
     static __device__ void run(const Operand& a, const Operand& b, int m0, int n0, int k0, int steps, const char* zeros,
                                char* lds, f32x4 (&acc)[MT][NT]) {
+        if (steps <= 0) return;
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         LA la;
         LB lb;
@@ -183,25 +193,45 @@ struct Product {
             la.issue(p, k0 + s * LHL_STEP, zeros, wave, lane);
             lb.issue(p + LA::kBytes, k0 + s * LHL_STEP, zeros, wave, lane);
         };
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s)
-            if (s < steps) issue(s);
-        for (int s = 0; s < steps; ++s) {
-            wait(s + STAGES - 2 >= steps);
-            if (s + STAGES - 1 < steps) issue(s + STAGES - 1);
+        struct Half {
+            u32x4 a[MT][NA], b[NT][NB];
+        } x, y;
+        auto read = [&](int s, int h, Half& f) {
             const char* p = lds + s % STAGES * kStage;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4 fa[MT][NA], fb[NT][NB];
+            for (int j = 0; j < NT; ++j) rb.read(p + LA::kBytes, j, h, f.b[j]);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) ra.read(p, i, h, fa[i]);
+            for (int i = 0; i < MT; ++i) ra.read(p, i, h, f.a[i]);
+            __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead of the products
+        };
+        auto multiply = [&](const Half& f) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) rb.read(p + LA::kBytes, j, h, fb[j]);
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int j = 0; j < NT; ++j) acc[i][j] = mfma_terms<NA, NB, MOST>(f.a[i], f.b[j], acc[i][j]);
+        };
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma_terms<NA, NB, MOST>(fa[i], fb[j], acc[i][j]);
+        for (int s = 0; s < STAGES; ++s)
+            if (s < steps) issue(s);
+        if (steps >= STAGES)
+            wait<STAGES - 1>();
+        else
+            wait<0>();
+        read(0, 0, x);
+        for (int s = 0; s < steps; ++s) {
+            read(s, 1, y);
+            multiply(x);
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 < steps) {
+                if (s + STAGES <= steps)  // the steps behind s + 1 are all on their way
+                    wait<STAGES >= 2 ? STAGES - 2 : 0>();
+                else
+                    wait<0>();
+                if (s + STAGES < steps) issue(s + STAGES);
+                read(s + 1, 0, x);
             }
+            multiply(y);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -238,56 +268,59 @@ struct Parts {
 };
 
 // ---- the rows that count ---------------------------------------------------------------
-// 64 rows to a workgroup, which counts the rows before its own by itself: four bytes a row,
-// next to the 2 KiB and more of a row's state.
+// 16 rows, a part of their columns to a workgroup, which counts the rows before its own by itself:
+// four bytes a row, next to the 2 KiB and more of a row's state.
+constexpr int kPrepRows = 16;
 template <int NT>
 __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, bool grad) {
-    __shared__ int before_sh[4], local[64], kept_sh;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * 64;
+    __shared__ int before_sh[4], local[kPrepRows], kept_sh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * kPrepRows;
     auto counts = [&](int r) {
         const int t = a.targets[r];
         return t >= 0 && t < a.vocab;
     };
     int before = 0;
+#pragma unroll 8
     for (int r = threadIdx.x; r < r0; r += 256) before += counts(r);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
     if (lane == 0) before_sh[wave] = before;
-    if (blockIdx.x == 0 && threadIdx.x < 64) reinterpret_cast<uint32_t*>(p.work + 256)[threadIdx.x] = 0;
+    const bool first = blockIdx.y == 0;
+    if (first && blockIdx.x == 0 && threadIdx.x < 64) reinterpret_cast<uint32_t*>(p.work + 256)[threadIdx.x] = 0;
     __syncthreads();
     before = before_sh[0] + before_sh[1] + before_sh[2] + before_sh[3];
     if (wave == 0) {
         const int r = r0 + lane;
-        const bool in = r < a.rows, kept = in && counts(r);
+        const bool in = lane < kPrepRows && r < a.rows, kept = in && counts(r);
         const uint64_t all = __ballot(kept);
         const int mine = __popcll(all & ((1ull << lane) - 1)), c = before + mine;
-        if (kept) {
-            local[mine] = r;
+        if (kept) local[mine] = r;
+        if (first && kept) {
             p.at<int>(p.w.rows_at)[c] = r;
             p.at<int>(p.w.target_at)[c] = a.targets[r];
             if (grad) {
                 p.at<float>(p.w.lse_at)[c] = a.lse[r];
                 p.at<float>(p.w.gl_at)[c] = a.grad_loss[r];
             }
-        } else if (in && !grad) {
+        } else if (first && in && !grad) {
             const float x = a.targets[r] < 0 ? 0.0f : __builtin_nanf("");
             if (a.loss) a.loss[r] = x;
             if (a.lse) a.lse[r] = x;
         }
-        if (in) p.at<int>(p.w.place_at)[r] = kept ? c : a.targets[r] < 0 ? -1 : -2;
+        if (first && in) p.at<int>(p.w.place_at)[r] = kept ? c : a.targets[r] < 0 ? -1 : -2;
         if (lane == 0) {
             kept_sh = __popcll(all);
-            if (r0 + 64 >= a.rows) *reinterpret_cast<int*>(p.work) = before + __popcll(all);
+            if (first && r0 + kPrepRows >= a.rows) *reinterpret_cast<int*>(p.work) = before + __popcll(all);
         }
     }
     __syncthreads();
     const int kept = kept_sh;
     uint16_t* out = p.at<uint16_t>(p.w.h_at);
-    const int parts = p.w.pitch / 8;
-    for (int u = threadIdx.x; u < kept * parts; u += 256) {
-        const int i = u / parts, e = 8 * (u % parts), c = before + i;
+    // this workgroup's parts of eight columns
+    const int parts = p.w.pitch / 8, e0 = parts * blockIdx.y / gridDim.y, n = parts * (blockIdx.y + 1) / gridDim.y - e0;
+    for (int u = threadIdx.x; u < kept * n; u += 256) {
+        const int i = u / n, e = 8 * (e0 + u % n), c = before + i;
         const int64_t src = (int64_t)local[i] * a.h_row + e;
-        float x[8];
         u32x4 t[NT];
         if constexpr (NT == 1) {
             const uint16_t* h = static_cast<const uint16_t*>(a.h) + src;
@@ -301,13 +334,18 @@ __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, P
             }
         } else {
             const float* h = static_cast<const float*>(a.h) + src;
+            float x[8];
+            if (e + 8 <= a.hidden) {
+                __builtin_memcpy(x, h, 32);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = e + j < a.hidden ? h[j] : 0.0f;
+                for (int j = 0; j < 8; ++j) x[j] = e + j < a.hidden ? h[j] : 0.0f;
+            }
             split8(x, t);
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<u32x4*>(out + ((size_t)n * a.rows + c) * p.w.pitch + e) = t[n];
+        for (int m = 0; m < NT; ++m)
+            *reinterpret_cast<u32x4*>(out + ((size_t)m * a.rows + c) * p.w.pitch + e) = t[m];
     }
 }
 
@@ -317,7 +355,7 @@ __device__ __forceinline__ Operand states_of(const lm_head_loss_args& a, const P
 }
 
 // Tiles of vocabulary x counted rows.  kGrad false: for each row the tile's maximum and sum of
-// exponentials above it, and the target's logit; true: D for vocabulary rows v0 .. of a piece.
+// exponentials above it (base 2), and the target's logit; true: D for vocabulary rows v0 .. of a piece.
 template <class P, int NT, bool kGrad>
 __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_args a, Parts p, int v0, int tm, int tn) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
@@ -334,6 +372,7 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int vw = vfirst + wave / P::WN * (P::BM / P::WM) + 4 * g;
     const int nw = n * P::BN + wave % P::WN * (P::BN / P::WN) + c;
+    const bool inside = vfirst + P::BM <= a.vocab;
     if constexpr (kGrad) {
 #pragma unroll
         for (int j = 0; j < P::NT; ++j) {
@@ -342,14 +381,17 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
             const float lse = p.at<float>(p.w.lse_at)[row], gl = p.at<float>(p.w.gl_at)[row];
             const int target = p.at<int>(p.w.target_at)[row];
             uint16_t* out = p.at<uint16_t>(p.w.d_at) + (size_t)row * p.w.piece;
+            const float lse2 = lse * kLog2e;
+            const int hit = target - vw;
 #pragma unroll
             for (int i = 0; i < P::MT; ++i) {
                 const int v = vw + 16 * i;
                 f32x4 d;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float y = exp2f((acc[i][j][e] - lse) * kLog2e);
-                    d[e] = v + e < a.vocab ? gl * (v + e == target ? y - 1.0f : y) : 0.0f;
+                    const float y = exp2_raw(__builtin_fmaf(acc[i][j][e], kLog2e, -lse2));
+                    d[e] = gl * (hit == 16 * i + e ? y - 1.0f : y);
+                    if (!inside && v + e >= a.vocab) d[e] = 0.0f;
                 }
                 u32x2 t[NT];
                 if constexpr (NT == 1) {
@@ -371,25 +413,34 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
 #pragma unroll
         for (int j = 0; j < P::NT; ++j) {
             const int row = nw + 16 * j;
-            const int target = row < count ? p.at<int>(p.w.target_at)[row] : -1;
             float top = -__builtin_inff(), sum = 0.0f;
+            if (!inside)
+#pragma unroll
+                for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (vw + 16 * i + e >= a.vocab) acc[i][j][e] = -__builtin_inff();
+            // the target's logit, where this lane has it
+            const int hit = (row < count ? p.at<int>(p.w.target_at)[row] : -1) - vw;
+            if (hit >= 0 && hit < 16 * P::MT && hit % 16 < 4)
+#pragma unroll
+                for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (hit == 16 * i + e) p.at<float>(p.w.logit_at)[row] = acc[i][j][e];
 #pragma unroll
             for (int i = 0; i < P::MT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int v = vw + 16 * i + e;
-                    if (v >= a.vocab) acc[i][j][e] = -__builtin_inff();
-                    if (v == target) p.at<float>(p.w.logit_at)[row] = acc[i][j][e];
-                    top = fmaxf(top, acc[i][j][e]);
-                }
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             // (a part past the vocabulary has no maximum: its terms are 0)
+            top *= kLog2e;
             const float ref = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
             for (int i = 0; i < P::MT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += exp2f((acc[i][j][e] - ref) * kLog2e);
+                for (int e = 0; e < 4; ++e) sum += exp2_raw(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (g == 0) red[wave / P::WN * P::BN + wave % P::WN * (P::BN / P::WN) + 16 * j + c] = {top, sum};
@@ -404,7 +455,7 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
 #pragma unroll
             for (int y = 0; y < P::WM; ++y) {
                 const float2 r = red[y * P::BN + x];
-                sum += r.x == -__builtin_inff() ? r.y : r.y * exp2f((r.x - top) * kLog2e);
+                sum += r.x == -__builtin_inff() ? r.y : r.y * exp2_raw(r.x - top);
             }
             p.at<float2>(p.w.part_at)[(size_t)row * tm + m] = {top, sum};
         }
@@ -420,11 +471,11 @@ __global__ __launch_bounds__(256) void lhl_loss_kernel(lm_head_loss_args a, Part
     for (int t = lane; t < tiles; t += 64) top = fmaxf(top, part[t].x);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    for (int t = lane; t < tiles; t += 64) sum += part[t].y * exp2f((part[t].x - top) * kLog2e);
+    for (int t = lane; t < tiles; t += 64) sum += part[t].y * exp2_raw(part[t].x - top);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if (lane == 0) {
-        const float lse = top + logf(sum);
+        const float lse = (top + log2f(sum)) * kLn2;
         const int r = p.at<int>(p.w.rows_at)[row];
         if (a.lse) a.lse[r] = lse;
         if (a.loss) a.loss[r] = lse - p.at<float>(p.w.logit_at)[row];
@@ -470,18 +521,28 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_h_kernel(lm_head_loss_ar
                 *reinterpret_cast<f32x4*>(sum + (size_t)(nw + 16 * j) * p.w.pitch + hw + 16 * i) = acc[i][j];
 }
 
-// grad_h's rows from the splits' sums; rows that do not count get 0 or NaN.
+// 256 columns of a row of grad_h from the splits' sums, four columns a lane and a quarter of the splits a
+// wavefront; rows that do not count get 0 or NaN.
 template <class T>
 __global__ __launch_bounds__(256) void lhl_finish_kernel(lm_head_loss_args a, Parts p) {
-    const int row = blockIdx.x, at = p.at<int>(p.w.place_at)[row];
-    T* out = static_cast<T*>(a.grad_h) + (int64_t)row * a.grad_h_row;
-    const float* sum = p.at<float>(p.w.sum_at) + (size_t)max(at, 0) * p.w.pitch;
-    for (int h = threadIdx.x; h < a.hidden; h += 256) {
-        float x = at == -2 ? __builtin_nanf("") : 0.0f;
-        if (at >= 0)
-            for (int s = 0; s < p.w.splits; ++s) x += sum[(size_t)s * a.rows * p.w.pitch + h];
-        out[h] = from_float<T>(x);
+    __shared__ f32x4 sh[4][64];
+    const int row = blockIdx.x, at = p.at<int>(p.w.place_at)[row], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = 256 * blockIdx.y + 4 * lane;
+    f32x4 x = {0, 0, 0, 0};
+    if (at >= 0 && h < p.w.pitch) {
+        const float* sum = p.at<float>(p.w.sum_at) + (size_t)at * p.w.pitch + h;
+        const int s0 = p.w.splits * wave / 4, s1 = p.w.splits * (wave + 1) / 4;
+#pragma unroll 8
+        for (int s = s0; s < s1; ++s) x += *reinterpret_cast<const f32x4*>(sum + (size_t)s * a.rows * p.w.pitch);
     }
+    sh[wave][lane] = x;
+    __syncthreads();
+    if (wave > 0) return;
+    x = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+    T* out = static_cast<T*>(a.grad_h) + (int64_t)row * a.grad_h_row + h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (h + e < a.hidden) out[e] = from_float<T>(at == -2 ? __builtin_nanf("") : x[e]);
 }
 
 // grad_table for vocabulary rows v0 .. v0 + width: tiles of h x vocabulary.
@@ -524,16 +585,18 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_los
 // ---- launches --------------------------------------------------------------------------
 template <int NT>
 hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStream_t s) {
-    lhl_prepare_kernel<NT><<<dim3((unsigned)std::max(1, (a.rows + 63) / 64)), 256, 0, s>>>(a, p, grad);
+    const unsigned columns = std::min(4, p.w.pitch / LHL_STEP);
+    lhl_prepare_kernel<NT>
+        <<<dim3((unsigned)std::max(1, (a.rows + kPrepRows - 1) / kPrepRows), columns), 256, 0, s>>>(a, p, grad);
     return hipGetLastError();
 }
 
-template <int BN, int NT, bool VEC, bool kGrad>
+template <int BM, int BN, int NT, bool VEC, bool kGrad>
 hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
-    constexpr int WN = BN == 128 ? 2 : 1, WM = 4 / WN;
-    constexpr int kStages = BN == 128 || !VEC ? 2 : 3;
-    using P = Product<LHL_TILE, BN, WM, WN, false, false, 1, NT, 3, VEC, kStages>;
-    const int tm = (width + LHL_TILE - 1) / LHL_TILE, tn = (a.rows + BN - 1) / BN;
+    constexpr int WN = BN == 256 ? 4 : BN == 128 ? 2 : 1, WM = (BM == 256 ? 8 : 4) / WN;
+    constexpr int kStages = BN >= 128 || !VEC ? 2 : 3;
+    using P = Product<BM, BN, WM, WN, false, false, 1, NT, 3, VEC, kStages>;
+    const int tm = (width + BM - 1) / BM, tn = (a.rows + BN - 1) / BN;
     lhl_logits_kernel<P, NT, kGrad>
         <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn);
     return hipGetLastError();
@@ -541,9 +604,11 @@ hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width,
 
 template <int NT, bool VEC, bool kGrad>
 hipError_t logits_of(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
-    if (a.rows <= 32) return logits<32, NT, VEC, kGrad>(a, p, v0, width, s);
-    if (a.rows <= 64) return logits<64, NT, VEC, kGrad>(a, p, v0, width, s);
-    return logits<128, NT, VEC, kGrad>(a, p, v0, width, s);
+    if (a.rows <= 32) return logits<128, 32, NT, VEC, kGrad>(a, p, v0, width, s);
+    if (a.rows <= 64) return logits<128, 64, NT, VEC, kGrad>(a, p, v0, width, s);
+    if constexpr (NT == 1 && VEC)
+        if (a.rows >= 1024) return logits<256, 256, NT, VEC, kGrad>(a, p, v0, width, s);
+    return logits<128, 128, NT, VEC, kGrad>(a, p, v0, width, s);
 }
 
 template <int NT, bool VEC>
@@ -551,7 +616,8 @@ hipError_t loss(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
     hipError_t e = prepare<NT>(a, p, false, s);
     if (e == hipSuccess) e = logits_of<NT, VEC, false>(a, p, 0, a.vocab, s);
     if (e != hipSuccess) return e;
-    lhl_loss_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s>>>(a, p, p.w.vtiles);
+    const int tiles = NT == 1 && VEC && a.rows >= 1024 ? (a.vocab + 255) / 256 : p.w.vtiles;
+    lhl_loss_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s>>>(a, p, tiles);
     return hipGetLastError();
 }
 
@@ -575,18 +641,32 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
             e = a.rows <= 64 ? grad_h<64, NT, VEC>(a, p, v0, width, s) : grad_h<128, NT, VEC>(a, p, v0, width, s);
         if (e == hipSuccess && a.grad_table) {
             constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 2^-16 of its terms
-            using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 2>;
+            if (NT == 1 && a.rows >= 1024) {
+                using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
+                const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
+                lhl_grad_table_kernel<P>
+                    <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+                e = hipGetLastError();
+                continue;
+            }
             const int tm = (p.w.pitch + 127) / 128, tn = (width + 127) / 128;
-            lhl_grad_table_kernel<P>
-                <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+            const dim3 grid(tile_grid((size_t)tm * tn));
+            if (a.rows <= LHL_STEP) {  // one step: its LDS for two workgroups more
+                using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 1>;
+                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+            } else {
+                using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 2>;
+                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+            }
             e = hipGetLastError();
         }
     }
     if (e != hipSuccess || !a.grad_h || a.rows == 0) return e;
+    const dim3 grid((unsigned)a.rows, (unsigned)((p.w.pitch + 255) / 256));
     if (NT == 1)
-        lhl_finish_kernel<uint16_t><<<dim3((unsigned)a.rows), 256, 0, s>>>(a, p);
+        lhl_finish_kernel<uint16_t><<<grid, 256, 0, s>>>(a, p);
     else
-        lhl_finish_kernel<float><<<dim3((unsigned)a.rows), 256, 0, s>>>(a, p);
+        lhl_finish_kernel<float><<<grid, 256, 0, s>>>(a, p);
     return hipGetLastError();
 }
 

@@ -75,6 +75,7 @@ const char* loss_pointers(const lm_head_loss_args* a, bool grad) {
     const size_t es = a->dtype == QWEN_BF16 ? 2 : 4;
     if (!a->table || !aligned(a->table, 2) || (a->vocab > 1 && a->table_row < a->hidden))
         return "table is NULL, not aligned to its elements, or its rows overlap";
+    if (a->table_row > 1 << 22) return "table's rows are more than 2^22 elements apart";
     if (grad && (!aligned(a->grad_table, 2) ||
                  (a->grad_table && a->vocab > 1 && a->grad_table_row < a->hidden)))
         return "grad_table is not aligned to its elements, or its rows overlap";

@@ -80,6 +80,6 @@ def check_all(gpu, h, table, t, gl):
 @pytest.mark.parametrize("dtype", [F, BF16])
 @pytest.mark.parametrize("rows,vocab,hidden", [
     (1, 1, 8), (1, 129, 64), (2, 1000, 8), (31, 300, 128), (33, 257, 72), (64, 128, 1024), (65, 640, 136), (130, 1111, 200),
-    (300, 2500, 320), (7, 50, 1), (40, 333, 33), (100, 700, 1001), (129, 131, 63)])
+    (300, 2500, 320), (7, 50, 1), (40, 333, 33), (100, 700, 1001), (129, 131, 63), (1100, 900, 320), (1025, 2305, 72)])
 def test_loss_and_gradients(gpu, rows, vocab, hidden, dtype):
     check_all(gpu, *inputs(rows, vocab, hidden, dtype))
