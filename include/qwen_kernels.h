@@ -553,8 +553,9 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  *
  * A row with a target below 0 is ignored, whatever h holds there: loss, lse and
  * its row of grad_h are 0.  A target of vocab or more gives NaN in the three,
- * and counts as ignored in grad_table.  A NaN or infinite logit gives its row a
- * NaN loss.
+ * and counts as ignored in grad_table.  Logits are finite and below 2e38 in
+ * magnitude; others give their row a NaN loss (with bf16 states -infinity counts
+ * as exp z = 0).
  *
  * bf16_dev_lm_head_loss writes loss and lse (either may be NULL);
  * bf16_dev_lm_head_loss_grad reads lse (of the same h, table and targets) and
@@ -564,7 +565,7 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  * caller's (calls that may overlap need one each).  Table rows that are 16-byte
  * aligned (pointer, stride, and hidden a multiple of 8) are streamed through LDS;
  * others are read through registers, more slowly.  hidden up to 65536, vocab up to
- * 2^28, rows up to 2^20.  Nothing is allocated and nothing waits: the calls can
+ * 2^28, rows up to 2^20, table_row up to 2^22.  Nothing is allocated and nothing waits: the calls can
  * be captured. */
 typedef struct lm_head_loss_args {
     float* loss;

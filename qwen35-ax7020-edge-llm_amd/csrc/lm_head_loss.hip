@@ -21,8 +21,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 
-// Exponentials in base 2: exp z = 2^(z log2 e), the product and the difference to a tile's maximum in
-// one rounding; the maximum is kept in base 2 too, so that its own rounding cancels.
+// Exponentials in base 2: exp z = 2^(z log2 e).
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: 0
 
@@ -53,6 +52,7 @@ struct Loader {
     int kc, k_end;        // first element along the sum of this lane's part of a step; the sum's end
     int col_left[I];      // VEC false, TR: columns from the part's first on
     int64_t step;         // bytes from one step to the next
+    u32x4 held[VEC ? 1 : I];  // VEC false: a step on its way to LDS
 
     static __device__ int swizzle(int k) { return (k & 3) | (k >> 1 & 4); }
     static __device__ int k_row(int q, int lane) { return 512 / B * (q % (B / 8)) + lane / (B / 8); }
@@ -79,23 +79,23 @@ struct Loader {
         }
     }
 
-    // Starts the copy of the step whose sum begins at k (from 0) and moves on.
+    // Starts the copy of the step whose sum begins at k (from 0) and moves on.  VEC false: only as far as
+    // the registers, from which put() takes it to LDS.
     __device__ void issue(char* lds, int k, const char* zeros, int wave, int lane) {
-        if (!VEC) {
+        if constexpr (!VEC) {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
                 const int q = wave * I + i, mine = k + (TR ? k_row(q, lane) : kc);
                 const int n = TR ? (mine < k_end ? col_left[i] : 0) : k_end - mine;
-                u32x4 v = {0, 0, 0, 0};
                 if (n >= 8) {
-                    __builtin_memcpy(&v, base[i] + off[i], 16);
+                    __builtin_memcpy(&held[i], base[i] + off[i], 16);
                 } else {
+                    held[i] = u32x4{0, 0, 0, 0};
                     const uint16_t* p = reinterpret_cast<const uint16_t*>(base[i] + off[i]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (j < n) v[j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
+                        if (j < n) held[i][j / 2] |= (uint32_t)p[j] << (j % 2 * 16);
                 }
-                *reinterpret_cast<u32x4*>(lds + q * 1024 + lane * 16) = v;
             }
         } else if (k + LHL_STEP <= k_end) {
 #pragma unroll
@@ -112,6 +112,12 @@ struct Loader {
         }
 #pragma unroll
         for (int i = 0; i < I; ++i) base[i] += step;
+    }
+    __device__ void put(char* lds, int wave, int lane) const {
+        if constexpr (!VEC)
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+                *reinterpret_cast<u32x4*>(lds + (wave * I + i) * 1024 + lane * 16) = held[i];
     }
 };
 
@@ -210,9 +216,14 @@ struct Product {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j] = mfma_terms<NA, NB, MOST>(f.a[i], f.b[j], acc[i][j]);
         };
+        // (VEC false: a's newest step waits in registers until the buffers' next barrier)
+        auto put = [&](int s) { la.put(lds + s % STAGES * kStage, wave, lane); };
 #pragma unroll
         for (int s = 0; s < STAGES; ++s)
-            if (s < steps) issue(s);
+            if (s < steps) {
+                issue(s);
+                if (!VEC && (s + 1 < STAGES || STAGES == 1)) put(s);
+            }
         if (steps >= STAGES)
             wait<STAGES - 1>();
         else
@@ -223,6 +234,7 @@ struct Product {
             multiply(x);
             __builtin_amdgcn_sched_barrier(0);
             if (s + 1 < steps) {
+                if (!VEC && s + STAGES - 1 < steps) put(s + STAGES - 1);
                 if (s + STAGES <= steps)  // the steps behind s + 1 are all on their way
                     wait<STAGES >= 2 ? STAGES - 2 : 0>();
                 else
@@ -381,7 +393,6 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
             const float lse = p.at<float>(p.w.lse_at)[row], gl = p.at<float>(p.w.gl_at)[row];
             const int target = p.at<int>(p.w.target_at)[row];
             uint16_t* out = p.at<uint16_t>(p.w.d_at) + (size_t)row * p.w.piece;
-            const float lse2 = lse * kLog2e;
             const int hit = target - vw;
 #pragma unroll
             for (int i = 0; i < P::MT; ++i) {
@@ -389,7 +400,7 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
                 f32x4 d;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float y = exp2_raw(__builtin_fmaf(acc[i][j][e], kLog2e, -lse2));
+                    const float y = exp2_raw((acc[i][j][e] - lse) * kLog2e);
                     d[e] = gl * (hit == 16 * i + e ? y - 1.0f : y);
                     if (!inside && v + e >= a.vocab) d[e] = 0.0f;
                 }
@@ -434,13 +445,23 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            // (a part past the vocabulary has no maximum: its terms are 0)
+            // z log2 e less the maximum in one rounding; the maximum is kept in base 2, so that its own
+            // rounding cancels.  Where that is too far from 0 for an exponent, the difference first.  (A part
+            // past the vocabulary has no maximum: its terms are 0.)
+            const float peak = top == -__builtin_inff() ? 0.0f : top;
             top *= kLog2e;
-            const float ref = top == -__builtin_inff() ? 0.0f : top;
+            if (__any(fabsf(peak) > 1e6f)) {
 #pragma unroll
-            for (int i = 0; i < P::MT; ++i)
+                for (int i = 0; i < P::MT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += exp2_raw(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
+                    for (int e = 0; e < 4; ++e) sum += exp2_raw((acc[i][j][e] - peak) * kLog2e);
+            } else {
+                const float ref = peak * kLog2e;
+#pragma unroll
+                for (int i = 0; i < P::MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += exp2_raw(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
+            }
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (g == 0) red[wave / P::WN * P::BN + wave % P::WN * (P::BN / P::WN) + 16 * j + c] = {top, sum};
@@ -594,7 +615,7 @@ hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStr
 template <int BM, int BN, int NT, bool VEC, bool kGrad>
 hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
     constexpr int WN = BN == 256 ? 4 : BN == 128 ? 2 : 1, WM = (BM == 256 ? 8 : 4) / WN;
-    constexpr int kStages = BN >= 128 || !VEC ? 2 : 3;
+    constexpr int kStages = BN >= 128 || !VEC || (BM == 256 && NT == 3) ? 2 : 3;
     using P = Product<BM, BN, WM, WN, false, false, 1, NT, 3, VEC, kStages>;
     const int tm = (width + BM - 1) / BM, tn = (a.rows + BN - 1) / BN;
     lhl_logits_kernel<P, NT, kGrad>
@@ -605,6 +626,8 @@ hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width,
 template <int NT, bool VEC, bool kGrad>
 hipError_t logits_of(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
     if (a.rows <= 32) return logits<128, 32, NT, VEC, kGrad>(a, p, v0, width, s);
+    if constexpr (VEC)
+        if (a.rows <= 64) return logits<256, 64, NT, VEC, kGrad>(a, p, v0, width, s);
     if (a.rows <= 64) return logits<128, 64, NT, VEC, kGrad>(a, p, v0, width, s);
     if constexpr (NT == 1 && VEC)
         if (a.rows >= 1024) return logits<256, 256, NT, VEC, kGrad>(a, p, v0, width, s);
@@ -616,14 +639,15 @@ hipError_t loss(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
     hipError_t e = prepare<NT>(a, p, false, s);
     if (e == hipSuccess) e = logits_of<NT, VEC, false>(a, p, 0, a.vocab, s);
     if (e != hipSuccess) return e;
-    const int tiles = NT == 1 && VEC && a.rows >= 1024 ? (a.vocab + 255) / 256 : p.w.vtiles;
+    const int tiles = VEC && ((NT == 1 && a.rows >= 1024) || (a.rows > 32 && a.rows <= 64)) ? (a.vocab + 255) / 256
+                                                                                             : p.w.vtiles;
     lhl_loss_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s>>>(a, p, tiles);
     return hipGetLastError();
 }
 
 template <int BN, int NT, bool VEC>
 hipError_t grad_h(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
-    using P = Product<128, BN, BN == 128 ? 2 : 4, BN == 128 ? 2 : 1, true, false, 1, NT, 3, VEC, 2>;
+    using P = Product<128, BN, BN == 128 ? 2 : 4, BN / 64, true, false, 1, NT, 3, VEC, 2>;
     const int tm = (p.w.pitch + 127) / 128, tn = (a.rows + BN - 1) / BN;
     lhl_grad_h_kernel<P>
         <<<dim3(tile_grid((size_t)tm * tn * p.w.splits)), P::kThreads, 0, s>>>(a, p, v0, width, tm, tn);

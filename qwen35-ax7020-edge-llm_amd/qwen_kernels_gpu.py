@@ -16,6 +16,7 @@ library raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
@@ -567,33 +568,39 @@ class SweepPlan:
 
 
 # ---- a text's tokens -------------------------------------------------------------------
+_HERE = contextlib.nullcontext()
+
+
 def _same_device(first, **tensors):
     """Every tensor on the device of `first`, a GPU; a context that makes it current."""
-    torch = _torch()
-    if not first.is_cuda:
+    cuda = _torch().cuda
+    device = first.device
+    if device.type != "cuda":
         raise ValueError("the tensors have to be on a GPU")
     for name, t in tensors.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
-    return torch.cuda.device(first.device)
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+    return _HERE if device.index == cuda.current_device() else cuda.device(device)
 
 
 def _rows_of(t, name, shape, dtype):
     """t of this shape and type, each of its rows contiguous -> the stride between rows."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name} has to be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
-    step = 1
-    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    stride, step = t.stride(), 1
+    for n, s in zip(shape[:0:-1], stride[:0:-1]):
         if n != 1 and s != step:
             raise ValueError(f"{name}: a row's elements have to be contiguous")
         step *= n
-    if t.shape[0] > 1 and t.stride(0) < step:
+    if shape[0] < 2:
+        return step
+    if stride[0] < step:
         raise ValueError(f"{name}: its rows overlap")
-    return t.stride(0) if t.shape[0] > 1 else step
+    return stride[0]
 
 
 def _flat(t, name, shape, dtype):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{name} has to be a contiguous {tuple(shape)} of {dtype}")
 
 
@@ -604,28 +611,23 @@ def _gdn_args(q, k, v, alpha, beta, scale, states, slots, out):
         raise ValueError("q, k, v are [rows, heads, dim] in float32 or bfloat16")
     rows, hk, dk = q.shape
     hv, dv = v.shape[1:]
-    a = gdn_dev_args()
-    a.q_row = _rows_of(q, "q", (rows, hk, dk), q.dtype)
-    a.k_row = _rows_of(k, "k", (rows, hk, dk), q.dtype)
-    a.v_row = _rows_of(v, "v", (rows, hv, dv), q.dtype)
-    a.out_row = _rows_of(out, "out", (rows, hv, dv), q.dtype)
-    a.gate_row = _rows_of(alpha, "alpha", (rows, hv), torch.float32)
-    if beta is not None and _rows_of(beta, "beta", (rows, hv), torch.float32) != a.gate_row:
-        raise ValueError("alpha and beta have to have the same row stride")
+    keys, values, gates, dtype = (rows, hk, dk), (rows, hv, dv), (rows, hv), q.dtype
     n_slots = None
+    at = {}
     for name, t in states.items():
         if t is not None:
             n_slots = t.shape[0] if n_slots is None else n_slots
             _flat(t, name, (n_slots, hv, dk * dv), torch.float32)
-            setattr(a, name, _dp(t))
-    if slots is not None:
-        a.slots = _dp(slots)
-    a.out, a.q, a.k, a.v, a.alpha = _dp(out), _dp(q), _dp(k), _dp(v), _dp(alpha)
-    a.beta = None if beta is None else _dp(beta)
-    a.rows, a.n_slots, a.heads_k, a.heads_v, a.dim_k, a.dim_v = rows, n_slots, hk, hv, dk, dv
-    a.dtype = QWEN_F32 if q.dtype == torch.float32 else QWEN_BF16
-    a.scale = scale
-    return a
+            at[name] = t.data_ptr()
+    gate_row = _rows_of(alpha, "alpha", gates, torch.float32)
+    if beta is not None and _rows_of(beta, "beta", gates, torch.float32) != gate_row:
+        raise ValueError("alpha and beta have to have the same row stride")
+    return gdn_dev_args(
+        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), alpha.data_ptr(),
+        None if beta is None else beta.data_ptr(), at.get("state_in"), at.get("state_out"),
+        None if slots is None else slots.data_ptr(), None, None, 0, _rows_of(q, "q", keys, dtype),
+        _rows_of(k, "k", keys, dtype), _rows_of(v, "v", values, dtype), _rows_of(out, "out", values, dtype), gate_row,
+        rows, 0, n_slots, hk, hv, dk, dv, QWEN_F32 if dtype == torch.float32 else QWEN_BF16, scale)
 
 
 def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0, state_in=None, state_out=None,

@@ -40,8 +40,8 @@ def inputs(rows, hk, hv, dk, dv, dtype, delta, n_state, seed=1, packed=True):
     q, k = (x / x.norm(dim=-1, keepdim=True).clamp(min=1e-6) for x in (q, k))
     k = 0.7 * k + 0.3 * k[:1] if rows else k  # keys that have much in common
     buf = torch.empty(rows, width + (0 if packed else 3)).to(dtype).cuda()
-    buf[:, : hk * dk] = q.reshape(rows, -1).to(dtype).cuda()
-    buf[:, hk * dk : 2 * hk * dk] = k.reshape(rows, -1).to(dtype).cuda()
+    buf[:, : hk * dk] = q.reshape(rows, hk * dk).to(dtype).cuda()
+    buf[:, hk * dk : 2 * hk * dk] = k.reshape(rows, hk * dk).to(dtype).cuda()
     buf[:, 2 * hk * dk : width] = qkv[:, 2 * hk * dk :].to(dtype).cuda()
     alpha = torch.sigmoid(2 * torch.randn(rows, hv, generator=g) + 2).cuda()
     beta = torch.sigmoid(torch.randn(rows, hv, generator=g)).cuda() if delta else None
@@ -112,13 +112,19 @@ def test_step(gpu, hk, hv, dk, dv, delta, dtype):
         near(st, wst)
 
 
+# many sequences (32 value columns a workgroup where there are heads enough), few, and one
+LENGTHS = {"many": [1, 0, 64, 63, 130, 65, 0, 200, 2], "few": [257, 70], "one": [449]}
+
+
 @pytest.mark.parametrize("dtype", [F, BF16])
 @pytest.mark.parametrize("delta", [True, False])
 @pytest.mark.parametrize("hk,hv,dk,dv", SHAPES)
-def test_prompt(gpu, hk, hv, dk, dv, delta, dtype):
-    lengths = [1, 0, 64, 63, 130, 65, 0, 200, 2]
+@pytest.mark.parametrize("which,packed", [("many", False), ("many", True), ("few", True), ("one", False)])
+def test_prompt(gpu, which, packed, hk, hv, dk, dv, delta, dtype):
+    """packed: rows of a projection as they are (16-byte aligned for most shapes); else three elements apart."""
+    lengths = LENGTHS[which]
     spans, starts = spans_of(lengths)
-    q, k, v, al, be, st = inputs(sum(lengths), hk, hv, dk, dv, dtype, delta, len(lengths), packed=False)
+    q, k, v, al, be, st = inputs(sum(lengths), hk, hv, dk, dv, dtype, delta, len(lengths), packed=packed)
     want, wst = oracle(q, k, v, al, be, 0.25, st, spans)
     out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, scale=0.25, state_in=st)
     near(out, want, dtype)
@@ -159,3 +165,189 @@ def test_state_is_the_decode_runtimes(gpu):
     near(torch.from_numpy(out).view(H, D), want[70])
     near(torch.from_numpy(host)[None], wst)
     assert np.allclose(ol.gdn_state_from_blocked(host, H, D), unblocked(wst, D, D)[0].numpy(), atol=1e-4)
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_long_sequence(gpu, dtype):
+    """Errors do not pile up over 60 chunks."""
+    q, k, v, al, be, st = inputs(3841, 1, 1, 128, 128, dtype, True, 1)
+    want, wst = oracle(q, k, v, al, be, 1.0, st, [(0, 3841)])
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, state_in=st)
+    near(out, want, dtype)
+    near(got, wst)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_decays_at_their_ends(gpu, delta, dtype):
+    """A decay of 0 forgets everything before it; 1 keeps it; tiny ones underflow; a beta of 0 writes nothing."""
+    q, k, v, al, be, st = inputs(200, 2, 2, 64, 64, dtype, delta, 1)
+    al[:] = 1.0
+    al[70, :] = 0.0
+    al[100:110, 0] = 1e-38
+    al[110:112, 1] = 1e-45  # subnormal
+    al[199, 1] = 0.0
+    if delta:
+        be[::3] = 0.0
+        be[1::3] = 1.0
+    want, wst = oracle(q, k, v, al, be, 1.0, st, [(0, 200)])
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, state_in=st)
+    near(out, want, dtype)
+    near(got, wst)
+    for t in range(0, 200):
+        o = gpu.linear_attention_step(q[t:t + 1], k[t:t + 1], v[t:t + 1], al[t:t + 1], None if be is None else be[t:t + 1],
+                                      st)
+        near(o, want[t:t + 1], dtype)
+    near(st, wst)
+
+
+@pytest.mark.parametrize("form", ["prompt", "step"])
+def test_slots(gpu, form):
+    """Slots in any order; empty places, slots outside the pool and a slot named before are skipped, their rows and
+    states left as they were, as are rows behind the last sequence."""
+    slots = [5, -1, 0, 9, 5, 2, 1000000, 3]
+    lengths = [1] * 8 if form == "step" else [70, 10, 0, 64, 3, 1, 20, 129]
+    spans, starts = spans_of(lengths)
+    rows = spans[-1][1] + (0 if form == "step" else 37)
+    q, k, v, al, be, st = inputs(rows, 2, 4, 64, 32, F, True, 9)
+    st[7] = float("nan")  # a state of no sequence
+    q[spans[1][0]:spans[1][1]] = float("nan")  # and rows that are skipped
+    if form == "prompt":
+        v[spans[-1][1]:] = float("nan")
+    taken = [s if s < 9 and i != 4 else -1 for i, s in enumerate(slots)]
+    want, wst = oracle(q, k, v, al, be, 1.0, st, spans, taken)
+    sl = torch.tensor(slots, dtype=torch.int32).cuda()
+    out = torch.full((rows, 4, 32), float("nan"), device="cuda")
+    if form == "step":
+        gpu.linear_attention_step(q, k, v, al, be, st, slots=sl, out=out)
+        state = st
+    else:
+        before = torch.full_like(st, 7.0)
+        _, state = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st, state_out=before, slots=sl, out=out)
+        for i in (1, 4, 6, 7, 8):
+            assert bool((state[i] == 7.0).all())
+            wst[i] = 7.0
+    near(out, want)
+    near(state, wst)
+
+
+def test_in_place_states_and_strided_gates(gpu):
+    q, k, v, al, be, st = inputs(140, 2, 2, 32, 32, F, True, 2)
+    spans, starts = spans_of([75, 65])
+    want, wst = oracle(q, k, v, al, be, 1.0, st, spans)
+    gates = torch.full((140, 7), float("nan"), device="cuda")
+    gates[:, :2], gates[:, 4:6] = al, be
+    wide = torch.full((140, 3, 32), 5.0, device="cuda")
+    _, got = gpu.linear_attention_prompt(q, k, v, gates[:, :2], gates[:, 4:6], starts, state_in=st, state_out=st,
+                                         out=wide[:, :2])
+    assert got is st
+    near(wide[:, :2], want)
+    near(st, wst)
+    assert bool((wide[:, 2] == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_nan_stays_in_its_sequence_head_and_time(gpu, dtype):
+    q, k, v, al, be, st = inputs(400, 2, 2, 64, 64, dtype, True, 2)
+    spans, starts = spans_of([200, 200])
+    v[130, 1, 3] = float("nan")
+    want, wst = oracle(q, k, v, al, be, 1.0, st, spans)
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[128:200, 1] = True  # from its chunk on
+    keep = ~bad
+    near(out[keep], want[keep.cpu()], dtype)
+    assert bool(torch.isnan(out[130:200, 1, 3]).all())
+    assert bool(torch.isfinite(got[1]).all()) and bool(torch.isfinite(got[0, 0]).all())
+    near(got[1], wst[1])
+
+
+def test_offsets_past_32_bits(gpu):
+    """A pool of states and rows far apart, both past 2^31 elements."""
+    n = 8200  # 8200 x 16 x 128 x 128 floats
+    pool = torch.empty(n, 16, 128 * 128, device="cuda")
+    q, k, v, al, be, st = inputs(3, 16, 16, 128, 128, F, True, 3)
+    at = [n - 1, 0, n - 7]
+    for i, s in enumerate(at):
+        pool[s] = st[i]
+    want, wst = oracle(q, k, v, al, be, 1.0, st, [(0, 1), (1, 2), (2, 3)])
+    out = gpu.linear_attention_step(q, k, v, al, be, pool, slots=torch.tensor(at, dtype=torch.int32).cuda())
+    near(out, want)
+    near(torch.stack([pool[s] for s in at]), wst)
+    del pool
+    q, k, v, al, be, st = inputs(150, 1, 1, 128, 128, BF16, True, 1)
+    want, wst = oracle(q, k, v, al, be, 1.0, st, [(0, 150)])
+    for far in ((1 << 24) - 8, 1 << 24):  # within and past what lanes hold as an offset
+        big = torch.empty(149 * far + 128, dtype=BF16, device="cuda")
+        vv = big.as_strided((150, 1, 128), (far, 128, 1))
+        vv.copy_(v)
+        out, got = gpu.linear_attention_prompt(q, k, vv, al, be, state_in=st)
+        near(out, want, BF16)
+        near(got, wst)
+        del big, vv
+
+
+def test_graph_stream_and_repeats(gpu):
+    """Captured on a stream of its own, replayed with other work between, and bit for bit the eager result."""
+    spans, starts = spans_of([100, 29, 300])
+    q, k, v, al, be, st = inputs(429, 4, 8, 64, 64, BF16, True, 3)
+    out0, state0 = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    step0 = gpu.linear_attention_step(q[:3], k[:3], v[:3], al[:3], be[:3], state0.clone())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out1, state1 = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+        again = state1.clone()
+        step1 = gpu.linear_attention_step(q[:3], k[:3], v[:3], al[:3], be[:3], again)
+    for i in range(3):
+        out1.zero_()
+        graph.replay()
+        other = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+        torch.cuda.synchronize()
+        for got, want in ((out1, out0), (state1, state0), (step1, step0), (other[0], out0), (other[1], state0)):
+            assert torch.equal(got, want), i
+    with torch.cuda.stream(side):
+        got = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    side.synchronize()
+    assert torch.equal(got[0], out0) and torch.equal(got[1], state0)
+
+
+def test_no_sequences_and_no_tokens(gpu):
+    q, k, v, al, be, st = inputs(0, 2, 2, 32, 32, F, True, 3)
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, torch.zeros(4, dtype=torch.int32).cuda(), state_in=st)
+    assert out.shape[0] == 0 and torch.equal(got, st)
+    _, got = gpu.linear_attention_prompt(q, k, v, al, be, torch.zeros(4, dtype=torch.int32).cuda())
+    assert bool((got == 0).all())
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, torch.zeros(1, dtype=torch.int32).cuda(), state_out=st[:0])
+    assert got.shape[0] == 0
+    assert gpu.linear_attention_step(q, k, v, al, be, st[:0]).shape[0] == 0
+
+
+def test_starts_outside_the_rows_are_held_inside(gpu):
+    """starts that leave the rows or fall do not reach memory outside: sequences are cut, or empty."""
+    q, k, v, al, be, st = inputs(100, 1, 1, 32, 32, F, True, 3)
+    starts = torch.tensor([-50, 40, 30, 100000], dtype=torch.int32).cuda()
+    want, wst = oracle(q, k, v, al, be, 1.0, st, [(0, 40), (40, 40), (30, 100)])
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    near(got[:2], wst[:2])  # (the last one's rows meet the first one's)
+    assert bool(torch.isfinite(out).all())
+
+
+def test_python_refusals(gpu):
+    q, k, v, al, be, st = inputs(4, 2, 4, 32, 32, F, True, 4)
+    step = gpu.linear_attention_step
+    for bad in (lambda: step(q.cpu(), k, v, al, be, st), lambda: step(q, k.cpu(), v, al, be, st),
+                lambda: step(q, k.to(BF16), v, al, be, st), lambda: step(q, k, v, al.double(), be, st),
+                lambda: step(q[:, :, ::2], k[:, :, ::2], v, al, be, st), lambda: step(q, k, v, al, be, st[:3]),
+                lambda: step(q, k, v, al, be, st, slots=torch.zeros(4, dtype=torch.int64, device="cuda")),
+                lambda: step(q, k, v, al, be, st, out=torch.empty(4, 4, 16, device="cuda")),
+                lambda: gpu.linear_attention_prompt(q, k, v, al, be, torch.zeros(7, dtype=torch.int32).cuda(), state_in=st),
+                lambda: gpu.linear_attention_prompt(q, k, v, al, be, slots=torch.zeros(1, dtype=torch.int32).cuda()),
+                lambda: step(q, k, v, al, be, st.transpose(0, 1).contiguous().transpose(0, 1))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        gpu.linear_attention_prompt(q, k, v, al, be, work=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError):  # 3 key heads do not divide 4 value heads
+        step(torch.zeros(4, 3, 32, device="cuda"), torch.zeros(4, 3, 32, device="cuda"), v, al, be, st)

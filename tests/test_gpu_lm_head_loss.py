@@ -83,3 +83,205 @@ def check_all(gpu, h, table, t, gl):
     (300, 2500, 320), (7, 50, 1), (40, 333, 33), (100, 700, 1001), (129, 131, 63), (1100, 900, 320), (1025, 2305, 72)])
 def test_loss_and_gradients(gpu, rows, vocab, hidden, dtype):
     check_all(gpu, *inputs(rows, vocab, hidden, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_strided_and_unaligned(gpu, dtype):
+    for pad in (1, 8):
+        check_all(gpu, *inputs(70, 400, 64, dtype, pad=pad))
+    h, table, t, gl = inputs(70, 401, 64, dtype)
+    check_all(gpu, h, table[1:], t.clamp(max=399), gl)
+    flat = torch.empty(400 * 64 + 1, dtype=BF16, device="cuda")
+    odd = flat[1:].view(400, 64)  # rows at odd 16-bit addresses
+    odd.copy_(table[:400])
+    check_all(gpu, h, odd, t.clamp(max=399), gl)
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF16, 8192, 18001), (F, 4096, 11000)])
+def test_several_pieces_of_the_vocabulary(gpu, dtype, rows, vocab):
+    check_all(gpu, *inputs(rows, vocab, 64, dtype, ignored=0.9))
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_ignored_rows_hold_anything(gpu, dtype):
+    h, table, t, gl = inputs(90, 300, 96, dtype)
+    t[3], t[50], t[89] = 300, 2 ** 31 - 1, -1
+    h[t < 0] = float("nan")
+    h[50] = float("inf")
+    check_all(gpu, h, table, t, torch.where(t < 0, float("nan"), gl))
+    for target in (-5, 300):
+        t[:] = target
+        loss, lse = gpu.lm_head_loss(h, table, t)
+        gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+        assert bool((gw == 0).all())
+        assert bool((gh == 0).all() if target < 0 else torch.isnan(gh).all())
+        assert bool((loss == 0).all() if target < 0 else torch.isnan(loss).all())
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_extreme_logits(gpu, dtype):
+    """Logits far apart, near the type's lowest value, and infinite."""
+    h = torch.zeros(5, 8, device="cuda")
+    h[:, 0] = torch.tensor([1.0, 1.0, -1.0, 1e-3, 0.0], device="cuda")
+    table = torch.zeros(300, 8, device="cuda", dtype=BF16)
+    table[:, 0] = torch.linspace(-3e4, 3e4, 300)
+    table[7, 0] = torch.finfo(BF16).min / 4
+    h = h.to(dtype)
+    t = torch.tensor([299, 0, 299, 3, 8], dtype=torch.int32, device="cuda")
+    loss, lse = gpu.lm_head_loss(h, table, t)
+    z = h.double().cpu() @ table.double().cpu().t()
+    want = torch.logsumexp(z, 1)
+    at = z.gather(1, t.long().cpu()[:, None])[:, 0]
+    for r in range(5):
+        assert abs(float(lse[r]) - float(want[r])) <= 2 ** -22 * abs(float(want[r])) + 1e-6, r
+        assert abs(float(loss[r]) - float(want[r] - at[r])) <= 2 ** -21 * float(want[r].abs() + at[r].abs()) + 1e-6, r
+    # infinities of the table: as a bf16 row's -infinity they count as nothing, else the row's loss is NaN
+    table[:] = 0.0
+    table[9, 1], table[11, 2] = float("-inf"), float("inf")
+    h = torch.zeros(2, 3, device="cuda")
+    h[0, 1], h[1, 2] = 1.0, 1.0
+    for r, col in ((0, [1]), (1, [2])):
+        loss, _ = gpu.lm_head_loss(h[r:r + 1, col].to(dtype), table[:, col], t[3:4])
+        if r == 0 and dtype == BF16:
+            assert abs(float(loss) - np.log(299)) < 1e-5
+        else:
+            assert bool(torch.isnan(loss).all())
+
+
+def test_gradient_is_the_differences(gpu):
+    """Central differences of the float32 loss; step 2^-5: the third derivative's part is below 2^-10 x the
+    largest third derivative / 6, and the losses' rounding 2 x 4e-5 / 2^-4 = 1.3e-3."""
+    h, table, t, gl = inputs(6, 200, 16, F, ignored=0.0)
+    loss, lse = gpu.lm_head_loss(h, table, t)
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+    eps = 2.0 ** -5
+    for r, c in ((0, 0), (3, 7), (5, 15)):
+        up, down = h.clone(), h.clone()
+        up[r, c] += eps
+        down[r, c] -= eps
+        d = ((gpu.lm_head_loss(up, table, t)[0] - gpu.lm_head_loss(down, table, t)[0]).double() * gl.double()).sum() / (2 * eps)
+        assert abs(float(d) - float(gh[r, c])) < 3e-3
+    for v, c in ((int(t[0]), 2), (11, 5)):
+        up, down = table.clone(), table.clone()
+        up[v, c] += eps
+        down[v, c] -= eps
+        width = float(up[v, c].double() - down[v, c].double())
+        d = ((gpu.lm_head_loss(h, up, t)[0] - gpu.lm_head_loss(h, down, t)[0]).double() * gl.double()).sum() / width
+        assert abs(float(d) - float(gw[v, c])) < 3e-3 + 2 ** -8 * abs(float(d))
+
+
+@pytest.mark.parametrize("rows", [20, 200])
+def test_one_gradient_alone(gpu, rows):
+    h, table, t, gl = inputs(rows, 500, 64, F)
+    _, lse = gpu.lm_head_loss(h, table, t)
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+    a, b = gpu.lm_head_loss_grad(h, table, t, lse, gl, need_table=False)
+    assert b is None and torch.equal(a, gh)
+    into = torch.full((500, 80), 3.0, dtype=BF16, device="cuda")
+    a, b = gpu.lm_head_loss_grad(h, table, t, lse, gl, need_h=False, grad_table=into[:, 5:69])
+    assert a is None and torch.equal(b, gw) and bool((into[:, :5] == 3).all()) and bool((into[:, 69:] == 3).all())
+    into = torch.full((rows, 71), 3.0, device="cuda")
+    a, _ = gpu.lm_head_loss_grad(h, table, t, lse, gl, need_table=False, grad_h=into[:, :64])
+    assert torch.equal(a, gh) and bool((into[:, 64:] == 3).all())
+
+
+def test_no_rows(gpu):
+    h, table, t, gl = inputs(0, 100, 64, F)
+    loss, lse = gpu.lm_head_loss(h, table, t)
+    assert loss.numel() == 0
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+    assert gh.shape == (0, 64) and bool((gw == 0).all())
+
+
+@pytest.mark.parametrize("rows,dtype", [(5, F), (300, BF16), (1100, BF16)])
+def test_graph_stream_and_repeats(gpu, rows, dtype):
+    h, table, t, gl = inputs(rows, 3000, 128, dtype)
+    loss0, lse0 = gpu.lm_head_loss(h, table, t)
+    g0 = gpu.lm_head_loss_grad(h, table, t, lse0, gl)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        loss1, lse1 = gpu.lm_head_loss(h, table, t)
+        g1 = gpu.lm_head_loss_grad(h, table, t, lse1, gl)
+    for i in range(3):
+        for x in (loss1, lse1, *g1):
+            x.zero_()
+        graph.replay()
+        loss2, lse2 = gpu.lm_head_loss(h, table, t)
+        g2 = gpu.lm_head_loss_grad(h, table, t, lse2, gl)
+        torch.cuda.synchronize()
+        for got, want in zip((loss1, lse1, *g1, loss2, lse2, *g2), (loss0, lse0, *g0) * 2):
+            assert torch.equal(got, want), i
+
+
+def test_table_past_32_bits(gpu):
+    """2.2 million rows of 1000: offsets past 2^31 elements."""
+    V, H = 2_200_000, 1000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = torch.empty(V, H, dtype=BF16, device="cuda")
+    for i in range(0, V, 200_000):
+        table[i:i + 200_000] = torch.randn(min(200_000, V - i), H, generator=g, device="cuda").to(BF16) * 0.05
+    h = torch.randn(3, H, generator=g, device="cuda")
+    t = torch.tensor([V - 1, 5, V - 4321], dtype=torch.int32, device="cuda")
+    loss, lse = gpu.lm_head_loss(h, table, t)
+    z = torch.cat([h.double() @ table[i:i + 100_000].double().t() for i in range(0, V, 100_000)], 1)
+    want = torch.logsumexp(z, 1)
+    near(lse, want.cpu(), 4e-5)
+    near(loss, (want - z.gather(1, t.long()[:, None])[:, 0]).cpu(), 4e-5)
+    gl = torch.ones(3, device="cuda")
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+    D = torch.exp(z - want[:, None])
+    D[torch.arange(3), t.long()] -= 1
+    gh_want = sum(D[:, i:i + 100_000] @ table[i:i + 100_000].double() for i in range(0, V, 100_000))
+    near(gh, gh_want.cpu(), 2e-4 * row_top(gh_want.cpu()))
+    for v in (0, 5, V - 4321, V - 1):
+        w = (D[:, v] @ h.double()).cpu()
+        near(gw[v], w, w.abs() * 2 ** -8 + 2e-4 * float(w.abs().max()))
+
+
+def test_reading_a_text(gpu):
+    """A prompt through a linear-attention layer, its score and the score's gradient, then the answer's first token
+    from the state that the prompt left."""
+    T, H, D, V = 210, 2, 64, 500
+    g = torch.Generator().manual_seed(8)
+    rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v = (torch.nn.functional.normalize(rnd(T + 1, H, D), dim=-1).cuda() for _ in range(3))
+    al, be = torch.sigmoid(rnd(T + 1, H) + 2).cuda(), torch.sigmoid(rnd(T + 1, H)).cuda()
+    table = rnd(V, H * D).to(BF16).cuda()
+    t = torch.randint(0, V, (T,), generator=g, dtype=torch.int32).cuda()
+    t[:50] = -100
+    ones = torch.full((T,), 1.0 / 160, device="cuda")
+    out, state = gpu.linear_attention_prompt(q[:T], k[:T], v[:T], al[:T], be[:T], scale=D ** -0.5)
+    h = out.view(T, H * D)
+    loss, lse = gpu.lm_head_loss(h, table, t)
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, ones)
+    nxt = gpu.linear_attention_step(q[T:], k[T:], v[T:], al[T:], be[T:], state, scale=D ** -0.5)
+    # the same in 64 bits
+    Q, K, W, A, B = (x.double().cpu() for x in (q, k, v, al, be))
+    S, outs = torch.zeros(H, D, D, dtype=torch.float64), []
+    for i in range(T + 1):
+        S = S * A[i][:, None, None]
+        u = B[i][:, None] * (W[i] - (S * K[i][:, :, None]).sum(1))
+        S = S + K[i][:, :, None] * u[:, None, :]
+        outs.append(D ** -0.5 * (S * Q[i][:, :, None]).sum(1))
+    O = torch.stack(outs)
+    near(nxt, O[T:], 2e-5 * float(O.abs().max()))
+    l0, _, g0, w0, _, _ = oracle(O[:T].reshape(T, -1), table, t, ones)
+    near(loss, l0, 1e-4)
+    near(gh, g0, 4e-4 * row_top(g0))
+    near(gw, w0, w0.abs() * 2 ** -8 + 4e-4 * row_top(w0))
+
+
+def test_python_refusals(gpu):
+    h, table, t, gl = inputs(4, 50, 16, F)
+    loss, lse = gpu.lm_head_loss(h, table, t)
+    for bad in (lambda: gpu.lm_head_loss(h.cpu(), table, t), lambda: gpu.lm_head_loss(h, table.float(), t),
+                lambda: gpu.lm_head_loss(h, table, t.long()), lambda: gpu.lm_head_loss(h, table[:, :8], t),
+                lambda: gpu.lm_head_loss(h.half(), table, t), lambda: gpu.lm_head_loss(h, table.t(), t),
+                lambda: gpu.lm_head_loss_grad(h, table, t, lse[:3], gl),
+                lambda: gpu.lm_head_loss_grad(h, table, t, lse, gl, grad_h=torch.empty(4, 16, dtype=BF16, device="cuda"))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        gpu.lm_head_loss(h, table, t, work=torch.empty(256, dtype=torch.uint8, device="cuda"))
