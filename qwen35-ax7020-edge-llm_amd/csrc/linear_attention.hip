@@ -833,7 +833,8 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
 // one pass over the state, whose bytes bound it.  A wavefront has COLS / 4 groups of
 // four value columns; lane 4 g + l has rows 4 (g + 16 n) .. + 3 of column l of each, one
 // 16-byte load and store each, 1 KiB a wavefront.
-template <int NI, int G, class T>
+// kStream: past the caches, for states that would not be found there again.
+template <int NI, int G, bool kStream, class T>
 __global__ __launch_bounds__(256) void gdn_step_kernel(gdn_dev_args a, int groups) {
     const int lane = threadIdx.x & 63, l = lane & 3, g = lane >> 2;
     const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);  // (sequence, head, run of G column groups)
@@ -853,9 +854,10 @@ __global__ __launch_bounds__(256) void gdn_step_kernel(gdn_dev_args a, int group
         for (int n = 0; n < NI; ++n) {
             const int ig = g + 16 * n;
             S[m][n] = f32x4{0, 0, 0, 0};
-            if (jg0 + m < groups && ig < ng && a.state_in)
-                S[m][n] = *reinterpret_cast<const f32x4*>(a.state_in + head_state +
-                                                          (((size_t)(jg0 + m) * ng + ig) * 4 + l) * 4);
+            if (jg0 + m < groups && ig < ng && a.state_in) {
+                const f32x4* at = reinterpret_cast<const f32x4*>(a.state_in + head_state) + ((jg0 + m) * ng + ig) * 4 + l;
+                S[m][n] = kStream ? __builtin_nontemporal_load(at) : *at;
+            }
         }
     const T* q = static_cast<const T*>(a.q) + (int64_t)seq * a.q_row + (int64_t)hk * a.dim_k;
     const T* k = static_cast<const T*>(a.k) + (int64_t)seq * a.k_row + (int64_t)hk * a.dim_k;
@@ -911,8 +913,11 @@ __global__ __launch_bounds__(256) void gdn_step_kernel(gdn_dev_args a, int group
                     f32x4 x;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(kf[n][e], u, al * S[m][n][e]);
-                    *reinterpret_cast<f32x4*>(a.state_out + head_state + (((size_t)(jg0 + m) * ng + ig) * 4 + l) * 4) =
-                        x;
+                    f32x4* at = reinterpret_cast<f32x4*>(a.state_out + head_state) + ((jg0 + m) * ng + ig) * 4 + l;
+                    if (kStream)
+                        __builtin_nontemporal_store(x, at);
+                    else
+                        *at = x;
                 }
             }
         }
@@ -961,16 +966,23 @@ hipError_t launch_prompt_of(const gdn_dev_args& a, const GdnWork& w, hipStream_t
     return a.beta ? launch_prompt<KS, 3, true>(a, w, s) : launch_prompt<KS, 3, false>(a, w, s);
 }
 
-template <int NI, int G>
+template <int NI, int G, bool kStream>
 hipError_t launch_step(const gdn_dev_args& a, hipStream_t s) {
     const int groups = a.dim_v / 4;
     const size_t units = (size_t)a.n_seq * a.heads_v * ((groups + G - 1) / G);
     const dim3 grid((unsigned)((units + 3) / 4));
     if (a.dtype == QWEN_BF16)
-        gdn_step_kernel<NI, G, uint16_t><<<grid, 256, 0, s>>>(a, groups);
+        gdn_step_kernel<NI, G, kStream, uint16_t><<<grid, 256, 0, s>>>(a, groups);
     else
-        gdn_step_kernel<NI, G, float><<<grid, 256, 0, s>>>(a, groups);
+        gdn_step_kernel<NI, G, kStream, float><<<grid, 256, 0, s>>>(a, groups);
     return hipGetLastError();
+}
+
+template <int G, bool kStream>
+hipError_t launch_step_of(const gdn_dev_args& a, hipStream_t s) {
+    if (a.dim_k <= 64) return launch_step<1, G, kStream>(a, s);
+    if (a.dim_k <= 128) return launch_step<2, G, kStream>(a, s);
+    return launch_step<4, G, kStream>(a, s);
 }
 
 }  // namespace
@@ -987,12 +999,9 @@ hipError_t gdn_launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_
 hipError_t gdn_launch_step(const gdn_dev_args& a, hipStream_t s) {
     // Four value columns a wavefront while there are few, to have more of them at work: 1 | 8 | 16 sequences of
     // 16 heads of 128 3.3 | 5.3 | 9.4 us; sixteen, four loads in flight a lane: 4.8 | 6.0 | 9.0, and 64 24 for 27.
-    if ((size_t)a.n_seq * a.heads_v * a.dim_v <= 16384) {
-        if (a.dim_k <= 64) return launch_step<1, 1>(a, s);
-        if (a.dim_k <= 128) return launch_step<2, 1>(a, s);
-        return launch_step<4, 1>(a, s);
-    }
-    if (a.dim_k <= 64) return launch_step<1, 4>(a, s);
-    if (a.dim_k <= 128) return launch_step<2, 4>(a, s);
-    return launch_step<4, 4>(a, s);
+    if ((size_t)a.n_seq * a.heads_v * a.dim_v <= 16384) return launch_step_of<1, false>(a, s);
+    // States of 128 MiB and more, with other layers' before they are next wanted, are not left in the 256 MiB
+    // of last-level cache: 256 sequences in turn over four pools 95 us for 107 (one pool again and again: 93 for 85).
+    if ((size_t)a.n_seq * a.heads_v * a.dim_k * a.dim_v * 4 < (size_t)128 << 20) return launch_step_of<4, false>(a, s);
+    return launch_step_of<4, true>(a, s);
 }

@@ -256,6 +256,34 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[MT][NT]) {
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 }
 
+// A wavefront's part of a result as bf16, whose lanes hold four rows of a column each, to memory in which the
+// rows are consecutive, 16 bytes a lane: through LDS, column by column, the 16-byte parts of column n at
+// positions part ^ n.  value(i, j): the four rows of acc[i][j]; store(n, m, x): eight rows from m of column n.
+template <class P, class Value, class Store>
+__device__ __forceinline__ void store_part(char* lds, Value&& value, Store&& store) {
+    constexpr int M = P::BM / P::WM, N = P::BN / P::WN, kParts = M / 8;
+    static_assert(P::kWaves * M * N * 2 <= P::kLds && N * kParts % 64 == 0, "a part fits");
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    char* mine = lds + (threadIdx.x >> 6) * (M * N * 2);
+#pragma unroll
+    for (int j = 0; j < P::NT; ++j)
+#pragma unroll
+        for (int i = 0; i < P::MT; ++i)
+            *reinterpret_cast<u32x2*>(mine + (16 * j + c) * M * 2 + ((2 * i + (g >> 1)) ^ (c % kParts)) * 16 +
+                                      (g & 1) * 8) = value(i, j);
+    asm volatile("" ::: "memory");  // (one wavefront's accesses to LDS are in order)
+#pragma unroll
+    for (int q = 0; q < N * kParts / 64; ++q) {
+        const int n = q * (64 / kParts) + lane / kParts, part = lane % kParts;
+        store(n, 8 * part, *reinterpret_cast<const u32x4*>(mine + n * M * 2 + (part ^ (n % 16 % kParts)) * 16));
+    }
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ u32x2 round4(f32x4 x) {
+    return u32x2{from_float<uint16_t>(x[0]) | (uint32_t)from_float<uint16_t>(x[1]) << 16,
+                 from_float<uint16_t>(x[2]) | (uint32_t)from_float<uint16_t>(x[3]) << 16};
+}
+
 // Tile t of tm x tn: workgroups go round the eight XCDs, so each XCD gets a run of tiles; in a run
 // 8 tiles of m take turns along n, so that the tiles at work in an XCD share their operands in its L2.
 __device__ __forceinline__ bool tile_of(int tm, int tn, int& m, int& n) {
@@ -385,41 +413,48 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
     const int vw = vfirst + wave / P::WN * (P::BM / P::WM) + 4 * g;
     const int nw = n * P::BN + wave % P::WN * (P::BN / P::WN) + c;
     const bool inside = vfirst + P::BM <= a.vocab;
+    __syncthreads();  // the tiles in LDS have been read
     if constexpr (kGrad) {
 #pragma unroll
         for (int j = 0; j < P::NT; ++j) {
-            const int row = nw + 16 * j;
-            if (row >= count) continue;
+            const int row = min(nw + 16 * j, count - 1);
             const float lse = p.at<float>(p.w.lse_at)[row], gl = p.at<float>(p.w.gl_at)[row];
-            const int target = p.at<int>(p.w.target_at)[row];
-            uint16_t* out = p.at<uint16_t>(p.w.d_at) + (size_t)row * p.w.piece;
-            const int hit = target - vw;
+            const int hit = p.at<int>(p.w.target_at)[row] - vw;
 #pragma unroll
-            for (int i = 0; i < P::MT; ++i) {
-                const int v = vw + 16 * i;
-                f32x4 d;
+            for (int i = 0; i < P::MT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float y = exp2_raw((acc[i][j][e] - lse) * kLog2e);
-                    d[e] = gl * (hit == 16 * i + e ? y - 1.0f : y);
-                    if (!inside && v + e >= a.vocab) d[e] = 0.0f;
+                    acc[i][j][e] = gl * (hit == 16 * i + e ? y - 1.0f : y);
+                    if (!inside && vw + 16 * i + e >= a.vocab) acc[i][j][e] = 0.0f;
                 }
-                u32x2 t[NT];
-                if constexpr (NT == 1) {
-                    // D rounded to nearest: half a step of each term of the sums that read it, as
-                    // independent as the logits are, so less than their own bf16 result's
-                    t[0][0] = from_float<uint16_t>(d[0]) | (uint32_t)from_float<uint16_t>(d[1]) << 16;
-                    t[0][1] = from_float<uint16_t>(d[2]) | (uint32_t)from_float<uint16_t>(d[3]) << 16;
-                } else {
-                    split4(d, t);
-                }
+        }
+        const int n0 = n * P::BN + wave % P::WN * (P::BN / P::WN);
+        const int m0 = m * P::BM + wave / P::WN * (P::BM / P::WM);
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
-                    *reinterpret_cast<u32x2*>(out + (size_t)x * a.rows * p.w.piece + (v - v0)) = t[x];
-            }
+        for (int t = 0; t < NT; ++t) {
+            uint16_t* out = p.at<uint16_t>(p.w.d_at) + ((size_t)t * a.rows + n0) * p.w.piece + m0;
+            store_part<P>(
+                lds,
+                [&](int i, int j) {
+                    // One term: rounded to nearest, half a step of each term of the sums that read it, as
+                    // independent as the logits are, so no more than their own bf16 result's.
+                    if constexpr (NT == 1) return round4(acc[i][j]);
+                    u32x2 x[1];
+                    split4(acc[i][j], x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float y = acc[i][j][e];
+                        cut(y);
+                        acc[i][j][e] = y;
+                    }
+                    return x[0];
+                },
+                [&](int row, int v, u32x4 x) {
+                    if (n0 + row < count) *reinterpret_cast<u32x4*>(out + (size_t)row * p.w.piece + v) = x;
+                });
         }
     } else {
-        __syncthreads();  // the tiles in LDS have been read
         float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
         for (int j = 0; j < P::NT; ++j) {
@@ -578,29 +613,24 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_los
     clear(acc);
     const Operand d{p.at<uint16_t>(p.w.d_at), p.w.piece, (int64_t)a.rows * p.w.piece, count, p.w.piece};
     P::run(states_of(a, p, count), d, m * P::BM, n * P::BN, 0, (count + LHL_STEP - 1) / LHL_STEP, p.zeros(), lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int hw = m * P::BM + wave / P::WN * (P::BM / P::WM) + 4 * g;
-    const int vw = v0 + n * P::BN + wave % P::WN * (P::BN / P::WN) + c;
-#pragma unroll
-    for (int j = 0; j < P::NT; ++j) {
-        const int v = vw + 16 * j;
-        if (v >= a.vocab) continue;
-        uint16_t* out = a.grad_table + (int64_t)v * a.grad_table_row;
-#pragma unroll
-        for (int i = 0; i < P::MT; ++i) {
-            const int h = hw + 16 * i;
-            uint16_t x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = from_float<uint16_t>(acc[i][j][e]);
-            if (wide && h + 4 <= a.hidden) {
-                *reinterpret_cast<u32x2*>(out + h) = u32x2{x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
+    const int wave = threadIdx.x >> 6;
+    const int h0 = m * P::BM + wave / P::WN * (P::BM / P::WM);
+    const int vfirst = v0 + n * P::BN + wave % P::WN * (P::BN / P::WN);
+    __syncthreads();  // the tiles in LDS have been read
+    store_part<P>(
+        lds, [&](int i, int j) { return round4(acc[i][j]); },
+        [&](int v, int h, u32x4 x) {
+            if (vfirst + v >= a.vocab) return;
+            h += h0;
+            uint16_t* out = a.grad_table + (int64_t)(vfirst + v) * a.grad_table_row + h;
+            if (wide && h + 8 <= a.hidden) {
+                *reinterpret_cast<u32x4*>(out) = x;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (h + e < a.hidden) out[h + e] = x[e];
+                for (int e = 0; e < 8; ++e)
+                    if (h + e < a.hidden) out[e] = (uint16_t)(x[e / 2] >> (e % 2 * 16));
             }
-        }
-    }
+        });
 }
 
 // ---- launches --------------------------------------------------------------------------
@@ -657,7 +687,7 @@ hipError_t grad_h(const lm_head_loss_args& a, const Parts& p, int v0, int width,
 template <int NT, bool VEC>
 hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
     hipError_t e = prepare<NT>(a, p, true, s);
-    const bool wide = ((uintptr_t)a.grad_table | (uintptr_t)(a.grad_table_row * 2)) % 8 == 0;
+    const bool wide = ((uintptr_t)a.grad_table | (uintptr_t)(a.grad_table_row * 2)) % 16 == 0;
     for (int v0 = 0; v0 < a.vocab && e == hipSuccess; v0 += p.w.piece) {
         const int width = std::min(p.w.piece, a.vocab - v0);
         if (a.rows > 0) e = logits_of<NT, VEC, true>(a, p, v0, width, s);

@@ -18,6 +18,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
+import struct
 from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 from typing import Optional, Sequence
@@ -89,6 +91,10 @@ class gdn_dev_args(ctypes.Structure):
         ("rows", c_int), ("n_seq", c_int), ("n_slots", c_int), ("heads_k", c_int), ("heads_v", c_int),
         ("dim_k", c_int), ("dim_v", c_int), ("dtype", c_int), ("scale", c_float),
     ]
+
+
+# gdn_dev_args in one packing: its 26 fields set one by one take longer than a short kernel
+_GDN_PACK = struct.Struct("@11PN5q8if4x")
 
 
 class lm_head_loss_args(ctypes.Structure):
@@ -571,22 +577,24 @@ class SweepPlan:
 _HERE = contextlib.nullcontext()
 
 
-def _same_device(first, **tensors):
+def _same_device(first, *tensors):
     """Every tensor on the device of `first`, a GPU; a context that makes it current."""
-    cuda = _torch().cuda
-    device = first.device
-    if device.type != "cuda":
+    device = first.get_device()
+    if device < 0:
         raise ValueError("the tensors have to be on a GPU")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-    return _HERE if device.index == cuda.current_device() else cuda.device(device)
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor of shape {tuple(t.shape)} is on {t.device}, not on {first.device}")
+    cuda = _torch().cuda
+    return _HERE if device == cuda.current_device() else cuda.device(device)
 
 
 def _rows_of(t, name, shape, dtype):
     """t of this shape and type, each of its rows contiguous -> the stride between rows."""
     if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name} has to be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    if t.is_contiguous():
+        return math.prod(shape[1:])
     stride, step = t.stride(), 1
     for n, s in zip(shape[:0:-1], stride[:0:-1]):
         if n != 1 and s != step:
@@ -604,30 +612,34 @@ def _flat(t, name, shape, dtype):
         raise ValueError(f"{name} has to be a contiguous {tuple(shape)} of {dtype}")
 
 
-def _gdn_args(q, k, v, alpha, beta, scale, states, slots, out):
-    """The arguments that both forms of the attention share."""
+def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out):
+    """The arguments of either form of the attention."""
     torch = _torch()
-    if q.dim() != 3 or v.dim() != 3 or q.dtype not in (torch.float32, torch.bfloat16):
+    dtype = q.dtype
+    if q.dim() != 3 or v.dim() != 3 or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("q, k, v are [rows, heads, dim] in float32 or bfloat16")
-    rows, hk, dk = q.shape
-    hv, dv = v.shape[1:]
-    keys, values, gates, dtype = (rows, hk, dk), (rows, hv, dv), (rows, hv), q.dtype
-    n_slots = None
-    at = {}
-    for name, t in states.items():
-        if t is not None:
-            n_slots = t.shape[0] if n_slots is None else n_slots
-            _flat(t, name, (n_slots, hv, dk * dv), torch.float32)
-            at[name] = t.data_ptr()
+    rows, hk, dk = keys = q.shape
+    _, hv, dv = values = torch.Size((rows, *v.shape[1:]))
+    gates = torch.Size((rows, hv))
+    n_slots = state_out.shape[0]
+    _flat(state_out, "state_out", (n_slots, hv, dk * dv), torch.float32)
+    if state_in is not None and state_in is not state_out:
+        _flat(state_in, "state_in", (n_slots, hv, dk * dv), torch.float32)
+    if slots is None:
+        if n_slots < n_seq:
+            raise ValueError("fewer states than sequences")
+    else:
+        _flat(slots, "slots", (n_seq,), torch.int32)
     gate_row = _rows_of(alpha, "alpha", gates, torch.float32)
     if beta is not None and _rows_of(beta, "beta", gates, torch.float32) != gate_row:
         raise ValueError("alpha and beta have to have the same row stride")
-    return gdn_dev_args(
-        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), alpha.data_ptr(),
-        None if beta is None else beta.data_ptr(), at.get("state_in"), at.get("state_out"),
-        None if slots is None else slots.data_ptr(), None, None, 0, _rows_of(q, "q", keys, dtype),
-        _rows_of(k, "k", keys, dtype), _rows_of(v, "v", values, dtype), _rows_of(out, "out", values, dtype), gate_row,
-        rows, 0, n_slots, hk, hv, dk, dv, QWEN_F32 if dtype == torch.float32 else QWEN_BF16, scale)
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    return gdn_dev_args.from_buffer_copy(_GDN_PACK.pack(
+        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), alpha.data_ptr(), at(beta), at(state_in),
+        state_out.data_ptr(), at(slots), at(starts), at(work), 0 if work is None else work.numel() * work.element_size(),
+        _rows_of(q, "q", keys, dtype), _rows_of(k, "k", keys, dtype), _rows_of(v, "v", values, dtype),
+        _rows_of(out, "out", values, dtype), gate_row, rows, n_seq, n_slots, hk, hv, dk, dv,
+        QWEN_F32 if dtype == torch.float32 else QWEN_BF16, scale))
 
 
 def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0, state_in=None, state_out=None,
@@ -645,30 +657,23 @@ def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0
     linear_attention_prompt_work_bytes, for callers that keep one.  The rest is
     gdn_dev_prompt's contract (include/qwen_kernels.h)."""
     torch = _torch()
-    with _same_device(q, k=k, v=v, alpha=alpha, beta=beta, starts=starts, state_in=state_in, state_out=state_out,
-                      slots=slots, out=out, work=work):
+    with _same_device(q, k, v, alpha, beta, starts, state_in, state_out, slots, out, work):
         n_seq = 1 if starts is None else starts.numel() - 1
         if starts is not None:
             _flat(starts, "starts", (max(n_seq, 0) + 1,), torch.int32)
-        if slots is not None:
-            _flat(slots, "slots", (n_seq,), torch.int32)
         if out is None:
             out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         if state_out is None:
             if slots is not None:
                 raise ValueError("slots need a state_out that holds them")
             state_out = torch.empty(n_seq, v.shape[1], q.shape[2] * v.shape[2], dtype=torch.float32, device=q.device)
-        a = _gdn_args(q, k, v, alpha, beta, scale, {"state_in": state_in, "state_out": state_out}, slots, out)
-        if slots is None and a.n_slots < n_seq:
-            raise ValueError("fewer states than sequences")
-        a.starts = None if starts is None else _dp(starts)
-        a.n_seq = n_seq
+        a = _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out)
         lib = load()
-        need = lib.gdn_dev_prompt_work_bytes(a)
-        if need and work is None:
-            work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        if work is not None:
-            a.work, a.work_bytes = _dp(work), work.numel() * work.element_size()
+        if work is None:
+            need = lib.gdn_dev_prompt_work_bytes(a)
+            if need:
+                work = torch.empty(need, dtype=torch.uint8, device=q.device)
+                a.work, a.work_bytes = work.data_ptr(), need
         check(lib.gdn_dev_prompt(a, _stream()), "linear_attention_prompt")
     return out, state_out
 
@@ -688,16 +693,10 @@ def linear_attention_step(q, k, v, alpha, beta, state, *, scale=1.0, slots=None,
     """One token for each sequence: row s of q, k, v updates the state in slot
     slots[s] (None: s) of `state` in place -> out.  Types and layouts as in
     linear_attention_prompt; gdn_dev_step (include/qwen_kernels.h)."""
-    torch = _torch()
-    with _same_device(q, k=k, v=v, alpha=alpha, beta=beta, state=state, slots=slots, out=out):
-        if slots is not None:
-            _flat(slots, "slots", (q.shape[0],), torch.int32)
+    with _same_device(q, k, v, alpha, beta, state, slots, out):
         if out is None:
-            out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        a = _gdn_args(q, k, v, alpha, beta, scale, {"state_in": state, "state_out": state}, slots, out)
-        if slots is None and a.n_slots < a.rows:
-            raise ValueError("fewer states than sequences")
-        a.n_seq = a.rows
+            out = _torch().empty(v.shape, dtype=v.dtype, device=v.device)
+        a = _gdn_args(q, k, v, alpha, beta, scale, state, state, slots, None, q.shape[0], None, out)
         check(load().gdn_dev_step(a, _stream()), "linear_attention_step")
     return out
 
@@ -738,7 +737,7 @@ def lm_head_loss(h, table, targets, *, work=None):
     gives NaN.  work: uint8 scratch of at least lm_head_loss_work_bytes.  The rest
     is bf16_dev_lm_head_loss's contract (include/qwen_kernels.h)."""
     torch = _torch()
-    with _same_device(h, table=table, targets=targets, work=work):
+    with _same_device(h, table, targets, work):
         a = _loss_args(h, table, targets)
         loss, lse = torch.empty(2, a.rows, dtype=torch.float32, device=h.device)
         a.loss, a.lse = _dp(loss), _dp(lse)
@@ -752,8 +751,7 @@ def lm_head_loss_grad(h, table, targets, lse, grad_loss, *, need_h=True, need_ta
     table's type, overwritten where given; None for one that is not needed.
     lse is lm_head_loss's; grad_loss float32 [rows]."""
     torch = _torch()
-    with _same_device(h, table=table, targets=targets, lse=lse, grad_loss=grad_loss, grad_h=grad_h,
-                      grad_table=grad_table, work=work):
+    with _same_device(h, table, targets, lse, grad_loss, grad_h, grad_table, work):
         a = _loss_args(h, table, targets)
         _flat(lse, "lse", (a.rows,), torch.float32)
         _flat(grad_loss, "grad_loss", (a.rows,), torch.float32)

@@ -313,6 +313,15 @@ def test_graph_stream_and_repeats(gpu):
     assert torch.equal(got[0], out0) and torch.equal(got[1], state0)
 
 
+def test_step_over_a_large_batch(gpu):
+    """States of more than 128 MiB, which pass the caches by."""
+    B = 140
+    q, k, v, al, be, st = inputs(B, 4, 16, 128, 128, BF16, True, B)
+    want, wst = oracle(q, k, v, al, be, 0.5, st, [(i, i + 1) for i in range(B)])
+    near(gpu.linear_attention_step(q, k, v, al, be, st, scale=0.5), want, BF16)
+    near(st, wst)
+
+
 def test_no_sequences_and_no_tokens(gpu):
     q, k, v, al, be, st = inputs(0, 2, 2, 32, 32, F, True, 3)
     out, got = gpu.linear_attention_prompt(q, k, v, al, be, torch.zeros(4, dtype=torch.int32).cuda(), state_in=st)
