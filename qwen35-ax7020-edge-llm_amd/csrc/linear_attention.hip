@@ -11,13 +11,14 @@
 //   O = scale (diag(2^g) Q S0 + P U),           P_ij = 2^(g_i - g_j) q_i.k_j      (j <= i)
 //   S0 <- 2^(g_C) S0 + K^T diag(2^(g_C - g)) U
 // gdn_chunk_kernel makes T = (I + L)^-1 diag(b), P and the decays of every chunk
-// side by side; gdn_scan_kernel takes the state from chunk to chunk, 16 of a
-// head's value columns in a workgroup (the columns do not mix).
+// side by side; gdn_scan_kernel takes the state from chunk to chunk, 16 or 32 of
+// a head's value columns in a workgroup (the columns do not mix).
 //
-// Arithmetic: every product runs on the bf16 matrix cores, a float32 operand as
-// the sum of three bf16 terms (bf16_terms.h), a product of two such sums as the
-// six pairs of terms above 2^-24.  What only a bf16 output sees (S0 in Q S0, P, U in P U) has two
-// terms: 2^-16, against the output's own 2^-9.
+// Arithmetic: every product of the scan, and K K^T and Q K^T, run on the bf16
+// matrix cores, a float32 operand as the sum of three bf16 terms (bf16_terms.h),
+// a product of two such sums as the six pairs of terms above 2^-24.  What only a
+// bf16 output sees (S0 in Q S0, P, U in P U) has two terms: 2^-16, against the
+// output's own 2^-9.
 #include "bf16_terms.h"
 #include "linear_attention.h"
 
@@ -80,6 +81,7 @@ __device__ __forceinline__ int slot_of(const gdn_dev_args& a, int s) {
     const int slot = a.slots[s];
     if (slot < 0 || slot >= a.n_slots) return -1;
     int twice = 0;
+#pragma unroll 8
     for (int i = threadIdx.x & 63; i < s; i += 64) twice |= a.slots[i] == slot;
     return __any(twice) ? -1 : slot;
 }
@@ -174,7 +176,9 @@ __device__ __forceinline__ void sync_lds() {
 // ---- chunks -------------------------------------------------------------------------
 // One chunk of one value head; wavefront w has tokens 16 w .. 16 w + 15.  What it writes is
 // in the order in which gdn_scan_kernel loads it.  direct: that kernel takes K and Q from
-// the inputs.
+// the inputs.  Memory bounds it: K and Q in, 31 KiB of T and P out; at 16,384 tokens of 16
+// heads of 128 in bf16 64 us, 4.1 TB/s.  Inverting (I + L) one column a lane over all 64 rows
+// left three wavefronts idle and took 145; in blocks of 16 all four work.
 template <int KS, int NT, bool kDelta>
 __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n_chunks, int full_q, int full_k,
                                                         int direct) {
@@ -376,6 +380,10 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
 // it some 30 cycles.  The state, the right side and U pass between wavefronts as bf16 terms in LDS, lane by
 // lane (see state_row).  Other fragments of the next chunk are loaded into each register as soon as it
 // is free.
+// The chain bounds it: at one sequence of 16,384 tokens, 16 heads of 128, bf16, 410 us, 1.6 us (3,600 cycles)
+// a chunk, of which the first four wavefronts work 1,100, 720 and 980 cycles between barriers and wait
+// for the others and for skew the rest; at 24 float32 prompts of 9,001 tokens in all 270 us.  The
+// same with four wavefronts that do everything and load for themselves: 1,190 and 620 us.
 template <int KS, int NT, int NC, bool kDelta, bool kDirect, class T>
 __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t n_chunks, int slices) {
     constexpr int NO = NT == 1 ? 2 : 3;
@@ -830,9 +838,9 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
 
 // ---- one token ------------------------------------------------------------------------
 // With the old state S: u = b (v - a S^T k), out = scale (a S^T q + (k.q) u), S <- a S + k u^T:
-// one pass over the state, whose bytes bound it.  A wavefront has COLS / 4 groups of
-// four value columns; lane 4 g + l has rows 4 (g + 16 n) .. + 3 of column l of each, one
-// 16-byte load and store each, 1 KiB a wavefront.
+// one pass over the state, whose bytes bound it (256 sequences of 16 heads of 128: 95 us, 5.7 TB/s).  A
+// wavefront has G groups of four value columns; lane 4 g + l has rows 4 (g + 16 n) .. + 3 of column l of
+// each, one 16-byte load and store each, 1 KiB a wavefront.
 // kStream: past the caches, for states that would not be found there again.
 template <int NI, int G, bool kStream, class T>
 __global__ __launch_bounds__(256) void gdn_step_kernel(gdn_dev_args a, int groups) {

@@ -12,6 +12,12 @@
 //   lhl_grad_table_kernel  h^T D
 // and lhl_loss_kernel / lhl_finish_kernel join the parts.  Every sum has one fixed
 // order: results repeat bit for bit.
+//
+// What bounds it.  Few rows: the table's bytes (one row of 65536 x 1024: 25 us of 26
+// at the rate of a copy).  Many: the matrix cores (4096 rows: the logits and their
+// statistics 470 us, 1.17 PFLOP/s; a library product of that shape alone 533).  The
+// gradient computes the logits again, in pieces of the vocabulary: 4096 rows, 3277 of
+// them counted, for each of four pieces 135 us of logits and D, 137 of grad_h, 108 of grad_table.
 #include "bf16_terms.h"
 #include "lm_head_loss.h"
 
@@ -642,6 +648,21 @@ hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStr
     return hipGetLastError();
 }
 
+// Vocabulary rows and counted rows of a tile of logits.  Up to 32 rows take tiles of 128 x 32, which leave two
+// workgroups of three stages a compute unit (one row: 25 us); up to 64 of 256 x 64 (48 float32 rows: 33 us, in
+// tiles of 128 x 64 45); many bf16 ones of 256 x 256 (4096: 515 us, in tiles of 128 x 128 550), whose operands
+// are the fewest bytes of LDS a product; the others, and float32's three terms, of 128 x 128.
+struct TileOf {
+    int vocab, rows;
+};
+template <int NT, bool VEC>
+TileOf tile_for(int rows) {
+    if (rows <= 32) return {128, 32};
+    if (rows <= 64) return {VEC ? 256 : 128, 64};
+    if (NT == 1 && VEC && rows >= 1024) return {256, 256};
+    return {128, 128};
+}
+
 template <int BM, int BN, int NT, bool VEC, bool kGrad>
 hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
     constexpr int WN = BN == 256 ? 4 : BN == 128 ? 2 : 1, WM = (BM == 256 ? 8 : 4) / WN;
@@ -655,12 +676,11 @@ hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width,
 
 template <int NT, bool VEC, bool kGrad>
 hipError_t logits_of(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
-    if (a.rows <= 32) return logits<128, 32, NT, VEC, kGrad>(a, p, v0, width, s);
-    if constexpr (VEC)
-        if (a.rows <= 64) return logits<256, 64, NT, VEC, kGrad>(a, p, v0, width, s);
-    if (a.rows <= 64) return logits<128, 64, NT, VEC, kGrad>(a, p, v0, width, s);
+    const TileOf t = tile_for<NT, VEC>(a.rows);
+    if (t.rows == 32) return logits<128, 32, NT, VEC, kGrad>(a, p, v0, width, s);
+    if (t.rows == 64) return logits<VEC ? 256 : 128, 64, NT, VEC, kGrad>(a, p, v0, width, s);
     if constexpr (NT == 1 && VEC)
-        if (a.rows >= 1024) return logits<256, 256, NT, VEC, kGrad>(a, p, v0, width, s);
+        if (t.rows == 256) return logits<256, 256, NT, VEC, kGrad>(a, p, v0, width, s);
     return logits<128, 128, NT, VEC, kGrad>(a, p, v0, width, s);
 }
 
@@ -669,8 +689,7 @@ hipError_t loss(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
     hipError_t e = prepare<NT>(a, p, false, s);
     if (e == hipSuccess) e = logits_of<NT, VEC, false>(a, p, 0, a.vocab, s);
     if (e != hipSuccess) return e;
-    const int tiles = VEC && ((NT == 1 && a.rows >= 1024) || (a.rows > 32 && a.rows <= 64)) ? (a.vocab + 255) / 256
-                                                                                             : p.w.vtiles;
+    const int tile = tile_for<NT, VEC>(a.rows).vocab, tiles = (a.vocab + tile - 1) / tile;
     lhl_loss_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s>>>(a, p, tiles);
     return hipGetLastError();
 }
@@ -695,7 +714,7 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
             e = a.rows <= 64 ? grad_h<64, NT, VEC>(a, p, v0, width, s) : grad_h<128, NT, VEC>(a, p, v0, width, s);
         if (e == hipSuccess && a.grad_table) {
             constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 2^-16 of its terms
-            if (NT == 1 && a.rows >= 1024) {
+            if (NT == 1 && a.rows >= 1024) {  // (4096 rows' piece 111 us, in tiles of 128 x 128 128)
                 using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
                 const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
                 lhl_grad_table_kernel<P>
