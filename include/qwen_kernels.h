@@ -504,9 +504,11 @@ void bfp8_plan_destroy(void* plan);
  * without tokens has its state copied.  Rows that no sequence holds are neither
  * read nor written.
  *
- * dim_k, dim_v: multiples of 4 up to 256; heads_v a multiple of heads_k; alpha
- * in [0, 1] (0 forgets the state), any beta.  state_in, state_out and work are
- * 16-byte aligned, the others aligned to their elements.  A NaN or infinity in a
+ * dim_k, dim_v: multiples of 4 up to 256; heads_v a multiple of heads_k, up to
+ * 65536; n_seq heads_v ceil(dim_v / 16) up to 2^22 and (rows / 64 + n_seq) heads_v
+ * up to 2^23; alpha in [0, 1] (0 forgets the state), any beta.  state_in, state_out
+ * and work are 16-byte aligned, the others aligned to their elements.  out overlaps
+ * nothing that the call reads.  A NaN or infinity in a
  * token gives NaN or infinite values in that sequence and head from that
  * chunk of 64 tokens on, and nowhere else.
  *
@@ -565,8 +567,9 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  * caller's (calls that may overlap need one each).  Table rows that are 16-byte
  * aligned (pointer, stride, and hidden a multiple of 8) are streamed through LDS;
  * others are read through registers, more slowly.  hidden up to 65536, vocab up to
- * 2^28, rows up to 2^20, table_row up to 2^22.  Nothing is allocated and nothing waits: the calls can
- * be captured. */
+ * 2^28, rows up to 2^20, ceil(vocab / 128) ceil(rows / 32) up to 2^25, table_row up
+ * to 2^22.  The results overlap nothing that the call reads.  Nothing is allocated
+ * and nothing waits: the calls can be captured. */
 typedef struct lm_head_loss_args {
     float* loss;
     float* lse;

@@ -4,7 +4,6 @@
 // state of the library is used.
 #include <hip/hip_runtime.h>
 
-#include <climits>
 #include <mutex>
 
 #include "host_internal.h"
@@ -37,9 +36,10 @@ const char* gdn_sizes(const gdn_dev_args* a) {
         a->dim_v % 4)
         return "dim_k and dim_v are multiples of 4 up to 256";
     if (a->rows < 0 || a->n_seq < 0 || a->n_slots < 0) return "rows, n_seq or n_slots below 0";
-    if ((size_t)a->n_seq * a->heads_v * ((a->dim_v + 3) / 4) > INT_MAX ||
-        ((size_t)a->rows / GDN_CHUNK + a->n_seq) * a->heads_v > INT_MAX)
-        return "too many sequences and heads for one call";
+    // a launch has fewer than 2^32 threads: 576 for 16 value columns of a sequence and head, 256 for a chunk and head
+    if ((size_t)a->n_seq * a->heads_v * ((a->dim_v + 15) / 16) > 1 << 22 ||
+        ((size_t)a->rows / GDN_CHUNK + a->n_seq) * a->heads_v > 1 << 23)
+        return "too many sequences, rows and heads for one call";
     return nullptr;
 }
 
@@ -66,7 +66,8 @@ const char* loss_sizes(const lm_head_loss_args* a) {
     if (a->rows < 0 || a->rows > 1 << 20) return "rows are 0 to 2^20";
     if (a->vocab < 1 || a->vocab > 1 << 28) return "vocab is 1 to 2^28";
     if (a->hidden < 1 || a->hidden > 65536) return "hidden is 1 to 65536";
-    if ((size_t)((a->vocab + LHL_TILE - 1) / LHL_TILE) * (size_t)((a->rows + 31) / 32) > INT_MAX / 16)
+    // a launch has fewer than 2^32 threads: 256 for a tile of 128 vocabulary rows and 32 or (above 64 rows) 128 rows
+    if ((size_t)((a->vocab + LHL_TILE - 1) / LHL_TILE) * (size_t)((a->rows + 31) / 32) > 1 << 25)
         return "too many logits for one call";
     return nullptr;
 }

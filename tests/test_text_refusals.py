@@ -36,7 +36,8 @@ def loss(**over):
 
 SIZES = [dict(dtype=2), dict(dtype=-1), dict(heads_k=0), dict(heads_v=3), dict(heads_v=1), dict(dim_k=0), dict(dim_k=66),
          dict(dim_k=260), dict(dim_v=2), dict(dim_v=512), dict(rows=-1), dict(n_seq=-1), dict(n_slots=-1),
-         dict(heads_k=1, heads_v=65540), dict(n_seq=1 << 30, rows=1 << 30)]
+         dict(heads_k=1, heads_v=65540), dict(n_seq=1 << 30, rows=1 << 30),
+         dict(n_seq=(1 << 18) + 1, rows=(1 << 18) + 1), dict(heads_k=16, heads_v=16, n_seq=4, rows=1 << 25)]
 POINTERS = [dict(state_out=None), dict(state_out=P + 4), dict(state_in=P + 8), dict(out=None), dict(q=None), dict(k=None),
             dict(v=None), dict(alpha=None), dict(q=P + 2), dict(out=P + 1, dtype=1), dict(alpha=P + 2), dict(beta=P + 1),
             dict(slots=P + 2), dict(q_row=64), dict(v_row=100), dict(out_row=0), dict(gate_row=2), dict(k_row=-256)]
@@ -70,8 +71,8 @@ def test_linear_attention_refuses_its_forms_own():
 
 @pytest.mark.parametrize("over", [
     dict(dtype=3), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(vocab=0), dict(vocab=(1 << 28) + 1), dict(hidden=0),
-    dict(hidden=65537), dict(rows=1 << 20, vocab=1 << 28), dict(table=None), dict(table=P + 1), dict(table_row=63),
-    dict(table_row=(1 << 22) + 1), dict(h=None), dict(targets=None), dict(h=P + 2), dict(targets=P + 2), dict(loss=P + 1),
+    dict(hidden=65537), dict(rows=1 << 20, vocab=1 << 28), dict(rows=2048, vocab=1 << 27), dict(table=None),
+    dict(table=P + 1), dict(table_row=63), dict(table_row=(1 << 22) + 1), dict(h=None), dict(targets=None), dict(h=P + 2), dict(targets=P + 2), dict(loss=P + 1),
     dict(lse=P + 2), dict(h_row=10), dict(work=None), dict(work=P + 16), dict(work_bytes=100)])
 def test_loss_refuses(over):
     lib = qk.load()
