@@ -314,20 +314,22 @@ struct Parts {
 };
 
 // ---- the rows that count ---------------------------------------------------------------
-// 16 rows, a part of their columns to a workgroup, which counts the rows before its own by itself:
-// four bytes a row, next to the 2 KiB and more of a row's state.
+// `runs` runs of 16 rows, a part of their columns to a workgroup, which counts the rows before its own by
+// itself: four bytes a row, next to the 2 KiB and more of a row's state.  Up to 512 workgroups along the rows,
+// so that what they count stays small (the loss of 2^20 rows over 1000 x 1024: 3.8 ms, with a workgroup for
+// every 16 rows 19).
 constexpr int kPrepRows = 16;
 template <int NT>
-__global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, bool grad) {
+__global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, int runs, bool grad) {
     __shared__ int before_sh[4], local[kPrepRows], kept_sh;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r0 = blockIdx.x * kPrepRows;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first_row = blockIdx.x * runs * kPrepRows;
     auto counts = [&](int r) {
         const int t = a.targets[r];
         return t >= 0 && t < a.vocab;
     };
     int before = 0;
 #pragma unroll 8
-    for (int r = threadIdx.x; r < r0; r += 256) before += counts(r);
+    for (int r = threadIdx.x; r < first_row; r += 256) before += counts(r);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
     if (lane == 0) before_sh[wave] = before;
@@ -335,63 +337,68 @@ __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, P
     if (first && blockIdx.x == 0 && threadIdx.x < 64) reinterpret_cast<uint32_t*>(p.work + 256)[threadIdx.x] = 0;
     __syncthreads();
     before = before_sh[0] + before_sh[1] + before_sh[2] + before_sh[3];
-    if (wave == 0) {
-        const int r = r0 + lane;
-        const bool in = lane < kPrepRows && r < a.rows, kept = in && counts(r);
-        const uint64_t all = __ballot(kept);
-        const int mine = __popcll(all & ((1ull << lane) - 1)), c = before + mine;
-        if (kept) local[mine] = r;
-        if (first && kept) {
-            p.at<int>(p.w.rows_at)[c] = r;
-            p.at<int>(p.w.target_at)[c] = a.targets[r];
-            if (grad) {
-                p.at<float>(p.w.lse_at)[c] = a.lse[r];
-                p.at<float>(p.w.gl_at)[c] = a.grad_loss[r];
-            }
-        } else if (first && in && !grad) {
-            const float x = a.targets[r] < 0 ? 0.0f : __builtin_nanf("");
-            if (a.loss) a.loss[r] = x;
-            if (a.lse) a.lse[r] = x;
-        }
-        if (first && in) p.at<int>(p.w.place_at)[r] = kept ? c : a.targets[r] < 0 ? -1 : -2;
-        if (lane == 0) {
-            kept_sh = __popcll(all);
-            if (first && r0 + kPrepRows >= a.rows) *reinterpret_cast<int*>(p.work) = before + __popcll(all);
-        }
-    }
-    __syncthreads();
-    const int kept = kept_sh;
     uint16_t* out = p.at<uint16_t>(p.w.h_at);
     // this workgroup's parts of eight columns
     const int parts = p.w.pitch / 8, e0 = parts * blockIdx.y / gridDim.y, n = parts * (blockIdx.y + 1) / gridDim.y - e0;
-    for (int u = threadIdx.x; u < kept * n; u += 256) {
-        const int i = u / n, e = 8 * (e0 + u % n), c = before + i;
-        const int64_t src = (int64_t)local[i] * a.h_row + e;
-        u32x4 t[NT];
-        if constexpr (NT == 1) {
-            const uint16_t* h = static_cast<const uint16_t*>(a.h) + src;
-            if (e + 8 <= a.hidden) {
-                __builtin_memcpy(&t[0], h, 16);
-            } else {
-                t[0] = u32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (e + j < a.hidden) t[0][j / 2] |= (uint32_t)h[j] << (j % 2 * 16);
+    for (int run = 0; run < runs; ++run) {
+        const int r0 = first_row + run * kPrepRows;
+        if (wave == 0) {
+            const int r = r0 + lane;
+            const bool in = lane < kPrepRows && r < a.rows, kept = in && counts(r);
+            const uint64_t all = __ballot(kept);
+            const int mine = __popcll(all & ((1ull << lane) - 1)), c = before + mine;
+            if (kept) local[mine] = r;
+            if (first && kept) {
+                p.at<int>(p.w.rows_at)[c] = r;
+                p.at<int>(p.w.target_at)[c] = a.targets[r];
+                if (grad) {
+                    p.at<float>(p.w.lse_at)[c] = a.lse[r];
+                    p.at<float>(p.w.gl_at)[c] = a.grad_loss[r];
+                }
+            } else if (first && in && !grad) {
+                const float x = a.targets[r] < 0 ? 0.0f : __builtin_nanf("");
+                if (a.loss) a.loss[r] = x;
+                if (a.lse) a.lse[r] = x;
             }
-        } else {
-            const float* h = static_cast<const float*>(a.h) + src;
-            float x[8];
-            if (e + 8 <= a.hidden) {
-                __builtin_memcpy(x, h, 32);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = e + j < a.hidden ? h[j] : 0.0f;
+            if (first && in) p.at<int>(p.w.place_at)[r] = kept ? c : a.targets[r] < 0 ? -1 : -2;
+            if (lane == 0) {
+                kept_sh = __popcll(all);
+                if (first && r0 + kPrepRows >= a.rows) *reinterpret_cast<int*>(p.work) = before + __popcll(all);
             }
-            split8(x, t);
         }
+        __syncthreads();
+        const int kept = kept_sh;
+        for (int u = threadIdx.x; u < kept * n; u += 256) {
+            const int i = u / n, e = 8 * (e0 + u % n), c = before + i;
+            const int64_t src = (int64_t)local[i] * a.h_row + e;
+            u32x4 t[NT];
+            if constexpr (NT == 1) {
+                const uint16_t* h = static_cast<const uint16_t*>(a.h) + src;
+                if (e + 8 <= a.hidden) {
+                    __builtin_memcpy(&t[0], h, 16);
+                } else {
+                    t[0] = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < NT; ++m)
-            *reinterpret_cast<u32x4*>(out + ((size_t)m * a.rows + c) * p.w.pitch + e) = t[m];
+                    for (int j = 0; j < 8; ++j)
+                        if (e + j < a.hidden) t[0][j / 2] |= (uint32_t)h[j] << (j % 2 * 16);
+                }
+            } else {
+                const float* h = static_cast<const float*>(a.h) + src;
+                float x[8];
+                if (e + 8 <= a.hidden) {
+                    __builtin_memcpy(x, h, 32);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = e + j < a.hidden ? h[j] : 0.0f;
+                }
+                split8(x, t);
+            }
+#pragma unroll
+            for (int m = 0; m < NT; ++m)
+                *reinterpret_cast<u32x4*>(out + ((size_t)m * a.rows + c) * p.w.pitch + e) = t[m];
+        }
+        before += kept;
+        __syncthreads();  // local and kept_sh have been read
     }
 }
 
@@ -643,8 +650,8 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_los
 template <int NT>
 hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStream_t s) {
     const unsigned columns = std::min(4, p.w.pitch / LHL_STEP);
-    lhl_prepare_kernel<NT>
-        <<<dim3((unsigned)std::max(1, (a.rows + kPrepRows - 1) / kPrepRows), columns), 256, 0, s>>>(a, p, grad);
+    const int blocks = std::max(1, (a.rows + kPrepRows - 1) / kPrepRows), runs = (blocks + 511) / 512;
+    lhl_prepare_kernel<NT><<<dim3((unsigned)((blocks + runs - 1) / runs), columns), 256, 0, s>>>(a, p, runs, grad);
     return hipGetLastError();
 }
 

@@ -103,6 +103,13 @@ def test_several_pieces_of_the_vocabulary(gpu, dtype, rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("rows", [8193, 16400])
+def test_many_rows(gpu, rows, dtype):
+    """More rows than the workgroups that gather them have at a time, whose last run is not full."""
+    check_all(gpu, *inputs(rows, 40, 72, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
 def test_ignored_rows_hold_anything(gpu, dtype):
     h, table, t, gl = inputs(90, 300, 96, dtype)
     t[3], t[50], t[89] = 300, 2 ** 31 - 1, -1
