@@ -490,7 +490,8 @@ void bfp8_plan_destroy(void* plan);
  * gdn_dev_prompt: sequence s is rows starts[s] .. starts[s + 1] - 1 (device
  * array of n_seq + 1 ascending values within 0 .. rows; NULL: n_seq is 1 and
  * the sequence is every row), of any length, none included.  Chunks of 64
- * tokens in two launches, whose work buffer is gdn_dev_prompt_work_bytes() of
+ * tokens in two launches (a third where sequences of up to 16 tokens go token by
+ * token), whose work buffer is gdn_dev_prompt_work_bytes() of
  * device memory, 16-byte aligned, the caller's (calls that may overlap need one
  * each).  gdn_dev_step: sequence s is row s (rows == n_seq; starts and work are
  * not used).

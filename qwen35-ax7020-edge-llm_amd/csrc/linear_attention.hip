@@ -180,8 +180,8 @@ __device__ __forceinline__ void sync_lds() {
 // heads of 128 in bf16 64 us, 4.1 TB/s.  Inverting (I + L) one column a lane over all 64 rows
 // left three wavefronts idle and took 145; in blocks of 16 all four work.
 template <int KS, int NT, bool kDelta>
-__global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n_chunks, int full_q, int full_k,
-                                                        int direct) {
+__global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n_chunks, int short_to, int full_q,
+                                                        int full_k, int direct) {
     constexpr int NO = NT == 1 ? 2 : 3, KP = 32 * KS + 8;
     __shared__ __attribute__((aligned(16))) uint16_t ksh[NT][C][KP];  // K, a row a token
     __shared__ __attribute__((aligned(16))) float lsh[kDelta ? C : 1][C + 4];
@@ -208,6 +208,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
     }
     int first, len;
     span(a, seq, first, len);
+    if (len <= short_to) return;
     const long c = (long)chunk - (first / C + seq);
     if (c < 0 || c * C >= len) return;
     const int row0 = first + (int)c * C, n = min(C, len - (int)c * C);
@@ -385,7 +386,8 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
 // for the others and for skew the rest; at 24 float32 prompts of 9,001 tokens in all 270 us.  The
 // same with four wavefronts that do everything and load for themselves: 1,190 and 620 us.
 template <int KS, int NT, int NC, bool kDelta, bool kDirect, class T>
-__global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t n_chunks, int slices) {
+__global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t n_chunks, int slices,
+                                                            int short_to) {
     constexpr int NO = NT == 1 ? 2 : 3;
     constexpr int TPW = KS >= 2 ? KS / 2 : 1;
     // chunks in LDS: three where they fit (their copies are on the way for a whole chunk), one where two
@@ -412,10 +414,11 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
     const int heads = a.n_seq * a.heads_v;
     const int sh = blockIdx.x % heads, slice = blockIdx.x / heads;
     const int seq = sh / a.heads_v, hv = sh % a.heads_v, hk = hv / (a.heads_v / a.heads_k);
-    const int slot = slot_of(a, seq);
-    if (slot < 0) return;
     int first, len;
     span(a, seq, first, len);
+    if (len <= short_to) return;
+    const int slot = slot_of(a, seq);
+    if (slot < 0) return;
     const int j0 = 16 * NC * slice + col;  // first value column
     const int nc = (len + C - 1) / C;
     Places at = L::at(a, n_chunks, (size_t)(first / C) + seq, hk, hv);
@@ -836,20 +839,69 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
     each_state([&](const f32x4& s, size_t i) { *reinterpret_cast<f32x4*>(a.state_out + i) = s; });
 }
 
-// ---- one token ------------------------------------------------------------------------
+// ---- token by token -------------------------------------------------------------------
+// A wavefront as four rows of 16 lanes, two registers at a time: what both have in the lower and in the upper
+// half, or in the even and in the odd rows.
+struct Pair {
+    float a, b;
+};
+__device__ __forceinline__ Pair swap32(float x, float y) {  // {x's | y's lower half, x's | y's upper half}
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ Pair swap16(float x, float y) {  // {x's | y's even rows, x's | y's odd rows}
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+template <int N>
+__device__ __forceinline__ float turned(float x) {  // by N lanes in each row
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + N, 15, 15, true));
+}
+// x summed over the 16 lanes of a column (lane % 4): one value in every lane, four the value of its row in each.
+__device__ __forceinline__ float over_lanes(const float (&x)[1]) {
+    Pair p = swap32(x[0], x[0]);
+    p = swap16(p.a + p.b, p.a + p.b);
+    float y = p.a + p.b;
+    y += turned<8>(y);
+    return y + turned<4>(y);
+}
+__device__ __forceinline__ float over_lanes(const float (&x)[4]) {
+    const Pair p = swap32(x[0], x[2]), q = swap32(x[1], x[3]);
+    const Pair r = swap16(p.a + p.b, q.a + q.b);
+    float y = r.a + r.b;
+    y += turned<8>(y);
+    return y + turned<4>(y);
+}
+// The rows' values to every lane.
+__device__ __forceinline__ void to_lanes(float x, float (&y)[1]) { y[0] = x; }
+__device__ __forceinline__ void to_lanes(float x, float (&y)[4]) {
+    const Pair r = swap16(x, x), p = swap32(r.a, r.a), q = swap32(r.b, r.b);
+    y[0] = p.a, y[1] = q.a, y[2] = p.b, y[3] = q.b;
+}
+
 // With the old state S: u = b (v - a S^T k), out = scale (a S^T q + (k.q) u), S <- a S + k u^T:
-// one pass over the state, whose bytes bound it (256 sequences of 16 heads of 128: 95 us, 5.7 TB/s).  A
+// one pass over the state, whose bytes bound one token (256 sequences of 16 heads of 128: 88 us, 6.1 TB/s).  A
 // wavefront has G groups of four value columns; lane 4 g + l has rows 4 (g + 16 n) .. + 3 of column l of
-// each, one 16-byte load and store each, 1 KiB a wavefront.
+// each, one 16-byte load and store each, 1 KiB a wavefront.  The sums over lanes stay in registers, and four
+// columns' share their steps (each by itself, through LDS: 95 us; 16 tokens of 64 sequences 73 us, each by itself 92).
 // kStream: past the caches, for states that would not be found there again.
-template <int NI, int G, bool kStream, class T>
-__global__ __launch_bounds__(256) void gdn_step_kernel(gdn_dev_args a, int groups) {
+// kText: the sequences of up to short_to tokens of a prompt call, the state in registers from token to token
+// and kAhead tokens' rows on their way; else one token a sequence.
+template <int NI, int G, bool kStream, bool kText, class T>
+__global__ __launch_bounds__(256) void gdn_token_kernel(gdn_dev_args a, int groups, int short_to) {
+    constexpr int kAhead = kText ? 4 : 1;
+    using Four = std::conditional_t<sizeof(T) == 2, u32x2, f32x4>;  // four elements as they are in memory
     const int lane = threadIdx.x & 63, l = lane & 3, g = lane >> 2;
     const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);  // (sequence, head, run of G column groups)
     const int runs = (groups + G - 1) / G, per_seq = a.heads_v * runs;
-    const int seq = unit / per_seq;
+    const int seq = __builtin_amdgcn_readfirstlane(unit / per_seq);
     if (seq >= a.n_seq) return;
-    const int hv = unit % per_seq / runs, jg0 = unit % runs * G;
+    const int hv = __builtin_amdgcn_readfirstlane(unit % per_seq / runs), jg0 = unit % runs * G;
+    int first = seq, len = 1;
+    if (kText) {
+        span(a, seq, first, len);
+        if (len > short_to) return;
+    }
     const int slot = slot_of(a, seq);
     if (slot < 0) return;
     const int hk = hv / (a.heads_v / a.heads_k);
@@ -867,69 +919,101 @@ __global__ __launch_bounds__(256) void gdn_step_kernel(gdn_dev_args a, int group
                 S[m][n] = kStream ? __builtin_nontemporal_load(at) : *at;
             }
         }
-    const T* q = static_cast<const T*>(a.q) + (int64_t)seq * a.q_row + (int64_t)hk * a.dim_k;
-    const T* k = static_cast<const T*>(a.k) + (int64_t)seq * a.k_row + (int64_t)hk * a.dim_k;
-    const T* v = static_cast<const T*>(a.v) + (int64_t)seq * a.v_row + (int64_t)hv * a.dim_v;
-    const float al = a.alpha[(int64_t)seq * a.gate_row + hv];
-    const float be = a.beta ? a.beta[(int64_t)seq * a.gate_row + hv] : 0.0f;
-    f32x4 kf[NI], qf[NI];
-    float qk = 0.0f;
+    // the column that this lane has a token's v and output of: in a row of lanes that of the row's group
+    const int group = jg0 + (G == 4 ? g >> 2 : 0), col = 4 * min(group, groups - 1) + l;
+    const bool writes = (G == 4 ? g & 3 : g) == 0 && group < groups;
+    struct Token {
+        Four k[NI], q[NI];
+        T v;
+        float al, be;
+    } tok[kAhead];
+    auto load = [&](int t, Token& x) {
+        const int64_t row = first + (kText ? min(t, len - 1) : 0);
+        const T* q = static_cast<const T*>(a.q) + row * a.q_row + (int64_t)hk * a.dim_k;
+        const T* k = static_cast<const T*>(a.k) + row * a.k_row + (int64_t)hk * a.dim_k;
+        const T* v = static_cast<const T*>(a.v) + row * a.v_row + (int64_t)hv * a.dim_v;
 #pragma unroll
-    for (int n = 0; n < NI; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = 4 * (g + 16 * n) + e;
-            kf[n][e] = i < a.dim_k ? to_float<T>(k[i]) : 0.0f;
-            qf[n][e] = i < a.dim_k ? to_float<T>(q[i]) : 0.0f;
-            qk = __builtin_fmaf(kf[n][e], qf[n][e], qk);
+        for (int n = 0; n < NI; ++n) {
+            const int i = 4 * min(g + 16 * n, ng - 1);
+            __builtin_memcpy(&x.k[n], k + i, sizeof(Four));
+            __builtin_memcpy(&x.q[n], q + i, sizeof(Four));
         }
-    float vj[G];
-#pragma unroll
-    for (int m = 0; m < G; ++m) vj[m] = jg0 + m < groups ? to_float<T>(v[4 * (jg0 + m) + l]) : 0.0f;
-    auto over_rows = [](float x) {  // the sum over the 16 lanes of a column, in each
-        x += __shfl_xor(x, 4);
-        x += __shfl_xor(x, 8);
-        x += __shfl_xor(x, 16);
-        return x + __shfl_xor(x, 32);
+        x.v = v[col];
+        x.al = a.alpha[row * a.gate_row + hv];
+        x.be = a.beta ? a.beta[row * a.gate_row + hv] : 0.0f;
     };
-    qk = over_rows(qk);
-    float kv[G], qs[G];
+    auto four = [&](const Four& x, int n) {
+        f32x4 y;
+        if constexpr (sizeof(T) == 2)
+            y = f32x4{__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xffff0000u), __uint_as_float(x[1] << 16),
+                      __uint_as_float(x[1] & 0xffff0000u)};
+        else
+            y = x;
+        return g + 16 * n < ng ? y : f32x4{0, 0, 0, 0};
+    };
+    auto take = [&](int t, const Token& x) {
+        f32x4 kf[NI], qf[NI];
+        float qk[1] = {0.0f}, kv[G], qs[G];
 #pragma unroll
-    for (int m = 0; m < G; ++m) {
-        kv[m] = qs[m] = 0.0f;
+        for (int n = 0; n < NI; ++n) {
+            kf[n] = four(x.k[n], n);
+            qf[n] = four(x.q[n], n);
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
+            for (int e = 0; e < 4; ++e) qk[0] = __builtin_fmaf(kf[n][e], qf[n][e], qk[0]);
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                kv[m] = __builtin_fmaf(S[m][n][e], kf[n][e], kv[m]);
-                qs[m] = __builtin_fmaf(S[m][n][e], qf[n][e], qs[m]);
-            }
-    }
+        for (int m = 0; m < G; ++m) {
+            kv[m] = qs[m] = 0.0f;
 #pragma unroll
-    for (int m = 0; m < G; ++m) {
-        qs[m] = over_rows(qs[m]);
-        float u = vj[m];
-        if (a.beta) u = be * (u - al * over_rows(kv[m]));
-        if (jg0 + m < groups) {
-            if (g == 0)
-                static_cast<T*>(a.out)[(int64_t)seq * a.out_row + (int64_t)hv * a.dim_v + 4 * (jg0 + m) + l] =
-                    from_float<T>(a.scale * __builtin_fmaf(qk, u, al * qs[m]));
+            for (int n = 0; n < NI; ++n)
 #pragma unroll
-            for (int n = 0; n < NI; ++n) {
-                const int ig = g + 16 * n;
-                if (ig < ng) {
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(kf[n][e], u, al * S[m][n][e]);
-                    f32x4* at = reinterpret_cast<f32x4*>(a.state_out + head_state) + ((jg0 + m) * ng + ig) * 4 + l;
-                    if (kStream)
-                        __builtin_nontemporal_store(x, at);
-                    else
-                        *at = x;
+                for (int e = 0; e < 4; ++e) {
+                    kv[m] = __builtin_fmaf(S[m][n][e], kf[n][e], kv[m]);
+                    qs[m] = __builtin_fmaf(S[m][n][e], qf[n][e], qs[m]);
                 }
+        }
+        float u = to_float<T>(x.v), us[G];
+        if (a.beta) u = x.be * (u - x.al * over_lanes(kv));
+        const float o = a.scale * __builtin_fmaf(over_lanes(qk), u, x.al * over_lanes(qs));
+        if (writes) static_cast<T*>(a.out)[(int64_t)(first + t) * a.out_row + (int64_t)hv * a.dim_v + col] = from_float<T>(o);
+        to_lanes(u, us);
+#pragma unroll
+        for (int m = 0; m < G; ++m)
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[m][n][e] = __builtin_fmaf(kf[n][e], us[m], x.al * S[m][n][e]);
+    };
+    if constexpr (kText) {
+        if (len > 0) {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) load(j, tok[j]);
+            for (int t = 0; t < len; t += kAhead) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (t + j < len) {
+                        take(t + j, tok[j]);
+                        load(t + j + kAhead, tok[j]);
+                    }
             }
         }
+    } else {
+        load(0, tok[0]);
+        take(0, tok[0]);
     }
+#pragma unroll
+    for (int m = 0; m < G; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int ig = g + 16 * n;
+            if (jg0 + m < groups && ig < ng) {
+                f32x4* at = reinterpret_cast<f32x4*>(a.state_out + head_state) + ((jg0 + m) * ng + ig) * 4 + l;
+                if (kStream)
+                    __builtin_nontemporal_store(S[m][n], at);
+                else
+                    *at = S[m][n];
+            }
+        }
 }
 
 bool rows_of_16(const void* p, int64_t row, int dim, int es) {
@@ -937,7 +1021,7 @@ bool rows_of_16(const void* p, int64_t row, int dim, int es) {
 }
 
 template <int KS, int NT, bool kDelta>
-hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
+hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, int short_to, hipStream_t s) {
     using T = std::conditional_t<NT == 1, uint16_t, float>;
     const int es = NT == 1 ? 2 : 4;
     const bool full_q = a.dim_k == 32 * KS && rows_of_16(a.q, a.q_row, a.dim_k, es);
@@ -946,12 +1030,12 @@ hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s)
                         a.k_row < 1 << 24 && a.v_row < 1 << 24;  // (offsets of 64 rows in 32 bits)
     if (a.rows > 0)
         gdn_chunk_kernel<KS, NT, kDelta>
-            <<<dim3((unsigned)(w.n_chunks * a.heads_v)), 256, 0, s>>>(a, w.n_chunks, full_q, full_k, direct);
+            <<<dim3((unsigned)(w.n_chunks * a.heads_v)), 256, 0, s>>>(a, w.n_chunks, short_to, full_q, full_k, direct);
     auto scan = [&](auto nc, auto from_inputs) {
         constexpr int NC = decltype(nc)::value;
         const int slices = (a.dim_v + 16 * NC - 1) / (16 * NC);
         gdn_scan_kernel<KS, NT, NC, kDelta, decltype(from_inputs)::value, T>
-            <<<dim3((unsigned)((size_t)a.n_seq * a.heads_v * slices)), 576, 0, s>>>(a, w.n_chunks, slices);
+            <<<dim3((unsigned)((size_t)a.n_seq * a.heads_v * slices)), 576, 0, s>>>(a, w.n_chunks, slices, short_to);
     };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, KS <= 4 ? 2 : 1>;
@@ -968,48 +1052,67 @@ hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s)
 }
 
 template <int KS>
-hipError_t launch_prompt_of(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
+hipError_t launch_prompt_of(const gdn_dev_args& a, const GdnWork& w, int short_to, hipStream_t s) {
     if (a.dtype == QWEN_BF16)
-        return a.beta ? launch_prompt<KS, 1, true>(a, w, s) : launch_prompt<KS, 1, false>(a, w, s);
-    return a.beta ? launch_prompt<KS, 3, true>(a, w, s) : launch_prompt<KS, 3, false>(a, w, s);
+        return a.beta ? launch_prompt<KS, 1, true>(a, w, short_to, s) : launch_prompt<KS, 1, false>(a, w, short_to, s);
+    return a.beta ? launch_prompt<KS, 3, true>(a, w, short_to, s) : launch_prompt<KS, 3, false>(a, w, short_to, s);
 }
 
-template <int NI, int G, bool kStream>
-hipError_t launch_step(const gdn_dev_args& a, hipStream_t s) {
+template <int NI, int G, bool kStream, bool kText>
+hipError_t launch_tokens(const gdn_dev_args& a, int short_to, hipStream_t s) {
     const int groups = a.dim_v / 4;
     const size_t units = (size_t)a.n_seq * a.heads_v * ((groups + G - 1) / G);
     const dim3 grid((unsigned)((units + 3) / 4));
     if (a.dtype == QWEN_BF16)
-        gdn_step_kernel<NI, G, kStream, uint16_t><<<grid, 256, 0, s>>>(a, groups);
+        gdn_token_kernel<NI, G, kStream, kText, uint16_t><<<grid, 256, 0, s>>>(a, groups, short_to);
     else
-        gdn_step_kernel<NI, G, kStream, float><<<grid, 256, 0, s>>>(a, groups);
+        gdn_token_kernel<NI, G, kStream, kText, float><<<grid, 256, 0, s>>>(a, groups, short_to);
     return hipGetLastError();
 }
 
-template <int G, bool kStream>
-hipError_t launch_step_of(const gdn_dev_args& a, hipStream_t s) {
-    if (a.dim_k <= 64) return launch_step<1, G, kStream>(a, s);
-    if (a.dim_k <= 128) return launch_step<2, G, kStream>(a, s);
-    return launch_step<4, G, kStream>(a, s);
+template <int G, bool kStream, bool kText>
+hipError_t launch_tokens_of(const gdn_dev_args& a, int short_to, hipStream_t s) {
+    if (a.dim_k <= 64) return launch_tokens<1, G, kStream, kText>(a, short_to, s);
+    if (a.dim_k <= 128) return launch_tokens<2, G, kStream, kText>(a, short_to, s);
+    return launch_tokens<4, G, kStream, kText>(a, short_to, s);
+}
+
+// Token by token: every sequence's one (kText false), or those sequences of a prompt call that have up to
+// short_to.
+template <bool kText>
+hipError_t tokens(const gdn_dev_args& a, int short_to, hipStream_t s) {
+    // Four value columns a wavefront while there are few, to have more of them at work: 4 | 8 | 16 sequences of
+    // 16 heads of 128 3.6 | 4.9 | 7.3 us, and 16 tokens of each 12.7 | 23 | 41; sixteen columns, four loads in
+    // flight a lane and as many sums over the lanes for four times the columns: 3.8 | 4.6 | 6.4 and 14 | 19 | 26.
+    if ((size_t)a.n_seq * a.heads_v * a.dim_v <= 8192) return launch_tokens_of<1, false, kText>(a, short_to, s);
+    // States of 128 MiB and more, with other layers' before they are next wanted, are not left in the 256 MiB
+    // of last-level cache: 256 sequences in turn over four pools 88 us for 103 (one pool again and again: 87 for 80).
+    if ((size_t)a.n_seq * a.heads_v * a.dim_k * a.dim_v * 4 < (size_t)128 << 20)
+        return launch_tokens_of<4, false, kText>(a, short_to, s);
+    return launch_tokens_of<4, true, kText>(a, short_to, s);
 }
 
 }  // namespace
 
 hipError_t gdn_launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
+    // Sequences of up to 16 tokens go token by token, past the latency of a chunk: one of 16 heads of 128 with
+    // 4 | 16 | 32 tokens in bf16 5.4 | 11 | 18 us, in a chunk 14; 64 of them with 4 | 16 tokens 44 | 73 us, in chunks
+    // 104 | 108.  That is a third launch where longer ones may be in the call too (their lengths are on the
+    // device); it is made if the chunks would go over the chip more than once and the average sequence is that short.
+    constexpr int kShort = 16;
+    const bool many = (size_t)a.n_seq * a.heads_v * ((a.dim_v + 31) / 32) > 256 &&
+                      (size_t)a.rows <= (size_t)kShort * a.n_seq;
+    const int short_to = a.rows <= kShort || many ? kShort : -1;
+    if (short_to >= 0) {
+        const hipError_t e = tokens<true>(a, short_to, s);
+        if (e != hipSuccess || a.rows <= short_to) return e;
+    }
     switch (w.ks) {
-        case 1: return launch_prompt_of<1>(a, w, s);
-        case 2: return launch_prompt_of<2>(a, w, s);
-        case 4: return launch_prompt_of<4>(a, w, s);
-        default: return launch_prompt_of<8>(a, w, s);
+        case 1: return launch_prompt_of<1>(a, w, short_to, s);
+        case 2: return launch_prompt_of<2>(a, w, short_to, s);
+        case 4: return launch_prompt_of<4>(a, w, short_to, s);
+        default: return launch_prompt_of<8>(a, w, short_to, s);
     }
 }
 
-hipError_t gdn_launch_step(const gdn_dev_args& a, hipStream_t s) {
-    // Four value columns a wavefront while there are few, to have more of them at work: 1 | 8 | 16 sequences of
-    // 16 heads of 128 3.3 | 5.3 | 9.4 us; sixteen, four loads in flight a lane: 4.8 | 6.0 | 9.0, and 64 24 for 27.
-    if ((size_t)a.n_seq * a.heads_v * a.dim_v <= 16384) return launch_step_of<1, false>(a, s);
-    // States of 128 MiB and more, with other layers' before they are next wanted, are not left in the 256 MiB
-    // of last-level cache: 256 sequences in turn over four pools 95 us for 107 (one pool again and again: 93 for 85).
-    if ((size_t)a.n_seq * a.heads_v * a.dim_k * a.dim_v * 4 < (size_t)128 << 20) return launch_step_of<4, false>(a, s);
-    return launch_step_of<4, true>(a, s);
-}
+hipError_t gdn_launch_step(const gdn_dev_args& a, hipStream_t s) { return tokens<false>(a, 1, s); }

@@ -131,6 +131,68 @@ def test_prompt(gpu, which, packed, hk, hv, dk, dv, delta, dtype):
     near(got, wst)
 
 
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("hk,hv,dk,dv", SHAPES)
+def test_prompt_of_short_sequences(gpu, hk, hv, dk, dv, delta, dtype):
+    """Sequences that go token by token: a few short ones alone, and many with longer ones between them."""
+    many = 256 // (8 * hv * -(-dv // 32)) + 1
+    for lengths in ([3, 0, 9, 1], [16], [1], [1, 0, 16, 17, 5, 70, 3, 2] * many):
+        spans, starts = spans_of(lengths)
+        q, k, v, al, be, st = inputs(sum(lengths), hk, hv, dk, dv, dtype, delta, len(lengths), packed=len(lengths) > 4)
+        want, wst = oracle(q, k, v, al, be, 0.5, st, spans)
+        out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, scale=0.5, state_in=st)
+        near(out, want, dtype)
+        near(got, wst)
+        _, other = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st, state_out=st, out=out)
+        assert other is st and torch.equal(st, got)
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv", [(2, 64, 16, 32), (16, 16, 128, 128)])
+def test_slots_of_short_sequences(gpu, hk, hv, dk, dv):
+    slots = [5, -1, 0, 9, 5, 2, 1000000, 3]
+    spans, starts = spans_of([12, 10, 0, 16, 3, 1, 2, 30])
+    q, k, v, al, be, st = inputs(spans[-1][1] + 37, hk, hv, dk, dv, F, True, 9)
+    q[spans[1][0]:spans[1][1]] = float("nan")
+    v[spans[-1][1]:] = float("nan")
+    st[7] = float("nan")
+    taken = [s if s < 9 and i != 4 else -1 for i, s in enumerate(slots)]
+    want, wst = oracle(q, k, v, al, be, 1.0, st, spans, taken)
+    out = torch.full(v.shape, float("nan"), device="cuda")
+    before = torch.full_like(st, 7.0)
+    _, state = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st, state_out=before, out=out,
+                                           slots=torch.tensor(slots, dtype=torch.int32).cuda())
+    for i in (1, 4, 6, 7, 8):
+        assert bool((state[i] == 7.0).all())
+        wst[i] = 7.0
+    near(out, want)
+    near(state, wst)
+
+
+def test_short_sequences_in_a_graph(gpu):
+    """Short and long ones in one captured call, replayed; states past 128 MiB; NaN stays with its tokens."""
+    lengths = [4, 16, 1, 0, 30] * 30
+    spans, starts = spans_of(lengths)
+    q, k, v, al, be, st = inputs(sum(lengths), 4, 16, 128, 128, BF16, True, len(lengths))
+    v[spans[1][0] + 7, 3, 5] = float("nan")
+    want, wst = oracle(q, k, v, al, be, 1.0, st, spans)
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    near(out, want, BF16)
+    near(got, wst)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again, state = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    for _ in range(3):
+        again.zero_()
+        state.zero_()
+        graph.replay()
+        other = gpu.linear_attention_step(q[:2], k[:2], v[:2], al[:2], be[:2], st[:2].clone())
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(other).all())
+        assert torch.equal(torch.nan_to_num(again), torch.nan_to_num(out))
+        assert torch.equal(torch.nan_to_num(state), torch.nan_to_num(got))
+
+
 def test_prompt_of_one_sequence_from_zeros(gpu):
     q, k, v, al, be, st = inputs(300, 4, 4, 64, 64, F, True, 1)
     want, wst = oracle(q, k, v, al, be, 1.0, torch.zeros_like(st), [(0, 300)])
