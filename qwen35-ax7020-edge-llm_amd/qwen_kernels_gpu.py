@@ -18,7 +18,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
 import struct
 from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
@@ -594,7 +593,7 @@ def _rows_of(t, name, shape, dtype):
     if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name} has to be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
     if t.is_contiguous():
-        return math.prod(shape[1:])
+        return t.stride()[0]  # (of one row: anything, and not used)
     stride, step = t.stride(), 1
     for n, s in zip(shape[:0:-1], stride[:0:-1]):
         if n != 1 and s != step:
@@ -605,6 +604,12 @@ def _rows_of(t, name, shape, dtype):
     if stride[0] < step:
         raise ValueError(f"{name}: its rows overlap")
     return stride[0]
+
+
+def _like(t):
+    """A contiguous tensor of t's shape and type."""
+    torch = _torch()
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _flat(t, name, shape, dtype):
@@ -619,9 +624,11 @@ def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n
     if q.dim() != 3 or v.dim() != 3 or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("q, k, v are [rows, heads, dim] in float32 or bfloat16")
     rows, hk, dk = keys = q.shape
-    _, hv, dv = values = torch.Size((rows, *v.shape[1:]))
-    gates = torch.Size((rows, hv))
-    n_slots = state_out.shape[0]
+    n_v, hv, dv = values = v.shape
+    if n_v != rows:
+        raise ValueError("q and v have to have the same rows")
+    gates = (rows, hv)
+    n_slots = state_out.size(0)
     _flat(state_out, "state_out", (n_slots, hv, dk * dv), torch.float32)
     if state_in is not None and state_in is not state_out:
         _flat(state_in, "state_in", (n_slots, hv, dk * dv), torch.float32)
@@ -630,16 +637,27 @@ def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n
             raise ValueError("fewer states than sequences")
     else:
         _flat(slots, "slots", (n_seq,), torch.int32)
-    gate_row = _rows_of(alpha, "alpha", gates, torch.float32)
-    if beta is not None and _rows_of(beta, "beta", gates, torch.float32) != gate_row:
-        raise ValueError("alpha and beta have to have the same row stride")
-    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    f32 = torch.float32
+    if (q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and out.is_contiguous() and alpha.is_contiguous()
+            and k.shape == keys and out.shape == values and alpha.shape == gates
+            and k.dtype == dtype and v.dtype == dtype and out.dtype == dtype and alpha.dtype == f32
+            and (beta is None or beta.is_contiguous() and beta.shape == gates and beta.dtype == f32)):
+        q_row = k_row = hk * dk  # (the usual step's, whose host time is its time: without a call for each)
+        v_row = out_row = hv * dv
+        gate_row = hv
+    else:
+        q_row, k_row = _rows_of(q, "q", keys, dtype), _rows_of(k, "k", keys, dtype)
+        v_row, out_row = _rows_of(v, "v", values, dtype), _rows_of(out, "out", values, dtype)
+        gate_row = _rows_of(alpha, "alpha", gates, f32)
+        if beta is not None and _rows_of(beta, "beta", gates, f32) != gate_row and rows > 1:
+            raise ValueError("alpha and beta have to have the same row stride")
     return gdn_dev_args.from_buffer_copy(_GDN_PACK.pack(
-        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), alpha.data_ptr(), at(beta), at(state_in),
-        state_out.data_ptr(), at(slots), at(starts), at(work), 0 if work is None else work.numel() * work.element_size(),
-        _rows_of(q, "q", keys, dtype), _rows_of(k, "k", keys, dtype), _rows_of(v, "v", values, dtype),
-        _rows_of(out, "out", values, dtype), gate_row, rows, n_seq, n_slots, hk, hv, dk, dv,
-        QWEN_F32 if dtype == torch.float32 else QWEN_BF16, scale))
+        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), alpha.data_ptr(),
+        0 if beta is None else beta.data_ptr(), 0 if state_in is None else state_in.data_ptr(), state_out.data_ptr(),
+        0 if slots is None else slots.data_ptr(), 0 if starts is None else starts.data_ptr(),
+        0 if work is None else work.data_ptr(), 0 if work is None else work.numel() * work.element_size(),
+        q_row, k_row, v_row, out_row, gate_row, rows, n_seq, n_slots, hk, hv, dk, dv,
+        QWEN_F32 if dtype == f32 else QWEN_BF16, scale))
 
 
 def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0, state_in=None, state_out=None,
@@ -662,7 +680,7 @@ def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0
         if starts is not None:
             _flat(starts, "starts", (max(n_seq, 0) + 1,), torch.int32)
         if out is None:
-            out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+            out = _like(v)
         if state_out is None:
             if slots is not None:
                 raise ValueError("slots need a state_out that holds them")
@@ -695,7 +713,7 @@ def linear_attention_step(q, k, v, alpha, beta, state, *, scale=1.0, slots=None,
     linear_attention_prompt; gdn_dev_step (include/qwen_kernels.h)."""
     with _same_device(q, k, v, alpha, beta, state, slots, out):
         if out is None:
-            out = _torch().empty(v.shape, dtype=v.dtype, device=v.device)
+            out = _like(v)
         a = _gdn_args(q, k, v, alpha, beta, scale, state, state, slots, None, q.shape[0], None, out)
         check(load().gdn_dev_step(a, _stream()), "linear_attention_step")
     return out
@@ -756,9 +774,9 @@ def lm_head_loss_grad(h, table, targets, lse, grad_loss, *, need_h=True, need_ta
         _flat(lse, "lse", (a.rows,), torch.float32)
         _flat(grad_loss, "grad_loss", (a.rows,), torch.float32)
         if need_h and grad_h is None:
-            grad_h = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+            grad_h = _like(h)
         if need_table and grad_table is None:
-            grad_table = torch.empty(table.shape, dtype=table.dtype, device=h.device)
+            grad_table = _like(table)
         a.lse, a.grad_loss = _dp(lse), _dp(grad_loss)
         if need_h:
             a.grad_h, a.grad_h_row = _dp(grad_h), _rows_of(grad_h, "grad_h", h.shape, h.dtype)

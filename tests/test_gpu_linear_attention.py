@@ -308,6 +308,20 @@ def test_in_place_states_and_strided_gates(gpu):
     assert bool((wide[:, 2] == 5.0).all())
 
 
+def test_step_of_parts_of_rows(gpu):
+    """Whole tensors and parts of a projection's rows give the same; one row's gates may lie anywhere."""
+    for rows in (1, 3):
+        q, k, v, al, be, st = inputs(rows, 2, 4, 64, 32, F, True, rows, packed=False)
+        want = gpu.linear_attention_step(q.contiguous(), k.contiguous(), v.contiguous(), al, be, st.clone())
+        gates = torch.cat([al, be, al], 1)
+        assert torch.equal(gpu.linear_attention_step(q, k, v, gates[:, :4], gates[:, 4:8], st.clone()), want)
+        if rows == 1:
+            assert torch.equal(gpu.linear_attention_step(q, k, v, al, gates[:, 4:8], st.clone()), want)
+        else:
+            with pytest.raises(ValueError, match="stride"):
+                gpu.linear_attention_step(q, k, v, al, gates[:, 4:8], st.clone())
+
+
 @pytest.mark.parametrize("dtype", [F, BF16])
 def test_nan_stays_in_its_sequence_head_and_time(gpu, dtype):
     q, k, v, al, be, st = inputs(400, 2, 2, 64, 64, dtype, True, 2)
