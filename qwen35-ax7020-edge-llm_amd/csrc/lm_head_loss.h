@@ -55,15 +55,21 @@ inline LossWork loss_work(const lm_head_loss_args& a, bool grad, bool grad_h) {
         w.part_at = put(8 * n * w.vtiles);
     } else {
         // pieces whose gradients stay under 128 MiB: they and their part of the table fit the 256 MiB
-        // last-level cache that they are read from again (4096 bf16 rows: 1.52 ms; 256 or 512 MiB 1.59)
+        // last-level cache that they are read from again (4096 bf16 rows: 1.52 ms; 256 or 512 MiB 1.59); powers
+        // of two, whose tiles go over the chip a whole number of times (4096 float32 rows: 4096 columns
+        // 4.8 ms, the 5120 that fit 5.8)
         const size_t whole = ((size_t)a.vocab + LHL_WIDE - 1) / LHL_WIDE * LHL_WIDE;
-        const size_t fit = ((size_t)128 << 20) / (2 * std::max<size_t>(n, 1) * w.terms) / 1024 * 1024;
-        w.piece = (int)std::min(whole, std::max<size_t>(fit, 1024));
+        size_t fit = 1024;
+        while (fit < whole && 2 * fit * 2 * n * w.terms <= (size_t)128 << 20) fit *= 2;
+        w.piece = (int)std::min(whole, fit);
         w.d_at = put(2 * n * w.terms * w.piece);
         if (grad_h) {
-            const size_t tiles = std::max<size_t>(1, (size_t)((w.pitch + 127) / 128) * ((n + 127) / 128));
+            // one tile's sum over the vocabulary split into as many as run at a time, once over the chip
+            const bool wide = w.terms == 3 && n > 64;  // (256 x 128, one a compute unit, else 128 x 128 or 64, two)
+            const size_t bm = wide ? 256 : 128, at_once = wide ? 256 : 512;
+            const size_t tiles = std::max<size_t>(1, (w.pitch + bm - 1) / bm * ((n + 127) / 128));
             const size_t steps = (size_t)w.piece / LHL_STEP;
-            w.splits = (int)std::max<size_t>(1, std::min(steps / 4, (512 + tiles - 1) / tiles));
+            w.splits = (int)std::max<size_t>(1, std::min(steps / 4, at_once / tiles));
             w.sum_at = put(4 * n * w.splits * w.pitch);
         }
     }

@@ -617,7 +617,7 @@ __global__ __launch_bounds__(256) void lhl_finish_kernel(lm_head_loss_args a, Pa
 // grad_table for vocabulary rows v0 .. v0 + width: tiles of h x vocabulary.
 template <class P>
 __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_loss_args a, Parts p, int v0, int tm,
-                                                                      int tn, int wide) {
+                                                                      int tn) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
     int m, n;
     if (!tile_of(tm, tn, m, n)) return;
@@ -636,8 +636,8 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_los
             if (vfirst + v >= a.vocab) return;
             h += h0;
             uint16_t* out = a.grad_table + (int64_t)(vfirst + v) * a.grad_table_row + h;
-            if (wide && h + 8 <= a.hidden) {
-                *reinterpret_cast<u32x4*>(out) = x;
+            if (h + 8 <= a.hidden) {
+                __builtin_memcpy(out, &x, 16);  // (rows may start at any element)
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -658,15 +658,19 @@ hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStr
 // Vocabulary rows and counted rows of a tile of logits.  Up to 32 rows take tiles of 128 x 32, which leave two
 // workgroups of three stages a compute unit (one row: 25 us); up to 64 of 256 x 64 (48 float32 rows: 33 us, in
 // tiles of 128 x 64 45); many bf16 ones of 256 x 256 (4096: 515 us, in tiles of 128 x 128 550), whose operands
-// are the fewest bytes of LDS a product; the others, and float32's three terms, of 128 x 128.
+// are the fewest bytes of LDS a product; the others of 128 x 128, but float32's three terms of 256 x 128 where
+// there is more than one such for a compute unit, whose LDS either fills: with eight wavefronts in place of
+// four (4096 x 65536 x 1024: 1.28 ms for 1.67; 200 x 3000 45 us for 37).
 struct TileOf {
     int vocab, rows;
 };
+bool more_than_units(size_t tiles) { return tiles > 256; }
 template <int NT, bool VEC>
-TileOf tile_for(int rows) {
+TileOf tile_for(int rows, int width) {
     if (rows <= 32) return {128, 32};
     if (rows <= 64) return {VEC ? 256 : 128, 64};
     if (NT == 1 && VEC && rows >= 1024) return {256, 256};
+    if (NT == 3 && more_than_units((size_t)((width + 127) / 128) * ((rows + 127) / 128))) return {256, 128};
     return {128, 128};
 }
 
@@ -683,11 +687,13 @@ hipError_t logits(const lm_head_loss_args& a, const Parts& p, int v0, int width,
 
 template <int NT, bool VEC, bool kGrad>
 hipError_t logits_of(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
-    const TileOf t = tile_for<NT, VEC>(a.rows);
+    const TileOf t = tile_for<NT, VEC>(a.rows, width);
     if (t.rows == 32) return logits<128, 32, NT, VEC, kGrad>(a, p, v0, width, s);
     if (t.rows == 64) return logits<VEC ? 256 : 128, 64, NT, VEC, kGrad>(a, p, v0, width, s);
     if constexpr (NT == 1 && VEC)
         if (t.rows == 256) return logits<256, 256, NT, VEC, kGrad>(a, p, v0, width, s);
+    if constexpr (NT == 3)
+        if (t.vocab == 256) return logits<256, 128, NT, VEC, kGrad>(a, p, v0, width, s);
     return logits<128, 128, NT, VEC, kGrad>(a, p, v0, width, s);
 }
 
@@ -696,36 +702,44 @@ hipError_t loss(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
     hipError_t e = prepare<NT>(a, p, false, s);
     if (e == hipSuccess) e = logits_of<NT, VEC, false>(a, p, 0, a.vocab, s);
     if (e != hipSuccess) return e;
-    const int tile = tile_for<NT, VEC>(a.rows).vocab, tiles = (a.vocab + tile - 1) / tile;
+    const int tile = tile_for<NT, VEC>(a.rows, a.vocab).vocab, tiles = (a.vocab + tile - 1) / tile;
     lhl_loss_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s>>>(a, p, tiles);
     return hipGetLastError();
 }
 
-template <int BN, int NT, bool VEC>
+template <int BM, int BN, int NT, bool VEC>
 hipError_t grad_h(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
-    using P = Product<128, BN, BN == 128 ? 2 : 4, BN / 64, true, false, 1, NT, 3, VEC, 2>;
-    const int tm = (p.w.pitch + 127) / 128, tn = (a.rows + BN - 1) / BN;
+    using P = Product<BM, BN, BN == 128 ? BM / 64 : 4, BN / 64, true, false, 1, NT, 3, VEC, 2>;
+    const int tm = (p.w.pitch + BM - 1) / BM, tn = (a.rows + BN - 1) / BN;
     lhl_grad_h_kernel<P>
         <<<dim3(tile_grid((size_t)tm * tn * p.w.splits)), P::kThreads, 0, s>>>(a, p, v0, width, tm, tn);
     return hipGetLastError();
 }
 
 template <int NT, bool VEC>
+hipError_t grad_h_of(const lm_head_loss_args& a, const Parts& p, int v0, int width, hipStream_t s) {
+    if (a.rows <= 64) return grad_h<128, 64, NT, VEC>(a, p, v0, width, s);
+    if constexpr (NT == 3)  // as for the logits (4096 rows' piece of 4096 columns 99 us)
+        if (more_than_units((size_t)((p.w.pitch + 127) / 128) * ((a.rows + 127) / 128) * p.w.splits))
+            return grad_h<256, 128, NT, VEC>(a, p, v0, width, s);
+    return grad_h<128, 128, NT, VEC>(a, p, v0, width, s);
+}
+
+template <int NT, bool VEC>
 hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
     hipError_t e = prepare<NT>(a, p, true, s);
-    const bool wide = ((uintptr_t)a.grad_table | (uintptr_t)(a.grad_table_row * 2)) % 16 == 0;
     for (int v0 = 0; v0 < a.vocab && e == hipSuccess; v0 += p.w.piece) {
         const int width = std::min(p.w.piece, a.vocab - v0);
         if (a.rows > 0) e = logits_of<NT, VEC, true>(a, p, v0, width, s);
         if (e == hipSuccess && a.grad_h && a.rows > 0)
-            e = a.rows <= 64 ? grad_h<64, NT, VEC>(a, p, v0, width, s) : grad_h<128, NT, VEC>(a, p, v0, width, s);
+            e = grad_h_of<NT, VEC>(a, p, v0, width, s);
         if (e == hipSuccess && a.grad_table) {
             constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 2^-16 of its terms
             if (NT == 1 && a.rows >= 1024) {  // (4096 rows' piece 111 us, in tiles of 128 x 128 128)
                 using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
                 const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
                 lhl_grad_table_kernel<P>
-                    <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+                    <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn);
                 e = hipGetLastError();
                 continue;
             }
@@ -733,10 +747,10 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
             const dim3 grid(tile_grid((size_t)tm * tn));
             if (a.rows <= LHL_STEP) {  // one step: its LDS for two workgroups more
                 using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 1>;
-                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
-            } else {
-                using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 2>;
-                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn, wide);
+                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn);
+            } else {  // (two terms' LDS leaves one workgroup a compute unit: of eight wavefronts)
+                using P = Product<128, 128, N2 == 2 ? 4 : 2, 2, true, true, N2, N2, N2, true, 2>;
+                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn);
             }
             e = hipGetLastError();
         }

@@ -103,6 +103,13 @@ def test_several_pieces_of_the_vocabulary(gpu, dtype, rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("rows,vocab,hidden", [(130, 20001, 520), (130, 20001, 513), (200, 17000, 257), (65, 33000, 264)])
+def test_more_tiles_than_compute_units(gpu, rows, vocab, hidden, dtype):
+    """Float32 states' wide tiles, with the last ones cut in each direction; table rows at odd elements."""
+    check_all(gpu, *inputs(rows, vocab, hidden, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
 @pytest.mark.parametrize("rows", [8193, 16400])
 def test_many_rows(gpu, rows, dtype):
     """More rows than the workgroups that gather them have at a time, whose last run is not full."""
