@@ -684,13 +684,15 @@ def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0
         if state_out is None:
             if slots is not None:
                 raise ValueError("slots need a state_out that holds them")
-            state_out = torch.empty(n_seq, v.shape[1], q.shape[2] * v.shape[2], dtype=torch.float32, device=q.device)
+            if q.dim() != 3 or v.dim() != 3:
+                raise ValueError("q, k, v are [rows, heads, dim]")
+            state_out = alpha.new_empty((n_seq, v.size(1), q.size(2) * v.size(2)), dtype=torch.float32)
         a = _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out)
         lib = load()
         if work is None:
             need = lib.gdn_dev_prompt_work_bytes(a)
             if need:
-                work = torch.empty(need, dtype=torch.uint8, device=q.device)
+                work = q.new_empty(need, dtype=torch.uint8)
                 a.work, a.work_bytes = work.data_ptr(), need
         check(lib.gdn_dev_prompt(a, _stream()), "linear_attention_prompt")
     return out, state_out
@@ -734,13 +736,12 @@ def _loss_args(h, table, targets):
     return a
 
 
-def _loss_call(name, a, work, device):
+def _loss_call(name, a, work, h):
     """Runs entry point `name` with the caller's work or a new one."""
-    torch = _torch()
     lib = load()
     need = getattr(lib, name + "_work_bytes")(a)
     if need and work is None:
-        work = torch.empty(need, dtype=torch.uint8, device=device)
+        work = h.new_empty(need, dtype=_torch().uint8)
     if work is not None:
         a.work, a.work_bytes = _dp(work), work.numel() * work.element_size()
     check(getattr(lib, name)(a, _stream()), name)
@@ -757,9 +758,9 @@ def lm_head_loss(h, table, targets, *, work=None):
     torch = _torch()
     with _same_device(h, table, targets, work):
         a = _loss_args(h, table, targets)
-        loss, lse = torch.empty(2, a.rows, dtype=torch.float32, device=h.device)
+        loss, lse = h.new_empty((2, a.rows), dtype=torch.float32)
         a.loss, a.lse = _dp(loss), _dp(lse)
-        _loss_call("bf16_dev_lm_head_loss", a, work, h.device)
+        _loss_call("bf16_dev_lm_head_loss", a, work, h)
     return loss, lse
 
 
@@ -783,7 +784,7 @@ def lm_head_loss_grad(h, table, targets, lse, grad_loss, *, need_h=True, need_ta
         if need_table:
             a.grad_table = _dp(grad_table)
             a.grad_table_row = _rows_of(grad_table, "grad_table", table.shape, table.dtype)
-        _loss_call("bf16_dev_lm_head_loss_grad", a, work, h.device)
+        _loss_call("bf16_dev_lm_head_loss_grad", a, work, h)
     return grad_h if need_h else None, grad_table if need_table else None
 
 
