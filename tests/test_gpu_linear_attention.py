@@ -389,6 +389,35 @@ def test_graph_stream_and_repeats(gpu):
     assert torch.equal(got[0], out0) and torch.equal(got[1], state0)
 
 
+@pytest.mark.parametrize("rows,n", [(200, 3), (600, 40), (2000, 40), (700, 70)])
+def test_replays_with_other_lengths(gpu, rows, n):
+    """A captured call reads the lengths when it runs: short for long, long for short, most of them none."""
+    q, k, v, al, be, st = inputs(rows, 4, 8, 64, 64, BF16, True, n)
+    ends = torch.zeros(n + 1, dtype=torch.int32)
+    ends[1:] = torch.arange(1, n + 1) * (rows // n)
+    starts = ends.cuda()
+    gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st)
+    g = torch.Generator().manual_seed(3)
+    for kind in range(4):
+        if kind == 1:
+            ends[1:] = torch.randint(0, rows + 1, (n,), generator=g).sort().values
+        elif kind == 2:
+            ends[1:] = rows
+        elif kind == 3:
+            ends[1:] = torch.arange(1, n + 1)
+        starts.copy_(ends)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        at = ends.tolist()
+        want, wst = oracle(q, k, v, al, be, 1.0, st, list(zip(at[:-1], at[1:])))
+        near(out, want, BF16)
+        near(got, wst)
+
+
 def test_step_over_a_large_batch(gpu):
     """States of more than 128 MiB, which pass the caches by."""
     B = 140
