@@ -552,7 +552,8 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  * has h's type, grad_table is bf16 (gradients are overwritten, not added to);
  * loss, lse, grad_loss: float32.  Row strides in elements.  The products of
  * float32 hidden states keep their 24 bits (three bf16 terms); sums, lse and D are
- * float32, D as an operand bf16 (dtype bf16) or 24 bits (float32).
+ * float32, D as an operand bf16 (dtype bf16, its weights over the call's largest finite
+ * |grad_loss|, so that equal ones are 1) or 24 bits (float32).
  *
  * A row with a target below 0 is ignored, whatever h holds there: loss, lse and
  * its row of grad_h are 0.  A target of vocab or more gives NaN in the three,

@@ -38,7 +38,7 @@ inline LossWork loss_work(const lm_head_loss_args& a, bool grad, bool grad_h) {
     w.terms = a.dtype == QWEN_BF16 ? 1 : 3;
     w.pitch = (a.hidden + LHL_STEP - 1) / LHL_STEP * LHL_STEP;
     w.vtiles = (a.vocab + LHL_TILE - 1) / LHL_TILE;
-    size_t at = 512;  // the count, and a line of zeros
+    size_t at = 512;  // the count, the largest weight, and a line of zeros
     auto put = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;

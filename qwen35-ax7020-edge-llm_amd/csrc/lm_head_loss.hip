@@ -4,6 +4,11 @@
 //   z_nv = w_v . h_n;  lse_n = log sum_v exp z_nv;  loss_n = lse_n - z_n,t_n
 //   D_nv = g_n (exp(z_nv - lse_n) - [v = t_n]);  grad_h = D W;  grad_w = D^T h
 //
+// With bf16 states D is an operand of one bf16 term, and holds g_n over the call's largest |g|, which both gradients
+// are multiplied by in float32.  Under a mean loss, whose weights are all the same, a target's entry is then -1 + p,
+// which bf16 holds almost exactly where p is small; g (-1 + p) would be rounded the same way in every row, by up to
+// 2^-8 that no sum takes out.
+//
 // lhl_prepare_kernel gathers the rows that count (a text's own prompt often does
 // not), as bf16 terms.  The rest are tiled products on the matrix cores:
 //   lhl_logits_kernel    W h^T; its epilogue leaves a tile's maximum and sum of
@@ -310,6 +315,7 @@ struct Parts {
         return reinterpret_cast<T*>(work + offset);
     }
     __device__ int count() const { return *reinterpret_cast<const int*>(work); }
+    __device__ float& top() const { return reinterpret_cast<float*>(work)[1]; }  // the largest weight (bf16 states)
     __device__ const char* zeros() const { return work + 256; }
 };
 
@@ -322,14 +328,26 @@ constexpr int kPrepRows = 16;
 template <int NT>
 __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, int runs, bool grad) {
     __shared__ int before_sh[4], local[kPrepRows], kept_sh;
+    __shared__ float top_sh[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first_row = blockIdx.x * runs * kPrepRows;
     auto counts = [&](int r) {
         const int t = a.targets[r];
         return t >= 0 && t < a.vocab;
     };
+    // the last workgroup looks at every row's target: it finds the largest weight too (of those that are finite)
+    const bool weighs = NT == 1 && grad && blockIdx.x + 1 == gridDim.x && blockIdx.y == 0;
+    auto weight = [&](int r) {
+        const float g = fabsf(a.grad_loss[r]);
+        return g < __builtin_inff() ? g : 0.0f;
+    };
     int before = 0;
+    float top = 0.0f;
 #pragma unroll 8
-    for (int r = threadIdx.x; r < first_row; r += 256) before += counts(r);
+    for (int r = threadIdx.x; r < first_row; r += 256) {
+        const bool kept = counts(r);
+        before += kept;
+        if (weighs) top = fmaxf(top, kept ? weight(r) : 0.0f);
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
     if (lane == 0) before_sh[wave] = before;
@@ -348,6 +366,7 @@ __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, P
             const uint64_t all = __ballot(kept);
             const int mine = __popcll(all & ((1ull << lane) - 1)), c = before + mine;
             if (kept) local[mine] = r;
+            if (weighs && kept) top = fmaxf(top, weight(r));
             if (first && kept) {
                 p.at<int>(p.w.rows_at)[c] = r;
                 p.at<int>(p.w.target_at)[c] = a.targets[r];
@@ -400,6 +419,14 @@ __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, P
         before += kept;
         __syncthreads();  // local and kept_sh have been read
     }
+    if (weighs) {
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        if (lane == 0) top_sh[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(top_sh[0], top_sh[1]), fmaxf(top_sh[2], top_sh[3]));
+        if (threadIdx.x == 0) p.top() = top > 0.0f ? top : 1.0f;
+    }
 }
 
 // ---- logits ---------------------------------------------------------------------------
@@ -408,7 +435,8 @@ __device__ __forceinline__ Operand states_of(const lm_head_loss_args& a, const P
 }
 
 // Tiles of vocabulary x counted rows.  kGrad false: for each row the tile's maximum and sum of
-// exponentials above it (base 2), and the target's logit; true: D for vocabulary rows v0 .. of a piece.
+// exponentials above it (base 2), and the target's logit; true: D for vocabulary rows v0 .. of a piece, with
+// bf16 states (NT 1) over the largest weight.
 template <class P, int NT, bool kGrad>
 __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_args a, Parts p, int v0, int tm, int tn) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
@@ -431,7 +459,9 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
 #pragma unroll
         for (int j = 0; j < P::NT; ++j) {
             const int row = min(nw + 16 * j, count - 1);
-            const float lse = p.at<float>(p.w.lse_at)[row], gl = p.at<float>(p.w.gl_at)[row];
+            const float lse = p.at<float>(p.w.lse_at)[row];
+            float gl = p.at<float>(p.w.gl_at)[row];
+            if (NT == 1) gl /= p.top();
             const int hit = p.at<int>(p.w.target_at)[row] - vw;
 #pragma unroll
             for (int i = 0; i < P::MT; ++i)
@@ -450,8 +480,9 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
             store_part<P>(
                 lds,
                 [&](int i, int j) {
-                    // One term: rounded to nearest, half a step of each term of the sums that read it, as
-                    // independent as the logits are, so no more than their own bf16 result's.
+                    // One term: rounded to nearest, half a step of each term of the sums that read it.  The p's
+                    // are as independent as the logits are; a target's entry, where its row has the largest weight,
+                    // is off by at most 2^-9, and by no more than p where p is below that.
                     if constexpr (NT == 1) return round4(acc[i][j]);
                     u32x2 x[1];
                     split4(acc[i][j], x);
@@ -608,14 +639,15 @@ __global__ __launch_bounds__(256) void lhl_finish_kernel(lm_head_loss_args a, Pa
     __syncthreads();
     if (wave > 0) return;
     x = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+    if (sizeof(T) == 2) x *= p.top();
     T* out = static_cast<T*>(a.grad_h) + (int64_t)row * a.grad_h_row + h;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (h + e < a.hidden) out[e] = from_float<T>(at == -2 ? __builtin_nanf("") : x[e]);
 }
 
-// grad_table for vocabulary rows v0 .. v0 + width: tiles of h x vocabulary.
-template <class P>
+// grad_table for vocabulary rows v0 .. v0 + width: tiles of h x vocabulary.  kTop: D is over the largest weight.
+template <class P, bool kTop>
 __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_loss_args a, Parts p, int v0, int tm,
                                                                       int tn) {
     __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
@@ -629,9 +661,10 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_table_kernel(lm_head_los
     const int wave = threadIdx.x >> 6;
     const int h0 = m * P::BM + wave / P::WN * (P::BM / P::WM);
     const int vfirst = v0 + n * P::BN + wave % P::WN * (P::BN / P::WN);
+    const float top = kTop ? p.top() : 1.0f;
     __syncthreads();  // the tiles in LDS have been read
     store_part<P>(
-        lds, [&](int i, int j) { return round4(acc[i][j]); },
+        lds, [&](int i, int j) { return round4(kTop ? acc[i][j] * top : acc[i][j]); },
         [&](int v, int h, u32x4 x) {
             if (vfirst + v >= a.vocab) return;
             h += h0;
@@ -738,7 +771,7 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
             if (NT == 1 && a.rows >= 1024) {  // (4096 rows' piece 111 us, in tiles of 128 x 128 128)
                 using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
                 const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
-                lhl_grad_table_kernel<P>
+                lhl_grad_table_kernel<P, NT == 1>
                     <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn);
                 e = hipGetLastError();
                 continue;
@@ -747,10 +780,10 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
             const dim3 grid(tile_grid((size_t)tm * tn));
             if (a.rows <= LHL_STEP) {  // one step: its LDS for two workgroups more
                 using P = Product<128, 128, 2, 2, true, true, N2, N2, N2, true, 1>;
-                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn);
+                lhl_grad_table_kernel<P, NT == 1><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn);
             } else {  // (two terms' LDS leaves one workgroup a compute unit: of eight wavefronts)
                 using P = Product<128, 128, N2 == 2 ? 4 : 2, 2, true, true, N2, N2, N2, true, 2>;
-                lhl_grad_table_kernel<P><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn);
+                lhl_grad_table_kernel<P, NT == 1><<<grid, P::kThreads, 0, s>>>(a, p, v0, tm, tn);
             }
             e = hipGetLastError();
         }

@@ -299,3 +299,66 @@ def test_python_refusals(gpu):
             bad()
     with pytest.raises(RuntimeError):
         gpu.lm_head_loss(h, table, t, work=torch.empty(256, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("weights", ["equal", "two", "negative"])
+@pytest.mark.parametrize("rows", [150, 1300])
+def test_weights_do_not_bias_bf16_gradients(gpu, rows, weights):
+    """bf16 states under a mean loss: every row's target has D = -g (1 - p) with the same g, whose rounding no sum
+    takes out.  1.0035 is rounded by 0.0035 of itself as a bf16.
+
+    What is allowed, in the norm of a gradient: a rounding to bf16 is off by at most 2^-8 of the value, and as a
+    uniform error by 2^-8 / sqrt 3 of the values' norm; that is taken for the result and for the terms p of D.
+    A target's entry -1 + p is off by at most min(p, 2^-9); where its row has another weight than the call's largest it
+    is rounded like any number, by up to 2^-8 of itself, in all rows of that weight the same way.  Along the gradient
+    itself independent roundings have a standard deviation of 2^-8 / sqrt 3 over sqrt(elements) for either of the two: 6 of
+    those, the targets' part, and 2^-13 for sums in float32."""
+    V, H = 4000, 128
+    h, table, _, _ = inputs(rows, V, H, BF16, ignored=0.0)
+    table = (table.float() * 0.5).to(BF16)
+    g = torch.Generator().manual_seed(5)
+    t = torch.randperm(V, generator=g)[:rows].to(torch.int32).cuda()  # (each its own row of the table)
+    gl = torch.full((rows,), 1.0035 / 1024)
+    if weights == "two":
+        gl[::3] *= 0.3
+    elif weights == "negative":
+        gl = -gl
+    gl = gl.cuda()
+    _, _, gh, gw, _, _ = oracle(h, table, t, gl)
+    _, lse = gpu.lm_head_loss(h, table, t)
+    got_h, got_w = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+    H64, W, G, T = h.double().cpu(), table.double().cpu(), gl.double().cpu(), t.long().cpu()
+    p = torch.softmax(H64 @ W.t(), 1)
+    off = p[torch.arange(rows), T].clamp(max=2.0 ** -9)
+    off[G.abs() < G.abs().max()] = 2.0 ** -8
+    p[torch.arange(rows), T] = 0.0
+    D2 = (p * G[:, None]) ** 2
+    step = 2.0 ** -8 / 3 ** 0.5
+    for got, want, of_rows, terms, share in ((got_h, gh, gh, D2 @ W ** 2, G.abs() * W[T].norm(dim=1)),
+                                             (got_w, gw, gw[T], D2.t() @ H64 ** 2, G.abs() * H64.norm(dim=1))):
+        got, top = got.double().cpu(), float(want.norm())
+        err = float((got - want).norm())
+        assert err <= step * (top + float(terms.sum()) ** 0.5) + float((off * share).norm()), err / top
+        along = float((got * want).sum()) / top ** 2 - 1
+        targets = float((off * share * of_rows.norm(dim=1)).sum()) / top ** 2
+        assert abs(along) <= 12 * step / want.numel() ** 0.5 + targets + 2.0 ** -13, along
+
+
+def test_weights_at_their_ends(gpu):
+    """bf16 states: weights of 0 alone, far apart, and next to one that is not finite, whose row and table rows alone
+    show it."""
+    h, table, t, gl = inputs(70, 300, 64, BF16, ignored=0.0)
+    _, lse = gpu.lm_head_loss(h, table, t)
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, torch.zeros_like(gl))
+    assert bool((gh == 0).all()) and bool((gw == 0).all())
+    far = gl.clone()
+    far[::2] *= 1e-30
+    far[0] = 0.0
+    check_all(gpu, h, table, t, far)
+    check_all(gpu, h, table, t, gl * 1e-40)  # (subnormal)
+    far[7] = float("inf")
+    gh, gw = gpu.lm_head_loss_grad(h, table, t, lse, far)
+    keep = torch.arange(70, device="cuda") != 7
+    want = gpu.lm_head_loss_grad(h, table, t, lse, torch.where(keep, far, 0.0))[0]
+    assert torch.equal(gh[keep], want[keep]) and not bool(torch.isfinite(gh[7]).any())
+    assert not bool(torch.isfinite(gw).any())  # every p is above 0
