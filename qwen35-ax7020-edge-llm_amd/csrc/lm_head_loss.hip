@@ -768,14 +768,15 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
             e = grad_h_of<NT, VEC>(a, p, v0, width, s);
         if (e == hipSuccess && a.grad_table) {
             constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 2^-16 of its terms
-            if (NT == 1 && a.rows >= 1024) {  // (4096 rows' piece 111 us, in tiles of 128 x 128 128)
-                using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
-                const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
-                lhl_grad_table_kernel<P, NT == 1>
-                    <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn);
-                e = hipGetLastError();
-                continue;
-            }
+            if constexpr (NT == 1)
+                if (a.rows >= 1024) {  // (4096 rows' piece 111 us, in tiles of 128 x 128 128)
+                    using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
+                    const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
+                    lhl_grad_table_kernel<P, true>
+                        <<<dim3(tile_grid((size_t)tm * tn)), P::kThreads, 0, s>>>(a, p, v0, tm, tn);
+                    e = hipGetLastError();
+                    continue;
+                }
             const int tm = (p.w.pitch + 127) / 128, tn = (width + 127) / 128;
             const dim3 grid(tile_grid((size_t)tm * tn));
             if (a.rows <= LHL_STEP) {  // one step: its LDS for two workgroups more
