@@ -16,9 +16,9 @@
 //
 // Arithmetic: every product of the scan, and K K^T and Q K^T, run on the bf16
 // matrix cores, a float32 operand as the sum of three bf16 terms (bf16_terms.h),
-// a product of two such sums as the six pairs of terms above 2^-24.  What only a
-// bf16 output sees (S0 in Q S0, P, U in P U) has two terms: 2^-16, against the
-// output's own 2^-9.
+// a product of two such sums as six pairs of terms: 2^-23.  What only a bf16 output
+// sees (S0 in Q S0, P and U in P U) has two terms, all pairs taken: 2^-16 and 2^-15,
+// against the output's own 2^-8.
 #include "bf16_terms.h"
 #include "linear_attention.h"
 
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                     u32x4 b[NO];
 #pragma unroll
                     for (int m = 0; m < NO; ++m) b[m] = ush[y][ts][m][lane];
-                    o[y] = mfma_terms<NO, NO, NO>(x.p[ts], b, o[y]);
+                    o[y] = mfma_terms<NO, NO, 3>(x.p[ts], b, o[y]);
                 }
             if (kSets == 1) load_p(x);
 #pragma unroll

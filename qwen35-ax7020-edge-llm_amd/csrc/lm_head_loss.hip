@@ -291,8 +291,7 @@ __device__ __forceinline__ void store_part(char* lds, Value&& value, Store&& sto
     asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ u32x2 round4(f32x4 x) {
-    return u32x2{from_float<uint16_t>(x[0]) | (uint32_t)from_float<uint16_t>(x[1]) << 16,
-                 from_float<uint16_t>(x[2]) | (uint32_t)from_float<uint16_t>(x[3]) << 16};
+    return u32x2{round2(x[0], x[1]), round2(x[2], x[3])};
 }
 
 // Tile t of tm x tn: workgroups go round the eight XCDs, so each XCD gets a run of tiles; in a run
@@ -484,15 +483,10 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
                     // are as independent as the logits are; a target's entry, where its row has the largest weight,
                     // is off by at most 2^-9, and by no more than p where p is below that.
                     if constexpr (NT == 1) return round4(acc[i][j]);
-                    u32x2 x[1];
-                    split4(acc[i][j], x);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float y = acc[i][j][e];
-                        cut(y);
-                        acc[i][j][e] = y;
-                    }
-                    return x[0];
+                    float y[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                    const u32x2 x = {take2(y[0], y[1]), take2(y[2], y[3])};
+                    acc[i][j] = f32x4{y[0], y[1], y[2], y[3]};  // (the next term's)
+                    return x;
                 },
                 [&](int row, int v, u32x4 x) {
                     if (n0 + row < count) *reinterpret_cast<u32x4*>(out + (size_t)row * p.w.piece + v) = x;
@@ -767,7 +761,7 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
         if (e == hipSuccess && a.grad_h && a.rows > 0)
             e = grad_h_of<NT, VEC>(a, p, v0, width, s);
         if (e == hipSuccess && a.grad_table) {
-            constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 2^-16 of its terms
+            constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 3 x 2^-16 of its terms
             if constexpr (NT == 1)
                 if (a.rows >= 1024) {  // (4096 rows' piece 111 us, in tiles of 128 x 128 128)
                     using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;

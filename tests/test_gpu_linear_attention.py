@@ -465,3 +465,15 @@ def test_python_refusals(gpu):
         gpu.linear_attention_prompt(q, k, v, al, be, work=torch.empty(16, dtype=torch.uint8, device="cuda"))
     with pytest.raises(RuntimeError):  # 3 key heads do not divide 4 value heads
         step(torch.zeros(4, 3, 32, device="cuda"), torch.zeros(4, 3, 32, device="cuda"), v, al, be, st)
+
+
+def test_products_of_a_state_keep_their_bits(gpu):
+    """One token's k u^T through the chunked form: each element a single product of two float32.  Six pairs of three
+    terms leave out 2^-23 of it, and the sums of the pairs in float32 are allowed a last place, 2^-23."""
+    q, k, v, al, _, _ = inputs(64, 16, 16, 128, 128, F, False, 1)
+    k, v = (3 * torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).cuda() for i, x in enumerate((k, v)))
+    v[:5], v[6:] = 0.0, 0.0
+    _, got = gpu.linear_attention_prompt(q, k, v, torch.ones_like(al))
+    want = k[5].double()[:, :, None] * v[5].double()[:, None, :]
+    off = (unblocked(got, 128, 128)[0].double() - want).abs() / want.abs()
+    assert float(off.max()) <= 2.0 ** -22, float(off.max()) * 2 ** 22
