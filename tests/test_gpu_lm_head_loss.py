@@ -362,3 +362,38 @@ def test_weights_at_their_ends(gpu):
     want = gpu.lm_head_loss_grad(h, table, t, lse, torch.where(keep, far, 0.0))[0]
     assert torch.equal(gh[keep], want[keep]) and not bool(torch.isfinite(gh[7]).any())
     assert not bool(torch.isfinite(gw).any())  # every p is above 0
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,pad,base", [
+    (1025, 2305, 73, 0, 0), (1100, 900, 321, 0, 0), (1030, 1400, 72, 5, 0), (1024, 641, 64, 0, 1), (1111, 2200, 128, 8, 0)])
+def test_many_bf16_rows_and_any_table(gpu, rows, vocab, hidden, pad, base):
+    """bf16 rows enough for wide tiles of grad_table, over table rows at any elements, whose logits' tiles are narrower:
+    columns of D that no tile of logits writes hold what the work buffer held, here NaN.
+
+    Besides the bounds of every element, the gradients' norms: the result's rounding and D's, 2^-8 / sqrt 3 of the
+    norms of values and of terms, and for the targets' entries, which need not be independent, 2^-8 of their sums."""
+    h, table, t, gl = inputs(rows, vocab, hidden, BF16, pad=pad)
+    if base:
+        flat = torch.empty(vocab * hidden + base, dtype=BF16, device="cuda")
+        odd = flat[base:].view(vocab, hidden)
+        odd.copy_(table)
+        table = odd
+    loss, lse, gh, gw, mags_h, mags_w = oracle(h, table, t, gl)
+    nan = lambda **kw: torch.full((gpu.lm_head_loss_work_bytes(rows, vocab, hidden, BF16, **kw),), 255,  # noqa: E731
+                                  dtype=torch.uint8, device="cuda")
+    got_loss, got_lse = gpu.lm_head_loss(h, table, t, work=nan())
+    near(got_loss, loss, 4e-5)
+    got_h, got_w = gpu.lm_head_loss_grad(h, table, t, got_lse, gl, work=nan(grad=True))
+    near(got_h, gh, gh.abs() * 2 ** -8 + 2e-4 * row_top(gh) + mags_h * 2 ** -8)
+    near(got_w, gw, gw.abs() * 2 ** -8 + 2e-4 * row_top(gw) + mags_w * 2 ** -8)
+    keep = (t >= 0).cpu()
+    H, W, T = h.double().cpu()[keep], table.double().cpu(), t.long().cpu()[keep]
+    D = torch.softmax(H @ W.t(), 1) * gl.double().cpu()[keep, None]
+    hit = D[torch.arange(len(T)), T] - gl.double().cpu()[keep]
+    D[torch.arange(len(T)), T] = 0.0
+    step = 2.0 ** -8 / 3 ** 0.5
+    sums = torch.zeros(vocab, hidden, dtype=torch.float64).index_add_(0, T, hit.abs()[:, None] * H.abs())
+    for got, want, terms, targets in ((got_h, gh, D ** 2 @ W ** 2, hit * W[T].norm(dim=1)),
+                                      (got_w, gw, (D ** 2).t() @ H ** 2, sums)):
+        off = float((got.double().cpu() - want).norm())
+        assert off <= step * (float(want.norm()) + float(terms.sum()) ** 0.5) + 2.0 ** -8 * float(targets.norm()), off
