@@ -484,8 +484,12 @@ void bfp8_plan_destroy(void* plan);
  * of dim_k one after the other, v and out heads_v of dim_v, alpha and beta
  * heads_v floats (gate_row between rows); the row strides let them be parts of
  * one projection's row.  q, k, v and out are all float32 or all bf16 (dtype);
- * sums, states and everything between two tokens are float32: in the prompt form
- * matrix operands are sums of bf16 terms that hold a float32's 24 bits.
+ * sums, states and everything between two tokens are float32.  In the prompt form
+ * matrix operands are sums of bf16 terms: three hold a float32's 24 bits, products of
+ * two such sums are off by up to 2^-23 of themselves.  With bf16 tensors what only out
+ * sees of a chunk (the state before it, its decayed q . k, its u) has two terms, 16 bits:
+ * 2^-15 of the products, against out's own 2^-8.  Float32 values of 3.396e38 (bf16's
+ * largest and half a step) or more count as infinite.
  *
  * gdn_dev_prompt: sequence s is rows starts[s] .. starts[s + 1] - 1 (device
  * array of n_seq + 1 ascending values within 0 .. rows; NULL: n_seq is 1 and
@@ -503,7 +507,9 @@ void bfp8_plan_destroy(void* plan);
  * slot of an earlier sequence of the call, is skipped: its rows of out and its
  * slot's state stay as they were but for the earlier sequence's work.  A sequence
  * without tokens has its state copied.  Rows that no sequence holds are neither
- * read nor written.
+ * read nor written.  The search for a slot's earlier sequences grows with the square of
+ * n_seq (4096 sequences of 16 heads of 128: 6 % of a step; 65,536 of 2 heads of 16:
+ * nine times the step): slots NULL does without it.
  *
  * dim_k, dim_v: multiples of 4 up to 256; heads_v a multiple of heads_k, up to
  * 65536; n_seq heads_v ceil(dim_v / 16) up to 2^22 and (rows / 64 + n_seq) heads_v
@@ -512,6 +518,10 @@ void bfp8_plan_destroy(void* plan);
  * nothing that the call reads.  A NaN or infinity in a
  * token gives NaN or infinite values in that sequence and head from that
  * chunk of 64 tokens on, and nowhere else.
+ *
+ * The same call gives the same bits.  In another call they may differ in rounding:
+ * whether a sequence of up to 16 tokens goes token by token, and how many value columns
+ * a workgroup takes, follow from rows, n_seq and the heads of the whole call.
  *
  * Nothing is allocated and nothing waits: the calls can be captured. */
 typedef struct gdn_dev_args {
@@ -551,9 +561,11 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  * h: rows x hidden, float32 or bf16 (dtype); table: vocab x hidden bf16; grad_h
  * has h's type, grad_table is bf16 (gradients are overwritten, not added to);
  * loss, lse, grad_loss: float32.  Row strides in elements.  The products of
- * float32 hidden states keep their 24 bits (three bf16 terms); sums, lse and D are
- * float32, D as an operand bf16 (dtype bf16, its weights over the call's largest finite
- * |grad_loss|, so that equal ones are 1) or 24 bits (float32).
+ * float32 hidden states keep their 24 bits (three bf16 terms) in the logits and in
+ * grad_h; in grad_table, whose results are bf16, they and D have 16 (two terms: 3 x 2^-16
+ * of the products).  Sums, lse and D are float32; D as grad_h's operand is bf16 (dtype
+ * bf16, its weights over the call's largest finite |grad_loss|, so that equal ones are 1)
+ * or has 24 bits (float32).  Float32 states of 3.396e38 or more count as infinite.
  *
  * A row with a target below 0 is ignored, whatever h holds there: loss, lse and
  * its row of grad_h are 0.  A target of vocab or more gives NaN in the three,
