@@ -507,7 +507,8 @@ void bfp8_plan_destroy(void* plan);
  * slot of an earlier sequence of the call, is skipped: its rows of out and its
  * slot's state stay as they were but for the earlier sequence's work.  A sequence
  * without tokens has its state copied.  Rows that no sequence holds are neither
- * read nor written.  The search for a slot's earlier sequences grows with the square of
+ * read nor written.  With zero_rest not 0, rows of out that are skipped or that no
+ * sequence holds are set to 0 instead (n_seq 0: not).  The search for a slot's earlier sequences grows with the square of
  * n_seq (4096 sequences of 16 heads of 128: 6 % of a step; 65,536 of 2 heads of 16:
  * nine times the step): slots NULL does without it.
  *
@@ -542,6 +543,7 @@ typedef struct gdn_dev_args {
     int heads_k, heads_v, dim_k, dim_v;
     int dtype;
     float scale;
+    int zero_rest;
 } gdn_dev_args;
 size_t gdn_dev_prompt_work_bytes(const gdn_dev_args* args); /* 0: invalid sizes */
 int gdn_dev_prompt(const gdn_dev_args* args, void* stream);

@@ -115,6 +115,23 @@ __device__ __forceinline__ int slot_of(const gdn_dev_args& a, int s) {
     return __any(twice) ? -1 : slot;
 }
 
+// Zeros in out's rows first .. end - 1, columns j0 .. j0 + n - 1 of head hv: thread i of threads.
+template <class T>
+__device__ __forceinline__ void zero_rows(const gdn_dev_args& a, int first, int end, int hv, int j0, int n, int i, int threads) {
+    for (size_t u = i; first < end && u < (size_t)(end - first) * n; u += threads) {
+        const int j = j0 + (int)(u % n);
+        if (j < a.dim_v)
+            static_cast<T*>(a.out)[(int64_t)(first + (int)(u / n)) * a.out_row + (int64_t)hv * a.dim_v + j] = T(0);
+    }
+}
+// zero_rest: the rows in front of the first sequence and behind the last, by whoever has that one.
+template <class T>
+__device__ __forceinline__ void zero_ends(const gdn_dev_args& a, int seq, int first, int len, int hv, int j0, int n, int i,
+                                          int threads) {
+    if (seq == 0) zero_rows<T>(a, 0, first, hv, j0, n, i, threads);
+    if (seq == a.n_seq - 1) zero_rows<T>(a, first + len, a.rows, hv, j0, n, i, threads);
+}
+
 // The byte offsets of the work buffer's parts for one chunk.
 struct Places {
     char *k, *q;                 // key head: the image of a KTile, Q fragments [4 row tiles][ks][nt] KiB
@@ -448,6 +465,10 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
     const int hk = hv / (a.heads_v / a.heads_k);
     if (len <= short_to) return;
     const int slot = slot_of(a, seq);
+    if (a.zero_rest) {
+        zero_ends<T>(a, seq, first, len, hv, 16 * NC * slice, 16 * NC, threadIdx.x, 576);
+        if (slot < 0) zero_rows<T>(a, first, first + len, hv, 16 * NC * slice, 16 * NC, threadIdx.x, 576);
+    }
     if (slot < 0) return;
     const int j0 = 16 * NC * slice + col;  // first value column
     const int nc = (len + C - 1) / C;
@@ -933,7 +954,11 @@ __global__ __launch_bounds__(256) void gdn_token_kernel(gdn_dev_args a, int grou
         if (len > short_to) return;
     }
     const int slot = slot_of(a, seq);
-    if (slot < 0) return;
+    if (kText && a.zero_rest) zero_ends<T>(a, seq, first, len, hv, 4 * jg0, 4 * G, lane, 64);
+    if (__builtin_expect(slot < 0, 0)) {  // (out of line: in line a step of one sequence took 15 us for 14)
+        if (a.zero_rest) zero_rows<T>(a, first, first + len, hv, 4 * jg0, 4 * G, lane, 64);
+        return;
+    }
     const int hk = hv / (a.heads_v / a.heads_k);
     const size_t head_state = ((size_t)slot * a.heads_v + hv) * a.dim_k * a.dim_v;
     const int ng = a.dim_k / 4;

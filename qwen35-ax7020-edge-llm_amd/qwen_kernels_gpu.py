@@ -88,12 +88,12 @@ class gdn_dev_args(ctypes.Structure):
         ("starts", c_void_p), ("work", c_void_p), ("work_bytes", c_size_t),
         ("q_row", c_int64), ("k_row", c_int64), ("v_row", c_int64), ("out_row", c_int64), ("gate_row", c_int64),
         ("rows", c_int), ("n_seq", c_int), ("n_slots", c_int), ("heads_k", c_int), ("heads_v", c_int),
-        ("dim_k", c_int), ("dim_v", c_int), ("dtype", c_int), ("scale", c_float),
+        ("dim_k", c_int), ("dim_v", c_int), ("dtype", c_int), ("scale", c_float), ("zero_rest", c_int),
     ]
 
 
-# gdn_dev_args in one packing: its 26 fields set one by one take longer than a short kernel
-_GDN_PACK = struct.Struct("@11PN5q8if4x")
+# gdn_dev_args in one packing: its 27 fields set one by one take longer than a short kernel
+_GDN_PACK = struct.Struct("@11PN5q8ifi")
 
 
 class lm_head_loss_args(ctypes.Structure):
@@ -617,7 +617,7 @@ def _flat(t, name, shape, dtype):
         raise ValueError(f"{name} has to be a contiguous {tuple(shape)} of {dtype}")
 
 
-def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out):
+def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out, zero_rest):
     """The arguments of either form of the attention."""
     torch = _torch()
     dtype = q.dtype
@@ -657,7 +657,7 @@ def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n
         0 if slots is None else slots.data_ptr(), 0 if starts is None else starts.data_ptr(),
         0 if work is None else work.data_ptr(), 0 if work is None else work.numel() * work.element_size(),
         q_row, k_row, v_row, out_row, gate_row, rows, n_seq, n_slots, hk, hv, dk, dv,
-        QWEN_F32 if dtype == f32 else QWEN_BF16, scale))
+        QWEN_F32 if dtype == f32 else QWEN_BF16, scale, zero_rest))
 
 
 def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0, state_in=None, state_out=None,
@@ -672,22 +672,25 @@ def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0
     starts from its slot of state_in (None: zeros) and leaves its state in that
     slot of state_out (None: a new tensor; it may be state_in).  slots: int32 on
     the device, None: slot s for sequence s.  work: uint8 scratch of at least
-    linear_attention_prompt_work_bytes, for callers that keep one.  The rest is
+    linear_attention_prompt_work_bytes, for callers that keep one.  Rows of out of
+    skipped sequences, and rows that no sequence holds, are left as they were where out is
+    given; in a new one they are 0 if slots are given, else undefined.  The rest is
     gdn_dev_prompt's contract (include/qwen_kernels.h)."""
     torch = _torch()
     with _same_device(q, k, v, alpha, beta, starts, state_in, state_out, slots, out, work):
         n_seq = 1 if starts is None else starts.numel() - 1
         if starts is not None:
             _flat(starts, "starts", (max(n_seq, 0) + 1,), torch.int32)
+        zero_rest = out is None and slots is not None
         if out is None:
-            out = _like(v)
+            out = _like(v) if n_seq else v.new_zeros(v.shape)  # (without sequences nothing is launched)
         if state_out is None:
             if slots is not None:
                 raise ValueError("slots need a state_out that holds them")
             if q.dim() != 3 or v.dim() != 3:
                 raise ValueError("q, k, v are [rows, heads, dim]")
             state_out = alpha.new_empty((n_seq, v.size(1), q.size(2) * v.size(2)), dtype=torch.float32)
-        a = _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out)
+        a = _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out, zero_rest)
         lib = load()
         if work is None:
             need = lib.gdn_dev_prompt_work_bytes(a)
@@ -711,12 +714,15 @@ def linear_attention_prompt_work_bytes(rows, n_seq, heads_k, heads_v, dim_k, dim
 
 def linear_attention_step(q, k, v, alpha, beta, state, *, scale=1.0, slots=None, out=None):
     """One token for each sequence: row s of q, k, v updates the state in slot
-    slots[s] (None: s) of `state` in place -> out.  Types and layouts as in
-    linear_attention_prompt; gdn_dev_step (include/qwen_kernels.h)."""
+    slots[s] (None: s) of `state` in place -> out.  Rows that are skipped (a slot
+    outside the states, or an earlier sequence's) are left as they were in an out that is
+    given and are 0 in a new one.  Types and layouts as in linear_attention_prompt;
+    gdn_dev_step (include/qwen_kernels.h)."""
     with _same_device(q, k, v, alpha, beta, state, slots, out):
+        zero_rest = out is None and slots is not None
         if out is None:
             out = _like(v)
-        a = _gdn_args(q, k, v, alpha, beta, scale, state, state, slots, None, q.shape[0], None, out)
+        a = _gdn_args(q, k, v, alpha, beta, scale, state, state, slots, None, q.shape[0], None, out, zero_rest)
         check(load().gdn_dev_step(a, _stream()), "linear_attention_step")
     return out
 

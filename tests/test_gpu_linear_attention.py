@@ -477,3 +477,36 @@ def test_products_of_a_state_keep_their_bits(gpu):
     want = k[5].double()[:, :, None] * v[5].double()[:, None, :]
     off = (unblocked(got, 128, 128)[0].double() - want).abs() / want.abs()
     assert float(off.max()) <= 2.0 ** -22, float(off.max()) * 2 ** 22
+
+
+def _new_memory_is_nan(like):
+    """What the allocator hands out next held NaN."""
+    x = [torch.full_like(like, float("nan")) for _ in range(3)]
+    torch.cuda.synchronize()
+    del x
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("heads,dv", [(2, 32), (16, 100)])
+@pytest.mark.parametrize("lengths", [[1] * 8, [12, 10, 0, 16, 3, 1, 2, 30], [70, 10, 0, 64, 3, 1, 20, 129], [3, 10, 90, 2, 1, 4, 5, 6],
+                                     [0, 100, 0, 0, 0, 0, 0, 0]])
+def test_rows_of_no_sequence_are_zero_in_a_new_output(gpu, lengths, heads, dv, dtype):
+    """Rows in front of the first sequence, behind the last and of skipped ones, whichever way each goes."""
+    slots = torch.tensor([-1, 4, 0, 9, 4, 2, 1000000, -5], dtype=torch.int32).cuda()
+    ends = np.cumsum([9] + lengths)
+    rows = int(ends[-1]) + 21
+    q, k, v, al, be, st = inputs(rows, heads, heads, 64, dv, dtype, True, 9)
+    starts = torch.tensor(ends, dtype=torch.int32).cuda()
+    taken = [-1, 4, 0, -1, -1, 2, -1, -1]
+    want, _ = oracle(q, k, v, al, be, 1.0, st, list(zip(ends[:-1].tolist(), ends[1:].tolist())), taken)
+    _new_memory_is_nan(v.contiguous())
+    out, _ = gpu.linear_attention_prompt(q, k, v, al, be, starts, state_in=st, state_out=st.clone(), slots=slots)
+    near(out, want.nan_to_num(0.0), dtype)
+    if lengths[0] == 1:
+        q, k, v, al, be = (x[:8].contiguous() for x in (q, k, v, al, be))
+        want, _ = oracle(q, k, v, al, be, 1.0, st, [(i, i + 1) for i in range(8)], taken)
+        _new_memory_is_nan(v)
+        near(gpu.linear_attention_step(q, k, v, al, be, st, slots=slots), want.nan_to_num(0.0), dtype)
+        none = torch.zeros(1, dtype=torch.int32).cuda()
+        _new_memory_is_nan(v)
+        assert bool((gpu.linear_attention_prompt(q, k, v, al, be, none)[0] == 0).all())
