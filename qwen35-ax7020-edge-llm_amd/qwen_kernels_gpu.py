@@ -617,6 +617,15 @@ def _flat(t, name, shape, dtype):
         raise ValueError(f"{name} has to be a contiguous {tuple(shape)} of {dtype}")
 
 
+def _work_of(work):
+    """Address and bytes of a caller's work buffer (None: 0, 0)."""
+    if work is None:
+        return 0, 0
+    if not work.is_contiguous():  # (an expanded or strided one has fewer bytes of its own, or others' between)
+        raise ValueError("work has to be contiguous")
+    return work.data_ptr(), work.numel() * work.element_size()
+
+
 def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n_seq, work, out, zero_rest):
     """The arguments of either form of the attention."""
     torch = _torch()
@@ -655,7 +664,7 @@ def _gdn_args(q, k, v, alpha, beta, scale, state_in, state_out, slots, starts, n
         out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), alpha.data_ptr(),
         0 if beta is None else beta.data_ptr(), 0 if state_in is None else state_in.data_ptr(), state_out.data_ptr(),
         0 if slots is None else slots.data_ptr(), 0 if starts is None else starts.data_ptr(),
-        0 if work is None else work.data_ptr(), 0 if work is None else work.numel() * work.element_size(),
+        *_work_of(work),
         q_row, k_row, v_row, out_row, gate_row, rows, n_seq, n_slots, hk, hv, dk, dv,
         QWEN_F32 if dtype == f32 else QWEN_BF16, scale, zero_rest))
 
@@ -748,8 +757,7 @@ def _loss_call(name, a, work, h):
     need = getattr(lib, name + "_work_bytes")(a)
     if need and work is None:
         work = h.new_empty(need, dtype=_torch().uint8)
-    if work is not None:
-        a.work, a.work_bytes = _dp(work), work.numel() * work.element_size()
+    a.work, a.work_bytes = _work_of(work)
     check(getattr(lib, name)(a, _stream()), name)
 
 

@@ -3,6 +3,7 @@ and work buffers give BFP8_EINVAL and a message before anything touches a GPU.""
 import ctypes
 
 import pytest
+import torch
 
 import qwen_kernels_gpu as qk
 
@@ -100,6 +101,22 @@ def test_loss_work():
     assert big[0] == big[1] < 256 << 20
     assert lib.bf16_dev_lm_head_loss(loss(rows=0), None) == qk.BFP8_OK
     assert lib.bf16_dev_lm_head_loss_grad(loss(grad_h=None, grad_table=None), None) == qk.BFP8_OK
+
+
+def test_work_has_to_be_contiguous():
+    """A view's elements times their size are not its bytes: one byte expanded would pass for any size."""
+    x = torch.zeros(64, dtype=torch.uint8)
+    assert qk._work_of(None) == (0, 0) and qk._work_of(x) == (x.data_ptr(), 64)
+    assert qk._work_of(torch.zeros(8)[2:])[1] == 24
+    for bad in (torch.zeros(1, dtype=torch.uint8).expand(1 << 30), x[::2], torch.zeros(4, 4).t()):
+        with pytest.raises(ValueError, match="contiguous"):
+            qk._work_of(bad)
+    q = torch.zeros(1, 1, 4)
+    gate, state = torch.zeros(1, 1), torch.zeros(1, 1, 16)
+    with pytest.raises(ValueError, match="contiguous"):
+        qk._gdn_args(q, q, q, gate, gate, 1.0, None, state, None, None, 1, x[::2], torch.zeros(1, 1, 4), False)
+    with pytest.raises(ValueError, match="contiguous"):
+        qk._loss_call("bf16_dev_lm_head_loss", loss(), x[::2], q)
 
 
 def test_structs_have_the_headers_layout():
