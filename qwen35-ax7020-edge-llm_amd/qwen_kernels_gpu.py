@@ -710,11 +710,22 @@ def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0
     return out, state_out
 
 
+def _sizes_of(a, dtype, **sizes):
+    """Sets the sizes of arguments `a` and its type (a c_int takes a larger number's lower half without a word)."""
+    torch = _torch()
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"float32 or bfloat16, not {dtype}")
+    for name, n in sizes.items():
+        if not 0 <= n < 1 << 31:
+            raise ValueError(f"{name}: {n} is not a size")
+        setattr(a, name, n)
+    a.dtype = QWEN_F32 if dtype == torch.float32 else QWEN_BF16
+
+
 def linear_attention_prompt_work_bytes(rows, n_seq, heads_k, heads_v, dim_k, dim_v, dtype) -> int:
     """Bytes of linear_attention_prompt's work for these sizes (dtype: of q, k, v)."""
     a = gdn_dev_args()
-    a.rows, a.n_seq, a.heads_k, a.heads_v, a.dim_k, a.dim_v = rows, n_seq, heads_k, heads_v, dim_k, dim_v
-    a.dtype = {_torch().float32: QWEN_F32, _torch().bfloat16: QWEN_BF16}[dtype]
+    _sizes_of(a, dtype, rows=rows, n_seq=n_seq, heads_k=heads_k, heads_v=heads_v, dim_k=dim_k, dim_v=dim_v)
     n = load().gdn_dev_prompt_work_bytes(a)
     if not n:
         check(BFP8_EINVAL, "linear_attention_prompt_work_bytes")
@@ -805,8 +816,7 @@ def lm_head_loss_grad(h, table, targets, lse, grad_loss, *, need_h=True, need_ta
 def lm_head_loss_work_bytes(rows, vocab, hidden, dtype, *, grad=False, need_h=True) -> int:
     """Bytes of lm_head_loss's work for these sizes (dtype: of h), or of lm_head_loss_grad's."""
     a = lm_head_loss_args()
-    a.rows, a.vocab, a.hidden = rows, vocab, hidden
-    a.dtype = {_torch().float32: QWEN_F32, _torch().bfloat16: QWEN_BF16}[dtype]
+    _sizes_of(a, dtype, rows=rows, vocab=vocab, hidden=hidden)
     a.grad_h = 1 if need_h else None  # only whether it is there
     lib = load()
     n = (lib.bf16_dev_lm_head_loss_grad_work_bytes if grad else lib.bf16_dev_lm_head_loss_work_bytes)(a)

@@ -119,6 +119,21 @@ def test_work_has_to_be_contiguous():
         qk._loss_call("bf16_dev_lm_head_loss", loss(), x[::2], q)
 
 
+def test_work_bytes_of_sizes_past_32_bits():
+    """A size whose lower half is valid is refused, not taken for that half; so is another type."""
+    f, g = qk.lm_head_loss_work_bytes, qk.linear_attention_prompt_work_bytes
+    assert f(5, 100, 64, torch.float32) > 0 and g(5, 1, 1, 1, 64, 64, torch.bfloat16) > 0
+    for far in ((1 << 32) + 5, 1 << 31, -(1 << 32) + 5, -1):
+        for bad in (lambda: f(far, 100, 64, torch.float32), lambda: f(5, far, 64, torch.float32),
+                    lambda: f(5, 100, far, torch.float32), lambda: g(far, 1, 1, 1, 64, 64, torch.float32),
+                    lambda: g(5, far, 1, 1, 64, 64, torch.float32)):
+            with pytest.raises(ValueError):
+                bad()
+    for bad in (lambda: f(5, 100, 64, torch.float16), lambda: g(5, 1, 1, 1, 64, 64, torch.float16)):
+        with pytest.raises(ValueError):
+            bad()
+
+
 def test_structs_have_the_headers_layout():
     assert ctypes.sizeof(qk.gdn_dev_args) == 12 * 8 + 5 * 8 + 9 * 4 + 4
     assert ctypes.sizeof(qk.lm_head_loss_args) == 10 * 8 + 4 * 8 + 4 * 4
