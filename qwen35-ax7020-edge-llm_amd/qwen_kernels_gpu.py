@@ -588,6 +588,11 @@ def _same_device(first, *tensors):
     return _HERE if device == cuda.current_device() else cuda.device(device)
 
 
+def _no_graph(who, why):
+    """Refuses inputs whose gradient autograd would be asked for: the results have no graph behind them."""
+    raise ValueError(f"{who}: an input requires a gradient, and {why}: detach it, or call under torch.no_grad()")
+
+
 def _rows_of(t, name, shape, dtype):
     """t of this shape and type, each of its rows contiguous -> the stride between rows."""
     if t.shape != shape or t.dtype != dtype:
@@ -683,9 +688,13 @@ def linear_attention_prompt(q, k, v, alpha, beta=None, starts=None, *, scale=1.0
     the device, None: slot s for sequence s.  work: uint8 scratch of at least
     linear_attention_prompt_work_bytes, for callers that keep one.  Rows of out of
     skipped sequences, and rows that no sequence holds, are left as they were where out is
-    given; in a new one they are 0 if slots are given, else undefined.  The rest is
-    gdn_dev_prompt's contract (include/qwen_kernels.h)."""
+    given; in a new one they are 0 if slots are given, else undefined.  There is no
+    backward pass: tensors that require a gradient are refused unless it is off.  The
+    rest is gdn_dev_prompt's contract (include/qwen_kernels.h)."""
     torch = _torch()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or alpha.requires_grad or any(
+            t is not None and t.requires_grad for t in (beta, state_in, state_out))):
+        _no_graph("linear_attention_prompt", "there is no backward pass")
     with _same_device(q, k, v, alpha, beta, starts, state_in, state_out, slots, out, work):
         n_seq = 1 if starts is None else starts.numel() - 1
         if starts is not None:
@@ -736,8 +745,11 @@ def linear_attention_step(q, k, v, alpha, beta, state, *, scale=1.0, slots=None,
     """One token for each sequence: row s of q, k, v updates the state in slot
     slots[s] (None: s) of `state` in place -> out.  Rows that are skipped (a slot
     outside the states, or an earlier sequence's) are left as they were in an out that is
-    given and are 0 in a new one.  Types and layouts as in linear_attention_prompt;
-    gdn_dev_step (include/qwen_kernels.h)."""
+    given and are 0 in a new one.  Types, layouts and refusals as in
+    linear_attention_prompt; gdn_dev_step (include/qwen_kernels.h)."""
+    if (q.requires_grad or k.requires_grad or v.requires_grad or alpha.requires_grad or state.requires_grad
+            or beta is not None and beta.requires_grad) and _torch().is_grad_enabled():
+        _no_graph("linear_attention_step", "there is no backward pass")
     with _same_device(q, k, v, alpha, beta, state, slots, out):
         zero_rest = out is None and slots is not None
         if out is None:
@@ -778,9 +790,13 @@ def lm_head_loss(h, table, targets, *, work=None):
 
     h [rows, hidden] float32 or bfloat16, table [vocab, hidden] bfloat16, targets
     int32 [rows]: below 0 the row is ignored (loss and lse 0), vocab or more
-    gives NaN.  work: uint8 scratch of at least lm_head_loss_work_bytes.  The rest
-    is bf16_dev_lm_head_loss's contract (include/qwen_kernels.h)."""
+    gives NaN.  work: uint8 scratch of at least lm_head_loss_work_bytes.  No autograd
+    graph is built: inputs that require a gradient are refused unless it is off, and
+    lm_head_loss_grad has the gradients.  The rest is bf16_dev_lm_head_loss's contract
+    (include/qwen_kernels.h)."""
     torch = _torch()
+    if (h.requires_grad or table.requires_grad) and torch.is_grad_enabled():
+        _no_graph("lm_head_loss", "its gradients are lm_head_loss_grad's")
     with _same_device(h, table, targets, work):
         a = _loss_args(h, table, targets)
         loss, lse = h.new_empty((2, a.rows), dtype=torch.float32)
@@ -793,7 +809,8 @@ def lm_head_loss_grad(h, table, targets, lse, grad_loss, *, need_h=True, need_ta
                       grad_table=None, work=None):
     """The gradients of sum(grad_loss * loss) -> (grad_h, grad_table), in h's and the
     table's type, overwritten where given; None for one that is not needed.
-    lse is lm_head_loss's; grad_loss float32 [rows]."""
+    lse is lm_head_loss's; grad_loss float32 [rows].  The gradients have no graph
+    behind them, as autograd's own without create_graph."""
     torch = _torch()
     with _same_device(h, table, targets, lse, grad_loss, grad_h, grad_table, work):
         a = _loss_args(h, table, targets)

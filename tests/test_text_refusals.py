@@ -134,6 +134,29 @@ def test_work_bytes_of_sizes_past_32_bits():
             bad()
 
 
+def test_inputs_that_require_a_gradient():
+    """Results without a graph would end the gradient without a word: refused, before the tensors are looked at (on
+    the CPU here), unless gradients are off."""
+    z = lambda *s: torch.zeros(*s)  # noqa: E731
+    q, gate, state = z(2, 1, 4), z(2, 1), z(2, 1, 16)
+    h, table, t = z(2, 4), z(5, 4), torch.zeros(2, dtype=torch.int32)
+    for i in range(6):
+        a = [q, q, q, gate, gate, state]
+        a[i] = a[i].clone().requires_grad_()
+        for f in (lambda: qk.linear_attention_step(*a), lambda: qk.linear_attention_prompt(*a[:5], state_in=a[5])):
+            with pytest.raises(ValueError, match="requires a gradient"):
+                f()
+            with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):
+                f()
+    for a in ((h.clone().requires_grad_(), table), (h, table.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="requires a gradient.*lm_head_loss_grad"):
+            qk.lm_head_loss(*a, t)
+        with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):
+            qk.lm_head_loss(*a, t)
+        with pytest.raises(ValueError, match="on a GPU"):  # (gradients of inputs that autograd knows are ordinary)
+            qk.lm_head_loss_grad(*a, t, z(2), z(2))
+
+
 def test_structs_have_the_headers_layout():
     assert ctypes.sizeof(qk.gdn_dev_args) == 12 * 8 + 5 * 8 + 9 * 4 + 4
     assert ctypes.sizeof(qk.lm_head_loss_args) == 10 * 8 + 4 * 8 + 4 * 4
