@@ -75,6 +75,11 @@ __device__ __forceinline__ void span(const gdn_dev_args& a, int s, int& first, i
     n = min(max(a.starts[s + 1], first), a.rows) - first;
 }
 
+// The place of sequence s's first chunk in the work buffer (GdnWork).
+__device__ __forceinline__ int first_place(int first, int s, int short_to) {
+    return short_to < 0 ? first / C + s : first / GDN_SHORT;
+}
+
 // The sequence with the r-th most chunks (of equal ones the first first) and its rows, where a wavefront holds
 // all lengths and the workgroups are more than the compute units; else sequence r.  Every lane of the wavefront:
 // bit by bit from the top, the lanes that the r-th may be.
@@ -238,13 +243,13 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
     const size_t chunk = blockIdx.x / a.heads_v;
     const int hv = blockIdx.x % a.heads_v, reach = a.heads_v / a.heads_k, hk = hv / reach;
 
-    // the sequence: the last s with starts[s] / 64 + s <= chunk
+    // the sequence: the last s whose first place is up to `chunk`
     int seq = 0;
     if (a.starts) {
         int lo = 0, hi = a.n_seq;  // key(lo) <= chunk < key(hi)
         while (hi - lo > 1) {
             const int step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
-            const bool le = at < hi && (size_t)(min(max(a.starts[at], 0), a.rows) / C + at) <= chunk;
+            const bool le = at < hi && (size_t)first_place(min(max(a.starts[at], 0), a.rows), at, short_to) <= chunk;
             const int below = __popcll(__ballot(le));
             const int nlo = lo + below * step;
             hi = min(hi, lo + (below + 1) * step);
@@ -255,7 +260,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
     int first, len;
     span(a, seq, first, len);
     if (len <= short_to) return;
-    const long c = (long)chunk - (first / C + seq);
+    const long c = (long)chunk - first_place(first, seq, short_to);
     if (c < 0 || c * C >= len) return;
     const int row0 = first + (int)c * C, n = min(C, len - (int)c * C);
     const Places at = Layout<KS, NT, NO>::at(a, n_chunks, chunk, hk, hv);
@@ -472,7 +477,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
     if (slot < 0) return;
     const int j0 = 16 * NC * slice + col;  // first value column
     const int nc = (len + C - 1) / C;
-    Places at = L::at(a, n_chunks, (size_t)(first / C) + seq, hk, hv);
+    Places at = L::at(a, n_chunks, first_place(first, seq, short_to), hk, hv);
     auto half = [&](u32x4(&x)[64], int tile) -> u32x2& { return reinterpret_cast<u32x2*>(&x[lane])[tile & 1]; };
 
     using lds_void = __attribute__((address_space(3))) void;
@@ -1076,21 +1081,20 @@ bool rows_of_16(const void* p, int64_t row, int dim, int es) {
 }
 
 template <int KS, int NT, bool kDelta>
-hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, int short_to, hipStream_t s) {
+hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
     using T = std::conditional_t<NT == 1, uint16_t, float>;
     const int es = NT == 1 ? 2 : 4;
     const bool full_q = a.dim_k == 32 * KS && rows_of_16(a.q, a.q_row, a.dim_k, es);
     const bool full_k = a.dim_k == 32 * KS && rows_of_16(a.k, a.k_row, a.dim_k, es);
     const bool direct = NT == 1 && full_q && full_k && rows_of_16(a.v, a.v_row, a.dim_v, es) &&
                         a.k_row < 1 << 24 && a.v_row < 1 << 24;  // (offsets of 64 rows in 32 bits)
-    if (a.rows > 0)
-        gdn_chunk_kernel<KS, NT, kDelta>
-            <<<dim3((unsigned)(w.n_chunks * a.heads_v)), 256, 0, s>>>(a, w.n_chunks, short_to, full_q, full_k, direct);
+    gdn_chunk_kernel<KS, NT, kDelta>
+        <<<dim3((unsigned)(w.places * a.heads_v)), 256, 0, s>>>(a, w.n_chunks, w.short_to, full_q, full_k, direct);
     auto scan = [&](auto nc, auto from_inputs) {
         constexpr int NC = decltype(nc)::value;
         const int slices = (a.dim_v + 16 * NC - 1) / (16 * NC);
         gdn_scan_kernel<KS, NT, NC, kDelta, decltype(from_inputs)::value, T>
-            <<<dim3((unsigned)((size_t)a.n_seq * a.heads_v * slices)), 576, 0, s>>>(a, w.n_chunks, slices, short_to);
+            <<<dim3((unsigned)((size_t)a.n_seq * a.heads_v * slices)), 576, 0, s>>>(a, w.n_chunks, slices, w.short_to);
     };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, KS <= 4 ? 2 : 1>;
@@ -1107,10 +1111,10 @@ hipError_t launch_prompt(const gdn_dev_args& a, const GdnWork& w, int short_to, 
 }
 
 template <int KS>
-hipError_t launch_prompt_of(const gdn_dev_args& a, const GdnWork& w, int short_to, hipStream_t s) {
+hipError_t launch_prompt_of(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
     if (a.dtype == QWEN_BF16)
-        return a.beta ? launch_prompt<KS, 1, true>(a, w, short_to, s) : launch_prompt<KS, 1, false>(a, w, short_to, s);
-    return a.beta ? launch_prompt<KS, 3, true>(a, w, short_to, s) : launch_prompt<KS, 3, false>(a, w, short_to, s);
+        return a.beta ? launch_prompt<KS, 1, true>(a, w, s) : launch_prompt<KS, 1, false>(a, w, s);
+    return a.beta ? launch_prompt<KS, 3, true>(a, w, s) : launch_prompt<KS, 3, false>(a, w, s);
 }
 
 template <int NI, int G, bool kStream, bool kText>
@@ -1150,23 +1154,15 @@ hipError_t tokens(const gdn_dev_args& a, int short_to, hipStream_t s) {
 }  // namespace
 
 hipError_t gdn_launch_prompt(const gdn_dev_args& a, const GdnWork& w, hipStream_t s) {
-    // Sequences of up to 16 tokens go token by token, past the latency of a chunk: one of 16 heads of 128 with
-    // 4 | 16 | 32 tokens in bf16 5.4 | 11 | 18 us, in a chunk 14; 64 of them with 4 | 16 tokens 44 | 73 us, in chunks
-    // 104 | 108.  That is a third launch where longer ones may be in the call too (their lengths are on the
-    // device); it is made if the chunks would go over the chip more than once and the average sequence is that short.
-    constexpr int kShort = 16;
-    const bool many = (size_t)a.n_seq * a.heads_v * ((a.dim_v + 31) / 32) > 256 &&
-                      (size_t)a.rows <= (size_t)kShort * a.n_seq;
-    const int short_to = a.rows <= kShort || many ? kShort : -1;
-    if (short_to >= 0) {
-        const hipError_t e = tokens<true>(a, short_to, s);
-        if (e != hipSuccess || a.rows <= short_to) return e;
+    if (w.short_to >= 0) {
+        const hipError_t e = tokens<true>(a, w.short_to, s);
+        if (e != hipSuccess || a.rows <= w.short_to) return e;
     }
     switch (w.ks) {
-        case 1: return launch_prompt_of<1>(a, w, short_to, s);
-        case 2: return launch_prompt_of<2>(a, w, short_to, s);
-        case 4: return launch_prompt_of<4>(a, w, short_to, s);
-        default: return launch_prompt_of<8>(a, w, short_to, s);
+        case 1: return launch_prompt_of<1>(a, w, s);
+        case 2: return launch_prompt_of<2>(a, w, s);
+        case 4: return launch_prompt_of<4>(a, w, s);
+        default: return launch_prompt_of<8>(a, w, s);
     }
 }
 

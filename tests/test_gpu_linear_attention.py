@@ -510,3 +510,21 @@ def test_rows_of_no_sequence_are_zero_in_a_new_output(gpu, lengths, heads, dv, d
         none = torch.zeros(1, dtype=torch.int32).cuda()
         _new_memory_is_nan(v)
         assert bool((gpu.linear_attention_prompt(q, k, v, al, be, none)[0] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("lengths", [[17] * 60 + [0] * 80, [1] * 300 + [400] + [2] * 60, [65, 0, 0, 0, 0, 0, 0, 0, 16, 0, 0, 0, 130] * 12,
+                                     [0] * 130 + [449], [200, 17, 3], [16] * 9])
+def test_work_is_as_large_as_it_says(gpu, lengths, dtype):
+    """Long sequences next to each other, behind and in front of many short ones: each chunk has a place of its own,
+    within the bytes asked for, whatever they held."""
+    spans, starts = spans_of(lengths)
+    rows = spans[-1][1]
+    q, k, v, al, be, st = inputs(rows, 2, 4, 64, 64, dtype, True, len(lengths))
+    need = gpu.linear_attention_prompt_work_bytes(rows, len(lengths), 2, 4, 64, 64, dtype)
+    work = torch.full((need + 65536,), 255, dtype=torch.uint8, device="cuda")
+    want, wst = oracle(q, k, v, al, be, 0.5, st, spans)
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, scale=0.5, state_in=st, work=work[:need])
+    near(out, want, dtype)
+    near(got, wst)
+    assert bool((work[need:] == 255).all())

@@ -157,6 +157,21 @@ def test_inputs_that_require_a_gradient():
             qk.lm_head_loss_grad(*a, t, z(2), z(2))
 
 
+def test_work_of_many_short_sequences():
+    """Sequences that go token by token have no place in the work buffer, whose size never falls with the rows or the
+    sequences (a buffer for the largest call does for the smaller ones)."""
+    f = qk.linear_attention_prompt_work_bytes
+    assert f(1024, 1024, 16, 16, 128, 128, torch.bfloat16) < 96 << 20
+    assert f(8192, 8192, 16, 16, 128, 128, torch.float32) < 3 << 29
+    sizes = sorted({0, 1, 15, 16, 17, 63, 64, 65, 255, 256, 257, 1000, 4095, 4096, 4097, 30000})
+    for heads, dim_v in ((1, 4), (3, 96), (16, 128)):
+        table = [[f(r, n, heads, heads, 64, dim_v, torch.bfloat16) for n in sizes[1:]] for r in sizes]
+        for row in table:
+            assert row == sorted(row)
+        for column in zip(*table):
+            assert list(column) == sorted(column)
+
+
 def test_structs_have_the_headers_layout():
     assert ctypes.sizeof(qk.gdn_dev_args) == 12 * 8 + 5 * 8 + 9 * 4 + 4
     assert ctypes.sizeof(qk.lm_head_loss_args) == 10 * 8 + 4 * 8 + 4 * 4
