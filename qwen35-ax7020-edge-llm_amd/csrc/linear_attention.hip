@@ -699,6 +699,9 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
 
     // the state: lane holds rows state_row(tile, grp) .. + 3 of column j0 + 16 x
     const size_t head_state = ((size_t)slot * a.heads_v + hv) * a.dim_k * a.dim_v;
+    // (with one step along dim_k two of the wavefronts have no tile; else the compiler has to know that all do: it leaves
+    // too few wait states between a matrix product, a branch around the next one, and the first use of the result)
+    auto has_tile = [&](int t) { return KS >= 2 || w * TPW + t < 2 * KS; };
     f32x4 S[NC][TPW];
     auto each_state = [&](auto&& f) {
 #pragma unroll
@@ -706,7 +709,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 const int i = state_row(w * TPW + t, grp), j = j0 + 16 * x;
-                if (j < a.dim_v && i < a.dim_k && w * TPW + t < 2 * KS)
+                if (j < a.dim_v && i < a.dim_k && has_tile(t))
                     f(S[x][t], head_state + (((size_t)(j / 4) * (a.dim_k / 4) + i / 4) * 4 + j % 4) * 4);
             }
     };
@@ -756,7 +759,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
         for (int x = 0; x < NC; ++x)
 #pragma unroll
             for (int t = 0; t < TPW; ++t)
-                if (w * TPW + t < 2 * KS) {
+                if (has_tile(t)) {
                     u32x2 y[3];
                     split4(S[x][t], y);
 #pragma unroll
@@ -882,7 +885,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                 for (int m = 0; m < 3; ++m) b[x][m] = dsh[x][ts][m][lane];
 #pragma unroll
             for (int t = 0; t < TPW; ++t)
-                if (w * TPW + t < 2 * KS) {
+                if (has_tile(t)) {
                     u32x4 kf[NT];
                     K::columns(kt, w * TPW + t, ts, lane, kf);
 #pragma unroll
