@@ -518,7 +518,8 @@ void bfp8_plan_destroy(void* plan);
  * and work are 16-byte aligned, the others aligned to their elements.  out overlaps
  * nothing that the call reads.  A NaN or infinity in a
  * token gives NaN or infinite values in that sequence and head from that
- * chunk of 64 tokens on, and nowhere else.
+ * token on (in q in that token's out alone, in v in its columns alone), and nowhere
+ * else; one in a state in its columns.
  *
  * The same call gives the same bits.  In another call they may differ in rounding:
  * whether a sequence of up to 16 tokens goes token by token, and how many value columns

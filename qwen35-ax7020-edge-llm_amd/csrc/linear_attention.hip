@@ -58,6 +58,8 @@ __device__ __forceinline__ void load_terms(const void* row, int i, int dim, bool
     }
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
 // 2^d, d <= 0 as a rule; the whole part exactly.
 __device__ __forceinline__ float exp2_of(double d) {
     const double w = floor(d);
@@ -238,6 +240,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
     __shared__ __attribute__((aligned(16))) float lsh[kDelta ? C : 1][C + 4];
     __shared__ double gsh[C];
     __shared__ float bsh[C];
+    __shared__ uint32_t bad_sh[4];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15,
               grp = lane >> 4;
     const size_t chunk = blockIdx.x / a.heads_v;
@@ -279,12 +282,30 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
         load_terms(krow, 32 * s + 8 * grp, a.dim_k, full_k, kf[s]);
         load_terms(qrow, 32 * s + 8 * grp, a.dim_k, full_q, qf[s]);
     }
+    // A token whose k, decay or beta is not finite: a matrix product takes 0 x NaN to the tokens before it too, so it
+    // goes in as zeros here, and the first such token's 2^g and 2^(g_C - g) are NaN, which gdn_scan_kernel meets.
+    using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, kf[s][0][j] & 0x7fff7fffu));
+    const uint64_t groups = __ballot(most[0] >= 0x7f80 || most[1] >= 0x7f80);
+    uint32_t bad_rows = (uint32_t)groups | (uint32_t)(groups >> 32);
+    bad_rows = (bad_rows | bad_rows >> 16) & 0xffff;
+    const bool bad_k = bad_rows >> col & 1;
+    if (lane == 0) bad_sh[w] = bad_rows;
+    uint64_t bad_gates = 0;
     if (w == 0) {
         // g in double: differences of large sums stay exact to a float32.  A decay of 0
         // counts as 2^-16384, which no product brings back.
         const int64_t grow = (int64_t)(row0 + min(lane, n - 1)) * a.gate_row + hv;
         const float al = a.alpha[grow], be = kDelta ? a.beta[grow] : 0.0f;
         double g = lane >= n ? 0.0 : al == 0.0f ? -16384.0 : log2((double)al);
+        const bool bad_al = !(fabs(g) < __builtin_inf());
+        if (bad_al) g = 0.0;
+        bad_gates = __ballot(bad_al || !finite(be));
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const double o = __shfl_up(g, d);
@@ -292,7 +313,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
         }
         const double gc = __shfl(g, 63);
         gsh[lane] = g;
-        bsh[lane] = lane < n ? be : 0.0f;
+        bsh[lane] = lane < n && finite(be) ? be : 0.0f;
         at.up[lane] = exp2_of(g);
         at.down[lane] = exp2_of(gc - g);
         if (lane == 0) at.last[0] = exp2_of(gc);
@@ -301,7 +322,8 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
     for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (r >= n) kf[s][t] = qf[s][t] = u32x4{0, 0, 0, 0};
+            if (r >= n) qf[s][t] = u32x4{0, 0, 0, 0};
+            if (r >= n || bad_k) kf[s][t] = u32x4{0, 0, 0, 0};
             *reinterpret_cast<u32x4*>(&ksh[t][r][32 * s + 8 * grp]) = kf[s][t];
             const int f = ((w * KS + s) * NT + t) * 64 + lane;
             if (keys && !direct) {
@@ -350,6 +372,11 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
         split8(x, p);
 #pragma unroll
         for (int m = 0; m < NO; ++m) reinterpret_cast<u32x4*>(at.p)[(tri_tile(w, ts) * NO + m) * 64 + lane] = p[m];
+    }
+    if (w == 0) {  // (which has the least to do up to here)
+        uint64_t bad = bad_gates | bad_sh[0] | (uint64_t)bad_sh[1] << 16 | (uint64_t)bad_sh[2] << 32 | (uint64_t)bad_sh[3] << 48;
+        if (n < C) bad &= (1ull << n) - 1;
+        if (bad && lane == __builtin_ctzll(bad)) at.up[lane] = at.down[lane] = __builtin_nanf("");
     }
     if constexpr (kDelta) {
         // X = (I + L)^-1 in blocks of 16.  The blocks on the diagonal by substitution, a column a
@@ -457,7 +484,14 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
     __shared__ u32x4 rsh[kDelta ? NC : 1][kDelta ? 2 : 1][3][64];
     __shared__ u32x4 ush[NC][2][NO][64];
     __shared__ u32x4 dsh[NC][2][3][64];
-    __shared__ __attribute__((aligned(16))) T osh[4][16][16];
+    // the output wavefronts' tiles on their way out, from a chunk's last barrier to the next one's first: R is idle then
+    using OutTile = T[16][16];
+    __shared__ __attribute__((aligned(16))) OutTile own_osh[kDelta ? 1 : 4];
+    static_assert(!kDelta || sizeof(rsh) >= 4 * sizeof(OutTile), "R's place holds them");
+    OutTile* const osh = kDelta ? reinterpret_cast<OutTile*>(&rsh[0][0][0][0]) : own_osh;
+    // A column's first token whose right side (without the delta rule: v) is not finite, counted in the sequence: its
+    // part of R or U is 0, for the sake of the tokens before it; outputs from it on are NaN, and so is the state.
+    __shared__ int bad_sh[NC][16], first_bad;  // of each column, of any
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3,
               col = lane & 15, grp = lane >> 4;
     // the longest sequences first, so that none is begun when the others are nearly done (24 of 9001
@@ -654,6 +688,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
             if (kDelta) sync_lds();
             load_q(x);
             sync_lds();
+            const bool some_bad = __any(first_bad < c * C + C);
 #pragma unroll
             for (int ts = 0; ts < 2; ++ts)
 #pragma unroll
@@ -665,10 +700,18 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                 }
             if (kSets == 1) load_p(x);
 #pragma unroll
+            for (int y = 0; y < NC; ++y) o[y] *= a.scale;
+            if (__builtin_expect(some_bad, 0))
+#pragma unroll
+                for (int y = 0; y < NC; ++y)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c * C + 16 * w + 4 * grp + e >= bad_sh[y][col]) o[y][e] = __builtin_nanf("");
+#pragma unroll
             for (int y = 0; y < NC; ++y) {
                 // the tile row by row (nobody else's part of LDS, and in order within a wavefront)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) osh[w][4 * grp + e][col] = from_float<T>(a.scale * o[y][e]);
+                for (int e = 0; e < 4; ++e) osh[w][4 * grp + e][col] = from_float<T>(o[y][e]);
                 struct alignas(EL * sizeof(T)) Part {
                     T x[EL];
                 };
@@ -774,8 +817,30 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
         load_down();
     }
     put_state();
+    if (w == 0 && grp == 0)
+#pragma unroll
+        for (int x = 0; x < NC; ++x) bad_sh[x][col] = first_bad = 0x7fffffff;
     for (int c = 0; c < nc; ++c) {
         const int nx = min(c + 1, nc - 1);
+        // Whether any of these is not finite (or their sum is not: then each is looked at).
+        auto any_bad = [](const f32x4(&r)[NC]) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < NC; ++x) sum += (r[x][0] + r[x][1]) + (r[x][2] + r[x][3]);
+            return __any(!finite(sum));
+        };
+        // Zeros for r where `by` is not finite.
+        auto leave_out = [&](f32x4(&r)[NC], const f32x4(&by)[NC]) {
+#pragma unroll
+            for (int x = 0; x < NC; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!finite(by[x][e])) {
+                        atomicMin(&bad_sh[x][col], c * C + 16 * w + 4 * grp + e);
+                        atomicMin(&first_bad, c * C);
+                        r[x][e] = 0.0f;
+                    }
+        };
         if (c + 1 < nc) L::next(a, at);
         const char* kt = ksh[c % kBufs];
         sync_lds();
@@ -790,7 +855,7 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                 for (int e = 0; e < 4; ++e)
                     v[x][e] = *reinterpret_cast<const T*>(vsh[c % kBufs] + (16 * w + 4 * grp + e) * kVRow + (16 * x + col) * 2);
         }
-        f32x4 u[NC];
+        f32x4 u[NC], into[NC];
         if constexpr (kDelta) {
             // R = V - 2^g K S0
             f32x4 ks[NC][2];
@@ -808,14 +873,26 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                     ks[x][s % 2] = mfma_terms<NT, 3, 3>(kf, b, ks[x][s % 2]);
                 }
             }
+            f32x4 rhs[NC];
+            float poison[NC];  // NaN for a column whose state ends here
 #pragma unroll
-            for (int x = 0; x < NC; ++x) {
-                f32x4 rhs;
+            for (int x = 0; x < NC; ++x)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    rhs[e] = __builtin_fmaf(-up[e], ks[x][0][e] + ks[x][1][e], to_float<T>(v[x][e]));
+                    rhs[x][e] = __builtin_fmaf(-up[e], ks[x][0][e] + ks[x][1][e], to_float<T>(v[x][e]));
+            const bool bad = any_bad(rhs);
+            if (__builtin_expect(bad, 0)) {
+#pragma unroll
+                for (int x = 0; x < NC; ++x) {
+                    const f32x4 z = rhs[x] * 0.0f;
+                    poison[x] = (z[0] + z[1]) + (z[2] + z[3]);
+                }
+                leave_out(rhs, rhs);
+            }
+#pragma unroll
+            for (int x = 0; x < NC; ++x) {
                 u32x2 y[3];
-                split4(rhs, y);
+                split4(rhs[x], y);
 #pragma unroll
                 for (int m = 0; m < 3; ++m) half(rsh[x][w / 2][m], w) = y[m];
             }
@@ -849,26 +926,35 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                         for (int x = 0; x < NC; ++x) u2[x][ts] = mfma(tf[ts][y], b[x][ts][z - y], u2[x][ts]);
             load_t();
 #pragma unroll
-            for (int x = 0; x < NC; ++x) u[x] = u2[x][0] + u2[x][1];
+            for (int x = 0; x < NC; ++x) {
+                u[x] = u2[x][0] + u2[x][1];
+                into[x] = u[x] * down;
+            }
+            if (__builtin_expect(bad, 0))
+#pragma unroll
+                for (int x = 0; x < NC; ++x) into[x] += poison[x];
         } else {
 #pragma unroll
-            for (int x = 0; x < NC; ++x)
+            for (int x = 0; x < NC; ++x) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     u[x][e] = c * C + 16 * w + 4 * grp + e < len ? to_float<T>(v[x][e]) : 0.0f;
+                into[x] = u[x] * down;
+            }
+            if (__builtin_expect(any_bad(into), 0)) leave_out(u, into);
             load_v(nx);
         }
-        const float keep = last;
 #pragma unroll
         for (int x = 0; x < NC; ++x) {
             u32x2 y[NO], d[3];
-            split4(u[x] * down, d);
+            split4(into[x], d);
 #pragma unroll
             for (int m = 0; m < 3; ++m) half(dsh[x][w / 2][m], w) = d[m];
             split4(u[x], y);
 #pragma unroll
             for (int m = 0; m < NO; ++m) half(ush[x][w / 2][m], w) = y[m];
         }
+        const float keep = last;
         load_down();
         sync_lds();
         // S0 <- 2^(g_C) S0 + K^T (2^(g_C - g) U)

@@ -528,3 +528,45 @@ def test_work_is_as_large_as_it_says(gpu, lengths, dtype):
     near(out, want, dtype)
     near(got, wst)
     assert bool((work[need:] == 255).all())
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("hk,hv,dk,dv,packed", [(2, 2, 64, 64, True), (16, 16, 128, 128, True), (2, 4, 128, 32, False), (1, 2, 20, 36, True),
+                                                (1, 1, 256, 32, True)])
+def test_nan_and_infinity_do_not_go_back(gpu, hk, hv, dk, dv, packed, delta, dtype):
+    """Whatever is not finite in a token shows from that token on, in its head (q: that token, v: its column; a state:
+    its column), as the recurrence has it: within a chunk, at its ends, in a last chunk that is not whole."""
+    spans, starts = spans_of([90, 200, 143])
+    h = hv - 1
+    for i, (kind, token) in enumerate([("q", 90 + 130), ("k", 90 + 64), ("v", 90 + 127), ("alpha", 90 + 100), ("beta", 90 + 31),
+                                       ("state", 0), ("k", 289), ("v", 90), ("v2", 90 + 40)]):
+        q, k, v, al, be, st = inputs(433, hk, hv, dk, dv, dtype, delta, 3, packed=packed)
+        value = float("nan") if i % 2 else float("inf")
+        if kind in ("q", "k"):
+            (q if kind == "q" else k)[token, hk - 1, dk // 2] = value
+        elif kind == "v":
+            v[token, h, dv // 2 + 1] = value
+        elif kind == "v2":  # two columns, two tokens of a chunk
+            v[token, h, 1], v[token + 9, h, dv - 1], v[token + 12, h, 1] = -value, value, value
+        elif kind == "alpha":
+            al[token, h] = float("nan")
+        elif kind == "beta":
+            if not delta:
+                continue
+            be[token, h] = value
+        else:
+            view = st.view(3, hv, dv // 4, dk // 4, 4, 4)
+            view[1, h, dv // 8, dk // 8, 2, 1] = value  # S[.., 4 (dv / 8) + 2] of sequence 1
+        want, wst = oracle(q, k, v, al, be, 0.5, st, spans)
+        out, got = gpu.linear_attention_prompt(q, k, v, al, be, starts, scale=0.5, state_in=st)
+        assert torch.equal(torch.isfinite(out).cpu(), torch.isfinite(want)), kind
+        nan = float("nan")
+        near(torch.where(torch.isfinite(out), out, nan), torch.where(torch.isfinite(want), want, nan), dtype)
+        if kind in ("k", "alpha", "beta"):  # (of such a state all is lost, whichever rows the recurrence keeps)
+            heads = range(h + 1 - hv // hk, hv) if kind == "k" else [h]
+            for x in heads:
+                assert not bool(torch.isfinite(got[1, x]).any()), kind
+                got[1, x], wst[1, x] = 0.0, 0.0
+        assert torch.equal(torch.isfinite(got).cpu(), torch.isfinite(wst)), kind
+        near(torch.where(torch.isfinite(got), got, nan), torch.where(torch.isfinite(wst), wst, nan))

@@ -16,6 +16,8 @@ ROOT = Path(__file__).resolve().parent.parent
 OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
 # wait states until a result may be used, as the compiler leaves them within a block
 WAITS = {"v_mfma_f32_16x16x32_bf16": 8, "v_mfma_f32_16x16x4_f32": 10, "v_mfma_i32_32x32x16_i8": 12}
+# (a load's own result comes from memory, later than any of these waits)
+LOAD, LOADED = re.compile(r"(global|buffer|flat|scratch)_load_(?!lds)|ds_read"), re.compile(r"^[^,]*,")
 LINE = re.compile(r"^\t(\S+)\s*(.*?)\s*// ([0-9A-F]{12}): ([0-9A-F]{8})")
 
 
@@ -67,7 +69,7 @@ def shortest(code, index, start):
                     break
                 if registers(parts[0]) & result:  # (the next product of the sum: it has its own way)
                     break
-            elif op[0] != "s" and registers(operands) & result:
+            elif op[0] != "s" and registers(LOADED.sub("", operands) if LOAD.match(op) else operands) & result:
                 best = (waits, code[i])
                 break
             waits += 1
