@@ -324,34 +324,41 @@ struct Parts {
 // so that what they count stays small (the loss of 2^20 rows over 1000 x 1024: 3.8 ms, with a workgroup for
 // every 16 rows 19).
 constexpr int kPrepRows = 16;
-template <int NT>
-__global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, int runs, bool grad) {
+template <int NT, bool kGrad>
+__global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, Parts p, int runs) {
     __shared__ int before_sh[4], local[kPrepRows], kept_sh;
-    __shared__ float top_sh[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first_row = blockIdx.x * runs * kPrepRows;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     auto counts = [&](int r) {
         const int t = a.targets[r];
         return t >= 0 && t < a.vocab;
     };
-    // the last workgroup looks at every row's target: it finds the largest weight too (of those that are finite)
-    const bool weighs = NT == 1 && grad && blockIdx.x + 1 == gridDim.x && blockIdx.y == 0;
-    auto weight = [&](int r) {
-        const float g = fabsf(a.grad_loss[r]);
-        return g < __builtin_inff() ? g : 0.0f;
-    };
-    int before = 0;
-    float top = 0.0f;
+    constexpr bool kWeigh = NT == 1 && kGrad;  // a workgroup of its own, the first, finds the largest finite weight
+    if (kWeigh && blockIdx.x == 0) {
+        __shared__ float top_sh[4];
+        if (blockIdx.y > 0) return;
+        float top = 0.0f;
 #pragma unroll 8
-    for (int r = threadIdx.x; r < first_row; r += 256) {
-        const bool kept = counts(r);
-        before += kept;
-        if (weighs) top = fmaxf(top, kept ? weight(r) : 0.0f);
+        for (int r = threadIdx.x; r < a.rows; r += 256) {
+            const float g = fabsf(a.grad_loss[r]);
+            top = counts(r) && g < __builtin_inff() ? fmaxf(top, g) : top;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        if (lane == 0) top_sh[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(top_sh[0], top_sh[1]), fmaxf(top_sh[2], top_sh[3]));
+        if (threadIdx.x == 0) p.top() = top > 0.0f ? top : 1.0f;
+        return;
     }
+    const int block = (int)blockIdx.x - kWeigh, first_row = block * runs * kPrepRows;
+    int before = 0;
+#pragma unroll 8
+    for (int r = threadIdx.x; r < first_row; r += 256) before += counts(r);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
     if (lane == 0) before_sh[wave] = before;
     const bool first = blockIdx.y == 0;
-    if (first && blockIdx.x == 0 && threadIdx.x < 64) reinterpret_cast<uint32_t*>(p.work + 256)[threadIdx.x] = 0;
+    if (first && block == 0 && threadIdx.x < 64) reinterpret_cast<uint32_t*>(p.work + 256)[threadIdx.x] = 0;
     __syncthreads();
     before = before_sh[0] + before_sh[1] + before_sh[2] + before_sh[3];
     uint16_t* out = p.at<uint16_t>(p.w.h_at);
@@ -365,15 +372,14 @@ __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, P
             const uint64_t all = __ballot(kept);
             const int mine = __popcll(all & ((1ull << lane) - 1)), c = before + mine;
             if (kept) local[mine] = r;
-            if (weighs && kept) top = fmaxf(top, weight(r));
             if (first && kept) {
                 p.at<int>(p.w.rows_at)[c] = r;
                 p.at<int>(p.w.target_at)[c] = a.targets[r];
-                if (grad) {
+                if (kGrad) {
                     p.at<float>(p.w.lse_at)[c] = a.lse[r];
                     p.at<float>(p.w.gl_at)[c] = a.grad_loss[r];
                 }
-            } else if (first && in && !grad) {
+            } else if (first && in && !kGrad) {
                 const float x = a.targets[r] < 0 ? 0.0f : __builtin_nanf("");
                 if (a.loss) a.loss[r] = x;
                 if (a.lse) a.lse[r] = x;
@@ -417,14 +423,6 @@ __global__ __launch_bounds__(256) void lhl_prepare_kernel(lm_head_loss_args a, P
         }
         before += kept;
         __syncthreads();  // local and kept_sh have been read
-    }
-    if (weighs) {
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-        if (lane == 0) top_sh[wave] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(top_sh[0], top_sh[1]), fmaxf(top_sh[2], top_sh[3]));
-        if (threadIdx.x == 0) p.top() = top > 0.0f ? top : 1.0f;
     }
 }
 
@@ -678,7 +676,11 @@ template <int NT>
 hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStream_t s) {
     const unsigned columns = std::min(4, p.w.pitch / LHL_STEP);
     const int blocks = std::max(1, (a.rows + kPrepRows - 1) / kPrepRows), runs = (blocks + 511) / 512;
-    lhl_prepare_kernel<NT><<<dim3((unsigned)((blocks + runs - 1) / runs), columns), 256, 0, s>>>(a, p, runs, grad);
+    const dim3 grid((unsigned)((blocks + runs - 1) / runs + (NT == 1 && grad)), columns);
+    if (grad)
+        lhl_prepare_kernel<NT, true><<<grid, 256, 0, s>>>(a, p, runs);
+    else
+        lhl_prepare_kernel<NT, false><<<grid, 256, 0, s>>>(a, p, runs);
     return hipGetLastError();
 }
 
