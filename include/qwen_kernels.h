@@ -567,8 +567,9 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  * float32 hidden states keep their 24 bits (three bf16 terms) in the logits and in
  * grad_h; in grad_table, whose results are bf16, they and D have 16 (two terms: 3 x 2^-16
  * of the products).  Sums, lse and D are float32; D as grad_h's operand is bf16 (dtype
- * bf16, its weights over the call's largest finite |grad_loss|, so that equal ones are 1)
- * or has 24 bits (float32).  Float32 states of 3.396e38 or more count as infinite.
+ * bf16, its weights over the call's largest finite |grad_loss|, so that equal ones are 1;
+ * of a row whose weight is below 2^-80 of that the smaller probabilities are lost) or
+ * has 24 bits (float32).  Float32 states of 3.396e38 or more count as infinite.
  *
  * A row with a target below 0 is ignored, whatever h holds there: loss, lse and
  * its row of grad_h are 0.  A target of vocab or more gives NaN in the three,
