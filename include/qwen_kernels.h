@@ -568,8 +568,9 @@ int gdn_dev_step(const gdn_dev_args* args, void* stream);
  * grad_h; in grad_table, whose results are bf16, they and D have 16 (two terms: 3 x 2^-16
  * of the products).  Sums, lse and D are float32; D as grad_h's operand is bf16 (dtype
  * bf16, its weights over the call's largest finite |grad_loss|, so that equal ones are 1;
- * of a row whose weight is below 2^-80 of that the smaller probabilities are lost) or
- * has 24 bits (float32).  Float32 states of 3.396e38 or more count as infinite.
+ * of a row whose weight is below 2^-80 of that the smaller probabilities are lost; what
+ * the rounding leaves out at a target goes to its row's grad_h in float32) or has 24 bits
+ * (float32).  Float32 states of 3.396e38 or more count as infinite.
  *
  * A row with a target below 0 is ignored, whatever h holds there: loss, lse and
  * its row of grad_h are 0.  A target of vocab or more gives NaN in the three,

@@ -25,6 +25,7 @@ struct LossWork {
     size_t place_at;    // int: original row -> counted row, -1 ignored, -2 no such target
     size_t logit_at;    // float: the target's logit
     size_t lse_at, gl_at;  // float: lse and the loss's gradient of each counted row
+    size_t rest_at;     // float: what the rounding of D left out at the target (the gradient of bf16 states)
     size_t h_at;        // bf16 [terms][rows][pitch]
     size_t part_at;     // float2 [rows][vtiles]: maximum and sum of exponentials of a tile's logits
     size_t d_at;        // bf16 [terms][rows][piece]
@@ -50,6 +51,7 @@ inline LossWork loss_work(const lm_head_loss_args& a, bool grad, bool grad_h) {
     w.logit_at = put(4 * n);
     w.lse_at = put(4 * n);
     w.gl_at = put(4 * n);
+    if (grad && w.terms == 1) w.rest_at = put(4 * n);
     w.h_at = put(2 * n * w.terms * w.pitch);
     if (!grad) {
         w.part_at = put(8 * n * w.vtiles);

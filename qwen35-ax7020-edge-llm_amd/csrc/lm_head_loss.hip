@@ -7,7 +7,8 @@
 // With bf16 states D is an operand of one bf16 term, and holds g_n over the call's largest |g|, which both gradients
 // are multiplied by in float32.  Under a mean loss, whose weights are all the same, a target's entry is then -1 + p,
 // which bf16 holds almost exactly where p is small; g (-1 + p) would be rounded the same way in every row, by up to
-// 2^-8 that no sum takes out.
+// 2^-8 that no sum takes out.  What the rounding leaves out at a target, the largest of its row's D, goes to grad_h with the
+// target's table row in float32.
 //
 // lhl_prepare_kernel gathers the rows that count (a text's own prompt often does
 // not), as bf16 terms.  The rest are tiled products on the matrix cores:
@@ -460,6 +461,20 @@ __global__ __launch_bounds__(P::kThreads) void lhl_logits_kernel(lm_head_loss_ar
             float gl = p.at<float>(p.w.gl_at)[row];
             if (NT == 1) gl /= p.top();
             const int hit = p.at<int>(p.w.target_at)[row] - vw;
+            if constexpr (NT == 1) {
+                // the target's entry once more, to its last bit: its logit halves the lane's values by a bit of its place
+                f32x4 of[P::MT];
+#pragma unroll
+                for (int i = 0; i < P::MT; ++i) of[i] = acc[i][j];
+#pragma unroll
+                for (int b = P::MT / 2; b > 0; b /= 2)
+#pragma unroll
+                    for (int i = 0; i < b; ++i) of[i] = hit & 16 * b ? of[i + b] : of[i];
+                const float even = hit & 2 ? of[0][2] : of[0][0], odd = hit & 2 ? of[0][3] : of[0][1];
+                const float at_target = gl * (exp2_raw(((hit & 1 ? odd : even) - lse) * kLog2e) - 1.0f);
+                if (hit >= 0 && hit < 16 * P::MT && hit % 16 < 4 && nw + 16 * j < count)
+                    p.at<float>(p.w.rest_at)[row] = at_target - to_float(from_float<uint16_t>(at_target));
+            }
 #pragma unroll
             for (int i = 0; i < P::MT; ++i)
 #pragma unroll
@@ -618,9 +633,22 @@ __global__ __launch_bounds__(P::kThreads) void lhl_grad_h_kernel(lm_head_loss_ar
 template <class T>
 __global__ __launch_bounds__(256) void lhl_finish_kernel(lm_head_loss_args a, Parts p) {
     __shared__ f32x4 sh[4][64];
-    const int row = blockIdx.x, at = p.at<int>(p.w.place_at)[row], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.x, at = p.at<int>(p.w.place_at)[row], target = a.targets[row];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int h = 256 * blockIdx.y + 4 * lane;
     f32x4 x = {0, 0, 0, 0};
+    float rest = 0.0f;
+    uint16_t w[4] = {0, 0, 0, 0};
+    if (sizeof(T) == 2 && at >= 0 && wave == 0) {  // (bf16 states: the target's part)
+        rest = p.at<float>(p.w.rest_at)[at];
+        const uint16_t* from = a.table + (int64_t)target * a.table_row + h;
+        if (h + 4 <= a.hidden)
+            __builtin_memcpy(w, from, 8);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (h + e < a.hidden) w[e] = from[e];
+    }
     if (at >= 0 && h < p.w.pitch) {
         const float* sum = p.at<float>(p.w.sum_at) + (size_t)at * p.w.pitch + h;
         const int s0 = p.w.splits * wave / 4, s1 = p.w.splits * (wave + 1) / 4;
@@ -631,7 +659,11 @@ __global__ __launch_bounds__(256) void lhl_finish_kernel(lm_head_loss_args a, Pa
     __syncthreads();
     if (wave > 0) return;
     x = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
-    if (sizeof(T) == 2) x *= p.top();
+    if (sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(rest, to_float(w[e]), x[e]);
+        x *= p.top();
+    }
     T* out = static_cast<T*>(a.grad_h) + (int64_t)row * a.grad_h_row + h;
 #pragma unroll
     for (int e = 0; e < 4; ++e)

@@ -397,3 +397,29 @@ def test_many_bf16_rows_and_any_table(gpu, rows, vocab, hidden, pad, base):
                                       (got_w, gw, (D ** 2).t() @ H ** 2, sums)):
         off = float((got.double().cpu() - want).norm())
         assert off <= step * (float(want.norm()) + float(terms.sum()) ** 0.5) + 2.0 ** -8 * float(targets.norm()), off
+
+
+@pytest.mark.parametrize("rows,vocab,hidden", [(40, 900, 73), (150, 4000, 128), (1300, 4000, 128), (1024, 2305, 321)])
+def test_states_gradients_have_their_targets_whole(gpu, rows, vocab, hidden):
+    """bf16 states with a weight for each sequence: a row's gradient is mostly its target's, whose part is kept in float32.
+    What is left of D's rounding are the other entries', 2^-8 / sqrt 3 of their terms' norm, besides the result's own; along
+    the gradient, which no weight may stretch, 6 standard deviations of either and 2^-13 for sums in float32."""
+    h, table, _, _ = inputs(rows, vocab, hidden, BF16, ignored=0.0)
+    table = (table.float() * 0.5).to(BF16)
+    t = torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(6), dtype=torch.int32).cuda()
+    lengths = torch.tensor([1.0, 173, 41, 331]).repeat_interleave((rows + 3) // 4)[:rows]
+    gl = (1.0 / lengths).cuda()
+    _, _, want, _, _, _ = oracle(h, table, t, gl)
+    _, lse = gpu.lm_head_loss(h, table, t)
+    got, _ = gpu.lm_head_loss_grad(h, table, t, lse, gl)
+    p = torch.softmax(h.double().cpu() @ table.double().cpu().t(), 1)
+    p[torch.arange(rows), t.long().cpu()] = 0.0
+    step = 2.0 ** -8 / 3 ** 0.5
+    terms = (p ** 2 @ table.double().cpu() ** 2).sum(1).sqrt() * gl.double().cpu()
+    got = got.double().cpu()
+    for first in range(0, rows, (rows + 3) // 4):  # each weight by itself
+        r = slice(first, first + (rows + 3) // 4)
+        top = float(want[r].norm())
+        assert float((got[r] - want[r]).norm()) <= step * (top + float(terms[r].norm()))
+        along = float((got[r] * want[r]).sum()) / top ** 2 - 1
+        assert abs(along) <= 12 * step / want[r].numel() ** 0.5 + 2.0 ** -13, along
