@@ -230,7 +230,7 @@ __device__ __forceinline__ void sync_lds() {
 // One chunk of one value head; wavefront w has tokens 16 w .. 16 w + 15.  What it writes is
 // in the order in which gdn_scan_kernel loads it.  direct: that kernel takes K and Q from
 // the inputs.  Memory bounds it: K and Q in, 31 KiB of T and P out; at 16,384 tokens of 16
-// heads of 128 in bf16 61 us, 4.3 TB/s.  Inverting (I + L) one column a lane over all 64 rows
+// heads of 128 in bf16 62 us, 4.2 TB/s.  Inverting (I + L) one column a lane over all 64 rows
 // left three wavefronts idle and took 145; in blocks of 16 all four work.
 template <int KS, int NT, bool kDelta>
 __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n_chunks, int short_to, int full_q,
@@ -459,9 +459,9 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(gdn_dev_args a, size_t n
 // it some 30 cycles.  The state, the right side and U pass between wavefronts as bf16 terms in LDS, lane by
 // lane (see state_row).  Other fragments of the next chunk are loaded into each register as soon as it
 // is free.
-// The chain bounds it: at one sequence of 16,384 tokens, 16 heads of 128, bf16, 413 us, 1.6 us (3,600 cycles)
+// The chain bounds it: at one sequence of 16,384 tokens, 16 heads of 128, bf16, 415 us, 1.6 us (3,600 cycles)
 // a chunk, of which the first four wavefronts work 1,100, 720 and 980 cycles between barriers and wait
-// for the others and for skew the rest; at 24 float32 prompts of 9,001 tokens in all 180 us.
+// for the others and for skew the rest; at 24 float32 prompts of 9,001 tokens in all 181 us.
 // With four wavefronts that do everything and load for themselves the first took 1,190 us.
 template <int KS, int NT, int NC, bool kDelta, bool kDirect, class T>
 __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t n_chunks, int slices,
@@ -1025,7 +1025,7 @@ __device__ __forceinline__ void to_lanes(float x, float (&y)[4]) {
 }
 
 // With the old state S: u = b (v - a S^T k), out = scale (a S^T q + (k.q) u), S <- a S + k u^T:
-// one pass over the state, whose bytes bound one token (256 sequences of 16 heads of 128: 86 us, 6.3 TB/s).  A
+// one pass over the state, whose bytes bound one token (256 sequences of 16 heads of 128: 87 us, 6.2 TB/s).  A
 // wavefront has G groups of four value columns; lane 4 g + l has rows 4 (g + 16 n) .. + 3 of column l of
 // each, one 16-byte load and store each, 1 KiB a wavefront.  The sums over lanes stay in registers, and four
 // columns' share their steps (each by itself, through LDS: 95 us; 16 tokens of 64 sequences 73 us, each by itself 92).

@@ -19,11 +19,11 @@
 // and lhl_loss_kernel / lhl_finish_kernel join the parts.  Every sum has one fixed
 // order: results repeat bit for bit.
 //
-// What bounds it.  Few rows: the table's bytes (one row of 65536 x 1024: the logits 26 us,
+// What bounds it.  Few rows: the table's bytes (one row of 65536 x 1024: the logits 25 us,
 // the table's at the rate of a copy 26).  Many: the matrix cores (4096 rows: the logits and their
-// statistics 476 us, 1.15 PFLOP/s; a library product of that shape alone 533).  The
+// statistics 490 us, 1.12 PFLOP/s; a library product of that shape alone 533).  The
 // gradient computes the logits again, in pieces of the vocabulary: 4096 rows, 3277 of
-// them counted, for each of four pieces 131 us of logits and D, 139 of grad_h, 106 of grad_table.
+// them counted, for each of four pieces 137 us of logits and D, 140 of grad_h, 110 of grad_table.
 #include "bf16_terms.h"
 #include "lm_head_loss.h"
 
@@ -717,8 +717,8 @@ hipError_t prepare(const lm_head_loss_args& a, const Parts& p, bool grad, hipStr
 }
 
 // Vocabulary rows and counted rows of a tile of logits.  Up to 32 rows take tiles of 128 x 32, which leave two
-// workgroups of three stages a compute unit (one row: 26 us); up to 64 of 256 x 64 (48 float32 rows: 29 us, in
-// tiles of 128 x 64 a third more); many bf16 ones of 256 x 256 (4096: 476 us, in tiles of 128 x 128 7 % more), whose
+// workgroups of three stages a compute unit (one row: 25 us); up to 64 of 256 x 64 (48 float32 rows: 30 us, in
+// tiles of 128 x 64 a third more); many bf16 ones of 256 x 256 (4096: 490 us, in tiles of 128 x 128 7 % more), whose
 // operands are the fewest bytes of LDS a product; the others of 128 x 128, but float32's three terms of 256 x 128 where
 // there is more than one such for a compute unit, whose LDS either fills: with eight wavefronts in place of
 // four (4096 x 65536 x 1024: 1.28 ms for 1.67; 200 x 3000 45 us for 37).
@@ -797,7 +797,7 @@ hipError_t grad(const lm_head_loss_args& a, const Parts& p, hipStream_t s) {
         if (e == hipSuccess && a.grad_table) {
             constexpr int N2 = NT == 1 ? 1 : 2;  // a bf16 result: 3 x 2^-16 of its terms
             if constexpr (NT == 1)
-                if (a.rows >= 1024) {  // (4096 rows' piece 106 us, in tiles of 128 x 128 15 % more)
+                if (a.rows >= 1024) {  // (4096 rows' piece 110 us, in tiles of 128 x 128 15 % more)
                     using P = Product<256, 256, 2, 4, true, true, 1, 1, 1, true, 2>;
                     const int tm = (p.w.pitch + 255) / 256, tn = (width + 255) / 256;
                     lhl_grad_table_kernel<P, true>
