@@ -58,7 +58,8 @@ __device__ __forceinline__ void load_terms(const void* row, int i, int dim, bool
     }
 }
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+// As bf16 terms: from bf16's largest value and half a step on the first one is infinite.
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < 0x1.ffp127f; }
 
 // 2^d, d <= 0 as a rule; the whole part exactly.
 __device__ __forceinline__ float exp2_of(double d) {
@@ -941,7 +942,18 @@ __global__ __launch_bounds__(576, 1) void gdn_scan_kernel(gdn_dev_args a, size_t
                     u[x][e] = c * C + 16 * w + 4 * grp + e < len ? to_float<T>(v[x][e]) : 0.0f;
                 into[x] = u[x] * down;
             }
-            if (__builtin_expect(any_bad(into), 0)) leave_out(u, into);
+            // (a bf16 that is finite fits; a float32 may fit only after its decay)
+            if (__builtin_expect(any_bad(into) || (NT == 3 && any_bad(u)), 0)) {
+                leave_out(u, into);
+                if constexpr (NT == 3) {
+#pragma unroll
+                    for (int x = 0; x < NC; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!finite(u[x][e])) into[x][e] = __builtin_nanf("");
+                    leave_out(u, u);
+                }
+            }
             load_v(nx);
         }
 #pragma unroll

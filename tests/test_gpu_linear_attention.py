@@ -570,3 +570,20 @@ def test_nan_and_infinity_do_not_go_back(gpu, hk, hv, dk, dv, packed, delta, dty
                 got[1, x], wst[1, x] = 0.0, 0.0
         assert torch.equal(torch.isfinite(got).cpu(), torch.isfinite(wst)), kind
         near(torch.where(torch.isfinite(got), got, nan), torch.where(torch.isfinite(wst), wst, nan))
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("kind", ["k", "v"])
+def test_values_past_bf16s_largest_do_not_go_back(gpu, kind, delta):
+    """A float32's largest value counts as infinite: what it is in shows it from its token on, and not before."""
+    q, k, v, al, be, st = inputs(150, 2, 2, 64, 64, F, delta, 1)
+    (k if kind == "k" else v)[100, 1, 7] = torch.finfo(F).max
+    want, _ = oracle(q, k, v, al, be, 1.0, st, [(0, 150)])
+    out, got = gpu.linear_attention_prompt(q, k, v, al, be, state_in=st)
+    near(out[:100], want[:100])
+    near(out[:, 0], want[:, 0])
+    columns = slice(None) if kind == "k" else 7
+    assert not bool(torch.isfinite(out[100:, 1, columns]).any())
+    if kind == "v":
+        keep = torch.arange(64) != 7
+        near(out[:, 1, keep.cuda()], want[:, 1, keep])
