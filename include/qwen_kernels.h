@@ -609,6 +609,157 @@ size_t bf16_dev_lm_head_loss_grad_work_bytes(const lm_head_loss_args* args);
 int bf16_dev_lm_head_loss(const lm_head_loss_args* args, void* stream);
 int bf16_dev_lm_head_loss_grad(const lm_head_loss_args* args, void* stream);
 
+/* Rotary positions.  Row r's head holds rot / 2 pairs (x_i, y_i) in its first rot
+ * elements: elements i and i + rot / 2, or with interleaved not 0 elements 2 i and
+ * 2 i + 1.  At position p = positions[r] (any int32), with t = p freqs[i]:
+ *
+ *   x' = amplitude (x cos t - y sin t);  y' = amplitude (x sin t + y cos t)
+ *
+ * and elements from rot on pass unchanged.  rope_dev_grad: the gradient to x, from
+ * the gradient of x' in args->x (the transposed rotation: sin t with its sign
+ * changed).  The engine's apply_rope on host arrays (04/qwen_real_engine.py:225-630)
+ * is its counterpart in the reference.
+ *
+ * freqs: rot / 2 doubles on the device, radians a position (a context's scaling is
+ * in them and in the amplitude).  t is made and brought into one turn in double, so that a far
+ * position's angle is off by 2^-53 of itself (at 2^20 radians 2^-33); its sine and
+ * cosine and the rotation are float32, and a bf16 result is rounded once.
+ *
+ * x, out: rows x heads x dim, float32 or bf16 (dtype), head h of row r at
+ * r * x_row + h * x_head elements.  out may be x with the same strides (elements from rot on are
+ * then not touched); other overlaps are not allowed.  rot even, 2 to dim; dim up to
+ * 1024, heads up to 65536, rows heads up to 2^28.  A NaN or infinity stays within its pair.
+ * Nothing is allocated and nothing waits: the calls can be captured. */
+typedef struct rope_dev_args {
+    void* out;
+    const void* x;
+    const int32_t* positions;
+    const double* freqs;
+    int64_t out_row, out_head, x_row, x_head;
+    int rows, heads, dim, rot;
+    int dtype, interleaved;
+    float amplitude;
+} rope_dev_args;
+int rope_dev_apply(const rope_dev_args* args, void* stream);
+int rope_dev_grad(const rope_dev_args* args, void* stream);
+
+/* A cache of keys and values in pages, and what a call adds to it.
+ *
+ * key_cache and value_cache hold `pages` pages of `page` tokens: head h of page
+ * p's token i is the dim elements at p * cache_page + i * cache_token +
+ * h * cache_head (elements; the same in both), 16-byte aligned.  Sequence s has its
+ * pages in tables[s * table_row ..], table_pages of them: place j of the
+ * sequence is token j % page of page tables[s * table_row + j / page].  Two sequences may
+ * share pages.  A place past the table, or whose table entry is not one of the pages (-1),
+ * does not exist: nothing is written there, and attention does not see it.
+ *
+ * cached[s]: tokens that sequence s holds before this call's own, the same number in
+ * every layer's calls.  Below 0 the sequence is skipped (an empty place of a padded
+ * batch).  The call's rows are packed: sequence s has rows starts[s] ..
+ * starts[s + 1] - 1 (device array of n_seq + 1 ascending values within 0 .. rows), of any number, none included;
+ * starts NULL: rows / n_seq each.  Row i of a sequence goes to place cached[s] + i.
+ * Rows that no sequence holds are neither read nor written.
+ *
+ * kv_dev_append writes a call's keys and values to their places.  With rot above 0 the
+ * keys are rotated on the way as rope_dev_apply does, at positions[row], or (NULL)
+ * at their place; q, if not NULL, is rotated to q_out in the same launch (of every row of a sequence
+ * that is not skipped; q_out may be q with the same strides).  rot 0: keys as they are, and no q.
+ * Places of one call have to be different: where two rows meet in one, each 16-byte part of it
+ * is from one of the two.
+ *
+ * dtype: of q, k, v and the cache (QWEN_F32, QWEN_BF16).  dim a multiple of 8 up
+ * to 256; heads_q (with q) a multiple of heads_k; rows of k, v, q and q_out have strides in
+ * elements as in rope_dev_args and are aligned to their elements; page up to 65536, page
+ * table_pages up to 2^30, rows heads up to 2^28.  Nothing the call reads overlaps what it writes.
+ * Nothing is allocated and nothing waits: the calls can be captured.  The engine's
+ * PagedAttentionPool (04/qwen_real_engine.py:225-630, pages of 16 tokens) is the host's counterpart. */
+typedef struct kv_dev_append_args {
+    void* key_cache;
+    void* value_cache;
+    void* q_out;
+    const void* k;
+    const void* v;
+    const void* q;
+    const int32_t* tables;
+    const int32_t* cached;
+    const int32_t* starts;
+    const int32_t* positions;
+    const double* freqs;
+    int64_t cache_page, cache_token, cache_head, table_row;
+    int64_t k_row, k_head, v_row, v_head, q_row, q_head, q_out_row, q_out_head;
+    int rows, n_seq, pages, page, table_pages;
+    int heads_q, heads_k, dim, rot;
+    int dtype, interleaved;
+    float amplitude;
+} kv_dev_append_args;
+int kv_dev_append(const kv_dev_append_args* args, void* stream);
+
+/* Attention over such a cache, this call's own tokens in it already.  Head h of row i of sequence
+ * s, on key head h / (heads_q / heads_k), sees the places j <= cached[s] + i, or with a mask the places
+ * j < cached[s] and, of the sequence's n rows' places, cached[s] + j for each j < n whose bit is set (word
+ * j / 32 of mask[row * mask_words ..], bit j % 32; words past mask_words count as 0):
+ *
+ *   o = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q . k_j)
+ *
+ * A row that sees nothing (or whose every score is -infinity) is 0.  A single token of each sequence is n = 1, a prompt
+ * any number, and drafted tokens that branch have attn_dev_tree's mask.
+ *
+ * Scores, maxima, sums and o are float32.  With bf16 the weights w_j are rounded to bf16 as an operand of their
+ * product with v, each by up to 2^-9 of itself either way, and the sum that divides takes the rounded ones, so that
+ * equal weights leave no error.  A NaN or infinity in a key or value shows in the rows that see it and in no
+ * other; one that no row sees (a later token's, a free place's) in none.
+ *
+ * Rows of a skipped sequence, and rows that no sequence holds, are left as they were; with zero_rest
+ * not 0 a skipped sequence's rows are set to 0.  work: device memory of attn_dev_paged_work_bytes() (which takes the
+ * sizes alone, not cached or tables), 256-byte aligned, the caller's (calls that may overlap need one each).
+ * The same call gives the same bits; in another call they may differ in rounding, as the
+ * keys are split over workgroups by the lengths of the whole call.
+ *
+ * scale finite and above 0; dim a multiple of 8 up to 256; heads_q a multiple of heads_k, rows heads_q up to 2^28;
+ * n_seq up to 2^20; mask_words up to 2^16 (mask NULL: not read).  q and out are aligned to their elements, the
+ * cache to 16 bytes (pointers and strides).  out overlaps nothing that the call reads.
+ * Nothing is allocated and nothing waits: the calls can be captured.  full_attn_f32 (04/qwen_attn.c:406) is the
+ * host's counterpart for one sequence. */
+typedef struct attn_dev_args {
+    void* out;
+    const void* q;
+    const void* key_cache;
+    const void* value_cache;
+    const int32_t* tables;
+    const int32_t* cached;
+    const int32_t* starts;
+    const int32_t* mask;
+    void* work;
+    size_t work_bytes;
+    int64_t cache_page, cache_token, cache_head, table_row;
+    int64_t q_row, q_head, out_row, out_head;
+    int rows, n_seq, pages, page, table_pages;
+    int heads_q, heads_k, dim, mask_words;
+    int dtype;
+    float scale;
+    int zero_rest;
+} attn_dev_args;
+size_t attn_dev_paged_work_bytes(const attn_dev_args* args); /* 0: invalid sizes */
+int attn_dev_paged(const attn_dev_args* args, void* stream);
+
+/* The mask and positions of drafted tokens from their tree.  parents[row] is the place among
+ * its sequence's rows of the token that a row's token follows, an earlier one; a value below 0
+ * (or not below the row's own place) makes it follow the cached text.  Bit j of a row is set where j is
+ * the row's own place or one of its ancestors', positions[row] = cached[s] + its number of ancestors
+ * (positions NULL: not written).  Rows of skipped sequences have no bits and position 0; rows that no
+ * sequence holds are left as they were.  Once for all layers of a step: the bits do not change
+ * between them.  words: of 32 bits, for each row; places of 32 words and more have no bit.
+ * rows words up to 2^28, n_seq up to 2^20. */
+typedef struct attn_dev_tree_args {
+    int32_t* mask;
+    int32_t* positions;
+    const int32_t* parents;
+    const int32_t* cached;
+    const int32_t* starts;
+    int rows, n_seq, words;
+} attn_dev_tree_args;
+int attn_dev_tree(const attn_dev_tree_args* args, void* stream);
+
 /* Synthetic reference-format planes on the device: mantissas uniform in
  * [-127, 127], exponents uniform in [e_lo, e_hi], from a counter-based hash
  * of (seed, index) -- bfp8_synth_planes_host gives the same bytes. */

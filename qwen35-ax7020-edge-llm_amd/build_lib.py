@@ -15,6 +15,8 @@ Translation units:
   csrc/batch_mfma.hip        the batched GEMV (up to 16 vectors) on the matrix cores, f32 flush-to-zero
   csrc/linear_attention.hip  gated linear attention over prompts and batches, IEEE
   csrc/lm_head_loss.hip      the bf16 head's loss and gradient, IEEE
+  csrc/kv_cache.hip          rotary positions, the paged cache's append, drafted tokens' masks, IEEE
+  csrc/paged_attention.hip   attention over the paged cache, IEEE
   csrc/qwen_kernels_api.cpp  C ABI host code (include/qwen_kernels.h)
   csrc/qwen_runtime_api.cpp  C ABI of the runtime kernels and the forward loop
   csrc/qwen_weights.cpp      manifest-driven weight-image loader
@@ -65,6 +67,8 @@ UNITS = {
     "noalloc.hip": [],
     "linear_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "lm_head_loss.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kv_cache.hip": [],
+    "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "qwen_kernels_api.cpp": [],
     "qwen_runtime_api.cpp": [],
     "qwen_weights.cpp": [],

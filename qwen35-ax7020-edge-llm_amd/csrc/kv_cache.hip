@@ -1,0 +1,310 @@
+// kv_cache.hip -- positions rotated into queries and keys, keys and values on their
+// way to a paged cache, and the masks of drafted tokens (rope_dev_apply, rope_dev_grad,
+// kv_dev_append, attn_dev_tree).
+//
+//   (x, y) -> A (x cos t - y sin t, x sin t + y cos t),  t = p f_i
+//
+// A workgroup has a few rows: their angles go to LDS once for all heads, then every thread
+// takes 16-byte pieces of the rows' heads.  What bounds it: few rows, the latency of a launch and
+// of the loads that depend on one another (sequence, length, page); many, memory.
+#include "bf16_terms.h"
+#include "kv_cache.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxRows = 4;       // of a workgroup
+constexpr int kMaxPairs = 512;    // of a head
+
+// Sine and cosine of p f: the angle is brought into one turn in double, where a float32 product would have lost the
+// turn's fraction (2^20 positions of 1 radian: 2^-4 of a radian), and -- as half turns of up to 1 -- is rounded to float32
+// only then, 2^-24 of an angle of up to pi.
+__device__ __forceinline__ float2 angle_of(int p, double f, float amplitude, bool back) {
+    const double turns = (double)p * f * 0.15915494309189533577;
+    float s, c;
+    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    return {amplitude * c, back ? -amplitude * s : amplitude * s};
+}
+
+template <class T, int N>
+struct Piece {
+    T x[N];
+};
+
+// How a head is taken apart: first `turned` units of pairs, then the units that pass unchanged.
+// VEC: 16 bytes a unit (from both halves of the rotated part in the half layout), else a pair or an element.
+template <class T, bool VEC, bool INTER>
+struct Head {
+    static constexpr int N = VEC ? 16 / sizeof(T) : 1;      // elements of a unit that passes
+    static constexpr int P = !VEC ? 1 : INTER ? N / 2 : N;  // pairs of a unit that is rotated
+    using V = Piece<T, N>;
+    using V2 = Piece<T, VEC && INTER ? N : 2 * P>;
+
+    static __device__ int turned(int rot) { return rot / 2 / P; }
+    static __device__ int passed(int dim, int rot) { return (dim - rot) / N; }
+
+    static __device__ __forceinline__ void turn(const T* x, T* y, int u, int rot, const float2* cs) {
+        float a[P], b[P];
+        if constexpr (INTER) {
+            V2 v;
+            load(v, x + u * 2 * P);
+#pragma unroll
+            for (int j = 0; j < P; ++j) a[j] = to_float(v.x[2 * j]), b[j] = to_float(v.x[2 * j + 1]);
+        } else {
+            V v, w;
+            load(v, x + u * P);
+            load(w, x + rot / 2 + u * P);
+#pragma unroll
+            for (int j = 0; j < P; ++j) a[j] = to_float(v.x[j]), b[j] = to_float(w.x[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const float2 t = cs[u * P + j];
+            const float xa = a[j], xb = b[j];
+            a[j] = __builtin_fmaf(xa, t.x, -(xb * t.y));
+            b[j] = __builtin_fmaf(xa, t.y, xb * t.x);
+        }
+        if constexpr (INTER) {
+            V2 v;
+#pragma unroll
+            for (int j = 0; j < P; ++j) v.x[2 * j] = from_float<T>(a[j]), v.x[2 * j + 1] = from_float<T>(b[j]);
+            store(y + u * 2 * P, v);
+        } else {
+            V v, w;
+#pragma unroll
+            for (int j = 0; j < P; ++j) v.x[j] = from_float<T>(a[j]), w.x[j] = from_float<T>(b[j]);
+            store(y + u * P, v);
+            store(y + rot / 2 + u * P, w);
+        }
+    }
+    static __device__ __forceinline__ void pass(const T* x, T* y, int u, int rot) {
+        V v;
+        load(v, x + rot + u * N);
+        store(y + rot + u * N, v);
+    }
+
+    template <class X>
+    static __device__ __forceinline__ void load(X& v, const T* p) {
+        if constexpr (sizeof(X) == 16)
+            v = __builtin_bit_cast(X, *reinterpret_cast<const u32x4*>(p));
+        else
+#pragma unroll
+            for (size_t j = 0; j < sizeof(X) / sizeof(T); ++j) v.x[j] = p[j];
+    }
+    template <class X>
+    static __device__ __forceinline__ void store(T* p, const X& v) {
+        if constexpr (sizeof(X) == 16)
+            *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, v);
+        else
+#pragma unroll
+            for (size_t j = 0; j < sizeof(X) / sizeof(T); ++j) p[j] = v.x[j];
+    }
+};
+
+// ---- rotation alone -------------------------------------------------------------------
+template <class T, bool VEC, bool INTER>
+__global__ __launch_bounds__(kThreads) void rope_kernel(rope_dev_args a, int each, int back, int copy) {
+    using H = Head<T, VEC, INTER>;
+    __shared__ float2 cs[kMaxRows * kMaxPairs];
+    const int half = a.rot / 2, turned = H::turned(a.rot), units = turned + (copy ? H::passed(a.dim, a.rot) : 0);
+    for (int64_t r0 = (int64_t)blockIdx.x * each; r0 < a.rows; r0 += (int64_t)gridDim.x * each) {
+        const int n = (int)min((int64_t)each, a.rows - r0);
+        for (int i = threadIdx.x; i < n * half; i += kThreads)
+            cs[i] = angle_of(a.positions[r0 + i / half], a.freqs[i % half], a.amplitude, back);
+        __syncthreads();
+        for (int i = threadIdx.x; i < n * a.heads * units; i += kThreads) {
+            const int head = i / units, u = i - head * units, r = head / a.heads, h = head - r * a.heads;
+            const T* x = static_cast<const T*>(a.x) + (r0 + r) * a.x_row + h * a.x_head;
+            T* y = static_cast<T*>(a.out) + (r0 + r) * a.out_row + h * a.out_head;
+            if (u < turned)
+                H::turn(x, y, u, a.rot, cs + r * half);
+            else
+                H::pass(x, y, u - turned, a.rot);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- to the cache -----------------------------------------------------------------------
+// A row's place: its sequence is not skipped; where in the cache (elements), -1 nowhere.
+struct Place {
+    int there;
+    int position;
+    int64_t at;
+};
+
+template <class T, bool VEC, bool INTER>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args a, Divisor page, int each, int copy_q,
+                                                             int copy_v) {
+    using H = Head<T, VEC, INTER>;
+    using C = Head<T, true, false>;  // values are copied 16 bytes at a time where they are aligned
+    __shared__ float2 cs[kMaxRows * kMaxPairs / 2];
+    __shared__ Place places[kMaxRows];
+    const int half = a.rot / 2, turned = H::turned(a.rot);
+    const int k_units = turned + H::passed(a.dim, a.rot), q_units = turned + (copy_q ? H::passed(a.dim, a.rot) : 0);
+    const int v_units = copy_v ? C::passed(a.dim, 0) : a.dim;
+    const int ks = a.heads_k * k_units, vs = a.heads_k * v_units, qs = a.q ? a.heads_q * q_units : 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * each; r0 < a.rows; r0 += (int64_t)gridDim.x * each) {
+        const int n = (int)min((int64_t)each, a.rows - r0);
+        if ((int)threadIdx.x < n) {
+            const int r = (int)r0 + threadIdx.x, s = owner_of(a.starts, a.rows, a.n_seq, r);
+            Place p{0, 0, -1};
+            if (s >= 0) {
+                const int held = a.cached[s];
+                if (held >= 0) {
+                    const int64_t place = (int64_t)held + r - span_of(a.starts, a.rows, a.n_seq, s).first;
+                    p.there = 1;
+                    p.position = a.positions ? a.positions[r] : (int)min(place, (int64_t)INT32_MAX);
+                    if (place < (int64_t)a.table_pages * a.page) {
+                        const uint32_t j = divide((uint32_t)place, page);
+                        const int id = a.tables[s * a.table_row + j];
+                        if ((unsigned)id < (unsigned)a.pages)
+                            p.at = id * a.cache_page + ((uint32_t)place - j * a.page) * a.cache_token;
+                    }
+                }
+            }
+            places[threadIdx.x] = p;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n * half; i += kThreads)
+            cs[i] = angle_of(places[i / half].position, a.freqs[i % half], a.amplitude, false);
+        if (half) __syncthreads();
+        for (int i = threadIdx.x; i < n * (ks + vs + qs); i += kThreads) {
+            const int r = i / (ks + vs + qs);
+            int u = i - r * (ks + vs + qs);
+            const Place p = places[r];
+            const int64_t row = r0 + r;
+            const float2* t = cs + r * half;
+            if (u < ks) {
+                if (p.at < 0) continue;
+                const int h = u / k_units;
+                u -= h * k_units;
+                const T* x = static_cast<const T*>(a.k) + row * a.k_row + h * a.k_head;
+                T* y = static_cast<T*>(a.key_cache) + p.at + h * a.cache_head;
+                if (u < turned)
+                    H::turn(x, y, u, a.rot, t);
+                else
+                    H::pass(x, y, u - turned, a.rot);
+            } else if (u < ks + vs) {
+                if (p.at < 0) continue;
+                u -= ks;
+                const int h = u / v_units;
+                u -= h * v_units;
+                const T* x = static_cast<const T*>(a.v) + row * a.v_row + h * a.v_head;
+                T* y = static_cast<T*>(a.value_cache) + p.at + h * a.cache_head;
+                if (copy_v)
+                    C::pass(x, y, u, 0);
+                else
+                    y[u] = x[u];
+            } else {
+                if (!p.there) continue;
+                u -= ks + vs;
+                const int h = u / q_units;
+                u -= h * q_units;
+                const T* x = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+                T* y = static_cast<T*>(a.q_out) + row * a.q_out_row + h * a.q_out_head;
+                if (u < turned)
+                    H::turn(x, y, u, a.rot, t);
+                else
+                    H::pass(x, y, u - turned, a.rot);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- drafted tokens' trees -----------------------------------------------------------------
+// A workgroup a sequence, a thread a word of a row's mask: it walks up the row's ancestors, whose places only fall,
+// until they are below its word; word 0's counts them all.
+constexpr int kTreeHeld = 4096;
+__global__ __launch_bounds__(kThreads) void attn_tree_kernel(attn_dev_tree_args a) {
+    __shared__ int32_t held_parents[kTreeHeld];
+    const int s = blockIdx.x;
+    const Span p = span_of(a.starts, a.rows, a.n_seq, s);
+    const int held = a.cached[s];
+    const int32_t* parents = a.parents + p.first;
+    const bool in_lds = p.count <= kTreeHeld;
+    if (in_lds) {
+        for (int i = threadIdx.x; i < p.count; i += kThreads) held_parents[i] = parents[i];
+        __syncthreads();
+    }
+    const int64_t items = (int64_t)p.count * a.words;
+    for (int64_t i = threadIdx.x; i < items; i += kThreads) {
+        const int r = (int)(i / a.words), w = (int)(i - (int64_t)r * a.words);
+        uint32_t bits = 0;
+        int depth = 0;
+        if (held >= 0)
+            for (int j = r; j >= 32 * w || (w == 0 && j >= 0);) {
+                if (j >> 5 == w) bits |= 1u << (j & 31);
+                const int up = in_lds ? held_parents[j] : parents[j];
+                if (up < 0 || up >= j) break;
+                ++depth;
+                j = up;
+            }
+        a.mask[(int64_t)p.first * a.words + i] = (int32_t)bits;
+        if (w == 0 && a.positions)
+            a.positions[p.first + r] = held < 0 ? 0 : (int)min((int64_t)held + depth, (int64_t)INT32_MAX);
+    }
+}
+
+bool whole(const void* p, int64_t row, int64_t head, size_t es) {
+    return ((uintptr_t)p | (uint64_t)row * es | (uint64_t)head * es) % 16 == 0;
+}
+// The rotated part falls into 16-byte pieces of whole pairs, what passes into 16-byte pieces.
+bool pieces(int dim, int rot, bool inter, size_t es) {
+    const int n = (int)(16 / es);
+    return rot % (inter ? n : 2 * n) == 0 && dim % n == 0;
+}
+
+}  // namespace
+
+hipError_t rope_launch(const rope_dev_args& a, bool back, hipStream_t s) {
+    const size_t es = a.dtype == QWEN_BF16 ? 2 : 4;
+    const bool vec = pieces(a.dim, a.rot, a.interleaved, es) && whole(a.x, a.x_row, a.x_head, es) &&
+                     whole(a.out, a.out_row, a.out_head, es);
+    const int copy = a.out != a.x, each = a.rows < 2048 ? 1 : kMaxRows;
+    const dim3 grid((unsigned)std::min((a.rows + each - 1) / each, 1 << 20));
+#define GO(T, V, I) rope_kernel<T, V, I><<<grid, kThreads, 0, s>>>(a, each, back, copy)
+    if (a.dtype == QWEN_BF16) {
+        if (a.interleaved)
+            vec ? GO(uint16_t, true, true) : GO(uint16_t, false, true);
+        else
+            vec ? GO(uint16_t, true, false) : GO(uint16_t, false, false);
+    } else {
+        if (a.interleaved)
+            vec ? GO(float, true, true) : GO(float, false, true);
+        else
+            vec ? GO(float, true, false) : GO(float, false, false);
+    }
+#undef GO
+    return hipGetLastError();
+}
+
+hipError_t kv_launch_append(const kv_dev_append_args& a, hipStream_t s) {
+    const size_t es = a.dtype == QWEN_BF16 ? 2 : 4;
+    const bool vec = pieces(a.dim, a.rot, a.interleaved, es) && whole(a.k, a.k_row, a.k_head, es) &&
+                     (!a.q || (whole(a.q, a.q_row, a.q_head, es) && whole(a.q_out, a.q_out_row, a.q_out_head, es)));
+    const int copy_q = a.q && a.q_out != a.q, copy_v = whole(a.v, a.v_row, a.v_head, es);
+    const int each = a.rows < 2048 ? 1 : kMaxRows;
+    const dim3 grid((unsigned)std::min((a.rows + each - 1) / each, 1 << 20));
+    const Divisor page = divisor(a.page);
+#define GO(T, V, I) kv_append_kernel<T, V, I><<<grid, kThreads, 0, s>>>(a, page, each, copy_q, copy_v)
+    if (a.dtype == QWEN_BF16) {
+        if (a.interleaved)
+            vec ? GO(uint16_t, true, true) : GO(uint16_t, false, true);
+        else
+            vec ? GO(uint16_t, true, false) : GO(uint16_t, false, false);
+    } else {
+        if (a.interleaved)
+            vec ? GO(float, true, true) : GO(float, false, true);
+        else
+            vec ? GO(float, true, false) : GO(float, false, false);
+    }
+#undef GO
+    return hipGetLastError();
+}
+
+hipError_t attn_launch_tree(const attn_dev_tree_args& a, hipStream_t s) {
+    attn_tree_kernel<<<dim3((unsigned)a.n_seq), kThreads, 0, s>>>(a);
+    return hipGetLastError();
+}

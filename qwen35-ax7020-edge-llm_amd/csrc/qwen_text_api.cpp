@@ -1,14 +1,17 @@
 // qwen_text_api.cpp -- C ABI of the operators over a text's tokens
-// (include/qwen_kernels.h): gated linear attention, the head's loss.  Arguments are
+// (include/qwen_kernels.h): gated linear attention, the head's loss, rotary positions,
+// the paged cache and the attention over it.  Arguments are
 // checked here; the library's lock is not held while a kernel is launched, and no
 // state of the library is used.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <mutex>
 
 #include "host_internal.h"
 #include "linear_attention.h"
 #include "lm_head_loss.h"
+#include "paged_attention.h"
 
 using namespace qhost;
 
@@ -99,6 +102,156 @@ size_t loss_bytes(const char* who, const lm_head_loss_args* a, bool grad) {
     return loss_work(*a, grad, grad && a->grad_h).total;
 }
 
+// ---- heads of rows and pages
+bool in(int64_t x, int64_t lo, int64_t hi) { return lo <= x && x <= hi; }
+constexpr int64_t kMaxStride = (int64_t)1 << 34;
+
+// An axis of a tensor whose innermost elements are `dim` in a run.
+struct Axis {
+    int64_t size, stride;
+};
+// The axes' places are `dim` elements each that do not overlap, within 2^60 elements.
+template <size_t N>
+bool apart(Axis (&axes)[N], int64_t dim) {
+    std::sort(axes, axes + N, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+    __int128 reach = dim;
+    for (const Axis& x : axes) {
+        if (x.size < 2) continue;
+        if (x.stride < reach) return false;
+        reach += (__int128)x.stride * (x.size - 1);
+    }
+    return reach <= (__int128)1 << 60;
+}
+bool heads_apart(int rows, int64_t row, int heads, int64_t head, int dim) {
+    Axis axes[] = {{rows, row}, {heads, head}};
+    return apart(axes, dim);
+}
+
+const char* rope_bad(const rope_dev_args* a) {
+    if (!a) return "no arguments";
+    if (a->dtype != QWEN_F32 && a->dtype != QWEN_BF16) return "dtype is neither QWEN_F32 nor QWEN_BF16";
+    if (!in(a->dim, 2, 1024) || !in(a->rot, 2, a->dim) || a->rot % 2) return "dim is 2 to 1024, rot even and 2 to dim";
+    if (a->rows < 0 || !in(a->heads, 1, 65536) || (int64_t)a->rows * a->heads > 1 << 28)
+        return "heads are 1 to 65536, rows times heads up to 2^28";
+    if (!std::isfinite(a->amplitude)) return "amplitude is not finite";
+    if (a->rows == 0) return nullptr;
+    const size_t es = a->dtype == QWEN_BF16 ? 2 : 4;
+    if (!a->out || !a->x || !a->positions || !a->freqs) return "out, x, positions or freqs is NULL";
+    if (!aligned(a->out, es) || !aligned(a->x, es) || !aligned(a->positions, 4) || !aligned(a->freqs, 8))
+        return "a pointer is not aligned to its elements";
+    if (!in(a->x_row, 0, kMaxStride) || !in(a->x_head, 0, kMaxStride) || !in(a->out_row, 0, kMaxStride) ||
+        !in(a->out_head, 0, kMaxStride))
+        return "a stride is below 0 or above 2^34";
+    if (!heads_apart(a->rows, a->out_row, a->heads, a->out_head, a->dim)) return "out's rows or heads overlap";
+    if (a->out == a->x && ((a->rows > 1 && a->x_row != a->out_row) || (a->heads > 1 && a->x_head != a->out_head)))
+        return "out is x, with other strides";
+    return nullptr;
+}
+
+// What kv_dev_append and attn_dev_paged ask of their cache and sequences.
+template <class A>
+const char* cache_sizes(const A* a) {
+    if (!a) return "no arguments";
+    if (a->dtype != QWEN_F32 && a->dtype != QWEN_BF16) return "dtype is neither QWEN_F32 nor QWEN_BF16";
+    if (!in(a->dim, 8, 256) || a->dim % 8) return "dim is a multiple of 8 up to 256";
+    if (!in(a->n_seq, 0, 1 << 20) || a->rows < 0) return "n_seq is 0 to 2^20, rows not below 0";
+    if (!in(a->heads_k, 1, 65536) || (int64_t)a->rows * a->heads_k > 1 << 28)
+        return "heads_k is 1 to 65536, rows times heads up to 2^28";
+    return nullptr;
+}
+template <class A>
+const char* cache_pointers(const A* a) {
+    if (!in(a->page, 1, 65536) || a->pages < 0 || a->table_pages < 0 || (int64_t)a->page * a->table_pages > 1 << 30)
+        return "page is 1 to 65536, page times table_pages up to 2^30, pages not below 0";
+    if (a->n_seq && !a->starts && a->rows % a->n_seq) return "without starts the rows are a multiple of n_seq";
+    if (a->n_seq == 0 || a->rows == 0) return nullptr;
+    if (!a->cached || !aligned(a->cached, 4) || !aligned(a->starts, 4) || !aligned(a->tables, 4))
+        return "cached is NULL, or cached, starts or tables not 4-byte aligned";
+    if (a->n_seq > 1 && !in(a->table_row, a->table_pages, kMaxStride)) return "the tables' rows overlap";
+    if (a->pages == 0 || a->table_pages == 0) return nullptr;
+    const int64_t part = a->dtype == QWEN_BF16 ? 8 : 4;
+    if (!a->tables || !a->key_cache || !a->value_cache) return "tables, key_cache or value_cache is NULL";
+    if (!aligned(a->key_cache, 16) || !aligned(a->value_cache, 16) || a->cache_page % part || a->cache_token % part ||
+        a->cache_head % part)
+        return "the caches and their strides are 16-byte aligned";
+    if (!in(a->cache_page, 0, (int64_t)1 << 40) || !in(a->cache_token, 0, kMaxStride) || !in(a->cache_head, 0, kMaxStride))
+        return "a stride of the caches is below 0 or too large";
+    Axis axes[] = {{a->pages, a->cache_page}, {a->page, a->cache_token}, {a->heads_k, a->cache_head}};
+    if (!apart(axes, a->dim)) return "the caches' pages, tokens or heads overlap";
+    return nullptr;
+}
+
+const char* append_bad(const kv_dev_append_args* a) {
+    if (const char* why = cache_sizes(a)) return why;
+    if (const char* why = cache_pointers(a)) return why;
+    if (!in(a->rot, 0, a->dim) || a->rot % 2) return "rot is even, 0 to dim";
+    if (!std::isfinite(a->amplitude)) return "amplitude is not finite";
+    if (a->q && (a->heads_q < a->heads_k || a->heads_q % a->heads_k || a->heads_q > 65536 ||
+                 (int64_t)a->rows * a->heads_q > 1 << 28))
+        return "heads_q is a multiple of heads_k, rows times heads up to 2^28";
+    if (a->q && a->rot == 0) return "q without a rotation";
+    if (a->n_seq == 0 || a->rows == 0) return nullptr;
+    const size_t es = a->dtype == QWEN_BF16 ? 2 : 4;
+    if (!a->k || !a->v || (a->q && !a->q_out) || (a->rot && !a->freqs)) return "k, v, q_out or freqs is NULL";
+    if (!aligned(a->k, es) || !aligned(a->v, es) || !aligned(a->positions, 4) || !aligned(a->freqs, 8) ||
+        (a->q && (!aligned(a->q, es) || !aligned(a->q_out, es))))
+        return "a pointer is not aligned to its elements";
+    for (const int64_t x : {a->k_row, a->k_head, a->v_row, a->v_head})
+        if (!in(x, 0, kMaxStride)) return "a stride is below 0 or above 2^34";
+    if (!a->q) return nullptr;
+    for (const int64_t x : {a->q_row, a->q_head, a->q_out_row, a->q_out_head})
+        if (!in(x, 0, kMaxStride)) return "a stride is below 0 or above 2^34";
+    if (!heads_apart(a->rows, a->q_out_row, a->heads_q, a->q_out_head, a->dim)) return "q_out's rows or heads overlap";
+    if (a->q_out == a->q &&
+        ((a->rows > 1 && a->q_row != a->q_out_row) || (a->heads_q > 1 && a->q_head != a->q_out_head)))
+        return "q_out is q, with other strides";
+    return nullptr;
+}
+
+const char* paged_sizes(const attn_dev_args* a) {
+    if (const char* why = cache_sizes(a)) return why;
+    if (a->heads_q < a->heads_k || a->heads_q % a->heads_k || (int64_t)a->rows * a->heads_q > 1 << 28 ||
+        a->heads_q > 1 << 20)
+        return "heads_q is a multiple of heads_k up to 2^20, rows times heads up to 2^28";
+    return nullptr;
+}
+const char* paged_bad(const attn_dev_args* a) {
+    if (const char* why = cache_pointers(a)) return why;
+    if (!std::isfinite(a->scale) || a->scale <= 0) return "scale is finite and above 0";
+    if (a->mask && (!in(a->mask_words, 0, 1 << 16) || !aligned(a->mask, 4)))
+        return "mask_words are 0 to 2^16, mask 4-byte aligned";
+    if (a->n_seq == 0 || a->rows == 0) return nullptr;
+    const size_t es = a->dtype == QWEN_BF16 ? 2 : 4;
+    if (!a->out || !a->q || !aligned(a->out, es) || !aligned(a->q, es))
+        return "out or q is NULL or not aligned to its elements";
+    for (const int64_t x : {a->q_row, a->q_head, a->out_row, a->out_head})
+        if (!in(x, 0, kMaxStride)) return "a stride is below 0 or above 2^34";
+    if (!heads_apart(a->rows, a->out_row, a->heads_q, a->out_head, a->dim)) return "out's rows or heads overlap";
+    return nullptr;
+}
+
+const char* tree_bad(const attn_dev_tree_args* a) {
+    if (!a) return "no arguments";
+    if (!in(a->n_seq, 0, 1 << 20) || a->rows < 0 || a->words < 0 || (int64_t)a->rows * a->words > 1 << 28)
+        return "n_seq is 0 to 2^20, rows times words up to 2^28";
+    if (a->n_seq && !a->starts && a->rows % a->n_seq) return "without starts the rows are a multiple of n_seq";
+    if (a->n_seq == 0 || a->rows == 0) return nullptr;
+    if (a->words < 1) return "no words for the rows' bits";
+    if (!a->mask || !a->parents || !a->cached) return "mask, parents or cached is NULL";
+    if (!aligned(a->mask, 4) || !aligned(a->positions, 4) || !aligned(a->parents, 4) || !aligned(a->cached, 4) ||
+        !aligned(a->starts, 4))
+        return "a pointer is not 4-byte aligned";
+    return nullptr;
+}
+
+int rope(const char* who, const rope_dev_args* a, bool back, void* stream) {
+    if (const char* why = rope_bad(a)) return refuse(who, why);
+    if (a->rows == 0) return BFP8_OK;
+    if (init() != BFP8_OK) return BFP8_EHIP;
+    HIP_OK(rope_launch(*a, back, pick_stream(stream)));
+    return BFP8_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -167,6 +320,47 @@ int bf16_dev_lm_head_loss_grad(const lm_head_loss_args* args, void* stream) {
         return refuse(who, "work is smaller than bf16_dev_lm_head_loss_grad_work_bytes() or not 256-byte aligned");
     if (init() != BFP8_OK) return BFP8_EHIP;
     HIP_OK(lhl_launch_grad(*args, w, pick_stream(stream)));
+    return BFP8_OK;
+}
+
+int rope_dev_apply(const rope_dev_args* args, void* stream) { return rope("rope_dev_apply", args, false, stream); }
+
+int rope_dev_grad(const rope_dev_args* args, void* stream) { return rope("rope_dev_grad", args, true, stream); }
+
+int kv_dev_append(const kv_dev_append_args* args, void* stream) {
+    if (const char* why = append_bad(args)) return refuse("kv_dev_append", why);
+    if (args->n_seq == 0 || args->rows == 0) return BFP8_OK;
+    if (init() != BFP8_OK) return BFP8_EHIP;
+    HIP_OK(kv_launch_append(*args, pick_stream(stream)));
+    return BFP8_OK;
+}
+
+size_t attn_dev_paged_work_bytes(const attn_dev_args* args) {
+    if (const char* why = paged_sizes(args)) {
+        set_error("attn_dev_paged_work_bytes: %s", why);
+        return 0;
+    }
+    return attn_plan(*args).total;
+}
+
+int attn_dev_paged(const attn_dev_args* args, void* stream) {
+    const char* who = "attn_dev_paged";
+    if (const char* why = paged_sizes(args)) return refuse(who, why);
+    if (const char* why = paged_bad(args)) return refuse(who, why);
+    if (args->n_seq == 0 || args->rows == 0) return BFP8_OK;
+    const AttnPlan p = attn_plan(*args);
+    if (!args->work || !aligned(args->work, 256) || args->work_bytes < p.total)
+        return refuse(who, "work is smaller than attn_dev_paged_work_bytes() or not 256-byte aligned");
+    if (init() != BFP8_OK) return BFP8_EHIP;
+    HIP_OK(attn_launch_paged(*args, p, pick_stream(stream)));
+    return BFP8_OK;
+}
+
+int attn_dev_tree(const attn_dev_tree_args* args, void* stream) {
+    if (const char* why = tree_bad(args)) return refuse("attn_dev_tree", why);
+    if (args->n_seq == 0 || args->rows == 0) return BFP8_OK;
+    if (init() != BFP8_OK) return BFP8_EHIP;
+    HIP_OK(attn_launch_tree(*args, pick_stream(stream)));
     return BFP8_OK;
 }
 

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 import struct
 from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
@@ -105,6 +106,63 @@ class lm_head_loss_args(ctypes.Structure):
         ("work_bytes", c_size_t), ("h_row", c_int64), ("table_row", c_int64), ("grad_h_row", c_int64),
         ("grad_table_row", c_int64), ("rows", c_int), ("vocab", c_int), ("hidden", c_int), ("dtype", c_int),
     ]
+
+
+class rope_dev_args(ctypes.Structure):
+    """Mirror of ``rope_dev_args`` (include/qwen_kernels.h)."""
+
+    _fields_ = [
+        ("out", c_void_p), ("x", c_void_p), ("positions", c_void_p), ("freqs", c_void_p),
+        ("out_row", c_int64), ("out_head", c_int64), ("x_row", c_int64), ("x_head", c_int64),
+        ("rows", c_int), ("heads", c_int), ("dim", c_int), ("rot", c_int), ("dtype", c_int), ("interleaved", c_int),
+        ("amplitude", c_float),
+    ]
+
+
+class kv_dev_append_args(ctypes.Structure):
+    """Mirror of ``kv_dev_append_args`` (include/qwen_kernels.h)."""
+
+    _fields_ = [
+        ("key_cache", c_void_p), ("value_cache", c_void_p), ("q_out", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q", c_void_p), ("tables", c_void_p), ("cached", c_void_p), ("starts", c_void_p), ("positions", c_void_p),
+        ("freqs", c_void_p),
+        ("cache_page", c_int64), ("cache_token", c_int64), ("cache_head", c_int64), ("table_row", c_int64),
+        ("k_row", c_int64), ("k_head", c_int64), ("v_row", c_int64), ("v_head", c_int64), ("q_row", c_int64),
+        ("q_head", c_int64), ("q_out_row", c_int64), ("q_out_head", c_int64),
+        ("rows", c_int), ("n_seq", c_int), ("pages", c_int), ("page", c_int), ("table_pages", c_int),
+        ("heads_q", c_int), ("heads_k", c_int), ("dim", c_int), ("rot", c_int), ("dtype", c_int), ("interleaved", c_int),
+        ("amplitude", c_float),
+    ]
+
+
+class attn_dev_args(ctypes.Structure):
+    """Mirror of ``attn_dev_args`` (include/qwen_kernels.h)."""
+
+    _fields_ = [
+        ("out", c_void_p), ("q", c_void_p), ("key_cache", c_void_p), ("value_cache", c_void_p), ("tables", c_void_p),
+        ("cached", c_void_p), ("starts", c_void_p), ("mask", c_void_p), ("work", c_void_p), ("work_bytes", c_size_t),
+        ("cache_page", c_int64), ("cache_token", c_int64), ("cache_head", c_int64), ("table_row", c_int64),
+        ("q_row", c_int64), ("q_head", c_int64), ("out_row", c_int64), ("out_head", c_int64),
+        ("rows", c_int), ("n_seq", c_int), ("pages", c_int), ("page", c_int), ("table_pages", c_int),
+        ("heads_q", c_int), ("heads_k", c_int), ("dim", c_int), ("mask_words", c_int), ("dtype", c_int),
+        ("scale", c_float), ("zero_rest", c_int),
+    ]
+
+
+class attn_dev_tree_args(ctypes.Structure):
+    """Mirror of ``attn_dev_tree_args`` (include/qwen_kernels.h)."""
+
+    _fields_ = [
+        ("mask", c_void_p), ("positions", c_void_p), ("parents", c_void_p), ("cached", c_void_p), ("starts", c_void_p),
+        ("rows", c_int), ("n_seq", c_int), ("words", c_int),
+    ]
+
+
+# these in one packing, as _GDN_PACK
+_ROPE_PACK = struct.Struct("@4P4q6if4x")
+_APPEND_PACK = struct.Struct("@11P12q11if")
+_ATTN_PACK = struct.Struct("@9PN8q10ifi")
+_TREE_PACK = struct.Struct("@5P3i4x")
 
 
 def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
@@ -247,6 +305,13 @@ def bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         getattr(lib, name + "_work_bytes").argtypes = [POINTER(lm_head_loss_args)]
         getattr(lib, name + "_work_bytes").restype = c_size_t
         getattr(lib, name).argtypes = [POINTER(lm_head_loss_args), vp]
+        getattr(lib, name).restype = i
+    lib.attn_dev_paged_work_bytes.argtypes = [POINTER(attn_dev_args)]
+    lib.attn_dev_paged_work_bytes.restype = c_size_t
+    for name, args in (("rope_dev_apply", rope_dev_args), ("rope_dev_grad", rope_dev_args),
+                       ("kv_dev_append", kv_dev_append_args), ("attn_dev_paged", attn_dev_args),
+                       ("attn_dev_tree", attn_dev_tree_args)):
+        getattr(lib, name).argtypes = [POINTER(args), vp]
         getattr(lib, name).restype = i
     lib.bfp8_stream.argtypes = []
     lib.bfp8_stream.restype = vp
@@ -839,4 +904,263 @@ def lm_head_loss_work_bytes(rows, vocab, hidden, dtype, *, grad=False, need_h=Tr
     n = (lib.bf16_dev_lm_head_loss_grad_work_bytes if grad else lib.bf16_dev_lm_head_loss_work_bytes)(a)
     if not n:
         check(BFP8_EINVAL, "lm_head_loss_work_bytes")
+    return n
+
+
+# ---- positions, the paged cache and the attention over it ---------------------------------
+def rotary_frequencies(rot, base=10000.0, *, scaling=None, factor=1.0, original=None, fast=32.0, slow=1.0,
+                       device="cuda"):
+    """Radians a position of each of rot / 2 pairs, base^(-2 i / rot) -> (freqs, amplitude): freqs float64 on
+    the device, amplitude for the rotation.
+
+    scaling, for contexts `factor` times as long as the model was trained on:
+    "linear": every frequency divided by it; "ntk": the base grown, so that the slowest is;
+    "yarn": pairs that turn more than `fast` times over the `original` context keep their frequency, those
+    that turn less than `slow` times are divided, in between a linear ramp over the pairs,
+    and the amplitude is 0.1 ln factor + 1 (Peng et al., 2023)."""
+    torch = _torch()
+    if rot < 2 or rot % 2 or not base > 0 or not factor > 0:
+        raise ValueError("rot is even and at least 2, base and factor are above 0")
+    if scaling == "ntk":
+        if rot < 4:
+            raise ValueError("ntk needs at least two pairs")
+        base = base * factor ** (rot / (rot - 2))
+    freqs = torch.tensor(float(base), dtype=torch.float64) ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    amplitude = 1.0
+    if scaling == "linear":
+        freqs /= factor
+    elif scaling == "yarn":
+        if not original or not fast > slow > 0 or not base > 1:
+            raise ValueError("yarn needs the original context's length, fast above slow above 0, and a base above 1")
+        # the pair, as a number with a fraction, that turns so many times over the original context
+        pair = lambda turns: rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
+        ramp = ((torch.arange(rot // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        freqs = freqs * (1 - ramp) + freqs / factor * ramp
+        amplitude = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"scaling is None, linear, ntk or yarn, not {scaling}")
+    return freqs.to(device), amplitude
+
+
+def _heads_of(t, name, shape, dtype):
+    """t of this [rows, heads, dim] and type, each head's elements contiguous -> strides of rows and heads."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} has to be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    row, head, one = t.stride()
+    if one != 1 and shape[2] > 1:
+        raise ValueError(f"{name}: a head's elements have to be contiguous")
+    return row, head
+
+
+def _rotate(who, x, positions, freqs, interleaved, amplitude, out):
+    torch = _torch()
+    with _same_device(x, positions, freqs, out):
+        if x.dim() != 3 or x.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("x is [rows, heads, dim] in float32 or bfloat16")
+        shape = rows, heads, dim = x.shape
+        if out is None:
+            out = _like(x)
+        _flat(positions, "positions", (rows,), torch.int32)
+        _flat(freqs, "freqs", (freqs.numel(),), torch.float64)
+        a = rope_dev_args.from_buffer_copy(_ROPE_PACK.pack(
+            out.data_ptr(), x.data_ptr(), positions.data_ptr(), freqs.data_ptr(), *_heads_of(out, "out", shape, x.dtype),
+            *_heads_of(x, "x", shape, x.dtype), rows, heads, dim, 2 * freqs.numel(),
+            QWEN_F32 if x.dtype == torch.float32 else QWEN_BF16, bool(interleaved), amplitude))
+        check(getattr(load(), who)(a, _stream()), who)
+    return out
+
+
+def rotary(x, positions, freqs, *, interleaved=False, amplitude=1.0, out=None):
+    """Rotary positions: each pair of a head's first 2 len(freqs) elements turned by position times
+    frequency -> out (a new contiguous tensor, or the one given, which may be x).
+
+    x [rows, heads, dim] float32 or bfloat16, with any strides of rows and heads; positions int32 [rows];
+    freqs float64, radians a position (rotary_frequencies).  Pairs are elements i and i + len(freqs), or with
+    interleaved 2 i and 2 i + 1; the rotation is multiplied by amplitude.  No autograd graph is built: an x that
+    requires a gradient is refused unless gradients are off, and rotary_grad has it.  The rest is rope_dev_apply's
+    contract (include/qwen_kernels.h)."""
+    if x.requires_grad and _torch().is_grad_enabled():
+        _no_graph("rotary", "its gradient is rotary_grad's")
+    return _rotate("rope_dev_apply", x, positions, freqs, interleaved, amplitude, out)
+
+
+def rotary_grad(grad, positions, freqs, *, interleaved=False, amplitude=1.0, out=None):
+    """The gradient to rotary's x from that of its result: the transposed rotation -> out (it may be grad)."""
+    return _rotate("rope_dev_grad", grad, positions, freqs, interleaved, amplitude, out)
+
+
+def _cache_of(key_cache, value_cache, dtype):
+    """Both caches [pages, page, heads, dim] with the same strides -> their shape and strides."""
+    shape = key_cache.shape
+    if len(shape) != 4 or value_cache.shape != shape or key_cache.dtype != dtype or value_cache.dtype != dtype:
+        raise ValueError(f"the caches have to be [pages, page, heads_k, dim] of {dtype}, both the same")
+    strides = key_cache.stride()
+    if value_cache.stride() != strides or strides[3] != 1:
+        raise ValueError("the caches have to have the same strides, a head's elements contiguous")
+    return shape, strides
+
+
+def _sequences_of(tables, cached, starts):
+    """-> the number of sequences, the tables' columns, the stride of their rows."""
+    int32 = _torch().int32
+    n = cached.numel()
+    _flat(cached, "cached", (n,), int32)
+    if starts is not None:
+        _flat(starts, "starts", (n + 1,), int32)
+    if tables.dim() != 2 or tables.size(0) != n or tables.dtype != int32:
+        raise ValueError("tables has to be [sequences, pages of a sequence] of int32")
+    row, one = tables.stride()
+    if one != 1 and tables.size(1) > 1:
+        raise ValueError("tables: a row's elements have to be contiguous")
+    return n, tables.size(1), row
+
+
+def kv_cache_append(k, v, key_cache, value_cache, tables, cached, starts=None, *, positions=None, freqs=None,
+                    interleaved=False, amplitude=1.0, q=None, q_out=None):
+    """Writes a call's keys and values to their places in the paged caches, the keys rotated on the way where
+    freqs is given; q is rotated in the same launch -> q_out (a new contiguous tensor, or the one
+    given, which may be q; None without q).
+
+    k, v [rows, heads_k, dim] float32 or bfloat16, q [rows, heads_q, dim]; key_cache and
+    value_cache [pages, page, heads_k, dim] of the same type, with any strides that are multiples of 16 bytes (the
+    same in both).  Sequence s has rows starts[s] to starts[s + 1] (int32 on the device; None: the same number each), its pages
+    in tables[s] (int32 [sequences, pages], -1: none), and held cached[s] tokens before (int32, below 0: skipped);
+    its row i goes to place cached[s] + i.  positions int32 [rows]: of the rotation, None: the
+    places.  Rows of q_out of skipped sequences, and that no sequence holds, are left as they were (undefined in a new
+    one).  There is no backward pass: tensors that require a gradient are refused unless it is off.  The rest is
+    kv_dev_append's contract (include/qwen_kernels.h)."""
+    torch = _torch()
+    if (k.requires_grad or v.requires_grad or key_cache.requires_grad or value_cache.requires_grad
+            or q is not None and q.requires_grad) and torch.is_grad_enabled():
+        _no_graph("kv_cache_append", "there is no backward pass")
+    with _same_device(k, v, key_cache, value_cache, tables, cached, starts, positions, freqs, q, q_out):
+        dtype = k.dtype
+        if k.dim() != 3 or dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("k and v are [rows, heads_k, dim] in float32 or bfloat16")
+        shape = rows, heads, dim = k.shape
+        cache, strides = _cache_of(key_cache, value_cache, dtype)
+        if cache[2] != heads or cache[3] != dim:
+            raise ValueError(f"the caches' heads are {tuple(cache[2:])}, not {(heads, dim)}")
+        n_seq, columns, table_row = _sequences_of(tables, cached, starts)
+        if positions is not None:
+            _flat(positions, "positions", (rows,), torch.int32)
+        if freqs is not None:
+            _flat(freqs, "freqs", (freqs.numel(),), torch.float64)
+        heads_q, q_strides = 0, (0, 0, 0, 0)
+        if q is not None:
+            if freqs is None:
+                raise ValueError("q is given to be rotated, and there are no freqs")
+            if q.dim() != 3:
+                raise ValueError("q is [rows, heads_q, dim]")
+            heads_q = q.size(1)
+            if q_out is None:
+                q_out = _like(q)
+            q_strides = (*_heads_of(q, "q", (rows, heads_q, dim), dtype),
+                         *_heads_of(q_out, "q_out", (rows, heads_q, dim), dtype))
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        ptr = _ptr_or_0
+        a = kv_dev_append_args.from_buffer_copy(_APPEND_PACK.pack(
+            key_cache.data_ptr(), value_cache.data_ptr(), ptr(q_out), k.data_ptr(), v.data_ptr(), ptr(q),
+            tables.data_ptr(), cached.data_ptr(), ptr(starts), ptr(positions), ptr(freqs), *strides[:3], table_row,
+            *_heads_of(k, "k", shape, dtype), *_heads_of(v, "v", shape, dtype), *q_strides,
+            rows, n_seq, cache[0], cache[1], columns, heads_q, heads, dim, 0 if freqs is None else 2 * freqs.numel(),
+            QWEN_F32 if dtype == torch.float32 else QWEN_BF16, bool(interleaved), amplitude))
+        check(load().kv_dev_append(a, _stream()), "kv_cache_append")
+    return q_out
+
+
+def _ptr_or_0(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def draft_tree(parents, cached, starts=None, *, longest=None, mask=None, positions=None):
+    """Drafted tokens' masks and positions from their tree -> (mask, positions), once for all layers of a step.
+
+    parents int32 [rows]: for each drafted token the place, among its sequence's rows, of the token that it follows,
+    an earlier one (below 0: the cached text).  mask int32 [rows, words]: bit j of a row (word j / 32,
+    bit j % 32) is set for the row's own place and its ancestors'; positions int32 [rows]: cached[s] plus the
+    number of its ancestors.  cached and starts as in kv_cache_append.  longest: the most rows that a sequence
+    has, for the words of a new mask (None: as many as there are rows, or without starts each has).
+    attn_dev_tree (include/qwen_kernels.h)."""
+    torch = _torch()
+    with _same_device(parents, cached, starts, mask, positions):
+        rows, n_seq = parents.numel(), cached.numel()
+        _flat(parents, "parents", (rows,), torch.int32)
+        _flat(cached, "cached", (n_seq,), torch.int32)
+        if starts is not None:
+            _flat(starts, "starts", (n_seq + 1,), torch.int32)
+        if mask is None:
+            if longest is None:
+                longest = rows if starts is not None or not n_seq else rows // n_seq
+            mask = parents.new_empty((rows, max(1, (longest + 31) // 32)))
+        words = mask.size(1) if mask.dim() == 2 else 0
+        _flat(mask, "mask", (rows, words), torch.int32)
+        if positions is None:
+            positions = parents.new_empty((rows,))
+        _flat(positions, "positions", (rows,), torch.int32)
+        a = attn_dev_tree_args.from_buffer_copy(_TREE_PACK.pack(
+            mask.data_ptr(), positions.data_ptr(), parents.data_ptr(), cached.data_ptr(), _ptr_or_0(starts),
+            rows, n_seq, words))
+        check(load().attn_dev_tree(a, _stream()), "draft_tree")
+    return mask, positions
+
+
+def paged_attention(q, key_cache, value_cache, tables, cached, starts=None, *, scale=None, mask=None, out=None, work=None):
+    """Attention of a call's tokens over the paged caches, their own keys and values in them already
+    (kv_cache_append) -> out.
+
+    q [rows, heads_q, dim], float32 or bfloat16 as the caches, heads_q a multiple of their heads; tables, cached
+    and starts as in kv_cache_append (cached: without this call's tokens, as there).  Row i of a sequence sees
+    the places up to cached[s] + i, or with a mask (draft_tree's, or any int32 [rows, words]) the cached ones and those of
+    the sequence's rows whose bit is set.  scale: of the scores, None: dim^-0.5.  work: uint8 scratch of at least
+    paged_attention_work_bytes, 256-byte aligned.  Rows of skipped sequences are left as they were where out is given, and 0 in a
+    new one; rows that no sequence holds are left as they were, undefined in a new one.  There is no backward
+    pass: tensors that require a gradient are refused unless it is off.  The rest is attn_dev_paged's contract
+    (include/qwen_kernels.h)."""
+    torch = _torch()
+    if (q.requires_grad or key_cache.requires_grad or value_cache.requires_grad) and torch.is_grad_enabled():
+        _no_graph("paged_attention", "there is no backward pass")
+    with _same_device(q, key_cache, value_cache, tables, cached, starts, mask, out, work):
+        dtype = q.dtype
+        if q.dim() != 3 or dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("q is [rows, heads_q, dim] in float32 or bfloat16")
+        shape = rows, heads_q, dim = q.shape
+        cache, strides = _cache_of(key_cache, value_cache, dtype)
+        if cache[3] != dim:
+            raise ValueError(f"the caches' heads have {cache[3]} elements, not {dim}")
+        n_seq, columns, table_row = _sequences_of(tables, cached, starts)
+        words = 0
+        if mask is not None:
+            words = mask.size(1) if mask.dim() == 2 else 0
+            _flat(mask, "mask", (rows, words), torch.int32)
+            if not words:
+                raise ValueError("mask has no words")
+        zero_rest = out is None
+        if out is None:
+            out = _like(q)
+        a = attn_dev_args.from_buffer_copy(_ATTN_PACK.pack(
+            out.data_ptr(), q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), tables.data_ptr(),
+            cached.data_ptr(), _ptr_or_0(starts), _ptr_or_0(mask), *_work_of(work), *strides[:3], table_row,
+            *_heads_of(q, "q", shape, dtype), *_heads_of(out, "out", shape, dtype),
+            rows, n_seq, cache[0], cache[1], columns, heads_q, cache[2], dim, words,
+            QWEN_F32 if dtype == torch.float32 else QWEN_BF16, dim ** -0.5 if scale is None else scale, zero_rest))
+        lib = load()
+        if work is None:
+            need = lib.attn_dev_paged_work_bytes(a)
+            if need:
+                work = q.new_empty(need, dtype=torch.uint8)
+                a.work, a.work_bytes = work.data_ptr(), need
+        check(lib.attn_dev_paged(a, _stream()), "paged_attention")
+    return out
+
+
+def paged_attention_work_bytes(rows, n_seq, heads_q, heads_k, dim, dtype) -> int:
+    """Bytes of paged_attention's work for these sizes (dtype: of q and the caches)."""
+    a = attn_dev_args()
+    _sizes_of(a, dtype, rows=rows, n_seq=n_seq, heads_q=heads_q, heads_k=heads_k, dim=dim)
+    n = load().attn_dev_paged_work_bytes(a)
+    if not n:
+        check(BFP8_EINVAL, "paged_attention_work_bytes")
     return n
