@@ -12,12 +12,15 @@ constexpr int ATTN_HELD = 1024;  // places whose tiles of keys a workgroup remem
 // head, row m being token m / group and query head m % group of it.
 struct AttnPlan {
     int group;    // query heads of a key head
+    int few;      // attn_step_kernel: up to 16 rows
     int dim;      // of the kernel: 64, 128 or 256
     int blocks;   // of 16 rows of a wavefront
     int waves;    // of a workgroup
-    int rows;     // of a tile: 16 blocks waves
+    int rows, rows_log;  // of a tile: 16 blocks waves, a power of two
+    int each;     // tiles of rows of a sequence, without starts
     int keys;     // of a tile of keys
     int grid;     // workgroups
+    int least;    // tiles of keys of a workgroup's share
     size_t desc_at;   // AttnDesc [grid]
     size_t stat_at;   // float2 [2 grid][rows]: a part's maximum and sum
     size_t part_at;   // float [2 grid][rows][dim]
@@ -34,10 +37,16 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     p.blocks = bf16 && mean > 16 ? 2 : 1;
     p.waves = mean <= (size_t)16 * p.blocks ? 1 : mean <= (size_t)32 * p.blocks ? 2 : mean <= (size_t)64 * p.blocks ? 4 : 8;
     p.rows = 16 * p.blocks * p.waves;
-    p.keys = bf16 && p.waves == 8 ? 64 : 32;
+    p.rows_log = 31 - __builtin_clz(p.rows);
+    p.each = a.starts || !a.n_seq ? 0 : (a.rows / a.n_seq * p.group + p.rows - 1) / p.rows;
+    p.few = mean <= 16;
+    p.keys = p.few || (bf16 && p.waves == 8) ? 64 : 32;
     // as many as are at work at a time, by LDS and registers (8 wavefronts a compute unit), up to four a unit
     const size_t lds = (size_t)4 * p.keys * p.dim * (bf16 ? 2 : 4) + ATTN_HELD * 4 + 256;
-    p.grid = 256 * (int)std::min<size_t>(std::min(4, 8 / p.waves), 160 * 1024 / lds);
+    p.grid = 256 * (p.few ? 2 : (int)std::min<size_t>(std::min(4, 8 / p.waves), 160 * 1024 / lds));
+    // A part is written and read again, 8 bytes an output: of many rows as much as several tiles of keys (one sequence of
+    // 6,000 tokens with 26 drafted ones: 1 | 2 | 4 | 8 tiles 94 | 60 | 46 | 50 us).
+    p.least = p.few ? 1 : 4;
     size_t at = 0;
     auto put = [&](size_t bytes) {
         const size_t here = at;
@@ -49,6 +58,29 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     p.part_at = put((size_t)2 * p.grid * p.rows * p.dim * 4);
     p.total = at;
     return p;
+}
+
+// Places in the cache as 32-bit multiples of the largest power of two that divides its strides, 16 bytes or more: a cache
+// may span 2^32 of them (64 GiB at least, 4 TiB with 1 KiB a token).
+struct AttnUnits {
+    Divisor divisor;       // by the tokens of a page
+    uint32_t page, token;  // their strides in units
+    int log;
+};
+inline AttnUnits attn_units(const attn_dev_args& a) {
+    const uint64_t es = a.dtype == QWEN_BF16 ? 2 : 4, page = a.cache_page * es, token = a.cache_token * es;
+    AttnUnits u{divisor(a.page), 0, 0, 4};
+    while (u.log < 31 && (page | token) >> u.log && ((page | token) >> u.log & 1) == 0) ++u.log;
+    u.page = (uint32_t)(page >> u.log);
+    u.token = (uint32_t)(token >> u.log);
+    return u;
+}
+// The last place's number is below 2^32 - 1.
+inline bool attn_units_fit(const attn_dev_args& a) {
+    const AttnUnits u = attn_units(a);
+    const uint64_t es = a.dtype == QWEN_BF16 ? 2 : 4;
+    if ((uint64_t)a.cache_page * es >> u.log > 0xffffffffull || (uint64_t)a.cache_token * es >> u.log > 0xffffffffull) return false;
+    return (unsigned __int128)u.page * std::max(a.pages - 1, 0) + (unsigned __int128)u.token * (a.page - 1) < 0xffffffffull;
 }
 
 hipError_t attn_launch_paged(const attn_dev_args& a, const AttnPlan& p, hipStream_t s);

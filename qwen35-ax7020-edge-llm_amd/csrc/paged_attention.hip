@@ -11,6 +11,8 @@
 // The tiles of keys of all tiles of rows are one long axis, divided evenly over the workgroups: a batch of
 // ragged lengths fills the device to the end, and one long sequence is shared by all.  A workgroup whose share begins
 // or ends inside a tile of rows leaves its maxima, sums and outputs, which attn_join_kernel joins in a fixed order.
+#include <type_traits>
+
 #include "bf16_terms.h"
 #include "paged_attention.h"
 
@@ -18,16 +20,30 @@ namespace {
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
+typedef __attribute__((address_space(1))) const char global_char;  // (where a pointer is one of two, the compiler has to be told)
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -INFINITY;  // the maximum of no scores
+constexpr uint32_t kNowhere = 0xffffffffu;
+// A row's maximum is raised, and what it has so far scaled down to it, only by a score that is this much above it: weights
+// then are up to 2^8, and float32 sums have the same bits.  (Each of 32 rows raises its own: without slack nearly
+// every 32 keys of the first thousand.)
+constexpr float kSlack = 8;
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: 0
 
 // 16 bytes that are read for keys that do not exist and elements past the head's: their weights are 0, but 0 times
 // what lies in a free page need not be.
-__device__ const uint4 kZeros = {0, 0, 0, 0};
+__device__ const uint4 kZeros[64] = {};  // (attn_step_kernel: a whole key's or value's)
+
+// 16 bytes a lane from `from` to 1 KiB of LDS, the same `to` in all lanes.  (The builtin of this instruction makes the compiler wait for all
+// copies in flight before the next read of LDS, whichever buffer that is from.
+// Whoever reads waits for itself: Pass::arrived.)
+__device__ __forceinline__ void copy_to_lds(global_char* from, char* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+}
 
 // A tile of rows that this workgroup's share ends in, and begins (AttnPlan::desc_at).
 struct AttnDesc {
@@ -52,17 +68,13 @@ struct Tile {
 struct Shape {
     const attn_dev_args& a;
     const AttnPlan& p;
-    __device__ int64_t places() const {
-        if (!a.starts) return (int64_t)a.n_seq * each();
-        return (int64_t)a.rows * p.group / p.rows + a.n_seq;
-    }
-    __device__ int each() const { return (int)(((int64_t)(a.rows / a.n_seq) * p.group + p.rows - 1) / p.rows); }
-    __device__ int64_t first_place(int s) const {
-        return (int64_t)min(max(a.starts[s], 0), a.rows) * p.group / p.rows + s;
-    }
-    __device__ Tile tile(int64_t place) const {
+    // (rows group is up to 2^28, a tile's rows are a power of two)
+    __device__ int tiles_of(int rows) const { return (rows * p.group) >> p.rows_log; }
+    __device__ int places() const { return a.starts ? tiles_of(a.rows) + a.n_seq : a.n_seq * p.each; }
+    __device__ int first_place(int s) const { return tiles_of(min(max(a.starts[s], 0), a.rows)) + s; }
+    __device__ Tile tile(int place) const {
         Tile t{};
-        int64_t in;
+        int in = 0;
         if (a.starts) {
             int lo = 0, hi = a.n_seq;
             while (hi - lo > 1) {
@@ -74,23 +86,23 @@ struct Shape {
             }
             t.seq = lo;
             in = place - first_place(lo);
+        } else if (p.each == 1) {
+            t.seq = place;
         } else {
-            const int n = each();
-            t.seq = n == 1 ? (int)place : (int)(place / n);
-            in = place - (int64_t)t.seq * n;
+            t.seq = place / p.each;
+            in = place - t.seq * p.each;
         }
         const Span span = span_of(a.starts, a.rows, a.n_seq, t.seq);
         t.first = span.first;
         t.count = span.count * p.group;
-        const int64_t m0 = in * p.rows;
-        if (in < 0 || m0 >= t.count) return t;
-        t.m0 = (int)m0;
+        if (in < 0 || in > (t.count - 1) >> p.rows_log) return t;  // (without rows: -1)
+        t.m0 = in << p.rows_log;
         t.held = a.cached[t.seq];
         if (t.held < 0) {
             t.tiles = a.zero_rest ? 1 : 0;
             return t;
         }
-        const int room = a.table_pages * a.page;  // (up to 2^30)
+        const int room = a.pages ? a.table_pages * a.page : 0;  // (up to 2^30)
         const int last = min(t.count, t.m0 + p.rows) - 1;
         const int seen = a.mask ? span.count : last / p.group + 1;
         t.places = (int)min((int64_t)t.held + seen, (int64_t)room);
@@ -100,58 +112,86 @@ struct Shape {
     }
 };
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+template <class T>
+__device__ __forceinline__ T uniform(T x) {  // the same in all lanes: to scalar registers
+    int w[sizeof(T) / 4];
+    __builtin_memcpy(w, &x, sizeof(T));
 #pragma unroll
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
+    for (size_t i = 0; i < sizeof(T) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+    __builtin_memcpy(&x, w, sizeof(T));
     return x;
 }
 
 // This workgroup's share: from which tile of keys on, how many.
 struct Share {
-    int64_t place, total;  // the place it begins in; tiles of keys of the call
-    int64_t from, to;      // of those
-    int64_t before;        // tiles of the places before
-    int workers;           // workgroups with a share
+    int64_t total;     // tiles of keys of the call
+    int64_t from, to;  // of those
+    int64_t before;    // tiles of the places before
+    int place;         // the place it begins in
+    int workers;       // workgroups with a share
 };
 
-// By one wavefront: the tiles of all places are counted, then the place is looked for in which the share begins.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {  // (a division of 64 bits is 20 times one of 32)
+    return (x | y) >> 32 ? x / y : (uint32_t)x / (uint32_t)y;
+}
+
+// By every wavefront for itself: the tiles of all places are counted (a chunk of 64 at a time: 2^25 each at most), then
+// the place is looked for in which the share begins.
 __device__ Share share_of(const Shape& sh, int* held, int least) {
     const int lane = threadIdx.x & 63, heads = sh.a.heads_k;
-    const int64_t n = sh.places();
+    const int n = sh.places();
+    auto scan = [&](uint32_t mine) {  // tiles of the chunk's places up to this one
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) {
+            const uint32_t x = __shfl_up(mine, i);
+            if (lane >= i) mine += x;
+        }
+        return mine;
+    };
     int64_t sum = 0;
-    for (int64_t at = lane; at < n; at += 64) {
-        const int t = sh.tile(at).tiles;
-        if (at < ATTN_HELD) held[at] = t;
-        sum += t;
+    uint32_t upto = 0, mine = 0;
+    for (int base = 0; base < n; base += 64) {
+        const int at = base + lane;
+        mine = at < n ? sh.tile(at).tiles : 0;
+        if (at < ATTN_HELD) held[at] = mine;
+        upto = scan(mine);
+        sum += (uint32_t)__shfl(upto, 63);
     }
     Share r{};
-    r.total = wave_sum(sum) * heads;
-    r.workers = (int)min((int64_t)gridDim.x, max((int64_t)1, r.total / least));
-    r.from = (int64_t)blockIdx.x * r.total / r.workers;
-    r.to = (int64_t)(blockIdx.x + 1) * r.total / r.workers;
+    r.total = sum * heads;
+    r.workers = (int)min((int64_t)gridDim.x, max((int64_t)1, quotient(r.total, least)));
+    r.from = quotient(blockIdx.x * r.total, r.workers);
+    r.to = quotient((blockIdx.x + 1) * r.total, r.workers);
     if ((int)blockIdx.x >= r.workers) r.from = r.to = 0;
     if (r.from >= r.to) return r;
     int64_t before = 0;
-    for (int64_t base = 0; base < n; base += 64) {
-        const int64_t at = base + lane;
-        int64_t mine = 0;
-        if (at < n) mine = (int64_t)(at < ATTN_HELD ? held[at] : sh.tile(at).tiles) * heads;
-        int64_t upto = mine;
-#pragma unroll
-        for (int i = 1; i < 64; i *= 2) {
-            const int64_t x = __shfl_up(upto, i);
-            if (lane >= i) upto += x;
+    for (int base = 0; base < n; base += 64) {
+        if (n > 64) {
+            const int at = base + lane;
+            mine = at >= n ? 0 : at < ATTN_HELD ? held[at] : sh.tile(at).tiles;
+            upto = scan(mine);
         }
-        const uint64_t over = __ballot(before + upto > r.from);
+        const uint64_t over = __ballot((before + upto) * heads > r.from);
         if (over) {
             const int l = __builtin_ctzll(over);
             r.place = base + l;
-            r.before = before + __shfl(upto - mine, l);
+            r.before = (before + (uint32_t)__shfl(upto - mine, l)) * heads;
             return r;
         }
-        before += __shfl(upto, 63);
+        before += (uint32_t)__shfl(upto, 63);
     }
     return r;
+}
+
+// Where key j of a sequence is, in units of the cache's strides (AttnPlan), kNowhere if it does not exist.
+__device__ __forceinline__ uint32_t key_at(const attn_dev_args& a, const AttnUnits& u, const Tile& t, int j) {
+    if (j >= t.places) return kNowhere;
+    const uint32_t n = divide((uint32_t)j, u.divisor);
+    const int id = a.tables[t.seq * a.table_row + n];
+    return (unsigned)id < (unsigned)a.pages ? (uint32_t)id * u.page + ((uint32_t)j - n * a.page) * u.token : kNowhere;
+}
+__device__ __forceinline__ global_char* in_cache(global_char* base, uint32_t at, const AttnUnits& u) {
+    return base + ((uint64_t)at << u.log);
 }
 
 __device__ __forceinline__ float pair_max(float x) {  // over the lanes of a row: those 16 apart
@@ -169,6 +209,11 @@ __device__ __forceinline__ float pair_sum(float x) {
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float sum2(uint32_t pair, float x) {  // x + both of a pair of bf16
+    using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3f803f80u), x, false);
 }
 
 template <class T>
@@ -205,7 +250,8 @@ __device__ __forceinline__ void add_kinds(f32x4& o, f32x4 kinds) {
 // ---- the pass over the keys ------------------------------------------------------------
 // T: uint16_t (bf16) or float.  D: elements of a head, padded.  RB blocks of 16 rows a wavefront, W wavefronts,
 // BN keys a tile.  A step is 32 keys: products of 16 keys by 16 rows by 32 (bf16) or 4 (float32) elements.
-template <class T, int D, int RB, int W, int BN>
+// FULL: heads have D elements.
+template <class T, int D, int RB, int W, int BN, bool FULL>
 struct Pass {
     static constexpr bool kBf16 = sizeof(T) == 2;
     static constexpr int E = 16 / sizeof(T);          // elements of a 16-byte part
@@ -219,21 +265,21 @@ struct Pass {
     static constexpr int kOut = D / 16;     // a lane's outputs of a row, in fours
     static constexpr int kFlip = D == 64 ? 4 : 8;  // 32-byte parts of a bf16 value that change places (v_swizzle)
 
-    static constexpr bool kTight = W == 8 && D == 256;  // little room in 256 registers
+    // Eight wavefronts leave each 256 registers: outputs and queries of 32 rows of 256 bf16 elements are 192 of them.
+    static constexpr bool kTight = W == 8 && D == 256;
 
     const attn_dev_args& a;
-    Divisor page;
+    AttnUnits units;
     int group;
     char* lds;
     int lane, wave;
     Tile t;
-    const char* kbase;
-    const char* vbase;
-    int first_token, last_token;  // of the wavefront's rows (last_token < 0: it has none)
-    int token[RB];                // of the lane's rows
+    global_char* kbase;
+    global_char* vbase;
+    int kv_head, last_token;  // last of the wavefront's rows (below 0: it has none)
     u32x4 q[RB][kQ];
     f32x4 o[RB][kOut];
-    float m[RB], l[RB];  // maximum of the scores as they are, this lane's part of the sum
+    float m[RB], l[RB];  // maximum of the scores (in base 2), or up to kSlack less, and this lane's part of the sum
     float c;
 
     // Positions of a key's parts in LDS: eight keys' parts of one place, which lanes of K Q^T read together, and
@@ -252,57 +298,59 @@ struct Pass {
         return kBf16 ? x[f][e] : x[f / 4 * 4 + e][f % 4];
     }
 
-    __device__ void begin(const Tile& tile, int head) {
+    __device__ __forceinline__ void begin(const Tile& tile, int head) {
         t = tile;
-        kbase = static_cast<const char*>(a.key_cache) + head * a.cache_head * (int64_t)sizeof(T);
-        vbase = static_cast<const char*>(a.value_cache) + head * a.cache_head * (int64_t)sizeof(T);
+        kv_head = head;
+        kbase = (global_char*)a.key_cache + head * a.cache_head * (int64_t)sizeof(T);
+        vbase = (global_char*)a.value_cache + head * a.cache_head * (int64_t)sizeof(T);
         const int r0 = t.m0 + wave * RB * 16, r1 = min(r0 + RB * 16, t.count) - 1;
-        first_token = r0 / group;
         last_token = r0 < t.count ? r1 / group : -1;
-        const bool vec = ((uintptr_t)a.q | (uint64_t)a.q_row * sizeof(T) | (uint64_t)a.q_head * sizeof(T)) % 16 == 0;
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            const int r = min(r0 + 16 * b + (lane & 15), t.count - 1);  // rows past the end: the last one's, not stored
-            token[b] = r / group;
-            const T* from = static_cast<const T*>(a.q) + (int64_t)(t.first + token[b]) * a.q_row +
-                            (int64_t)(head * group + r % group) * a.q_head;
-#pragma unroll
-            for (int k = 0; k < kQ; ++k) {
-                const int d = (k * 4 + (lane >> 4)) * E;
-                q[b][k] = u32x4{0, 0, 0, 0};
-                if (d < a.dim) {
-                    if (vec)
-                        q[b][k] = *reinterpret_cast<const u32x4*>(from + d);
-                    else
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if constexpr (kBf16)
-                                q[b][k][j] = from[d + 2 * j] | (uint32_t)from[d + 2 * j + 1] << 16;
-                            else
-                                q[b][k][j] = __float_as_uint(from[d + j]);
-                        }
-                }
-            }
             m[b] = kNone;
             l[b] = 0;
 #pragma unroll
             for (int f = 0; f < kOut; ++f) o[b][f] = f32x4{0, 0, 0, 0};
         }
     }
-
-    // Where key j of the sequence is (elements), -1 nowhere.
-    __device__ int64_t key_at(int j) const {
-        if (j >= t.places) return -1;
-        const uint32_t n = divide((uint32_t)j, page);
-        const int id = a.tables[t.seq * a.table_row + n];
-        return (unsigned)id < (unsigned)a.pages ? id * a.cache_page + ((uint32_t)j - n * a.page) * a.cache_token : -1;
+    __device__ __forceinline__ int token_of(int b) const {  // rows past the end: the last one, not stored
+        return min(t.m0 + (wave * RB + b) * 16 + (lane & 15), t.count - 1) / group;
+    }
+    __device__ __forceinline__ void load_q() {
+        const bool vec = ((uintptr_t)a.q | (uint64_t)a.q_row * sizeof(T) | (uint64_t)a.q_head * sizeof(T)) % 16 == 0;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            const int r = min(t.m0 + (wave * RB + b) * 16 + (lane & 15), t.count - 1);
+            const T* from = static_cast<const T*>(a.q) + (int64_t)(t.first + r / group) * a.q_row +
+                            (int64_t)(kv_head * group + r % group) * a.q_head;
+#pragma unroll
+            for (int k = 0; k < kQ; ++k) {
+                const int d = (k * 4 + (lane >> 4)) * E;
+                u32x4 x = {0, 0, 0, 0};
+                if (d < a.dim) {
+                    if (vec)
+                        x = *reinterpret_cast<const u32x4*>(from + d);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if constexpr (kBf16)
+                                x[j] = from[d + 2 * j] | (uint32_t)from[d + 2 * j + 1] << 16;
+                            else
+                                x[j] = __float_as_uint(from[d + j]);
+                        }
+                }
+                q[b][k] = x;
+            }
+        }
     }
 
+    __device__ uint32_t key_at(int j) const { return ::key_at(a, units, t, j); }
+
     // Starts the copies of a tile whose keys are at `at` (key i's in lane i): 1 KiB a wave instruction, to consecutive
-    // bytes of LDS; the parts' positions are in the addresses.  WHOLE: every key exists, heads have D elements.
+    // bytes of LDS; the parts' positions are in the addresses.  WHOLE: every key exists.
     template <bool WHOLE>
-    __device__ __forceinline__ void copy_of(int stage, int64_t at) const {
-        const char* zeros = reinterpret_cast<const char*>(&kZeros);
+    __device__ __forceinline__ void copy(int stage, uint32_t at) const {
+        global_char* zeros = (global_char*)kZeros;
         char* to = lds + stage * kStage;
         int lane = this->lane;
         if (kTight || !WHOLE) asm volatile("" : "+v"(lane));  // (addresses are not kept in registers across the loop)
@@ -310,19 +358,14 @@ struct Pass {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int n = wave * kLoads + i, r = n * (64 / kParts) + lane / kParts;
-            const int64_t from = __shfl(at, r) * (int64_t)sizeof(T);
+            const uint32_t from = __shfl(at, r);
             const int kp = part ^ k_swizzle(r), vp = part ^ v_swizzle(r);
-            const char* ks = WHOLE || (from >= 0 && kp * E < a.dim) ? kbase + from + kp * 16 : zeros;
-            const char* vs = WHOLE || (from >= 0 && vp * E < a.dim) ? vbase + from + vp * 16 : zeros;
-            __builtin_amdgcn_global_load_lds((global_void*)ks, (lds_void*)(to + n * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((global_void*)vs, (lds_void*)(to + kTile + n * 1024), 16, 0, 0);
+            const bool there = WHOLE || from != kNowhere;
+            global_char* ks = there && (FULL || kp * E < a.dim) ? in_cache(kbase, from, units) + kp * 16 : zeros;
+            global_char* vs = there && (FULL || vp * E < a.dim) ? in_cache(vbase, from, units) + vp * 16 : zeros;
+            copy_to_lds(ks, to + n * 1024);
+            copy_to_lds(vs, to + kTile + n * 1024);
         }
-    }
-    __device__ __forceinline__ void copy(int stage, int64_t at) const {
-        if (a.dim == D && __all(at >= 0))
-            copy_of<true>(stage, at);
-        else
-            copy_of<false>(stage, at);
     }
     static __device__ void sync() {  // LDS alone: copies stay in flight
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
@@ -340,12 +383,12 @@ struct Pass {
     // Which of the 32 keys from k0 on row b of this lane sees, of those that exist.
     __device__ uint32_t seen(int b, int k0, uint32_t there) const {
         if (!a.mask) {
-            const int upto = t.held + token[b] - k0;
+            const int upto = t.held + token_of(b) - k0;
             return upto < 0 ? 0 : upto >= 31 ? there : there & ((2u << upto) - 1);
         }
         const int j = k0 - t.held;
         if (j <= -32) return there;
-        const int32_t* words = a.mask + (int64_t)(t.first + token[b]) * a.mask_words;
+        const int32_t* words = a.mask + (int64_t)(t.first + token_of(b)) * a.mask_words;
         if (j < 0) {
             const uint32_t w = a.mask_words > 0 ? words[0] : 0;
             return there & (w << -j | ((1u << -j) - 1));
@@ -357,7 +400,7 @@ struct Pass {
 
     // Byte of LDS, from a step's first key on, of the values that product f reads with ds_read_tr16_b64: lane n of 16
     // reads 8 bytes of key 4 g + n / 4 (and of that 16 keys on), and gets element n of four keys.
-    __device__ __forceinline__ int tr_at() const {
+    static __device__ __forceinline__ int tr_at(int lane) {
         const int n = lane & 15, r = 4 * (lane >> 4) + (n >> 2);
         return r * kRow + (v_swizzle(r) ^ (n >> 1 & 1)) * 16 + (n & 1) * 8;
     }
@@ -373,30 +416,18 @@ struct Pass {
         return *reinterpret_cast<const f32x4*>(v + r * kRow + ((16 * f + (lane & 15)) ^ v_swizzle(r)) * 16);
     }
 
-    // O += the values of 32 keys (from v on) times their weights.
-    __device__ __forceinline__ void add_values(const char* v, const float (&w)[RB][2][4], const u32x4 (&wb)[RB]) {
-        if constexpr (kBf16) {
-            int at = tr_at();
-            asm volatile("" : "+v"(at));  // (one operation a product, not a register each)
-#pragma unroll
-            for (int f = 0; f < kOut; ++f) {
-                const u32x4 y = tr_read(v, at, f);
-#pragma unroll
-                for (int b = 0; b < RB; ++b) o[b][f] = mfma(y, wb[b], o[b][f]);
-            }
-        } else {
-#pragma unroll
-            for (int f = 0; f < kOut / 4; ++f)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const f32x4 y = row_read(v, i, f);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int b = 0; b < RB; ++b)
-                            o[b][4 * f + j] = mfma4(y[j], w[b][i / 4][i % 4], o[b][4 * f + j]);
-                }
-        }
+    // The operands of the step's products, read kDeep - 1 ahead of them.  Keys: part 4 i + g of keys 16 h + lane % 16.
+    // Values (operand t of kValues): bf16 a product's, 32 keys by 16 elements; float32 four products', four keys by 64 elements.
+    static constexpr int kDeep = kBf16 ? 4 : 3;
+    static constexpr int kKeys = 2 * kQ, kValues = kBf16 ? kOut : 2 * kOut;
+    using Operand = u32x4;
+    static __device__ __forceinline__ Operand read_key(const char* k, int at, int t) {
+        const int i = t / 2, h = t % 2;  // (of eight parts that change places the second four are the first's neighbours)
+        return *reinterpret_cast<const Operand*>(k + (at ^ i % 2 * 64) + 16 * h * kRow + i / 2 * 128);
+    }
+    __device__ __forceinline__ Operand read_value(const char* v, int at, int t) const {
+        if constexpr (kBf16) return tr_read(v, at, t);
+        return __builtin_bit_cast(Operand, row_read(v, t % 8, t / 8));
     }
 
     // The values of 32 keys (from v on) that are not finite, to the rows that see them: counted by a product, their kinds
@@ -413,7 +444,7 @@ struct Pass {
 #pragma unroll
             for (int i = 0; i < 4; ++i) seeb[b][i] = round2(see[b][2 * i], see[b][2 * i + 1]);
         }
-        const int at = kBf16 ? tr_at() : 0;
+        const int at = kBf16 ? tr_at(lane) : 0;
 #pragma unroll
         for (int f = 0; f < (kBf16 ? kOut : kOut / 4); ++f) {
             __builtin_amdgcn_sched_barrier(0);
@@ -476,53 +507,68 @@ struct Pass {
         sync();  // (and the flags can be written again)
     }
 
-    // The keys k0 .. k0 + 31, at rows k .. of the tile in `stage`.
+    // The keys k0 .. k0 + 31, at rows k .. of the tile in `stage`.  ALL: every row sees every one of them.
+    template <bool ALL>
     __device__ __forceinline__ void step(int stage, int k, int k0, uint32_t there) {
         const char* ks = lds + stage * kStage;
         const char* vs = ks + kTile;
-        const int n = lane & 15, g = lane >> 4;
-        int at[2];  // parts 4 i + g of a key: eight of them change places
+        // (before the products: no branch stands between them and the first use of their results)
+        uint32_t sees[RB];
+        if (!ALL)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) at[i] = n * kRow + ((4 * i + g) ^ k_swizzle(n)) * 16;
+            for (int b = 0; b < RB; ++b) sees[b] = seen(b, k0, there) >> (4 * (this->lane >> 4));
+        int lane = this->lane;
+        if (kTight) asm volatile("" : "+v"(lane));  // (addresses are made again, not kept)
+        const int at = (lane & 15) * kRow + ((lane >> 4) ^ k_swizzle(lane & 15)) * 16;
+        ks += k * kRow;
+        vs += k * kRow;
+        Operand x[kDeep];
+#pragma unroll
+        for (int i = 0; i < kDeep - 1; ++i) x[i] = read_key(ks, at, i);
         f32x4 s[RB][2];
 #pragma unroll
         for (int b = 0; b < RB; ++b) s[b][0] = s[b][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kQ; ++i)
+        for (int i = 0; i < kKeys; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + kDeep - 1 < kKeys) x[(i + kDeep - 1) % kDeep] = read_key(ks, at, i + kDeep - 1);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(ks + (k + 16 * h) * kRow + at[i % 2] + i / 2 * 128);
+            for (int b = 0; b < RB; ++b) {
+                f32x4& z = s[b][i % 2];
+                if constexpr (kBf16) {
+                    z = mfma(x[i % kDeep], q[b][i / 2], z);
+                } else {
 #pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    if constexpr (kBf16) {
-                        s[b][h] = mfma(x, q[b][i], s[b][h]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            s[b][h] = mfma4(__uint_as_float(x[j]), __uint_as_float(q[b][i][j]), s[b][h]);
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        z = mfma4(__uint_as_float(x[i % kDeep][j]), __uint_as_float(q[b][i / 2][j]), z);
                 }
             }
-        // scores and the maximum before any branch: the first use of the products
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        int vat = kBf16 ? tr_at(lane) : 0;
+        asm volatile("" : "+v"(vat));  // (one operation an operand, not a register each)
+#pragma unroll
+        for (int i = 0; i < kDeep - 1; ++i) x[i] = read_value(vs, vat, i);
         float top[RB];
-        const bool all = there == 0xffffffffu && (a.mask ? k0 + 32 <= t.held : k0 + 31 <= t.held + first_token);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            const uint32_t bits = (all ? 0xffffffffu : seen(b, k0, there)) >> (4 * g);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (!(bits >> (16 * (i / 4) + i % 4) & 1)) s[b][i / 4][i % 4] = kNone;
+            {
+                s[b][i / 4][i % 4] *= c;
+                if (!ALL && !(sees[b] >> (16 * (i / 4) + i % 4) & 1)) s[b][i / 4][i % 4] = kNone;
+            }
             const f32x4 x = s[b][0], y = s[b][1];
             top[b] = pair_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
         }
         bool grows = false;
 #pragma unroll
-        for (int b = 0; b < RB; ++b) grows |= top[b] > m[b];
+        for (int b = 0; b < RB; ++b) grows |= top[b] > m[b] + kSlack;
         if (__any(grows)) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
                 const float now = fmaxf(m[b], top[b]);
-                const float f = m[b] == kNone ? 1.0f : exp2_raw(m[b] * c - now * c);  // (nothing yet but clean()'s)
+                const float f = m[b] == kNone ? 1.0f : exp2_raw(m[b] - now);  // (nothing yet but clean()'s)
                 m[b] = now;
                 l[b] *= f;
 #pragma unroll
@@ -533,47 +579,89 @@ struct Pass {
         u32x4 wb[RB];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            const float mc = m[b] == kNone ? 0.0f : m[b] * c;
+            const float most = m[b] == kNone ? 0.0f : m[b];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[b][i / 4][i % 4] = exp2_raw(__builtin_fmaf(s[b][i / 4][i % 4], c, -mc));
+            for (int i = 0; i < 8; ++i) w[b][i / 4][i % 4] = exp2_raw(s[b][i / 4][i % 4] - most);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x = w[b][i / 2][i % 2 * 2], y = w[b][i / 2][i % 2 * 2 + 1];
-                if (kBf16) {
+                const float x = w[b][i / 2][i % 2 * 2], y = w[b][i / 2][i % 2 * 2 + 1];
+                if constexpr (kBf16) {
                     wb[b][i] = round2(x, y);
-                    x = __uint_as_float(wb[b][i] << 16);
-                    y = __uint_as_float(wb[b][i] & 0xffff0000u);
+                    l[b] = sum2(wb[b][i], l[b]);  // (the rounded ones)
+                } else {
+                    l[b] += x;
+                    l[b] += y;
                 }
-                l[b] += x;
-                l[b] += y;
             }
         }
-        add_values(vs + k * kRow, w, wb);
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + kDeep - 1 < kValues) x[(i + kDeep - 1) % kDeep] = read_value(vs, vat, i + kDeep - 1);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                if constexpr (kBf16) {
+                    o[b][i] = mfma(x[i % kDeep], wb[b], o[b][i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        f32x4& z = o[b][i / 8 * 4 + j];
+                        z = mfma4(__uint_as_float(x[i % kDeep][j]), w[b][i % 8 / 4][i % 4], z);
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 
-    // The tiles of keys k0 .. k1 - 1 of this tile of rows.
-    __device__ void run(int k0, int k1, int* flags) {
-        arrived();  // (the tile of rows before is done with LDS)
-        int64_t next = key_at(k0 * BN + lane % BN);
-        copy(0, next);
-        uint64_t there = __ballot(next >= 0);
-        next = k0 + 1 < k1 ? key_at((k0 + 1) * BN + lane % BN) : -1;
+    // The tiles of keys k0 .. k1 - 1, a tile ahead.  ALL: those below `full` whose keys all exist, which every row sees;
+    // else the others.  -> the first tile below `full` that some key of does not exist (ALL).
+    template <bool ALL>
+    __device__ __forceinline__ int pass(int k0, int k1, int full, int* flags) {
+        int first_bad = full;
+        arrived();  // (whoever used LDS before is done)
+        uint32_t next = key_at(k0 * BN + lane % BN);
+        // (ALL: a tile with absent keys is left to the other loop, so the first place does for them; there is one, as
+        // places, and so tiles below `full`, are 0 without pages)
+        copy<ALL>(0, ALL && next == kNowhere ? 0 : next);
+        uint64_t there = __ballot(next != kNowhere);
+        next = k0 + 1 < k1 ? key_at((k0 + 1) * BN + lane % BN) : kNowhere;
         for (int k = k0; k < k1; ++k) {
             const uint64_t now = there;
             const int stage = (k - k0) & 1;
             arrived();
             if (k + 1 < k1) {
-                copy(stage ^ 1, next);
-                there = __ballot(next >= 0);
+                copy<ALL>(stage ^ 1, ALL && next == kNowhere ? 0 : next);
+                there = __ballot(next != kNowhere);
                 if (k + 2 < k1) next = key_at((k + 2) * BN + lane % BN);
             }
-            if (now != ~0ull || (a.mask ? (k + 1) * BN > t.held : (k + 1) * BN - 1 > t.held + t.m0 / group))
-                clean(stage, k * BN, now, flags);
-#pragma unroll
+            if (ALL != (k < full && now == ~0ull)) {
+                if (ALL) first_bad = min(first_bad, k);
+                continue;
+            }
+            if (!ALL) clean(stage, k * BN, now, flags);
+#pragma unroll 1
             for (int i = 0; i < BN / 32; ++i) {
                 const int from = k * BN + 32 * i;
-                if (last_token >= 0 && (a.mask || from <= t.held + last_token)) step(stage, 32 * i, from, (uint32_t)(now >> 32 * i));
+                if (last_token >= 0 && (ALL || a.mask || from <= t.held + last_token))
+                    step<ALL>(stage, 32 * i, from, (uint32_t)(now >> 32 * i));
             }
+        }
+        return first_bad;
+    }
+
+    // The tiles of keys k0 .. k1 - 1 of this tile of rows: those that need no masks first, in a loop without them.
+    __device__ __forceinline__ void run(int k0, int k1, int* flags) {
+        const int seen_by_all = min(a.mask ? t.held : t.held + t.m0 / group + 1, t.places);
+        const int full = min(max(seen_by_all / BN, k0), k1);
+        int rest = full;
+        if (full > k0) {
+            load_q();
+            rest = pass<true>(k0, full, full, flags);
+        }
+        if (rest < k1) {
+            load_q();  // (again, so that what the masks need does not push it out of the first loop's registers)
+            pass<false>(rest, k1, full, flags);
         }
     }
 };
@@ -595,39 +683,34 @@ __device__ __forceinline__ bool quads(const attn_dev_args& a) {  // four element
     return ((uintptr_t)a.out | (uint64_t)a.out_row * sizeof(T) | (uint64_t)a.out_head * sizeof(T)) % (4 * sizeof(T)) == 0;
 }
 
-template <class T, int D, int RB, int W, int BN>
-__global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan p, Divisor page, int least) {
-    using P = Pass<T, D, RB, W, BN>;
+template <class T, int D, int RB, int W, int BN, bool FULL>
+__global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan p, AttnUnits units) {
+    using P = Pass<T, D, RB, W, BN, FULL>;
     __shared__ __attribute__((aligned(1024))) char lds[2 * P::kStage];
     __shared__ int held[ATTN_HELD];
-    __shared__ Share share_sh;
     __shared__ int flags[W];
     const Shape shape{a, p};
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (wave == 0) {
-        const Share s = share_of(shape, held, least);
-        if (threadIdx.x == 0) share_sh = s;
-    }
-    __syncthreads();
-    const Share share = share_sh;
+    const Share share = uniform(share_of(shape, held, p.least));
     AttnDesc* desc = reinterpret_cast<AttnDesc*>(static_cast<char*>(a.work) + p.desc_at) + blockIdx.x;
     float2* stats = reinterpret_cast<float2*>(static_cast<char*>(a.work) + p.stat_at);
     f32x4* parts = reinterpret_cast<f32x4*>(static_cast<char*>(a.work) + p.part_at);
     AttnDesc left{};
-    P pass{a, page, p.group, lds, (int)(threadIdx.x & 63), wave};
+    P pass{a, units, p.group, lds, (int)(threadIdx.x & 63), wave};
     pass.c = a.scale * kLog2e;
-    int64_t at = share.from, place = share.place, before = share.before;
-    const int64_t places = shape.places();
+    int64_t at = share.from, before = share.before;
+    int place = share.place;
+    const int places = shape.places();
     const bool vec = quads<T>(a);
     while (at < share.to && place < places) {
-        const Tile t = shape.tile(place);
+        const Tile t = uniform(shape.tile(place));
         const int64_t in = at - before, all = (int64_t)t.tiles * a.heads_k;
         if (in >= all) {
             before += all;
             ++place;
             continue;
         }
-        const int head = (int)(in / t.tiles), k0 = (int)(in - (int64_t)head * t.tiles);
+        const int head = (int)quotient(in, t.tiles), k0 = (int)(in - (int64_t)head * t.tiles);
         const int k1 = (int)min((int64_t)t.tiles, k0 + (share.to - at));
         at += k1 - k0;
         pass.begin(t, head);
@@ -635,7 +718,7 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
         asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");  // the last products' results, whatever way the loop was left
         if (k0 == 0 && k1 < t.tiles)
             left = AttnDesc{1, t.first, t.m0, t.count, head,
-                            (int)(((at - k1 + t.tiles) * share.workers - 1) / share.total)};
+                            (int)quotient((at - k1 + t.tiles) * share.workers - 1, share.total)};
         const int n = threadIdx.x & 15, slot = 2 * blockIdx.x + (k0 == 0);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -655,7 +738,7 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
                     if (d < a.dim) store4(to + d, x, vec);
                 }
             } else {
-                if (threadIdx.x % 64 < 16) stats[(int64_t)slot * p.rows + 16 * block + n] = float2{pass.m[b] * pass.c, sum};
+                if (threadIdx.x % 64 < 16) stats[(int64_t)slot * p.rows + 16 * block + n] = float2{pass.m[b], sum};
                 f32x4* to = parts + ((int64_t)slot * (p.rows / 16) + block) * P::kOut * 64 + (threadIdx.x & 63);
 #pragma unroll
                 for (int i = 0; i < P::kOut; ++i) to[i * 64] = pass.o[b][i];
@@ -667,6 +750,7 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
 
 // The parts of a tile of rows, 16 rows and 64 elements to a workgroup: its first part is the last of workgroup
 // blockIdx.x, the others are the first of those that follow.  Four wavefronts take every fourth.
+constexpr int kAtOnce = 4;
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(attn_dev_args a, AttnPlan p) {
     const AttnDesc d = reinterpret_cast<const AttnDesc*>(static_cast<const char*>(a.work) + p.desc_at)[blockIdx.x];
@@ -682,17 +766,36 @@ __global__ __launch_bounds__(256) void attn_join_kernel(attn_dev_args a, AttnPla
     f32x4 o[4] = {};
     float m = kNone, l = 0;
     if (mine)
-        for (int w = first + wave; w <= d.last; w += 4) {
-            const int slot = w == first ? 2 * first + 1 : 2 * w;
-            const float2 s = stats[(int64_t)slot * p.rows + 16 * block + n];
-            const f32x4* from = parts + (((int64_t)slot * (p.rows / 16) + block) * kOut + 4 * blockIdx.z) * 64 + lane;
-            const float now = fmaxf(m, s.x);
-            if (now == kNone) continue;
-            const float f = exp2_raw(m - now), e = exp2_raw(s.x - now);
-            m = now;
-            l = l * f + s.y * e;
+        for (int w0 = first + wave; w0 <= d.last; w0 += 4 * kAtOnce) {
+            // (a part past the last: the last again, with no weight)
+            float2 s[kAtOnce];
+            f32x4 x[kAtOnce][4];
+            float now = m;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = o[i] * f + from[i * 64] * e;
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int w = min(w0 + 4 * j, d.last), slot = w == first ? 2 * first + 1 : 2 * w;
+                s[j] = stats[(int64_t)slot * p.rows + 16 * block + n];
+                const f32x4* from = parts + (((int64_t)slot * (p.rows / 16) + block) * kOut + 4 * blockIdx.z) * 64 + lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = from[i * 64];
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+                if (w0 + 4 * j <= d.last) now = fmaxf(now, s[j].x);
+            if (now == kNone) continue;
+            const float f = exp2_raw(m - now);
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] *= f;
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                if (w0 + 4 * j > d.last) break;
+                const float e = exp2_raw(s[j].x - now);
+                l += s[j].y * e;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] += x[j][i] * e;
+            }
         }
     tops[wave][lane] = float2{m, l};
 #pragma unroll
@@ -722,16 +825,445 @@ __global__ __launch_bounds__(256) void attn_join_kernel(attn_dev_args a, AttnPla
     if (at < a.dim) store4(to + at, x, quads<T>(a));
 }
 
+// ---- few rows ----------------------------------------------------------------------------
+// Up to 16 rows on a key head: bound by the cache's bytes.  Every wavefront has keys of its own, 16 at a time, straight
+// to registers: as the left operands of K Q^T and, with float32 weights and values widened, of V^T W^T, whose 16 by
+// 16 by 4 products take a lane's 16 bytes of a value as that many products' operands.  (bf16 products of V would need
+// its transpose, from LDS: the float32 ones are a third of the time that the bytes take.)  The wavefronts' outputs meet in
+// LDS at the end.
+// FULL: heads have D elements.
+template <class T, int D, bool FULL>
+struct Few {
+    static constexpr bool kBf16 = sizeof(T) == 2;
+    static constexpr int W = 4;
+    static constexpr int E = 16 / sizeof(T);
+    static constexpr int kQ = D / (4 * E);               // a lane's parts of a key
+    static constexpr int kN = D / 16 < E ? D / 16 : E;   // elements of a lane's part of a value, next to each other
+    static constexpr int kV = D / (16 * kN);             // such parts
+    static constexpr int kPitch = D + 4;                 // floats of a row in LDS
+    using VPart = std::conditional_t<kN * sizeof(T) == 16, u32x4, u32x2>;
+
+    const attn_dev_args& a;
+    AttnUnits units;
+    int lane, wave;
+    Tile t;
+    global_char* kbase;
+    global_char* vbase;
+    const u32x4* q;  // in LDS: part k of lane l at [k][l]
+    int token;       // of the lane's row
+    f32x4 o[kV][kN];
+    float m, l, c;
+    u32x4 kr[kQ];
+    VPart vr[4][kV];
+
+    __device__ uint32_t key_at(int j) const { return ::key_at(a, units, t, j); }
+    // Lane n of 16 reads key n; parts past the head's elements are read as the first and zeroed.
+    __device__ __forceinline__ void load_keys(uint32_t at) {
+        const int g = lane >> 4;
+        using Part = __attribute__((address_space(1))) const u32x4;
+        global_char* from = at == kNowhere ? (global_char*)kZeros : in_cache(kbase, at, units);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) kr[i] = *(Part*)(from + (FULL || (4 * i + g) * E < a.dim ? (4 * i + g) * 16 : 0));
+    }
+    // Lane n of 16, group g: elements of key 4 g + i, which is at `at` of lane 4 g + i.
+    __device__ __forceinline__ global_char* value_at(uint32_t at, int i) const {
+        const uint32_t x = __shfl(at, 4 * (lane >> 4) + i);
+        return x == kNowhere ? (global_char*)kZeros : in_cache(vbase, x, units);
+    }
+    __device__ __forceinline__ void load_value(global_char* from, int i) {
+#pragma unroll
+        for (int f = 0; f < kV; ++f) {
+            const int d = (16 * f + (lane & 15)) * kN;
+            vr[i][f] = *(__attribute__((address_space(1))) const VPart*)(from + (FULL || d < a.dim ? d : 0) * (int)sizeof(T));
+        }
+    }
+    __device__ __forceinline__ float value(int i, int f, int j) const {
+        if constexpr (!kBf16) return __uint_as_float(vr[i][f][j]);
+        const uint32_t x = vr[i][f][j / 2];
+        return __uint_as_float(j % 2 ? x & 0xffff0000u : x << 16);
+    }
+
+    // Which of the 16 keys from k0 on the lane's row sees, of those that exist (Pass::seen).
+    __device__ uint32_t seen(int k0, uint32_t there) const {
+        if (!a.mask) {
+            const int upto = t.held + token - k0;
+            return upto < 0 ? 0 : upto >= 15 ? there : there & ((2u << upto) - 1);
+        }
+        const int j = k0 - t.held;
+        if (j <= -16) return there;
+        const int32_t* words = a.mask + (int64_t)(t.first + token) * a.mask_words;
+        if (j < 0) {
+            const uint32_t w = a.mask_words > 0 ? words[0] : 0;
+            return there & (w << -j | ((1u << -j) - 1));
+        }
+        const int n = j >> 5, sh = j & 31;
+        const uint32_t lo = n < a.mask_words ? words[n] : 0, hi = n + 1 < a.mask_words ? words[n + 1] : 0;
+        return there & (uint32_t)(((uint64_t)hi << 32 | lo) >> sh);
+    }
+
+    // The 16 keys from k0 on, in the registers; next: where the wavefront's next ones are, whose loads begin as soon as
+    // the products have read a register.  ALL: every row sees every key.
+    template <bool ALL, bool MORE>
+    __device__ __forceinline__ void step(int k0, uint32_t there, uint32_t next) {
+        const int g = lane >> 4;
+        // (before the products, as in Pass::step)
+        const uint32_t sees = ALL ? 0xffffu : seen(k0, there);
+        f32x4 s = {0, 0, 0, 0};
+        if constexpr (kBf16) {
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                u32x4 x = kr[i];
+                if (!FULL) x = (4 * i + g) * E < a.dim ? x : u32x4{0, 0, 0, 0};
+                s = mfma(x, q[i * 64 + lane], s);
+            }
+        } else {
+            f32x4 part[4] = {};  // (a product waits for the one before in its sum)
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                const f32x4 x = __builtin_bit_cast(f32x4, kr[i]), y = __builtin_bit_cast(f32x4, q[i * 64 + lane]);
+                const bool in = FULL || (4 * i + g) * E < a.dim;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[j] = mfma4(in ? x[j] : 0.0f, y[j], part[j]);
+            }
+            s = (part[0] + part[1]) + (part[2] + part[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            s[i] *= c;
+            if (!ALL && !(sees >> (4 * g + i) & 1)) s[i] = kNone;
+        }
+        const float top = pair_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+        global_char* from[4];
+        if (MORE) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_keys(next);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) from[i] = value_at(next, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__any(top > m + kSlack)) {
+            const float now = fmaxf(m, top);
+            const float f = m == kNone ? 1.0f : exp2_raw(m - now);  // (nothing yet but values that are not finite)
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < kV; ++i)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) o[i][j] *= f;
+        }
+        const float most = m == kNone ? 0.0f : m;
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = exp2_raw(s[i] - most);
+            l += w[i];
+        }
+        if (!ALL) clean(sees);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int f = 0; f < kV; ++f)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) o[f][j] = mfma4(value(i, f, j), w[i], o[f][j]);
+            if (MORE) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_value(from[i], i);
+            }
+        }
+    }
+
+    // Values that are not finite: to the rows that see them, and 0 in their place (Pass::clean).
+    __device__ __forceinline__ void clean(uint32_t sees) {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int f = 0; f < kV; ++f)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) odd |= is_odd(value(i, f, j));
+        if (!__any(odd)) return;
+        float see[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) see[i] = (float)(sees >> (4 * (lane >> 4) + i) & 1);
+#pragma unroll
+        for (int f = 0; f < kV; ++f) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                f32x4 kinds = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kinds = mfma4(kind_of(value(i, f, j)), see[i], kinds);
+                add_kinds(o[f][j], kinds);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kN * (int)sizeof(T) / 4; ++j) {
+                    if constexpr (kBf16)
+                        vr[i][f][j] = round2(finite(value(i, f, 2 * j)), finite(value(i, f, 2 * j + 1)));
+                    else
+                        vr[i][f][j] = __float_as_uint(finite(value(i, f, j)));
+                }
+        }
+    }
+    int group;
+
+    // The tiles of 64 keys k0 .. k1 - 1: keys 16 wave .. of each.  First those that every row sees, in a loop without
+    // masks; then the rest (the last ones, and those of absent pages), one by one.
+    __device__ __forceinline__ void run(int k0, int k1) {
+        const int n = lane & 15;
+        auto first = [&](int k) { return k * 16 * W + 16 * wave; };
+        auto load = [&](uint32_t at) {
+            load_keys(at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_value(value_at(at, i), i);
+        };
+        const int spare = min(a.mask ? t.held : t.held + t.m0 / group + 1, t.places) - 16 - 16 * wave;
+        const int full = min(max(spare < 0 ? 0 : spare / (16 * W) + 1, k0), k1);
+        int rest = full;
+        if (k0 < full) {
+            // Tables are read two tiles ahead, before the next tile's loads: waiting for them waits for nothing newer.
+            uint32_t at = key_at(first(k0) + n), next = k0 + 1 < full ? key_at(first(k0 + 1) + n) : kNowhere;
+            load(at);
+            int k = k0;
+            auto turn = [&](auto more) {
+                const uint32_t after = k + 2 < full ? key_at(first(k + 2) + n) : kNowhere;
+                if (__all(at != kNowhere)) {
+                    step<true, decltype(more)::value>(first(k), 0xffff, next);
+                } else {
+                    rest = min(rest, k);
+                    if (decltype(more)::value) load(next);
+                }
+                at = next;
+                next = after;
+                ++k;
+            };
+            while (k + 1 < full) turn(std::true_type{});
+            turn(std::false_type{});  // (apart: with a branch around its loads the compiler would wait for them at once)
+        }
+        for (int k = rest; k < k1; ++k) {
+            const uint32_t at = key_at(first(k) + n), there = (uint32_t)__ballot(at != kNowhere) & 0xffff;
+            if (there == 0 || (k < full && there == 0xffff)) continue;
+            load(at);
+            step<false, false>(first(k), there, kNowhere);
+        }
+    }
+};
+
+// Four consecutive elements of a row of out.
+template <class T>
+__device__ __forceinline__ void store_row(const attn_dev_args& a, int group, int first, int r, int head, int d, const float (&x)[4]) {
+    if (d >= a.dim) return;
+    T* to = static_cast<T*>(a.out) + (int64_t)(first + r / group) * a.out_row + (int64_t)(head * group + r % group) * a.out_head + d;
+    store4(to, x, quads<T>(a));
+}
+
+template <class T, int D, bool FULL>
+__global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, AttnPlan p, AttnUnits units) {
+    using P = Few<T, D, FULL>;
+    __shared__ int held[ATTN_HELD];
+    __shared__ u32x4 q[P::kQ * 64];
+    __shared__ float2 tops[P::W][16];
+    __shared__ __attribute__((aligned(16))) float sums[P::W][16][P::kPitch];
+    const Shape shape{a, p};
+    const Share share = uniform(share_of(shape, held, p.least));
+    AttnDesc* desc = reinterpret_cast<AttnDesc*>(static_cast<char*>(a.work) + p.desc_at) + blockIdx.x;
+    float2* stats = reinterpret_cast<float2*>(static_cast<char*>(a.work) + p.stat_at);
+    float* parts = reinterpret_cast<float*>(static_cast<char*>(a.work) + p.part_at);
+    AttnDesc left{};
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    P few{a, units, lane, wave};
+    few.c = a.scale * kLog2e;
+    few.q = q;
+    few.group = p.group;
+    int64_t at = share.from, before = share.before;
+    int place = share.place;
+    const int places = shape.places();
+    while (at < share.to && place < places) {
+        const Tile t = uniform(shape.tile(place));
+        const int64_t in = at - before, all = (int64_t)t.tiles * a.heads_k;
+        if (in >= all) {
+            before += all;
+            ++place;
+            continue;
+        }
+        const int head = (int)quotient(in, t.tiles), k0 = (int)(in - (int64_t)head * t.tiles);
+        const int k1 = (int)min((int64_t)t.tiles, k0 + (share.to - at));
+        at += k1 - k0;
+        if (k0 == 0 && k1 < t.tiles)
+            left = AttnDesc{1, t.first, t.m0, t.count, head,
+                            (int)quotient((at - k1 + t.tiles) * share.workers - 1, share.total)};
+        // q to LDS, a part a thread at a time
+        const int rows = min(16, t.count - t.m0);
+        few.t = t;
+        few.token = (t.m0 + min(n, rows - 1)) / p.group;
+        few.kbase = (global_char*)a.key_cache + head * a.cache_head * (int64_t)sizeof(T);
+        few.vbase = (global_char*)a.value_cache + head * a.cache_head * (int64_t)sizeof(T);
+        const bool vec = ((uintptr_t)a.q | (uint64_t)a.q_row * sizeof(T) | (uint64_t)a.q_head * sizeof(T)) % 16 == 0;
+        for (int i = wave; i < P::kQ; i += P::W) {
+            const int r = t.m0 + min(n, rows - 1), d = (4 * i + g) * P::E;
+            const T* from = static_cast<const T*>(a.q) + (int64_t)(t.first + r / p.group) * a.q_row +
+                            (int64_t)(head * p.group + r % p.group) * a.q_head + d;
+            u32x4 x = {0, 0, 0, 0};
+            if (d < a.dim) {
+                if (vec)
+                    x = *reinterpret_cast<const u32x4*>(from);
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (P::kBf16)
+                            x[j] = from[2 * j] | (uint32_t)from[2 * j + 1] << 16;
+                        else
+                            x[j] = __float_as_uint(from[j]);
+                    }
+            }
+            q[i * 64 + lane] = x;
+        }
+        few.m = kNone;
+        few.l = 0;
+#pragma unroll
+        for (int f = 0; f < P::kV; ++f)
+#pragma unroll
+            for (int j = 0; j < P::kN; ++j) few.o[f][j] = f32x4{0, 0, 0, 0};
+        __syncthreads();
+        if (t.held >= 0) few.run(k0, k1);
+        asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");  // the last products' results, whatever way the loop was left
+        // a row's maximum over the wavefronts, and what each has, scaled to it
+        const float sum = pair_sum(few.l);
+        if (g == 0) tops[wave][n] = float2{few.m, sum};
+        __syncthreads();
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < P::W; ++w) top = fmaxf(top, tops[w][n].x);
+        const float f = few.m == kNone ? 1.0f : exp2_raw(few.m - top);
+        if (n < rows)
+#pragma unroll
+            for (int v = 0; v < P::kV; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < P::kN; j += 4)
+                        *reinterpret_cast<f32x4*>(&sums[wave][n][(16 * v + 4 * g + e) * P::kN + j]) =
+                            f32x4{few.o[v][j][e], few.o[v][j + 1][e], few.o[v][j + 2][e], few.o[v][j + 3][e]} * f;
+        __syncthreads();
+        const int slot = 2 * blockIdx.x + (k0 == 0);
+        for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            f32x4 x = {0, 0, 0, 0};
+            float most = kNone, all_l = 0;
+#pragma unroll
+            for (int w = 0; w < P::W; ++w) {
+                x += *reinterpret_cast<const f32x4*>(&sums[w][r][d]);
+                most = fmaxf(most, tops[w][r].x);
+            }
+#pragma unroll
+            for (int w = 0; w < P::W; ++w) {
+                const float2 s = tops[w][r];
+                all_l += s.x == kNone ? 0.0f : s.y * exp2_raw(s.x - most);
+            }
+            if (k0 == 0 && k1 == t.tiles) {
+                const float y = 1.0f / all_l;
+                float z[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = all_l == 0 ? 0.0f : x[e] * y;
+                store_row<T>(a, p.group, t.first, t.m0 + r, head, d, z);
+            } else {
+                *reinterpret_cast<f32x4*>(parts + ((int64_t)slot * 16 + r) * D + d) = x;
+                if (d == 0) stats[slot * 16 + r] = float2{most, all_l};
+            }
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *desc = left;
+}
+
+// The parts of a row, a row to a workgroup: D / 4 lanes a part, kJoin parts at a time, two of them of each lane.
+constexpr int kJoin = 16;
+template <class T, int D>
+__global__ __launch_bounds__(kJoin * (D / 4)) void attn_step_join_kernel(attn_dev_args a, AttnPlan p) {
+    const AttnDesc d = reinterpret_cast<const AttnDesc*>(static_cast<const char*>(a.work) + p.desc_at)[blockIdx.x];
+    const int r = blockIdx.y;
+    if (!d.there || d.m0 + r >= d.count) return;
+    const float2* stats = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.stat_at);
+    const float* parts = reinterpret_cast<const float*>(static_cast<const char*>(a.work) + p.part_at);
+    __shared__ f32x4 sums[kJoin][D / 4];
+    __shared__ float2 tops[kJoin];
+    const int lane = threadIdx.x % (D / 4), group = threadIdx.x / (D / 4), first = blockIdx.x;
+    f32x4 o = {0, 0, 0, 0};
+    float m = kNone, l = 0;
+    constexpr int kEach = 4;
+    for (int w0 = first + group; w0 <= d.last; w0 += kJoin * kEach) {
+        float2 s[kEach];
+        f32x4 x[kEach];
+        float now = m;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {  // (past the last: the last again, with no weight)
+            const int w = min(w0 + kJoin * j, d.last), slot = w == first ? 2 * first + 1 : 2 * w;
+            s[j] = stats[slot * 16 + r];
+            x[j] = *reinterpret_cast<const f32x4*>(parts + ((int64_t)slot * 16 + r) * D + 4 * lane);
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (w0 + kJoin * j <= d.last) now = fmaxf(now, s[j].x);
+        const float f = m == kNone ? 1.0f : exp2_raw(m - now);
+        m = now;
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            if (w0 + kJoin * j > d.last) break;
+            const float e = s[j].x == kNone ? 1.0f : exp2_raw(s[j].x - now);  // (values that are not finite alone)
+            l += s[j].y * e;
+            o += x[j] * e;
+        }
+    }
+    sums[group][lane] = o;
+    if (lane == 0) tops[group] = float2{m, l};
+    __syncthreads();
+    if (group) return;
+    float top = kNone, all = 0;
+#pragma unroll
+    for (int w = 0; w < kJoin; ++w) top = fmaxf(top, tops[w].x);
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kJoin; ++w) {
+        const float e = tops[w].x == kNone ? 1.0f : exp2_raw(tops[w].x - top);
+        all += tops[w].y * e;
+        x += sums[w][lane] * e;
+    }
+    const float y = 1.0f / all;
+    float z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = all == 0 ? 0.0f : x[e] * y;
+    store_row<T>(a, p.group, d.first, d.m0 + r, d.head, 4 * lane, z);
+}
+
+template <class T, int D>
+hipError_t launch_step(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
+    const AttnUnits units = attn_units(a);
+    if (a.dim == D)
+        attn_step_kernel<T, D, true><<<dim3((unsigned)p.grid), 256, 0, s>>>(a, p, units);
+    else
+        attn_step_kernel<T, D, false><<<dim3((unsigned)p.grid), 256, 0, s>>>(a, p, units);
+    attn_step_join_kernel<T, D><<<dim3((unsigned)p.grid, 16), kJoin * (D / 4), 0, s>>>(a, p);
+    return hipGetLastError();
+}
+
 template <class T, int D, int RB, int W, int BN>
 hipError_t launch(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
-    attn_kernel<T, D, RB, W, BN><<<dim3((unsigned)p.grid), 64 * W, 0, s>>>(a, p, divisor(a.page), 1);
+    const AttnUnits units = attn_units(a);
+    if (a.dim == D)
+        attn_kernel<T, D, RB, W, BN, true><<<dim3((unsigned)p.grid), 64 * W, 0, s>>>(a, p, units);
+    else
+        attn_kernel<T, D, RB, W, BN, false><<<dim3((unsigned)p.grid), 64 * W, 0, s>>>(a, p, units);
     attn_join_kernel<T, D><<<dim3((unsigned)p.grid, (unsigned)(p.rows / 16), D / 64), 256, 0, s>>>(a, p);
     return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_bf16(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
-    if (p.blocks == 1) return launch<uint16_t, D, 1, 1, 32>(a, p, s);
+    if (p.few) return launch_step<uint16_t, D>(a, p, s);
     switch (p.waves) {
         case 1: return launch<uint16_t, D, 2, 1, 32>(a, p, s);
         case 2: return launch<uint16_t, D, 2, 2, 32>(a, p, s);
@@ -741,8 +1273,8 @@ hipError_t launch_bf16(const attn_dev_args& a, const AttnPlan& p, hipStream_t s)
 }
 template <int D>
 hipError_t launch_f32(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
+    if (p.few) return launch_step<float, D>(a, p, s);
     switch (p.waves) {
-        case 1: return launch<float, D, 1, 1, 32>(a, p, s);
         case 2: return launch<float, D, 1, 2, 32>(a, p, s);
         case 4: return launch<float, D, 1, 4, 32>(a, p, s);
         default: return launch<float, D, 1, 8, 32>(a, p, s);

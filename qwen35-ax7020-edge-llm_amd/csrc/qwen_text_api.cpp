@@ -221,6 +221,7 @@ const char* paged_bad(const attn_dev_args* a) {
     if (a->mask && (!in(a->mask_words, 0, 1 << 16) || !aligned(a->mask, 4)))
         return "mask_words are 0 to 2^16, mask 4-byte aligned";
     if (a->n_seq == 0 || a->rows == 0) return nullptr;
+    if (!attn_units_fit(*a)) return "the caches span more places than 32 bits number";
     const size_t es = a->dtype == QWEN_BF16 ? 2 : 4;
     if (!a->out || !a->q || !aligned(a->out, es) || !aligned(a->q, es))
         return "out or q is NULL or not aligned to its elements";
