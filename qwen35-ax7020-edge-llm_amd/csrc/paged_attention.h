@@ -20,7 +20,8 @@ struct AttnPlan {
     int each;     // tiles of rows of a sequence, without starts
     int keys;     // of a tile of keys
     int grid;     // workgroups
-    int least;    // tiles of keys of a workgroup's share
+    int extra;    // tiles of keys that a tile of rows counts for besides its own
+    int least;    // tiles of a workgroup's share
     size_t desc_at;   // AttnDesc [grid]
     size_t stat_at;   // float2 [2 grid][rows]: a part's maximum and sum
     size_t part_at;   // float [2 grid][rows][dim]
@@ -45,8 +46,13 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     const size_t lds = (size_t)4 * p.keys * p.dim * (bf16 ? 2 : 4) + ATTN_HELD * 4 + 256;
     p.grid = 256 * (p.few ? 2 : (int)std::min<size_t>(std::min(4, 8 / p.waves), 160 * 1024 / lds));
     // A part is written and read again, 8 bytes an output: of many rows as much as several tiles of keys (one sequence of
-    // 6,000 tokens with 26 drafted ones: 1 | 2 | 4 | 8 tiles 94 | 60 | 46 | 50 us).
+    // 6,000 tokens with 26 drafted ones: 1 | 2 | 4 | 8 tiles 96 | 57 | 42 | 40 us; a prompt of 2,048 73 | 71 | 71 | 87).
     p.least = p.few ? 1 : 4;
+    // What a tile of rows costs by itself, its first keys' latency, masks and results, in tiles of keys.  Left out, the
+    // workgroups with a sequence's first rows, many tiles of rows with few keys, are the last by far: a prompt of 16,384
+    // tokens with 0 | 2 | 4 | 8 tiles of 64 keys 1,764 | 1,468 | 1,245 | 1,160 us; 8,192 of 16 heads of 128 589 | 435 |
+    // 372 | 381; float32 prompts with 0 | 1 | 2 | 4 tiles of 32 107 | 98 | 98 | 105.
+    p.extra = p.few ? 1 : bf16 ? std::max(256, 2 * p.dim) / p.keys : 2;
     size_t at = 0;
     auto put = [&](size_t bytes) {
         const size_t here = at;

@@ -8,7 +8,7 @@
 // turned round (K Q^T, V^T W^T), so that a lane holds scores, weights and outputs of one row: the weights
 // are the next product's operand as they lie, maxima and sums need two exchanges between lanes.
 //
-// The tiles of keys of all tiles of rows are one long axis, divided evenly over the workgroups: a batch of
+// The tiles of keys of all tiles of rows, and some more for what a tile of rows costs by itself, are one long axis, divided evenly over the workgroups: a batch of
 // ragged lengths fills the device to the end, and one long sequence is shared by all.  A workgroup whose share begins
 // or ends inside a tile of rows leaves its maxima, sums and outputs, which attn_join_kernel joins in a fixed order.
 #include <type_traits>
@@ -63,6 +63,7 @@ struct Tile {
     int seq, first, count, m0;  // the sequence, its first row, group times its tokens, the tile's first row of those
     int held, places;           // tokens before the call's, places that exist (both as int32: 2^30 at most)
     int tiles;                  // of keys (0: nothing to do)
+    int cost;                   // on the axis that is divided: and AttnPlan::extra
 };
 
 struct Shape {
@@ -99,7 +100,7 @@ struct Shape {
         t.m0 = in << p.rows_log;
         t.held = a.cached[t.seq];
         if (t.held < 0) {
-            t.tiles = a.zero_rest ? 1 : 0;
+            t.tiles = t.cost = a.zero_rest ? 1 : 0;
             return t;
         }
         const int room = a.pages ? a.table_pages * a.page : 0;  // (up to 2^30)
@@ -108,6 +109,7 @@ struct Shape {
         t.places = (int)min((int64_t)t.held + seen, (int64_t)room);
         t.held = min(t.held, 1 << 30);
         t.tiles = max(1, (t.places + p.keys - 1) / p.keys);
+        t.cost = t.tiles + p.extra;
         return t;
     }
 };
@@ -152,7 +154,7 @@ __device__ Share share_of(const Shape& sh, int* held, int least) {
     uint32_t upto = 0, mine = 0;
     for (int base = 0; base < n; base += 64) {
         const int at = base + lane;
-        mine = at < n ? sh.tile(at).tiles : 0;
+        mine = at < n ? sh.tile(at).cost : 0;
         if (at < ATTN_HELD) held[at] = mine;
         upto = scan(mine);
         sum += (uint32_t)__shfl(upto, 63);
@@ -168,7 +170,7 @@ __device__ Share share_of(const Shape& sh, int* held, int least) {
     for (int base = 0; base < n; base += 64) {
         if (n > 64) {
             const int at = base + lane;
-            mine = at >= n ? 0 : at < ATTN_HELD ? held[at] : sh.tile(at).tiles;
+            mine = at >= n ? 0 : at < ATTN_HELD ? held[at] : sh.tile(at).cost;
             upto = scan(mine);
         }
         const uint64_t over = __ballot((before + upto) * heads > r.from);
@@ -347,22 +349,22 @@ struct Pass {
     __device__ uint32_t key_at(int j) const { return ::key_at(a, units, t, j); }
 
     // Starts the copies of a tile whose keys are at `at` (key i's in lane i): 1 KiB a wave instruction, to consecutive
-    // bytes of LDS; the parts' positions are in the addresses.  WHOLE: every key exists.
-    template <bool WHOLE>
+    // bytes of LDS; the parts' positions are in the addresses.  The first place stands for keys that do not exist: no
+    // row sees them, and clean() takes care that their values do no harm.
     __device__ __forceinline__ void copy(int stage, uint32_t at) const {
+        if (at == kNowhere) at = 0;
         global_char* zeros = (global_char*)kZeros;
         char* to = lds + stage * kStage;
         int lane = this->lane;
-        if (kTight || !WHOLE) asm volatile("" : "+v"(lane));  // (addresses are not kept in registers across the loop)
+        if (kTight || !FULL) asm volatile("" : "+v"(lane));  // (addresses are not kept in registers across the loop)
         const int part = lane % kParts;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int n = wave * kLoads + i, r = n * (64 / kParts) + lane / kParts;
             const uint32_t from = __shfl(at, r);
             const int kp = part ^ k_swizzle(r), vp = part ^ v_swizzle(r);
-            const bool there = WHOLE || from != kNowhere;
-            global_char* ks = there && (FULL || kp * E < a.dim) ? in_cache(kbase, from, units) + kp * 16 : zeros;
-            global_char* vs = there && (FULL || vp * E < a.dim) ? in_cache(vbase, from, units) + vp * 16 : zeros;
+            global_char* ks = FULL || kp * E < a.dim ? in_cache(kbase, from, units) + kp * 16 : zeros;
+            global_char* vs = FULL || vp * E < a.dim ? in_cache(vbase, from, units) + vp * 16 : zeros;
             copy_to_lds(ks, to + n * 1024);
             copy_to_lds(vs, to + kTile + n * 1024);
         }
@@ -418,7 +420,7 @@ struct Pass {
 
     // The operands of the step's products, read kDeep - 1 ahead of them.  Keys: part 4 i + g of keys 16 h + lane % 16.
     // Values (operand t of kValues): bf16 a product's, 32 keys by 16 elements; float32 four products', four keys by 64 elements.
-    static constexpr int kDeep = kBf16 ? 4 : 3;
+    static constexpr int kDeep = kBf16 && !kTight ? 4 : 3;
     static constexpr int kKeys = 2 * kQ, kValues = kBf16 ? kOut : 2 * kOut;
     using Operand = u32x4;
     static __device__ __forceinline__ Operand read_key(const char* k, int at, int t) {
@@ -614,54 +616,69 @@ struct Pass {
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // The tiles of keys k0 .. k1 - 1, a tile ahead.  ALL: those below `full` whose keys all exist, which every row sees;
-    // else the others.  -> the first tile below `full` that some key of does not exist (ALL).
-    template <bool ALL>
-    __device__ __forceinline__ int pass(int k0, int k1, int full, int* flags) {
-        int first_bad = full;
+    // A run of tiles of keys, a tile ahead.
+    int ahead, end, stage;  // the tile whose copy is in flight or done, the first that is not wanted, where it goes
+    uint32_t next;          // places of the tile after it
+    uint64_t exist;         // its keys that exist
+    __device__ __forceinline__ void start(int k0, int k1) {
         arrived();  // (whoever used LDS before is done)
-        uint32_t next = key_at(k0 * BN + lane % BN);
-        // (ALL: a tile with absent keys is left to the other loop, so the first place does for them; there is one, as
-        // places, and so tiles below `full`, are 0 without pages)
-        copy<ALL>(0, ALL && next == kNowhere ? 0 : next);
-        uint64_t there = __ballot(next != kNowhere);
-        next = k0 + 1 < k1 ? key_at((k0 + 1) * BN + lane % BN) : kNowhere;
-        for (int k = k0; k < k1; ++k) {
-            const uint64_t now = there;
-            const int stage = (k - k0) & 1;
-            arrived();
-            if (k + 1 < k1) {
-                copy<ALL>(stage ^ 1, ALL && next == kNowhere ? 0 : next);
-                there = __ballot(next != kNowhere);
-                if (k + 2 < k1) next = key_at((k + 2) * BN + lane % BN);
-            }
-            if (ALL != (k < full && now == ~0ull)) {
-                if (ALL) first_bad = min(first_bad, k);
-                continue;
-            }
-            if (!ALL) clean(stage, k * BN, now, flags);
-#pragma unroll 1
-            for (int i = 0; i < BN / 32; ++i) {
-                const int from = k * BN + 32 * i;
-                if (last_token >= 0 && (ALL || a.mask || from <= t.held + last_token))
-                    step<ALL>(stage, 32 * i, from, (uint32_t)(now >> 32 * i));
-            }
+        ahead = k0, end = k1, stage = 0;
+        next = key_at(k0 * BN + lane % BN);
+        copy(0, next);
+        exist = __ballot(next != kNowhere);
+        if (k0 + 1 < k1) next = key_at((k0 + 1) * BN + lane % BN);
+    }
+    __device__ __forceinline__ uint64_t take() {  // tile `ahead` is in LDS -> its keys that exist; the next one is on its way
+        const uint64_t now = exist;
+        arrived();
+        ++ahead;
+        stage ^= 1;
+        if (ahead < end) {
+            copy(stage, next);
+            exist = __ballot(next != kNowhere);
+            if (ahead + 1 < end) next = key_at((ahead + 1) * BN + lane % BN);
         }
-        return first_bad;
+        return now;
+    }
+    // The products of tile k, in the stage that take() left.
+    template <bool ALL>
+    __device__ __forceinline__ void steps(int k, uint64_t now) {
+#pragma unroll 1
+        for (int i = 0; i < BN / 32; ++i) {
+            const int from = k * BN + 32 * i;
+            if (last_token >= 0 && (ALL || a.mask || from <= t.held + last_token))
+                step<ALL>(stage ^ 1, 32 * i, from, (uint32_t)(now >> 32 * i));
+        }
     }
 
-    // The tiles of keys k0 .. k1 - 1 of this tile of rows: those that need no masks first, in a loop without them.
+    // The tiles of keys k0 .. k1 - 1 of this tile of rows: first those that every row sees, in a loop without masks (but
+    // for those with absent pages: they come last).
     __device__ __forceinline__ void run(int k0, int k1, int* flags) {
+        if (t.places == 0) return;
         const int seen_by_all = min(a.mask ? t.held : t.held + t.m0 / group + 1, t.places);
         const int full = min(max(seen_by_all / BN, k0), k1);
         int rest = full;
-        if (full > k0) {
-            load_q();
-            rest = pass<true>(k0, full, full, flags);
+        start(k0, k1);
+        load_q();
+        for (int k = k0; k < full; ++k) {
+            const uint64_t now = take();
+            if (now == ~0ull)
+                steps<true>(k, now);
+            else
+                rest = min(rest, k);
         }
-        if (rest < k1) {
-            load_q();  // (again, so that what the masks need does not push it out of the first loop's registers)
-            pass<false>(rest, k1, full, flags);
+        if (full == k1 && rest == full) return;
+        load_q();  // (again, so that what the masks need does not push it out of the first loop's registers)
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+            const int from = part ? rest : full, to = part ? full : k1;
+            if (part && from < to) start(from, to);
+            for (int k = from; k < to; ++k) {
+                const uint64_t now = take();
+                if (k < full && now == ~0ull) continue;
+                clean(stage ^ 1, k * BN, now, flags);
+                steps<false>(k, now);
+            }
         }
     }
 };
@@ -704,21 +721,23 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
     const bool vec = quads<T>(a);
     while (at < share.to && place < places) {
         const Tile t = uniform(shape.tile(place));
-        const int64_t in = at - before, all = (int64_t)t.tiles * a.heads_k;
+        const int64_t in = at - before, all = (int64_t)t.cost * a.heads_k;
         if (in >= all) {
             before += all;
             ++place;
             continue;
         }
-        const int head = (int)quotient(in, t.tiles), k0 = (int)(in - (int64_t)head * t.tiles);
-        const int k1 = (int)min((int64_t)t.tiles, k0 + (share.to - at));
-        at += k1 - k0;
+        const int head = (int)quotient(in, t.cost), c0 = (int)(in - (int64_t)head * t.cost);
+        const int c1 = (int)min((int64_t)t.cost, c0 + (share.to - at));
+        at += c1 - c0;
+        const int k0 = max(c0 - (t.cost - t.tiles), 0), k1 = c1 - (t.cost - t.tiles);
+        if (k0 >= k1) continue;
         pass.begin(t, head);
         if (t.held >= 0) pass.run(k0, k1, flags);
         asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");  // the last products' results, whatever way the loop was left
         if (k0 == 0 && k1 < t.tiles)
             left = AttnDesc{1, t.first, t.m0, t.count, head,
-                            (int)quotient((at - k1 + t.tiles) * share.workers - 1, share.total)};
+                            (int)quotient((at - c1 + t.cost) * share.workers - 1, share.total)};
         const int n = threadIdx.x & 15, slot = 2 * blockIdx.x + (k0 == 0);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -1082,18 +1101,20 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
     const int places = shape.places();
     while (at < share.to && place < places) {
         const Tile t = uniform(shape.tile(place));
-        const int64_t in = at - before, all = (int64_t)t.tiles * a.heads_k;
+        const int64_t in = at - before, all = (int64_t)t.cost * a.heads_k;
         if (in >= all) {
             before += all;
             ++place;
             continue;
         }
-        const int head = (int)quotient(in, t.tiles), k0 = (int)(in - (int64_t)head * t.tiles);
-        const int k1 = (int)min((int64_t)t.tiles, k0 + (share.to - at));
-        at += k1 - k0;
+        const int head = (int)quotient(in, t.cost), c0 = (int)(in - (int64_t)head * t.cost);
+        const int c1 = (int)min((int64_t)t.cost, c0 + (share.to - at));
+        at += c1 - c0;
+        const int k0 = max(c0 - (t.cost - t.tiles), 0), k1 = c1 - (t.cost - t.tiles);
+        if (k0 >= k1) continue;
         if (k0 == 0 && k1 < t.tiles)
             left = AttnDesc{1, t.first, t.m0, t.count, head,
-                            (int)quotient((at - k1 + t.tiles) * share.workers - 1, share.total)};
+                            (int)quotient((at - c1 + t.cost) * share.workers - 1, share.total)};
         // q to LDS, a part a thread at a time
         const int rows = min(16, t.count - t.m0);
         few.t = t;
