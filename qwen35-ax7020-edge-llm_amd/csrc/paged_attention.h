@@ -6,6 +6,7 @@
 
 #include "kv_cache.h"
 
+constexpr int ATTN_MOST = 1024;  // workgroups of a call, at most
 constexpr int ATTN_HELD = 1024;  // places whose tiles of keys a workgroup remembers
 
 // How a call is laid out: from its sizes alone.  A tile of rows is `rows` rows of one sequence on one key
@@ -22,7 +23,10 @@ struct AttnPlan {
     int grid;     // workgroups
     int extra;    // tiles of keys that a tile of rows counts for besides its own
     int least;    // tiles of a workgroup's share
+    int rows_most;    // of a sequence and key head, as far as the host knows
+    int shared;   // tiles of rows and key heads, at most, if they are few and each in many parts; else 0
     size_t desc_at;   // AttnDesc [grid]
+    size_t flag_at;   // int [grid]: there is one
     size_t stat_at;   // float2 [2 grid][rows]: a part's maximum and sum
     size_t part_at;   // float [2 grid][rows][dim]
     size_t total;
@@ -53,6 +57,10 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     // tokens with 0 | 2 | 4 | 8 tiles of 64 keys 1,764 | 1,468 | 1,245 | 1,160 us; 8,192 of 16 heads of 128 589 | 435 |
     // 372 | 381; float32 prompts with 0 | 1 | 2 | 4 tiles of 32 107 | 98 | 98 | 105.
     p.extra = p.few ? 1 : bf16 ? std::max(256, 2 * p.dim) / p.keys : 2;
+    p.rows_most = a.starts || !a.n_seq ? p.rows : a.rows / a.n_seq * p.group;
+    // Where there are about eight parts or more of each, 16 wavefronts join them (4 | 16: one sequence of 4,096 tokens xxx).
+    const size_t units = (a.starts ? (size_t)a.rows * p.group / p.rows + a.n_seq : (size_t)a.n_seq * p.each) * a.heads_k;
+    p.shared = units * 8 <= (size_t)p.grid ? (int)units : 0;
     size_t at = 0;
     auto put = [&](size_t bytes) {
         const size_t here = at;
@@ -60,6 +68,7 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
         return here;
     };
     p.desc_at = put((size_t)p.grid * 32);
+    p.flag_at = put((size_t)p.grid * 4);
     p.stat_at = put((size_t)2 * p.grid * p.rows * 8);
     p.part_at = put((size_t)2 * p.grid * p.rows * p.dim * 4);
     p.total = at;

@@ -42,7 +42,7 @@ __device__ const uint4 kZeros[64] = {};  // (attn_step_kernel: a whole key's or 
 // Whoever reads waits for itself: Pass::arrived.)
 __device__ __forceinline__ void copy_to_lds(global_char* from, char* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
 }
 
 // A tile of rows that this workgroup's share ends in, and begins (AttnPlan::desc_at).
@@ -764,84 +764,139 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
             }
         }
     }
-    if (threadIdx.x == 0) *desc = left;
+    if (threadIdx.x == 0) {
+        *desc = left;
+        reinterpret_cast<int*>(static_cast<char*>(a.work) + p.flag_at)[blockIdx.x] = left.there;
+    }
 }
 
-// The parts of a tile of rows, 16 rows and 64 elements to a workgroup: its first part is the last of workgroup
-// blockIdx.x, the others are the first of those that follow.  Four wavefronts take every fourth.
+// The workgroup whose share ends in the tile of rows that a workgroup joins: workgroup blockIdx.x; or (p.shared: few
+// tiles, and only so many workgroups) the blockIdx.x-th that left one, by their flags.  -1: none.
+template <int THREADS>
+__device__ __forceinline__ int first_of(const attn_dev_args& a, const AttnPlan& p) {
+    const int* flags = reinterpret_cast<const int*>(static_cast<const char*>(a.work) + p.flag_at);
+    if (!p.shared) return flags[blockIdx.x] ? (int)blockIdx.x : -1;
+    constexpr int kRounds = (ATTN_MOST + THREADS - 1) / THREADS, kWaves = THREADS / 64;
+    __shared__ uint64_t sets[kRounds * kWaves];
+    bool there[kRounds];
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        const int at = i * THREADS + threadIdx.x;
+        there[i] = at < p.grid && flags[at];
+    }
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        const uint64_t set = __ballot(there[i]);
+        if (threadIdx.x % 64 == 0) sets[i * kWaves + threadIdx.x / 64] = set;
+    }
+    __syncthreads();
+    // (a wavefront's lane has a set of 64 flags)
+    const int lane = threadIdx.x & 63;
+    uint64_t set = lane < kRounds * kWaves ? sets[lane] : 0;
+    static_assert(kRounds * kWaves <= 64, "a lane for each set");
+    int upto = __popcll(set);
+    const int mine = upto;
+#pragma unroll
+    for (int i = 1; i < kRounds * kWaves; i *= 2) {
+        const int x = __shfl_up(upto, i);
+        if (lane >= i) upto += x;
+    }
+    const uint64_t over = __ballot(upto > (int)blockIdx.x);
+    if (!over) return -1;
+    const int l = __builtin_ctzll(over);
+    int left = (int)blockIdx.x - (upto - mine);
+    while (left-- > 0 && lane == l) set &= set - 1;
+    return l * 64 + __shfl(lane == l ? __builtin_ctzll(set | 1ull << 63) : 0, l);
+}
+
+// The parts of a tile of rows, 16 rows to a workgroup: its first part is the last of workgroup first_of(), the others are
+// the first of those that follow.  A wavefront has 64 elements of the rows and every G-th part, kAtOnce of them in
+// flight; Z wavefronts side by side, D / 64 / Z workgroups.
 constexpr int kAtOnce = 4;
-template <class T, int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(attn_dev_args a, AttnPlan p) {
-    const AttnDesc d = reinterpret_cast<const AttnDesc*>(static_cast<const char*>(a.work) + p.desc_at)[blockIdx.x];
+template <class T, int D, int G, int Z>
+__global__ __launch_bounds__(64 * Z * G) void attn_join_kernel(attn_dev_args a, AttnPlan p) {
+    const int first = first_of<64 * Z * G>(a, p);
+    if (first < 0) return;
+    const AttnDesc d = reinterpret_cast<const AttnDesc*>(static_cast<const char*>(a.work) + p.desc_at)[first];
     const int block = blockIdx.y, m0 = d.m0 + 16 * block;
-    if (!d.there || m0 >= d.count) return;
+    if (m0 >= d.count) return;
     constexpr int kOut = D / 16;
     const float2* stats = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.stat_at);
     const f32x4* parts = reinterpret_cast<const f32x4*>(static_cast<const char*>(a.work) + p.part_at);
-    __shared__ f32x4 sums[4][4][64];
-    __shared__ float2 tops[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, first = blockIdx.x;
-    const bool mine = m0 + n < d.count;
+    __shared__ f32x4 sums[G > 1 ? G - 1 : 1][Z][4][64];
+    __shared__ float2 tops[G][Z][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15;
+    const int at_z = wave % Z, z = Z * blockIdx.z + at_z, group = wave / Z;
     f32x4 o[4] = {};
     float m = kNone, l = 0;
-    if (mine)
-        for (int w0 = first + wave; w0 <= d.last; w0 += 4 * kAtOnce) {
+    if (m0 + n < d.count)
+        for (int w0 = first + group; w0 <= d.last; w0 += G * kAtOnce) {
             // (a part past the last: the last again, with no weight)
             float2 s[kAtOnce];
             f32x4 x[kAtOnce][4];
             float now = m;
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
-                const int w = min(w0 + 4 * j, d.last), slot = w == first ? 2 * first + 1 : 2 * w;
+                const int w = min(w0 + G * j, d.last), slot = w == first ? 2 * first + 1 : 2 * w;
                 s[j] = stats[(int64_t)slot * p.rows + 16 * block + n];
-                const f32x4* from = parts + (((int64_t)slot * (p.rows / 16) + block) * kOut + 4 * blockIdx.z) * 64 + lane;
+                const f32x4* from = parts + (((int64_t)slot * (p.rows / 16) + block) * kOut + 4 * z) * 64 + lane;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[j][i] = from[i * 64];
             }
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j)
-                if (w0 + 4 * j <= d.last) now = fmaxf(now, s[j].x);
-            if (now == kNone) continue;
-            const float f = exp2_raw(m - now);
+                if (w0 + G * j <= d.last) now = fmaxf(now, s[j].x);
+            const float f = m == kNone ? 1.0f : exp2_raw(m - now);
             m = now;
             l *= f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] *= f;
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
-                if (w0 + 4 * j > d.last) break;
-                const float e = exp2_raw(s[j].x - now);
+                if (w0 + G * j > d.last) break;
+                const float e = s[j].x == kNone ? 1.0f : exp2_raw(s[j].x - now);  // (values that are not finite alone)
                 l += s[j].y * e;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[i] += x[j][i] * e;
             }
         }
-    tops[wave][lane] = float2{m, l};
+    if constexpr (G > 1) {
+        tops[group][at_z][lane] = float2{m, l};
+        if (group)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][i][lane] = o[i];
-    __syncthreads();
-    if (!mine) return;
-    // each wavefront a quarter: its own four outputs of the lane's row
-    float top = kNone;
+            for (int i = 0; i < 4; ++i) sums[group - 1][at_z][i][lane] = o[i];
+        __syncthreads();
+        if (group) return;
+        float top = kNone;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w][lane].x);
-    float sum = 0, x[4] = {0, 0, 0, 0};
+        for (int g = 0; g < G; ++g) top = fmaxf(top, tops[g][at_z][lane].x);
+        const float f = m == kNone ? 1.0f : exp2_raw(m - top);
+        l *= f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float2 s = tops[w][lane];
-        const float f = s.x == kNone ? 0.0f : exp2_raw(s.x - top);
-        sum += s.y * f;
+        for (int i = 0; i < 4; ++i) o[i] *= f;
+#pragma unroll 3
+        for (int g = 1; g < G; ++g) {
+            const float2 s = tops[g][at_z][lane];
+            const float e = s.x == kNone ? 1.0f : exp2_raw(s.x - top);
+            l += s.y * e;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += (sizeof(T) == 2 ? sums[w][wave][lane][e] : sums[w][e][lane][wave]) * f;
+            for (int i = 0; i < 4; ++i) o[i] += sums[g - 1][at_z][i][lane] * e;
+        }
     }
-    const float f = 1.0f / sum;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = sum == 0 ? 0.0f : x[e] * f;
-    const int g = lane >> 4, at = 64 * blockIdx.z + (sizeof(T) == 2 ? 16 * wave + 4 * g : 16 * g + 4 * wave);
-    const int r = m0 + n;
+    const int r = m0 + n, g = lane >> 4;
+    if (r >= d.count) return;
+    const float f = 1.0f / l;
     T* to = static_cast<T*>(a.out) + (int64_t)(d.first + r / p.group) * a.out_row +
             (int64_t)(d.head * p.group + r % p.group) * a.out_head;
-    if (at < a.dim) store4(to + at, x, quads<T>(a));
+    const bool vec = quads<T>(a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // (Pass::quad_at)
+        const int at = 64 * z + (sizeof(T) == 2 ? 16 * i + 4 * g : 16 * g + 4 * i);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = l == 0 ? 0.0f : (sizeof(T) == 2 ? o[i][e] : o[e][i]) * f;
+        if (at < a.dim) store4(to + at, x, vec);
+    }
 }
 
 // ---- few rows ----------------------------------------------------------------------------
@@ -1196,44 +1251,47 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
         }
         __syncthreads();
     }
-    if (threadIdx.x == 0) *desc = left;
+    if (threadIdx.x == 0) {
+        *desc = left;
+        reinterpret_cast<int*>(static_cast<char*>(a.work) + p.flag_at)[blockIdx.x] = left.there;
+    }
 }
 
-// The parts of a row, a row to a workgroup: D / 4 lanes a part, kJoin parts at a time, two of them of each lane.
-constexpr int kJoin = 16;
-template <class T, int D>
-__global__ __launch_bounds__(kJoin * (D / 4)) void attn_step_join_kernel(attn_dev_args a, AttnPlan p) {
-    const AttnDesc d = reinterpret_cast<const AttnDesc*>(static_cast<const char*>(a.work) + p.desc_at)[blockIdx.x];
+// The parts of a row, a row to a workgroup: D / 4 lanes have every G-th part, kAtOnce of them in flight.
+template <class T, int D, int G>
+__global__ __launch_bounds__(G * (D / 4)) void attn_step_join_kernel(attn_dev_args a, AttnPlan p) {
+    const int first = first_of<G * (D / 4)>(a, p);
+    if (first < 0) return;
+    const AttnDesc d = reinterpret_cast<const AttnDesc*>(static_cast<const char*>(a.work) + p.desc_at)[first];
     const int r = blockIdx.y;
-    if (!d.there || d.m0 + r >= d.count) return;
+    if (d.m0 + r >= d.count) return;
     const float2* stats = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.stat_at);
     const float* parts = reinterpret_cast<const float*>(static_cast<const char*>(a.work) + p.part_at);
-    __shared__ f32x4 sums[kJoin][D / 4];
-    __shared__ float2 tops[kJoin];
-    const int lane = threadIdx.x % (D / 4), group = threadIdx.x / (D / 4), first = blockIdx.x;
+    __shared__ f32x4 sums[G][D / 4];
+    __shared__ float2 tops[G];
+    const int lane = threadIdx.x % (D / 4), group = threadIdx.x / (D / 4);
     f32x4 o = {0, 0, 0, 0};
     float m = kNone, l = 0;
-    constexpr int kEach = 4;
-    for (int w0 = first + group; w0 <= d.last; w0 += kJoin * kEach) {
-        float2 s[kEach];
-        f32x4 x[kEach];
+    for (int w0 = first + group; w0 <= d.last; w0 += G * kAtOnce) {
+        float2 s[kAtOnce];
+        f32x4 x[kAtOnce];
         float now = m;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {  // (past the last: the last again, with no weight)
-            const int w = min(w0 + kJoin * j, d.last), slot = w == first ? 2 * first + 1 : 2 * w;
+        for (int j = 0; j < kAtOnce; ++j) {  // (past the last: the last again, with no weight)
+            const int w = min(w0 + G * j, d.last), slot = w == first ? 2 * first + 1 : 2 * w;
             s[j] = stats[slot * 16 + r];
             x[j] = *reinterpret_cast<const f32x4*>(parts + ((int64_t)slot * 16 + r) * D + 4 * lane);
         }
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
-            if (w0 + kJoin * j <= d.last) now = fmaxf(now, s[j].x);
+        for (int j = 0; j < kAtOnce; ++j)
+            if (w0 + G * j <= d.last) now = fmaxf(now, s[j].x);
         const float f = m == kNone ? 1.0f : exp2_raw(m - now);
         m = now;
         l *= f;
         o *= f;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            if (w0 + kJoin * j > d.last) break;
+        for (int j = 0; j < kAtOnce; ++j) {
+            if (w0 + G * j > d.last) break;
             const float e = s[j].x == kNone ? 1.0f : exp2_raw(s[j].x - now);  // (values that are not finite alone)
             l += s[j].y * e;
             o += x[j] * e;
@@ -1245,10 +1303,10 @@ __global__ __launch_bounds__(kJoin * (D / 4)) void attn_step_join_kernel(attn_de
     if (group) return;
     float top = kNone, all = 0;
 #pragma unroll
-    for (int w = 0; w < kJoin; ++w) top = fmaxf(top, tops[w].x);
+    for (int w = 0; w < G; ++w) top = fmaxf(top, tops[w].x);
     f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < kJoin; ++w) {
+    for (int w = 0; w < G; ++w) {
         const float e = tops[w].x == kNone ? 1.0f : exp2_raw(tops[w].x - top);
         all += tops[w].y * e;
         x += sums[w][lane] * e;
@@ -1267,7 +1325,11 @@ hipError_t launch_step(const attn_dev_args& a, const AttnPlan& p, hipStream_t s)
         attn_step_kernel<T, D, true><<<dim3((unsigned)p.grid), 256, 0, s>>>(a, p, units);
     else
         attn_step_kernel<T, D, false><<<dim3((unsigned)p.grid), 256, 0, s>>>(a, p, units);
-    attn_step_join_kernel<T, D><<<dim3((unsigned)p.grid, 16), kJoin * (D / 4), 0, s>>>(a, p);
+    const dim3 grid((unsigned)(p.shared ? p.shared : p.grid), (unsigned)std::min(16, p.rows_most));
+    if (p.shared)
+        attn_step_join_kernel<T, D, 16><<<grid, 4 * D, 0, s>>>(a, p);
+    else
+        attn_step_join_kernel<T, D, 4><<<grid, D, 0, s>>>(a, p);
     return hipGetLastError();
 }
 
@@ -1278,7 +1340,11 @@ hipError_t launch(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
         attn_kernel<T, D, RB, W, BN, true><<<dim3((unsigned)p.grid), 64 * W, 0, s>>>(a, p, units);
     else
         attn_kernel<T, D, RB, W, BN, false><<<dim3((unsigned)p.grid), 64 * W, 0, s>>>(a, p, units);
-    attn_join_kernel<T, D><<<dim3((unsigned)p.grid, (unsigned)(p.rows / 16), D / 64), 256, 0, s>>>(a, p);
+    const unsigned blocks = (std::min(p.rows, p.rows_most) + 15) / 16;
+    if (p.shared)
+        attn_join_kernel<T, D, 16, 1><<<dim3(p.shared, blocks, D / 64), 1024, 0, s>>>(a, p);
+    else
+        attn_join_kernel<T, D, 1, D / 64><<<dim3(p.grid, blocks), D, 0, s>>>(a, p);
     return hipGetLastError();
 }
 
