@@ -7,7 +7,7 @@
 
 #include "qwen_kernels.h"
 
-// n / d for 0 <= n < 2^31 by one product (d 1 to 65536): with l = ceil(log2 d) and
+// n / d for 0 <= n < 2^31 by one product (d 1 to 2^31): with l = ceil(log2 d) and
 // m = floor(2^(31 + l) / d) + 1, n m / 2^(31 + l) is off by less than 2^-l <= 1 / d from above.
 struct Divisor {
     uint32_t m;
@@ -33,20 +33,6 @@ __device__ __forceinline__ Span span_of(const int32_t* starts, int rows, int n_s
     }
     const int lo = min(max(starts[s], 0), rows), hi = min(max(starts[s + 1], lo), rows);
     return {lo, hi - lo};
-}
-// The sequence that holds row r, or -1.
-__device__ __forceinline__ int owner_of(const int32_t* starts, int rows, int n_seq, int r) {
-    if (!starts) return r / (rows / n_seq);
-    int lo = 0, hi = n_seq;  // starts[lo] <= r < starts[hi], as far as it is known
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (starts[mid] <= r)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const Span p = span_of(starts, rows, n_seq, lo);
-    return r >= p.first && r < p.first + p.count ? lo : -1;
 }
 #endif
 

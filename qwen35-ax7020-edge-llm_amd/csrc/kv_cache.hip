@@ -7,6 +7,9 @@
 // A workgroup has a few rows: their angles go to LDS once for all heads, then every thread
 // takes 16-byte pieces of the rows' heads.  What bounds it: few rows, the latency of a launch and
 // of the loads that depend on one another (sequence, length, page); many, memory.
+#include <algorithm>
+#include <type_traits>
+
 #include "bf16_terms.h"
 #include "kv_cache.h"
 
@@ -40,8 +43,8 @@ struct Head {
     using V = Piece<T, N>;
     using V2 = Piece<T, VEC && INTER ? N : 2 * P>;
 
-    static __device__ int turned(int rot) { return rot / 2 / P; }
-    static __device__ int passed(int dim, int rot) { return (dim - rot) / N; }
+    static __host__ __device__ int turned(int rot) { return rot / 2 / P; }
+    static __host__ __device__ int passed(int dim, int rot) { return (dim - rot) / N; }
 
     static __device__ __forceinline__ void turn(const T* x, T* y, int u, int rot, const float2* cs) {
         float a[P], b[P];
@@ -103,17 +106,18 @@ struct Head {
 
 // ---- rotation alone -------------------------------------------------------------------
 template <class T, bool VEC, bool INTER>
-__global__ __launch_bounds__(kThreads) void rope_kernel(rope_dev_args a, int each, int back, int copy) {
+__global__ __launch_bounds__(kThreads) void rope_kernel(rope_dev_args a, int each, int back, int units, Divisor by_units,
+                                                        Divisor by_heads) {
     using H = Head<T, VEC, INTER>;
     __shared__ float2 cs[kMaxRows * kMaxPairs];
-    const int half = a.rot / 2, turned = H::turned(a.rot), units = turned + (copy ? H::passed(a.dim, a.rot) : 0);
+    const int half = a.rot / 2, turned = H::turned(a.rot);
     for (int64_t r0 = (int64_t)blockIdx.x * each; r0 < a.rows; r0 += (int64_t)gridDim.x * each) {
         const int n = (int)min((int64_t)each, a.rows - r0);
         for (int i = threadIdx.x; i < n * half; i += kThreads)
             cs[i] = angle_of(a.positions[r0 + i / half], a.freqs[i % half], a.amplitude, back);
         __syncthreads();
         for (int i = threadIdx.x; i < n * a.heads * units; i += kThreads) {
-            const int head = i / units, u = i - head * units, r = head / a.heads, h = head - r * a.heads;
+            const int head = divide(i, by_units), u = i - head * units, r = divide(head, by_heads), h = head - r * a.heads;
             const T* x = static_cast<const T*>(a.x) + (r0 + r) * a.x_row + h * a.x_head;
             T* y = static_cast<T*>(a.out) + (r0 + r) * a.out_row + h * a.out_head;
             if (u < turned)
@@ -133,21 +137,40 @@ struct Place {
     int64_t at;
 };
 
+// How a row's 16-byte pieces (or elements) follow one another: the keys' heads, the values', the queries'.
+struct Units {
+    int k, v, q;              // of a head
+    int ks, vs, all;          // of the keys' heads, the values', all
+    Divisor by_k, by_v, by_q, by_all;
+};
+
+// The sequence that holds row r, or -1, by a wavefront: 64 of the starts at a time (a binary search would wait for
+// five loads one after the other for 24 sequences).
+__device__ __forceinline__ int owner_by_wave(const int32_t* starts, int rows, int n_seq, int r) {
+    if (!starts) return r / (rows / n_seq);
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = n_seq;  // starts[lo] <= r < starts[lo + n], as far as it is known
+    while (n > 1) {
+        const int step = (n + 63) / 64, at = lo + lane * step;
+        const uint64_t upto = __ballot(lane * step < n && (lane == 0 || starts[at] <= r));
+        lo += (63 - __builtin_clzll(upto)) * step;
+        n = min(step, n_seq - lo);
+    }
+    const Span p = span_of(starts, rows, n_seq, lo);
+    return r >= p.first && r < p.first + p.count ? lo : -1;
+}
+
 template <class T, bool VEC, bool INTER>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args a, Divisor page, int each, int copy_q,
-                                                             int copy_v) {
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args a, Divisor page, int each, Units n, int copy_v) {
     using H = Head<T, VEC, INTER>;
     using C = Head<T, true, false>;  // values are copied 16 bytes at a time where they are aligned
-    __shared__ float2 cs[kMaxRows * kMaxPairs / 2];
+    __shared__ float2 cs[kMaxRows * kMaxPairs / 4];
     __shared__ Place places[kMaxRows];
-    const int half = a.rot / 2, turned = H::turned(a.rot);
-    const int k_units = turned + H::passed(a.dim, a.rot), q_units = turned + (copy_q ? H::passed(a.dim, a.rot) : 0);
-    const int v_units = copy_v ? C::passed(a.dim, 0) : a.dim;
-    const int ks = a.heads_k * k_units, vs = a.heads_k * v_units, qs = a.q ? a.heads_q * q_units : 0;
+    const int half = a.rot / 2, turned = H::turned(a.rot), wave = threadIdx.x >> 6;
     for (int64_t r0 = (int64_t)blockIdx.x * each; r0 < a.rows; r0 += (int64_t)gridDim.x * each) {
-        const int n = (int)min((int64_t)each, a.rows - r0);
-        if ((int)threadIdx.x < n) {
-            const int r = (int)r0 + threadIdx.x, s = owner_of(a.starts, a.rows, a.n_seq, r);
+        const int rows = (int)min((int64_t)each, a.rows - r0);
+        if (wave < rows) {
+            const int r = (int)r0 + wave, s = owner_by_wave(a.starts, a.rows, a.n_seq, r);
             Place p{0, 0, -1};
             if (s >= 0) {
                 const int held = a.cached[s];
@@ -163,51 +186,52 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args 
                     }
                 }
             }
-            places[threadIdx.x] = p;
+            places[wave] = p;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < n * half; i += kThreads)
-            cs[i] = angle_of(places[i / half].position, a.freqs[i % half], a.amplitude, false);
-        if (half) __syncthreads();
-        for (int i = threadIdx.x; i < n * (ks + vs + qs); i += kThreads) {
-            const int r = i / (ks + vs + qs);
-            int u = i - r * (ks + vs + qs);
+        if (half) {
+            for (int i = threadIdx.x; i < rows * half; i += kThreads)
+                cs[i] = angle_of(places[i / half].position, a.freqs[i % half], a.amplitude, false);
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < rows * n.all; i += kThreads) {
+            const int r = divide(i, n.by_all);
+            int u = i - r * n.all;
             const Place p = places[r];
             const int64_t row = r0 + r;
             const float2* t = cs + r * half;
-            if (u < ks) {
+            const T* x;
+            T* y;
+            if (u < n.ks) {
                 if (p.at < 0) continue;
-                const int h = u / k_units;
-                u -= h * k_units;
-                const T* x = static_cast<const T*>(a.k) + row * a.k_row + h * a.k_head;
-                T* y = static_cast<T*>(a.key_cache) + p.at + h * a.cache_head;
-                if (u < turned)
-                    H::turn(x, y, u, a.rot, t);
-                else
-                    H::pass(x, y, u - turned, a.rot);
-            } else if (u < ks + vs) {
+                const int h = divide(u, n.by_k);
+                u -= h * n.k;
+                x = static_cast<const T*>(a.k) + row * a.k_row + h * a.k_head;
+                y = static_cast<T*>(a.key_cache) + p.at + h * a.cache_head;
+            } else if (u < n.ks + n.vs) {
                 if (p.at < 0) continue;
-                u -= ks;
-                const int h = u / v_units;
-                u -= h * v_units;
-                const T* x = static_cast<const T*>(a.v) + row * a.v_row + h * a.v_head;
-                T* y = static_cast<T*>(a.value_cache) + p.at + h * a.cache_head;
+                u -= n.ks;
+                const int h = divide(u, n.by_v);
+                u -= h * n.v;
+                x = static_cast<const T*>(a.v) + row * a.v_row + h * a.v_head;
+                y = static_cast<T*>(a.value_cache) + p.at + h * a.cache_head;
                 if (copy_v)
                     C::pass(x, y, u, 0);
                 else
                     y[u] = x[u];
+                continue;
             } else {
                 if (!p.there) continue;
-                u -= ks + vs;
-                const int h = u / q_units;
-                u -= h * q_units;
-                const T* x = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
-                T* y = static_cast<T*>(a.q_out) + row * a.q_out_row + h * a.q_out_head;
-                if (u < turned)
-                    H::turn(x, y, u, a.rot, t);
-                else
-                    H::pass(x, y, u - turned, a.rot);
+                u -= n.ks + n.vs;
+                const int h = divide(u, n.by_q);
+                u -= h * n.q;
+                x = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+                y = static_cast<T*>(a.q_out) + row * a.q_out_row + h * a.q_out_head;
             }
+            if (u < turned)
+                H::turn(x, y, u, a.rot, t);
+            else
+                H::pass(x, y, u - turned, a.rot);
         }
         __syncthreads();
     }
@@ -256,27 +280,55 @@ bool pieces(int dim, int rot, bool inter, size_t es) {
     return rot % (inter ? n : 2 * n) == 0 && dim % n == 0;
 }
 
+template <class T, bool VEC, bool INTER>
+void launch_rope(const rope_dev_args& a, bool back, hipStream_t s) {
+    using H = Head<T, VEC, INTER>;
+    const int each = a.rows < 2048 ? 1 : kMaxRows, grid = std::min((a.rows + each - 1) / each, 1 << 20);
+    const int units = H::turned(a.rot) + (a.out != a.x ? H::passed(a.dim, a.rot) : 0);
+    rope_kernel<T, VEC, INTER>
+        <<<dim3((unsigned)grid), kThreads, 0, s>>>(a, each, back, units, divisor(units), divisor(a.heads));
+}
+
+template <class T, bool VEC, bool INTER>
+void launch_append(const kv_dev_append_args& a, hipStream_t s) {
+    using H = Head<T, VEC, INTER>;
+    const int each = a.rows < 2048 ? 1 : kMaxRows, grid = std::min((a.rows + each - 1) / each, 1 << 20);
+    const int copy_v = whole(a.v, a.v_row, a.v_head, sizeof(T));
+    Units n{};
+    n.k = H::turned(a.rot) + H::passed(a.dim, a.rot);
+    n.v = copy_v ? a.dim * (int)sizeof(T) / 16 : a.dim;
+    n.q = H::turned(a.rot) + (a.q_out != a.q ? H::passed(a.dim, a.rot) : 0);
+    n.ks = a.heads_k * n.k;
+    n.vs = a.heads_k * n.v;
+    n.all = n.ks + n.vs + (a.q ? a.heads_q * n.q : 0);
+    n.by_k = divisor(n.k);
+    n.by_v = divisor(n.v);
+    n.by_q = divisor(std::max(n.q, 1));
+    n.by_all = divisor(n.all);
+    kv_append_kernel<T, VEC, INTER><<<dim3((unsigned)grid), kThreads, 0, s>>>(a, divisor(a.page), each, n, copy_v);
+}
+
+// f(T{}, VEC, INTER) for a call's type, alignment and layout
+template <class F>
+void choose(int dtype, bool vec, bool inter, F&& f) {
+    using Yes = std::true_type;
+    using No = std::false_type;
+    auto of = [&](auto t) { vec ? (inter ? f(t, Yes{}, Yes{}) : f(t, Yes{}, No{})) : (inter ? f(t, No{}, Yes{}) : f(t, No{}, No{})); };
+    if (dtype == QWEN_BF16)
+        of(uint16_t{});
+    else
+        of(float{});
+}
+
 }  // namespace
 
 hipError_t rope_launch(const rope_dev_args& a, bool back, hipStream_t s) {
     const size_t es = a.dtype == QWEN_BF16 ? 2 : 4;
     const bool vec = pieces(a.dim, a.rot, a.interleaved, es) && whole(a.x, a.x_row, a.x_head, es) &&
                      whole(a.out, a.out_row, a.out_head, es);
-    const int copy = a.out != a.x, each = a.rows < 2048 ? 1 : kMaxRows;
-    const dim3 grid((unsigned)std::min((a.rows + each - 1) / each, 1 << 20));
-#define GO(T, V, I) rope_kernel<T, V, I><<<grid, kThreads, 0, s>>>(a, each, back, copy)
-    if (a.dtype == QWEN_BF16) {
-        if (a.interleaved)
-            vec ? GO(uint16_t, true, true) : GO(uint16_t, false, true);
-        else
-            vec ? GO(uint16_t, true, false) : GO(uint16_t, false, false);
-    } else {
-        if (a.interleaved)
-            vec ? GO(float, true, true) : GO(float, false, true);
-        else
-            vec ? GO(float, true, false) : GO(float, false, false);
-    }
-#undef GO
+    choose(a.dtype, vec, a.interleaved, [&](auto t, auto v, auto i) {
+        launch_rope<decltype(t), decltype(v)::value, decltype(i)::value>(a, back, s);
+    });
     return hipGetLastError();
 }
 
@@ -284,23 +336,9 @@ hipError_t kv_launch_append(const kv_dev_append_args& a, hipStream_t s) {
     const size_t es = a.dtype == QWEN_BF16 ? 2 : 4;
     const bool vec = pieces(a.dim, a.rot, a.interleaved, es) && whole(a.k, a.k_row, a.k_head, es) &&
                      (!a.q || (whole(a.q, a.q_row, a.q_head, es) && whole(a.q_out, a.q_out_row, a.q_out_head, es)));
-    const int copy_q = a.q && a.q_out != a.q, copy_v = whole(a.v, a.v_row, a.v_head, es);
-    const int each = a.rows < 2048 ? 1 : kMaxRows;
-    const dim3 grid((unsigned)std::min((a.rows + each - 1) / each, 1 << 20));
-    const Divisor page = divisor(a.page);
-#define GO(T, V, I) kv_append_kernel<T, V, I><<<grid, kThreads, 0, s>>>(a, page, each, copy_q, copy_v)
-    if (a.dtype == QWEN_BF16) {
-        if (a.interleaved)
-            vec ? GO(uint16_t, true, true) : GO(uint16_t, false, true);
-        else
-            vec ? GO(uint16_t, true, false) : GO(uint16_t, false, false);
-    } else {
-        if (a.interleaved)
-            vec ? GO(float, true, true) : GO(float, false, true);
-        else
-            vec ? GO(float, true, false) : GO(float, false, false);
-    }
-#undef GO
+    choose(a.dtype, vec, a.interleaved, [&](auto t, auto v, auto i) {
+        launch_append<decltype(t), decltype(v)::value, decltype(i)::value>(a, s);
+    });
     return hipGetLastError();
 }
 

@@ -448,7 +448,8 @@ def _torch():
 
 
 def _stream():
-    return _torch().cuda.current_stream().cuda_stream
+    torch = _torch()  # (its current_stream() makes an object: 2.6 us of a call's 10)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _dp(t) -> int:
