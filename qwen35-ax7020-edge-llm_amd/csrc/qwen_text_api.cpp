@@ -217,7 +217,7 @@ const char* paged_sizes(const attn_dev_args* a) {
 }
 const char* paged_bad(const attn_dev_args* a) {
     if (const char* why = cache_pointers(a)) return why;
-    if (!std::isfinite(a->scale) || a->scale <= 0) return "scale is finite and above 0";
+    if (!std::isnormal(a->scale) || a->scale < 0 || a->scale > 1e38f) return "scale is a normal number of up to 1e38, above 0";
     if (a->mask && (!in(a->mask_words, 0, 1 << 16) || !aligned(a->mask, 4)))
         return "mask_words are 0 to 2^16, mask 4-byte aligned";
     if (a->n_seq == 0 || a->rows == 0) return nullptr;

@@ -225,6 +225,14 @@ def test_absent_places(gpu, dtype):
     none = tables[:, :0]
     assert bool((gpu.paged_attention(q, K, V, none, cached, starts) == 0).all())
     assert bool((gpu.paged_attention(q, K[:0], V[:0], short, cached, starts) == 0).all())
+    # few rows on a key head
+    few, fstarts = case([4, 1, 2, 3], [100, -1, 40, 700], 4, 2, 64, 16, dtype)
+    few[3][0, 1] = -1
+    few[3][0, 4] = 2 ** 31 - 1
+    few[3][2] = -7
+    few[3][3, 5:40:7] = few[1].shape[0]
+    check(gpu, few, fstarts, dtype)
+    assert bool((gpu.paged_attention(few[0], K[:0], V[:0], *few[3:], fstarts) == 0).all())
     # rows in front of and behind the sequences, and of skipped ones, stay as they were
     q2 = torch.cat((q, q, q))
     out = torch.full_like(q2, 5.0)
@@ -260,7 +268,7 @@ def test_masks(gpu, hq, hk, dim, page, dtype):
 def test_values_that_are_not_finite(gpu, dim, dtype):
     """A NaN or infinity in a value shows in the rows that see it, in its element, and in no other; in a
     key in all elements of them; what no row sees nowhere.  Causal and with a mask; first in a tile and inside."""
-    for new, cached, masked in (([40, 3], [0, 70], False), ([100], [29], False), ([40, 20], [3, 40], True)):
+    for new, cached, masked in (([40, 3], [0, 70], False), ([100], [29], False), ([40, 20], [3, 40], True), ([300], [0], False)):
         args, starts = case(new, cached, 4, 2, dim, 16, dtype, free=INF)
         q, K, V, tables, held = args
         mask = random_mask(sum(new), 2) if masked else None
@@ -279,6 +287,43 @@ def test_values_that_are_not_finite(gpu, dim, dtype):
         got = check(gpu, args, starts, dtype, mask=mask)
         if not masked:
             assert bool(torch.isnan(got[20:new[0], 2:]).all()) and bool(torch.isfinite(got[new[0] :]).all())
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+def test_values_that_are_not_finite_few_rows(gpu, dim, dtype):
+    """The same with up to 16 rows on a key head, at a place that a wavefront has last and one that it has first."""
+    for cached, masked in ((0, False), (59, False), (64, False), (200, True), (14, True)):
+        args, starts = case([7, 1], [cached, 33], 4, 2, dim, 16, dtype, free=NAN)
+        q, K, V, tables, held = args
+        mask = random_mask(8, 1) if masked else None
+        for j, d, x in ((0, 0, NAN), (1, 1, INF), (3, 1, -INF), (4, dim - 1, -INF), (5, 2, INF), (2, 3, INF)):
+            V[int(tables[0, (cached + j) // 16]), (cached + j) % 16, 1, d] = x
+        got = check(gpu, args, starts, dtype, mask=mask)
+        assert bool(torch.isfinite(got[:, :2]).all()) and bool(torch.isfinite(got[7]).all())
+        if not masked:
+            assert bool(torch.isnan(got[:7, 2:, 0]).all()) and bool(torch.isinf(got[1:3, 2:, 1]).all())
+        K[int(tables[0, (cached + 5) // 16]), (cached + 5) % 16, 1, 3] = NAN
+        got = check(gpu, args, starts, dtype, mask=mask)
+        if not masked:
+            assert bool(torch.isnan(got[5:7, 2:]).all())
+
+
+def test_two_streams_at_once(gpu):
+    """Two calls that overlap, each with its own work."""
+    a, sa = case([1] * 3, [3000, 200, 9000], 8, 2, 256, 16, BF16)
+    b, sb = case([40], [7000], 8, 2, 128, 16, BF16)
+    want = gpu.paged_attention(*a), gpu.paged_attention(*b, sb)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        for s, args, starts in ((streams[0], a, None), (streams[1], b, sb)):
+            with torch.cuda.stream(s):
+                outs.append(gpu.paged_attention(*args, starts))
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, want[i % 2])
 
 
 @pytest.mark.parametrize("dtype", [F, BF16])
