@@ -238,36 +238,66 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args 
 }
 
 // ---- drafted tokens' trees -----------------------------------------------------------------
-// A workgroup a sequence, a thread a word of a row's mask: it walks up the row's ancestors, whose places only fall,
-// until they are below its word; word 0's counts them all.
-constexpr int kTreeHeld = 4096;
+// A workgroup a sequence.  A draft of up to kTreeWalk tokens: a thread a word of a row's mask, which walks up the row's
+// ancestors, whose places only fall, until they are below its word; word 0's counts them all.  Of more tokens a walk
+// could be as long as the text: a thread has a word of every row, one row after the other, as its parent's word and its own
+// bit (and word 0's thread the positions, as the parent's and one).
+constexpr int kTreeWalk = kThreads;
 __global__ __launch_bounds__(kThreads) void attn_tree_kernel(attn_dev_tree_args a) {
-    __shared__ int32_t held_parents[kTreeHeld];
-    const int s = blockIdx.x;
+    __shared__ int32_t up[kThreads];
+    const int s = blockIdx.x, t0 = blockIdx.y * kThreads + threadIdx.x, threads = gridDim.y * kThreads;
     const Span p = span_of(a.starts, a.rows, a.n_seq, s);
     const int held = a.cached[s];
     const int32_t* parents = a.parents + p.first;
-    const bool in_lds = p.count <= kTreeHeld;
-    if (in_lds) {
-        for (int i = threadIdx.x; i < p.count; i += kThreads) held_parents[i] = parents[i];
+    int32_t* mask = a.mask + (int64_t)p.first * a.words;
+    int32_t* positions = a.positions ? a.positions + p.first : nullptr;
+    if (p.count <= kTreeWalk) {
+        if ((int)threadIdx.x < p.count) up[threadIdx.x] = parents[threadIdx.x];
         __syncthreads();
+        const int64_t items = (int64_t)p.count * a.words;
+        for (int64_t i = t0; i < items; i += threads) {
+            const int r = (int)(i / a.words), w = (int)(i - (int64_t)r * a.words);
+            uint32_t bits = 0;
+            int depth = 0;
+            if (held >= 0)
+                for (int j = r; j >> 5 >= w;) {
+                    if (j >> 5 == w) bits |= 1u << (j & 31);
+                    if (up[j] < 0 || up[j] >= j) break;
+                    ++depth;
+                    j = up[j];
+                }
+            mask[i] = (int32_t)bits;
+            if (w == 0 && positions) positions[r] = held < 0 ? 0 : (int)min((int64_t)held + depth, (int64_t)INT32_MAX);
+        }
+        return;
     }
-    const int64_t items = (int64_t)p.count * a.words;
-    for (int64_t i = threadIdx.x; i < items; i += kThreads) {
-        const int r = (int)(i / a.words), w = (int)(i - (int64_t)r * a.words);
-        uint32_t bits = 0;
-        int depth = 0;
-        if (held >= 0)
-            for (int j = r; j >= 32 * w || (w == 0 && j >= 0);) {
-                if (j >> 5 == w) bits |= 1u << (j & 31);
-                const int up = in_lds ? held_parents[j] : parents[j];
-                if (up < 0 || up >= j) break;
-                ++depth;
-                j = up;
+    for (int w0 = blockIdx.y * kThreads; w0 < a.words; w0 += threads) {
+        const int w = w0 + threadIdx.x;
+        const bool mine = w < a.words, first = w == 0 && positions;
+        uint32_t last = 0;  // of the row before
+        int last_position = 0;
+        for (int r0 = 0; r0 < p.count; r0 += kThreads) {
+            const int n = min(kThreads, p.count - r0);
+            __syncthreads();
+            if ((int)threadIdx.x < n) up[threadIdx.x] = parents[r0 + threadIdx.x];
+            __syncthreads();
+            if (!mine) continue;
+            for (int i = 0; i < n; ++i) {
+                const int r = r0 + i, j = up[i];
+                const bool has = held >= 0 && j >= 0 && j < r;
+                uint32_t bits = 0;
+                int position = max(held, 0);
+                if (has) {
+                    if (j >> 5 >= w) bits = j == r - 1 ? last : (uint32_t)mask[(int64_t)j * a.words + w];
+                    if (first) position = min(j == r - 1 ? last_position : positions[j], INT32_MAX - 1) + 1;
+                }
+                if (held >= 0 && r >> 5 == w) bits |= 1u << (r & 31);
+                mask[(int64_t)r * a.words + w] = (int32_t)bits;
+                if (first) positions[r] = position;
+                last = bits;
+                last_position = position;
             }
-        a.mask[(int64_t)p.first * a.words + i] = (int32_t)bits;
-        if (w == 0 && a.positions)
-            a.positions[p.first + r] = held < 0 ? 0 : (int)min((int64_t)held + depth, (int64_t)INT32_MAX);
+        }
     }
 }
 
@@ -343,6 +373,8 @@ hipError_t kv_launch_append(const kv_dev_append_args& a, hipStream_t s) {
 }
 
 hipError_t attn_launch_tree(const attn_dev_tree_args& a, hipStream_t s) {
-    attn_tree_kernel<<<dim3((unsigned)a.n_seq), kThreads, 0, s>>>(a);
+    // (more workgroups a sequence where a row's words are more than the threads, and the sequences do not fill the device)
+    const int more = a.n_seq <= 256 ? std::min((a.words + kThreads - 1) / kThreads, 64) : 1;
+    attn_tree_kernel<<<dim3((unsigned)a.n_seq, (unsigned)more), kThreads, 0, s>>>(a);
     return hipGetLastError();
 }

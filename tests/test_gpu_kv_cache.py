@@ -305,6 +305,29 @@ def test_trees(gpu):
         gpu.draft_tree(p[:-1], c)
 
 
+@pytest.mark.parametrize("n", [256, 257, 20000])
+def test_long_trees(gpu, n):
+    """Chains, and two that take turns (a token follows the one before the last), as long as a text: the bits by their
+    formula.  And several sequences of them, some skipped."""
+    device = dict(dtype=torch.int32, device="cuda")
+    words = -(-n // 32)
+    word, row = torch.arange(words, device="cuda")[None], torch.arange(n, device="cuda")[:, None]
+    upto = (row - 32 * word).clamp(-1, 31)  # the last bit that a row has in a word
+    ones = (torch.ones_like(upto) << (upto + 1)) - 1
+    for stride, bits in ((1, ones), (2, ones & torch.where(row % 2 == 0, 0x55555555, 0xAAAAAAAA))):
+        parents = torch.arange(n, **device) - stride
+        want = bits.to(torch.int32), (7 + row[:, 0] // stride).to(torch.int32)
+        got = gpu.draft_tree(parents, torch.tensor([7], **device))
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        if n < 1000:
+            several = gpu.draft_tree(parents.repeat(3), torch.tensor([7, -1, 2 ** 31 - 3], **device))
+            for x, y in zip(several, want):
+                assert torch.equal(x[:n], y) and bool((x[n : 2 * n] == 0).all())
+            assert torch.equal(several[0][2 * n :], want[0])
+            far = (want[1].long() - 7 + 2 ** 31 - 3).clamp(max=2 ** 31 - 1)
+            assert torch.equal(several[1][2 * n :].long(), far)
+
+
 # ---- together --------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F, BF16])
 def test_a_layer_reads_drafts_and_goes_on(gpu, dtype):
