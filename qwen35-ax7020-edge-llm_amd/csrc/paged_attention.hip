@@ -185,6 +185,17 @@ __device__ Share share_of(const Shape& sh, int* held, int least) {
     return r;
 }
 
+// The first place after this one that has something to do: a batch's skipped and empty sequences, 64 at a time.
+__device__ __forceinline__ int place_after(const Shape& sh, const int* held, int place) {
+    const int lane = threadIdx.x & 63, n = sh.places();
+    for (int base = place + 1; base < n; base += 64) {
+        const int at = base + lane;
+        const uint64_t some = __ballot(at < n && (at < ATTN_HELD ? held[at] : sh.tile(at).cost) > 0);
+        if (some) return base + __builtin_ctzll(some);
+    }
+    return n;
+}
+
 // Where key j of a sequence is, in units of the cache's strides (AttnPlan), kNowhere if it does not exist.
 __device__ __forceinline__ uint32_t key_at(const attn_dev_args& a, const AttnUnits& u, const Tile& t, int j) {
     if (j >= t.places) return kNowhere;
@@ -555,8 +566,7 @@ struct Pass {
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-            {
+            for (int i = 0; i < 8; ++i) {
                 s[b][i / 4][i % 4] *= c;
                 if (!ALL && !(sees[b] >> (16 * (i / 4) + i % 4) & 1)) s[b][i / 4][i % 4] = kNone;
             }
@@ -724,7 +734,7 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
         const int64_t in = at - before, all = (int64_t)t.cost * a.heads_k;
         if (in >= all) {
             before += all;
-            ++place;
+            place = __builtin_amdgcn_readfirstlane(place_after(shape, held, place));
             continue;
         }
         const int head = (int)quotient(in, t.cost), c0 = (int)(in - (int64_t)head * t.cost);
@@ -1002,8 +1012,7 @@ struct Few {
             s = (part[0] + part[1]) + (part[2] + part[3]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
+        for (int i = 0; i < 4; ++i) {
             s[i] *= c;
             if (!ALL && !(sees >> (4 * g + i) & 1)) s[i] = kNone;
         }
@@ -1159,7 +1168,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
         const int64_t in = at - before, all = (int64_t)t.cost * a.heads_k;
         if (in >= all) {
             before += all;
-            ++place;
+            place = __builtin_amdgcn_readfirstlane(place_after(shape, held, place));
             continue;
         }
         const int head = (int)quotient(in, t.cost), c0 = (int)(in - (int64_t)head * t.cost);

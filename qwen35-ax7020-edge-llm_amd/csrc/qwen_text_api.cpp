@@ -225,6 +225,7 @@ const char* paged_bad(const attn_dev_args* a) {
     const size_t es = a->dtype == QWEN_BF16 ? 2 : 4;
     if (!a->out || !a->q || !aligned(a->out, es) || !aligned(a->q, es))
         return "out or q is NULL or not aligned to its elements";
+    if (a->out == a->q) return "out is q";
     for (const int64_t x : {a->q_row, a->q_head, a->out_row, a->out_head})
         if (!in(x, 0, kMaxStride)) return "a stride is below 0 or above 2^34";
     if (!heads_apart(a->rows, a->out_row, a->heads_q, a->out_head, a->dim)) return "out's rows or heads overlap";

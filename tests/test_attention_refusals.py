@@ -32,7 +32,7 @@ def append(**over):
 
 
 def paged(**over):
-    return made(qk.attn_dev_args(), over, **CACHE, out=P, q=P, mask=P, work=P, work_bytes=1 << 40, q_row=256, q_head=64,
+    return made(qk.attn_dev_args(), over, **CACHE, out=2 * P, q=P, mask=P, work=P, work_bytes=1 << 40, q_row=256, q_head=64,
                 out_row=256, out_head=64, mask_words=1, scale=0.125)
 
 
@@ -84,7 +84,7 @@ def test_append_refuses(over):
 @pytest.mark.parametrize("over", SHARED + [
     dict(scale=0.0), dict(scale=-1.0), dict(scale=NAN), dict(scale=INF), dict(scale=1e-39), dict(scale=2e38), dict(mask_words=-1), dict(mask_words=65537),
     dict(mask=P + 1), dict(out=None), dict(q=None), dict(out=P + 1), dict(q=P + 1), dict(q_row=-1), dict(out_head=-1),
-    dict(cache_page=1 << 39, pages=1 << 20),
+    dict(cache_page=1 << 39, pages=1 << 20), dict(out=P),
     dict(out_row=64), dict(out_head=8), dict(work=None), dict(work=P + 16), dict(work_bytes=1000)])
 def test_attention_refuses(over):
     refused(qk.load().attn_dev_paged, paged(**over))

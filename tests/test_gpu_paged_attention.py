@@ -309,6 +309,17 @@ def test_values_that_are_not_finite_few_rows(gpu, dim, dtype):
             assert bool(torch.isnan(got[5:7, 2:]).all())
 
 
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_mostly_empty_batches(gpu, dtype):
+    """Long runs of skipped and of empty sequences between those that are at work, more than a workgroup remembers."""
+    live = {3: 700, 70: 5, 300: 64, 1290: 1500}
+    for new, rest in ((1, -1), (2, -1), (40, -1), (1, 0), (40, 0)):  # rest 0: the others have no rows, with tokens held
+        lens = [new if s in live or rest < 0 and new < 40 else 0 for s in range(1300)]
+        held = [live.get(s, rest) for s in range(1300)]
+        args, starts = case(lens, held, 4, 2, 64, 16, dtype)
+        check(gpu, args, starts, dtype, pass_starts=len(set(lens)) > 1)
+
+
 def test_two_streams_at_once(gpu):
     """Two calls that overlap, each with its own work."""
     a, sa = case([1] * 3, [3000, 200, 9000], 8, 2, 256, 16, BF16)
