@@ -73,20 +73,35 @@ struct Shape {
     __device__ int tiles_of(int rows) const { return (rows * p.group) >> p.rows_log; }
     __device__ int places() const { return a.starts ? tiles_of(a.rows) + a.n_seq : a.n_seq * p.each; }
     __device__ int first_place(int s) const { return tiles_of(min(max(a.starts[s], 0), a.rows)) + s; }
-    __device__ Tile tile(int place) const {
+    // The last sequence whose first place is not past this one.
+    __device__ int seq_of(int place) const {
+        int lo = 0, hi = a.n_seq;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first_place(mid) <= place)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        return lo;
+    }
+    // The same for places (of any lanes) that are up to 64 sequences past lo, by a load of all lanes and exchanges between
+    // them; lo + 64 if they are more (1,024 sequences, two at work: a search in memory for every place 81 us, so 58).
+    __device__ __forceinline__ int seq_from(int lo, int place) const {
+        const int next = lo + 1 + (threadIdx.x & 63), first = next < a.n_seq ? first_place(next) : INT32_MAX;
+        int past = 0;
+#pragma unroll
+        for (int i = 32; i; i /= 2)
+            if (__shfl(first, past + i - 1) <= place) past += i;
+        return lo + past + (__shfl(first, past) <= place);
+    }
+    __device__ Tile tile(int place) const { return tile(place, a.starts ? seq_of(place) : 0); }
+    __device__ Tile tile(int place, int seq) const {  // (seq: with starts)
         Tile t{};
         int in = 0;
         if (a.starts) {
-            int lo = 0, hi = a.n_seq;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (first_place(mid) <= place)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            t.seq = lo;
-            in = place - first_place(lo);
+            t.seq = seq;
+            in = place - first_place(seq);
         } else if (p.each == 1) {
             t.seq = place;
         } else {
@@ -130,6 +145,7 @@ struct Share {
     int64_t from, to;  // of those
     int64_t before;    // tiles of the places before
     int place;         // the place it begins in
+    int seq;           // a sequence that is not past that place's
     int workers;       // workgroups with a share
 };
 
@@ -152,9 +168,13 @@ __device__ Share share_of(const Shape& sh, int* held, int least) {
     };
     int64_t sum = 0;
     uint32_t upto = 0, mine = 0;
+    int seq = 0, far = 0;  // the sequence of the last place so far, and of the last one of `held`
     for (int base = 0; base < n; base += 64) {
         const int at = base + lane;
-        mine = at < n ? sh.tile(at).cost : 0;
+        if (base == ATTN_HELD) far = seq;
+        const int own = sh.a.starts ? sh.seq_from(seq, at) : 0;
+        mine = at < n ? sh.tile(at, own).cost : 0;
+        seq = __shfl(own, 63);
         if (at < ATTN_HELD) held[at] = mine;
         upto = scan(mine);
         sum += (uint32_t)__shfl(upto, 63);
@@ -167,10 +187,18 @@ __device__ Share share_of(const Shape& sh, int* held, int least) {
     if ((int)blockIdx.x >= r.workers) r.from = r.to = 0;
     if (r.from >= r.to) return r;
     int64_t before = 0;
+    seq = far;
     for (int base = 0; base < n; base += 64) {
         if (n > 64) {
             const int at = base + lane;
-            mine = at >= n ? 0 : at < ATTN_HELD ? held[at] : sh.tile(at).cost;
+            if (base >= ATTN_HELD) {
+                const int own = sh.a.starts ? sh.seq_from(seq, at) : 0;
+                mine = at < n ? sh.tile(at, own).cost : 0;
+                r.seq = seq;
+                seq = __shfl(own, 63);
+            } else {
+                mine = at < n ? held[at] : 0;
+            }
             upto = scan(mine);
         }
         const uint64_t over = __ballot((before + upto) * heads > r.from);
@@ -194,6 +222,12 @@ __device__ __forceinline__ int place_after(const Shape& sh, const int* held, int
         if (some) return base + __builtin_ctzll(some);
     }
     return n;
+}
+
+// The sequence of a place that lies further on than lo's.
+__device__ __forceinline__ int next_seq(const Shape& sh, int lo, int place) {
+    const int seq = __builtin_amdgcn_readfirstlane(sh.seq_from(lo, place));
+    return seq < lo + 64 ? seq : __builtin_amdgcn_readfirstlane(sh.seq_of(place));
 }
 
 // Where key j of a sequence is, in units of the cache's strides (AttnPlan), kNowhere if it does not exist.
@@ -726,11 +760,12 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
     P pass{a, units, p.group, lds, (int)(threadIdx.x & 63), wave};
     pass.c = a.scale * kLog2e;
     int64_t at = share.from, before = share.before;
-    int place = share.place;
+    int place = share.place, seq = share.seq;
     const int places = shape.places();
     const bool vec = quads<T>(a);
     while (at < share.to && place < places) {
-        const Tile t = uniform(shape.tile(place));
+        if (a.starts) seq = next_seq(shape, seq, place);
+        const Tile t = uniform(shape.tile(place, seq));
         const int64_t in = at - before, all = (int64_t)t.cost * a.heads_k;
         if (in >= all) {
             before += all;
@@ -747,7 +782,7 @@ __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan 
         asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");  // the last products' results, whatever way the loop was left
         if (k0 == 0 && k1 < t.tiles)
             left = AttnDesc{1, t.first, t.m0, t.count, head,
-                            (int)quotient((at - c1 + t.cost) * share.workers - 1, share.total)};
+                            min((int)quotient((at - c1 + t.cost) * share.workers - 1, share.total), share.workers - 1)};
         const int n = threadIdx.x & 15, slot = 2 * blockIdx.x + (k0 == 0);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -1161,10 +1196,11 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
     few.q = q;
     few.group = p.group;
     int64_t at = share.from, before = share.before;
-    int place = share.place;
+    int place = share.place, seq = share.seq;
     const int places = shape.places();
     while (at < share.to && place < places) {
-        const Tile t = uniform(shape.tile(place));
+        if (a.starts) seq = next_seq(shape, seq, place);
+        const Tile t = uniform(shape.tile(place, seq));
         const int64_t in = at - before, all = (int64_t)t.cost * a.heads_k;
         if (in >= all) {
             before += all;
@@ -1178,7 +1214,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
         if (k0 >= k1) continue;
         if (k0 == 0 && k1 < t.tiles)
             left = AttnDesc{1, t.first, t.m0, t.count, head,
-                            (int)quotient((at - c1 + t.cost) * share.workers - 1, share.total)};
+                            min((int)quotient((at - c1 + t.cost) * share.workers - 1, share.total), share.workers - 1)};
         // q to LDS, a part a thread at a time
         const int rows = min(16, t.count - t.m0);
         few.t = t;
