@@ -715,10 +715,11 @@ int kv_dev_append(const kv_dev_append_args* args, void* stream);
  * The same call gives the same bits; in another call they may differ in rounding, as the
  * keys are split over workgroups by the lengths of the whole call.
  *
- * scale above 0, a normal number of up to 1e38; dim a multiple of 8 up to 256; heads_q a multiple of heads_k, rows heads_q up to 2^28;
- * n_seq up to 2^20; mask_words up to 2^16 (mask NULL: not read).  q and out are aligned to their elements, the
- * cache to 16 bytes (pointers and strides); from a head's first place to its last a cache spans less than 2^32 times
- * the largest power of two that divides its pages' and tokens' strides (so 64 GiB or more, 4 TiB with 1 KiB a token).  out overlaps nothing that the call reads.
+ * scale above 0, a normal number of up to 1e38; dim a multiple of 8 up to 256; heads_q a multiple of heads_k,
+ * rows heads_q up to 2^28; n_seq up to 2^20; mask_words up to 2^16 (mask NULL: not read).  q and out are
+ * aligned to their elements, the cache to 16 bytes (pointers and strides); from a head's first place to its last a
+ * cache spans less than 2^32 times the largest power of two that divides its pages' and tokens' strides (so 64 GiB
+ * or more, 4 TiB with 1 KiB a token).  out overlaps nothing that the call reads.
  * Nothing is allocated and nothing waits: the calls can be captured.  full_attn_f32 (04/qwen_attn.c:406) is the
  * host's counterpart for one sequence. */
 typedef struct attn_dev_args {

@@ -39,12 +39,22 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     p.dim = a.dim <= 64 ? 64 : a.dim <= 128 ? 128 : 256;
     // rows of an average sequence and key head
     const size_t mean = ((size_t)a.rows * p.group + std::max(a.n_seq, 1) - 1) / std::max(a.n_seq, 1);
-    p.blocks = bf16 && mean > 16 ? 2 : 1;
-    p.waves = mean <= (size_t)16 * p.blocks ? 1 : mean <= (size_t)32 * p.blocks ? 2 : mean <= (size_t)64 * p.blocks ? 4 : 8;
+    // Up to 16 rows: attn_step_kernel (64 sequences of 4,000 keys, 16 rows of 256 bf16 elements, 130 us, by attn_kernel
+    // 135; 32 of 2,000, 128 float32 ones, 47 for 61; but 48 of 2,000 and 16 rows on average, many with more, 71 for
+    // 55).
+    p.few = mean <= 16;
+    // More: as many rows to a tile as there are, so that its keys are read once.  Two wavefronts at least, to copy (one
+    // | two: 48 sequences of 28 rows of 128 elements 70 | 62 us, 64 of 32 rows of 256 174 | 149).  Of 256 bf16 elements
+    // four wavefronts with their 340 registers are one workgroup a compute unit, two are two (two | four | eight at 64
+    // sequences of 128 rows 223 | 240 | 241, one of 128 rows 44 | 45 | 51, at 160 rows 271 | - | 235); of 128 elements
+    // two are (48 of 125 rows, two | four | eight: 108 | 93 | 116).
+    p.blocks = bf16 && !p.few ? 2 : 1;
+    p.waves = p.few ? 1 : mean <= (size_t)32 * p.blocks ? 2 : mean <= (size_t)64 * p.blocks ? 4 : 8;
+    if (bf16 && p.dim == 256 && p.waves == 4) p.waves = 2;
     p.rows = 16 * p.blocks * p.waves;
     p.rows_log = 31 - __builtin_clz(p.rows);
     p.each = a.starts || !a.n_seq ? 0 : (a.rows / a.n_seq * p.group + p.rows - 1) / p.rows;
-    p.few = mean <= 16;
+    // (64 keys: half as many waits for the copies; four wavefronts gained nothing by it)
     p.keys = p.few || (bf16 && p.waves == 8) ? 64 : 32;
     // as many as are at work at a time, by LDS and registers (8 wavefronts a compute unit), up to four a unit
     const size_t lds = (size_t)4 * p.keys * p.dim * (bf16 ? 2 : 4) + ATTN_HELD * 4 + 256;
@@ -58,7 +68,8 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     // 372 | 381; float32 prompts with 0 | 1 | 2 | 4 tiles of 32 107 | 98 | 98 | 105.
     p.extra = p.few ? 1 : bf16 ? std::max(256, 2 * p.dim) / p.keys : 2;
     p.rows_most = a.starts || !a.n_seq ? p.rows : a.rows / a.n_seq * p.group;
-    // Where there are about eight parts or more of each, 16 wavefronts join them (4 | 16: one sequence of 4,096 tokens xxx).
+    // Where there are about eight parts or more of each, 16 wavefronts join them, by a workgroup for each tile and not
+    // each share (without | with: a token of one sequence of 4,096 19.0 | 15.7 us, 26 drafted ones of 6,000 64 | 33).
     const size_t units = (a.starts ? (size_t)a.rows * p.group / p.rows + a.n_seq : (size_t)a.n_seq * p.each) * a.heads_k;
     p.shared = units * 8 <= (size_t)p.grid ? (int)units : 0;
     size_t at = 0;

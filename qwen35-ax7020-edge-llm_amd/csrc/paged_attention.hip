@@ -8,9 +8,10 @@
 // turned round (K Q^T, V^T W^T), so that a lane holds scores, weights and outputs of one row: the weights
 // are the next product's operand as they lie, maxima and sums need two exchanges between lanes.
 //
-// The tiles of keys of all tiles of rows, and some more for what a tile of rows costs by itself, are one long axis, divided evenly over the workgroups: a batch of
-// ragged lengths fills the device to the end, and one long sequence is shared by all.  A workgroup whose share begins
-// or ends inside a tile of rows leaves its maxima, sums and outputs, which attn_join_kernel joins in a fixed order.
+// The tiles of keys of all tiles of rows, and some more for what a tile of rows costs by itself, are one long axis,
+// divided evenly over the workgroups: a batch of ragged lengths fills the device to the end, and one long sequence is
+// shared by all.  A workgroup whose share begins or ends inside a tile of rows leaves its maxima, sums and outputs,
+// which attn_join_kernel joins in a fixed order.
 #include <type_traits>
 
 #include "bf16_terms.h"
@@ -27,9 +28,9 @@ using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -INFINITY;  // the maximum of no scores
 constexpr uint32_t kNowhere = 0xffffffffu;
-// A row's maximum is raised, and what it has so far scaled down to it, only by a score that is this much above it: weights
-// then are up to 2^8, and float32 sums have the same bits.  (Each of 32 rows raises its own: without slack nearly
-// every 32 keys of the first thousand.)
+// A row's maximum is raised, and what it has so far scaled down to it, only by a score that is this much above it:
+// weights then are up to 2^8, and float32 sums have the same bits.  (Each of 32 rows raises its own: without slack
+// nearly every 32 keys of the first thousand.)
 constexpr float kSlack = 8;
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: 0
 
@@ -37,9 +38,9 @@ __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp
 // what lies in a free page need not be.
 __device__ const uint4 kZeros[64] = {};  // (attn_step_kernel: a whole key's or value's)
 
-// 16 bytes a lane from `from` to 1 KiB of LDS, the same `to` in all lanes.  (The builtin of this instruction makes the compiler wait for all
-// copies in flight before the next read of LDS, whichever buffer that is from.
-// Whoever reads waits for itself: Pass::arrived.)
+// 16 bytes a lane from `from` to 1 KiB of LDS, the same `to` in all lanes.  (The builtin of this instruction makes the
+// compiler wait for all copies in flight before the next read of LDS, whichever buffer that is from. Whoever reads
+// waits for itself: Pass::arrived.)
 __device__ __forceinline__ void copy_to_lds(global_char* from, char* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory");
@@ -85,8 +86,9 @@ struct Shape {
         }
         return lo;
     }
-    // The same for places (of any lanes) that are up to 64 sequences past lo, by a load of all lanes and exchanges between
-    // them; lo + 64 if they are more (1,024 sequences, two at work: a search in memory for every place 81 us, so 58).
+    // The same for places (of any lanes) that are up to 64 sequences past lo, by a load of all lanes and exchanges
+    // between them; lo + 64 if they are more (1,024 sequences, two at work: a search in memory for every place 81 us,
+    // so 58).
     __device__ __forceinline__ int seq_from(int lo, int place) const {
         const int next = lo + 1 + (threadIdx.x & 63), first = next < a.n_seq ? first_place(next) : INT32_MAX;
         int past = 0;
@@ -464,7 +466,8 @@ struct Pass {
     }
 
     // The operands of the step's products, read kDeep - 1 ahead of them.  Keys: part 4 i + g of keys 16 h + lane % 16.
-    // Values (operand t of kValues): bf16 a product's, 32 keys by 16 elements; float32 four products', four keys by 64 elements.
+    // Values (operand t of kValues): bf16 a product's, 32 keys by 16 elements; float32 four products', four keys by 64
+    // elements.
     static constexpr int kDeep = kBf16 && !kTight ? 4 : 3;
     static constexpr int kKeys = 2 * kQ, kValues = kBf16 ? kOut : 2 * kOut;
     using Operand = u32x4;
@@ -521,8 +524,8 @@ struct Pass {
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // A tile of which some row does not see every key: a value that is not finite must not reach such a row as 0 times it.
-    // If there are any, those rows that see them get them here, and 0 takes their place.
+    // A tile of which some row does not see every key: a value that is not finite must not reach such a row as 0 times
+    // it. If there are any, those rows that see them get them here, and 0 takes their place.
     __device__ void clean(int stage, int k0, uint64_t there, int* flags) {
         char* v = lds + stage * kStage + kTile;
         bool odd = false;
@@ -744,6 +747,12 @@ __device__ __forceinline__ bool quads(const attn_dev_args& a) {  // four element
     return ((uintptr_t)a.out | (uint64_t)a.out_row * sizeof(T) | (uint64_t)a.out_head * sizeof(T)) % (4 * sizeof(T)) == 0;
 }
 
+// What bounds it.  Many rows: the matrix cores and LDS together (a prompt of 16,384 tokens, 8 heads of 256, bf16: 1.16
+// ms for 1.1 TFLOP, 0.95 PFLOP/s).  A step of 32 keys by 32 rows of 256 elements is 64 products, 32 KiB from LDS and 16
+// exponentials a lane; two wavefronts a SIMD take turns with them.  Tens of rows on thousands of keys: the copies and
+// the reads of LDS (1,500 drafted tokens of 48 sequences on 100,000 keys, 4 key heads of 128: 79 us for 205 MB, 2.6
+// TB/s); one sequence: the latency of finding its share, of a few tiles of keys and of the join (26 tokens on 6,000: 24
+// us and 7).  float32: the 16 x 16 x 4 products (9 prompts, 3,001 tokens on 5,000, 80 of 128 elements used: 88 us).
 template <class T, int D, int RB, int W, int BN, bool FULL>
 __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan p, AttnUnits units) {
     using P = Pass<T, D, RB, W, BN, FULL>;
@@ -854,9 +863,10 @@ __device__ __forceinline__ int first_of(const attn_dev_args& a, const AttnPlan& 
     return l * 64 + __shfl(lane == l ? __builtin_ctzll(set | 1ull << 63) : 0, l);
 }
 
-// The parts of a tile of rows, 16 rows to a workgroup: its first part is the last of workgroup first_of(), the others are
-// the first of those that follow.  A wavefront has 64 elements of the rows and every G-th part, kAtOnce of them in
-// flight; Z wavefronts side by side, D / 64 / Z workgroups.
+// The parts of a tile of rows, 16 rows to a workgroup: its first part is the last of workgroup first_of(), the others
+// are the first of those that follow.  A wavefront has 64 elements of the rows and every G-th part, kAtOnce of them in
+// flight; Z wavefronts side by side, D / 64 / Z workgroups.  Bound by the parts' latency where there are few tiles (7
+// us for one sequence's 26 tokens in 512 parts), else by their bytes (48 trees: 13 us, a prompt of 16,384 tokens 29).
 constexpr int kAtOnce = 4;
 template <class T, int D, int G, int Z>
 __global__ __launch_bounds__(64 * Z * G) void attn_join_kernel(attn_dev_args a, AttnPlan p) {
@@ -945,12 +955,13 @@ __global__ __launch_bounds__(64 * Z * G) void attn_join_kernel(attn_dev_args a, 
 }
 
 // ---- few rows ----------------------------------------------------------------------------
-// Up to 16 rows on a key head: bound by the cache's bytes.  Every wavefront has keys of its own, 16 at a time, straight
-// to registers: as the left operands of K Q^T and, with float32 weights and values widened, of V^T W^T, whose 16 by
-// 16 by 4 products take a lane's 16 bytes of a value as that many products' operands.  (bf16 products of V would need
-// its transpose, from LDS: the float32 ones are a third of the time that the bytes take.)  The wavefronts' outputs meet in
-// LDS at the end.
-// FULL: heads have D elements.
+// Up to 16 rows on a key head: bound by the cache's bytes (64 sequences of 4,096 keys, 2 key heads of 256, bf16: 537 MB
+// in 110 us, 4.9 TB/s, what a copy reaches; 139 us when the keys came through LDS), or where they are few by the
+// latency of a share (one sequence: 11 us).  Every wavefront has keys of its own, 16 at a time, straight to registers:
+// as the left operands of K Q^T and, with float32 weights and values widened, of V^T W^T, whose 16 by 16 by 4 products
+// take a lane's 16 bytes of a value as that many products' operands.  (bf16 products of V would need its transpose,
+// from LDS: the float32 ones are a third of the time that the bytes take.)  The wavefronts' outputs meet in LDS at the
+// end. FULL: heads have D elements.
 template <class T, int D, bool FULL>
 struct Few {
     static constexpr bool kBf16 = sizeof(T) == 2;
@@ -1302,7 +1313,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
     }
 }
 
-// The parts of a row, a row to a workgroup: D / 4 lanes have every G-th part, kAtOnce of them in flight.
+// The parts of a row, a row to a workgroup: D / 4 lanes have every G-th part, kAtOnce of them in flight.  Latency: 5 us.
 template <class T, int D, int G>
 __global__ __launch_bounds__(G * (D / 4)) void attn_step_join_kernel(attn_dev_args a, AttnPlan p) {
     const int first = first_of<G * (D / 4)>(a, p);
@@ -1396,12 +1407,10 @@ hipError_t launch(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
 template <int D>
 hipError_t launch_bf16(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
     if (p.few) return launch_step<uint16_t, D>(a, p, s);
-    switch (p.waves) {
-        case 1: return launch<uint16_t, D, 2, 1, 32>(a, p, s);
-        case 2: return launch<uint16_t, D, 2, 2, 32>(a, p, s);
-        case 4: return launch<uint16_t, D, 2, 4, 32>(a, p, s);
-        default: return launch<uint16_t, D, 2, 8, 64>(a, p, s);
-    }
+    if (p.waves == 2) return launch<uint16_t, D, 2, 2, 32>(a, p, s);
+    if constexpr (D < 256)
+        if (p.waves == 4) return launch<uint16_t, D, 2, 4, 32>(a, p, s);
+    return launch<uint16_t, D, 2, 8, 64>(a, p, s);
 }
 template <int D>
 hipError_t launch_f32(const attn_dev_args& a, const AttnPlan& p, hipStream_t s) {
