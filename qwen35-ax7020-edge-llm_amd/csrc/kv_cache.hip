@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args 
 // A workgroup a sequence.  A draft of up to kTreeWalk tokens: a thread a word of a row's mask, which walks up the row's
 // ancestors, whose places only fall, until they are below its word; word 0's counts them all.  Of more tokens a walk
 // could be as long as the text: a thread has a word of every row, one row after the other, as its parent's word and its
-// own bit (and word 0's thread the positions, as the parent's and one). Latency bounds both: 26 tokens 2.7 us, 48 trees
+// own bit (and word 0's thread the positions, as the parent's and one). Latency bounds both: 26 tokens 3.4 us, 48 trees
 // of 1,500 4.8. (One sequence, a chain of 64 | 256 | 1,000 | 20,000 tokens: walked 11 | 109 us, row after row 50 | 178
 // | 3,437 of 256 and more.)
 constexpr int kTreeWalk = 128;

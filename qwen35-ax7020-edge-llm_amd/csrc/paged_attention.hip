@@ -751,7 +751,7 @@ __device__ __forceinline__ bool quads(const attn_dev_args& a) {  // four element
 // ms for 1.1 TFLOP, 0.95 PFLOP/s).  A step of 32 keys by 32 rows of 256 elements is 64 products, 32 KiB from LDS and 16
 // exponentials a lane; two wavefronts a SIMD take turns with them.  Tens of rows on thousands of keys: the copies and
 // the reads of LDS (1,500 drafted tokens of 48 sequences on 100,000 keys, 4 key heads of 128: 79 us for 205 MB, 2.6
-// TB/s); one sequence: the latency of finding its share, of a few tiles of keys and of the join (26 tokens on 6,000: 24
+// TB/s); one sequence: the latency of finding its share, of a few tiles of keys and of the join (26 tokens on 6,000: 22
 // us and 7).  float32: the 16 x 16 x 4 products (9 prompts, 3,001 tokens on 5,000, 80 of 128 elements used: 88 us).
 template <class T, int D, int RB, int W, int BN, bool FULL>
 __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan p, AttnUnits units) {
@@ -866,7 +866,7 @@ __device__ __forceinline__ int first_of(const attn_dev_args& a, const AttnPlan& 
 // The parts of a tile of rows, 16 rows to a workgroup: its first part is the last of workgroup first_of(), the others
 // are the first of those that follow.  A wavefront has 64 elements of the rows and every G-th part, kAtOnce of them in
 // flight; Z wavefronts side by side, D / 64 / Z workgroups.  Bound by the parts' latency where there are few tiles (7
-// us for one sequence's 26 tokens in 512 parts), else by their bytes (48 trees: 13 us, a prompt of 16,384 tokens 29).
+// us for one sequence's 26 tokens in 200 parts), else by their bytes (48 trees: 13 us, a prompt of 16,384 tokens 29).
 constexpr int kAtOnce = 4;
 template <class T, int D, int G, int Z>
 __global__ __launch_bounds__(64 * Z * G) void attn_join_kernel(attn_dev_args a, AttnPlan p) {
