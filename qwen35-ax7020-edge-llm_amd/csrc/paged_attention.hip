@@ -331,10 +331,13 @@ struct Pass {
     float m[RB], l[RB];  // maximum of the scores (in base 2), or up to kSlack less, and this lane's part of the sum
     float c;
 
-    // Positions of a key's parts in LDS: eight keys' parts of one place, which lanes of K Q^T read together, and
-    // the 32 bytes of each of eight keys that ds_read_tr16_b64 reads lie in different banks.
-    static __device__ int k_swizzle(int r) { return r & 7; }
-    static __device__ int v_swizzle(int r) { return !kBf16 ? r & 7 : (D == 64 ? r >> 1 & 3 : r & 7) << 1; }
+    // Positions of a key's parts in LDS.  16 lanes whose 16 bytes are read at once have to have them in different
+    // sixteenths of 256 bytes: those of K Q^T, with parts 4 i and 4 i + 1 of eight keys each, change places
+    // by their key; the 32 bytes of each of eight keys that ds_read_tr16_b64 reads too.  float32 values are read along the
+    // key.  (Among eight parts only, every read of keys met itself: 1,159 us for 1,149 of the prompt below.)
+    static constexpr int kTurn = kParts < 16 ? 8 : 16;
+    static __device__ int k_swizzle(int r) { return r & (kTurn - 1); }
+    static __device__ int v_swizzle(int r) { return !kBf16 ? 0 : (D == 64 ? r >> 1 & 3 : r & 7) << 1; }
 
     // Output e of f of a lane's row is element out_at(f, e); four of them are next to each other.
     // (float32: 16 bytes of a value are the left operands of four products, so that a product's 16
@@ -462,7 +465,7 @@ struct Pass {
     // float32: parts 16 f + lane % 16 of key 16 (i / 4) + 4 g + i % 4
     __device__ __forceinline__ f32x4 row_read(const char* v, int i, int f) const {
         const int r = 16 * (i / 4) + 4 * (lane >> 4) + i % 4;
-        return *reinterpret_cast<const f32x4*>(v + r * kRow + ((16 * f + (lane & 15)) ^ v_swizzle(r)) * 16);
+        return *reinterpret_cast<const f32x4*>(v + r * kRow + (16 * f + (lane & 15)) * 16);
     }
 
     // The operands of the step's products, read kDeep - 1 ahead of them.  Keys: part 4 i + g of keys 16 h + lane % 16.
@@ -472,8 +475,8 @@ struct Pass {
     static constexpr int kKeys = 2 * kQ, kValues = kBf16 ? kOut : 2 * kOut;
     using Operand = u32x4;
     static __device__ __forceinline__ Operand read_key(const char* k, int at, int t) {
-        const int i = t / 2, h = t % 2;  // (of eight parts that change places the second four are the first's neighbours)
-        return *reinterpret_cast<const Operand*>(k + (at ^ i % 2 * 64) + 16 * h * kRow + i / 2 * 128);
+        const int i = t / 2, h = t % 2;  // (kTurn parts change places with one another)
+        return *reinterpret_cast<const Operand*>(k + (at ^ i % (kTurn / 4) * 64) + 16 * h * kRow + i / (kTurn / 4) * (kTurn * 16));
     }
     __device__ __forceinline__ Operand read_value(const char* v, int at, int t) const {
         if constexpr (kBf16) return tr_read(v, at, t);
@@ -747,12 +750,14 @@ __device__ __forceinline__ bool quads(const attn_dev_args& a) {  // four element
     return ((uintptr_t)a.out | (uint64_t)a.out_row * sizeof(T) | (uint64_t)a.out_head * sizeof(T)) % (4 * sizeof(T)) == 0;
 }
 
-// What bounds it.  Many rows: the matrix cores and LDS together (a prompt of 16,384 tokens, 8 heads of 256, bf16: 1.16
-// ms for 1.1 TFLOP, 0.95 PFLOP/s).  A step of 32 keys by 32 rows of 256 elements is 64 products, 32 KiB from LDS and 16
-// exponentials a lane; two wavefronts a SIMD take turns with them.  Tens of rows on thousands of keys: the copies and
-// the reads of LDS (1,500 drafted tokens of 48 sequences on 100,000 keys, 4 key heads of 128: 79 us for 205 MB, 2.6
+// What bounds it.  Many rows: what a step does one after the other (a prompt of 16,384 tokens, 8 heads of 256, bf16:
+// 1.15 ms for 1.1 TFLOP, 0.96 PFLOP/s; matrix cores 42 % of the time, other vector instructions 32, LDS 23).  A step of
+// 32 keys by 32 rows of 256 elements is 64 products, 32 KiB from LDS, 16 exponentials a lane and a maximum over lanes;
+// two wavefronts a SIMD take turns with them, for more there are no registers.  Tens of rows on thousands of keys: the copies'
+// latency and the parts (1,500 drafted tokens of 48 sequences on 100,000 keys, 4 key heads of 128: 79 us for 205 MB, 2.6
 // TB/s); one sequence: the latency of finding its share, of a few tiles of keys and of the join (26 tokens on 6,000: 22
-// us and 7).  float32: the 16 x 16 x 4 products (9 prompts, 3,001 tokens on 5,000, 80 of 128 elements used: 88 us).
+// us and 7).  float32: the 16 x 16 x 4 products, 59 % of the time (9 prompts, 3,001 tokens on 5,000, 80 of 128 elements
+// used: 87 us).
 template <class T, int D, int RB, int W, int BN, bool FULL>
 __global__ __launch_bounds__(64 * W) void attn_kernel(attn_dev_args a, AttnPlan p, AttnUnits units) {
     using P = Pass<T, D, RB, W, BN, FULL>;
