@@ -1297,7 +1297,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(attn_dev_args a, Attn
 #pragma unroll
             for (int w = 0; w < P::W; ++w) {
                 const float2 s = tops[w][r];
-                all_l += s.x == kNone ? 0.0f : s.y * exp2_raw(s.x - most);
+                all_l += s.x == kNone ? s.y : s.y * exp2_raw(s.x - most);  // (no maximum: no sum, or every score NaN)
             }
             if (k0 == 0 && k1 == t.tiles) {
                 const float y = 1.0f / all_l;
