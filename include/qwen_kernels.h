@@ -651,7 +651,8 @@ int rope_dev_grad(const rope_dev_args* args, void* stream);
  * pages in tables[s * table_row ..], table_pages of them: place j of the
  * sequence is token j % page of page tables[s * table_row + j / page].  Two sequences may
  * share pages.  A place past the table, or whose table entry is not one of the pages (-1),
- * does not exist: nothing is written there, and attention does not see it.
+ * does not exist: nothing is written there, and attention does not see it.  With pages or table_pages 0 none does;
+ * the caches and tables may then be NULL.
  *
  * cached[s]: tokens that sequence s holds before this call's own, the same number in
  * every layer's calls.  Below 0 the sequence is skipped (an empty place of a padded

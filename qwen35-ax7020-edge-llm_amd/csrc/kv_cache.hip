@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args 
                     const int64_t place = (int64_t)held + r - span_of(a.starts, a.rows, a.n_seq, s).first;
                     p.there = 1;
                     p.position = a.positions ? a.positions[r] : (int)min(place, (int64_t)INT32_MAX);
-                    if (place < (int64_t)a.table_pages * a.page) {
+                    if (place < (a.pages ? (int64_t)a.table_pages * a.page : 0)) {  // (without pages tables may be NULL)
                         const uint32_t j = divide((uint32_t)place, page);
                         const int id = a.tables[s * a.table_row + j];
                         if ((unsigned)id < (unsigned)a.pages)

@@ -1,5 +1,5 @@
-"""Edges of the attention over the paged cache and of the append: scores that are all NaN, and what a batch
-does with them.  A row is NaN or it is not: what is finite has the tolerances of test_gpu_paged_attention.py."""
+"""Edges of the attention over the paged cache and of the append: scores that are all NaN, a pool without pages.
+A row is NaN or it is not: what is finite has the tolerances of test_gpu_paged_attention.py."""
 import pytest
 import torch
 
@@ -47,3 +47,26 @@ def test_keys_that_are_all_nan(gpu, dim, dtype):
         mask[2] = 2
         got = check(gpu, args, starts, dtype, mask=mask)
         assert bool(torch.isnan(got[1, :2]).all()) and bool((got[0] == 0).all()) and bool(torch.isfinite(got[2]).all())
+
+
+@pytest.mark.parametrize("dtype,code", [(F, 0), (BF16, 1)])
+def test_a_pool_without_pages(gpu, dtype, code):
+    """No caches and no tables (NULL), as the entry points allow it where there are no pages: the queries are rotated
+    as ever, attention gives 0."""
+    rows, n, hq, hk, dim = 6, 3, 4, 2, 64
+    q, k = torch.randn(rows, hq, dim, device="cuda").to(dtype), torch.randn(rows, hk, dim, device="cuda").to(dtype)
+    cached = torch.tensor([0, 5, -1], dtype=torch.int32, device="cuda")
+    freqs, _ = gpu.rotary_frequencies(32)
+    out = torch.full_like(q, 7)
+    sizes = dict(cached=cached.data_ptr(), rows=rows, n_seq=n, pages=0, page=16, table_pages=4, table_row=4, heads_q=hq, heads_k=hk,
+                 dim=dim, dtype=code, q=q.data_ptr(), q_row=hq * dim, q_head=dim)
+    a = gpu.kv_dev_append_args(k=k.data_ptr(), v=k.data_ptr(), q_out=out.data_ptr(), freqs=freqs.data_ptr(), k_row=hk * dim, k_head=dim,
+                               v_row=hk * dim, v_head=dim, q_out_row=hq * dim, q_out_head=dim, rot=32, amplitude=1.0, **sizes)
+    gpu.check(gpu.load().kv_dev_append(a, None), "append")
+    positions = torch.tensor([0, 1, 5, 6, 0, 0], dtype=torch.int32, device="cuda")
+    assert torch.equal(out[:4], gpu.rotary(q, positions, freqs)[:4]) and bool((out[4:] == 7).all())
+    work = torch.empty(gpu.paged_attention_work_bytes(rows, n, hq, hk, dim, dtype), dtype=torch.uint8, device="cuda")
+    a = gpu.attn_dev_args(out=out.data_ptr(), out_row=hq * dim, out_head=dim, work=work.data_ptr(), work_bytes=work.numel(), scale=0.125,
+                          **sizes)
+    gpu.check(gpu.load().attn_dev_paged(a, None), "attention")
+    assert bool((out[:4] == 0).all()) and bool((out[4:] == 7).all())
