@@ -1,4 +1,5 @@
-"""Edges of the attention over the paged cache and of the append: scores that are all NaN, a pool without pages.
+"""Edges of the attention over the paged cache and of the append: scores that are all NaN, a pool without pages, drafts
+in a stretched context.
 A row is NaN or it is not: what is finite has the tolerances of test_gpu_paged_attention.py."""
 import pytest
 import torch
@@ -70,3 +71,27 @@ def test_a_pool_without_pages(gpu, dtype, code):
                           **sizes)
     gpu.check(gpu.load().attn_dev_paged(a, None), "attention")
     assert bool((out[:4] == 0).all()) and bool((out[4:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+def test_drafts_in_a_stretched_context(gpu, dtype):
+    """Frequencies and amplitude of a context four times as long: drafted tokens that follow one another get the keys
+    and queries, to the bit, that the same tokens get as text, and attention sees the same."""
+    freqs, amplitude = gpu.rotary_frequencies(64, 1e6, scaling="yarn", factor=4.0, original=512)
+    assert amplitude > 1.1
+    args, starts = case([7, 0, 21], [40, 9, 1000], 8, 2, 128, 16, dtype)
+    q, K, V, tables, cached = args
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(28, 2, 128, generator=g).to(dtype).cuda() for _ in range(2))
+    parents = torch.tensor([*range(-1, 6), *range(-1, 20)], dtype=torch.int32, device="cuda")
+    mask, positions = gpu.draft_tree(parents, cached, starts, longest=21)
+    results = []
+    for drafted in (False, True):
+        k_cache, v_cache = K.clone(), V.clone()
+        turned = gpu.kv_cache_append(k, v, k_cache, v_cache, tables, cached, starts, q=q, positions=positions if drafted else None,
+                                     freqs=freqs, amplitude=amplitude)
+        check(gpu, (turned, k_cache, v_cache, tables, cached), starts, dtype, mask=mask if drafted else None)
+        results.append((turned, k_cache.nan_to_num(9.0), v_cache.nan_to_num(9.0)))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    want = gpu.rotary(q, positions, freqs, amplitude=amplitude)
+    assert torch.equal(results[1][0], want)
