@@ -707,8 +707,9 @@ int kv_dev_append(const kv_dev_append_args* args, void* stream);
  *
  * Scores, maxima, sums and o are float32.  With bf16 the weights w_j are rounded to bf16 as an operand of their
  * product with v, each by up to 2^-9 of itself either way, and the sum that divides takes the rounded ones, so that
- * equal weights leave no error.  A NaN or infinity in a key or value shows in the rows that see it and in no
- * other; one that no row sees (a later token's, a free place's) in none.
+ * equal weights leave no error.  A row whose query is NaN, or that sees a key with a NaN, is NaN; a score of infinity
+ * makes its row NaN, one of -infinity is a weight of 0.  A NaN or infinity in a value shows in the rows that see it, in
+ * its element.  None of these shows in any other row, and one that no row sees (a later token's, a free place's) in none.
  *
  * Rows of a skipped sequence, and rows that no sequence holds, are left as they were; with zero_rest
  * not 0 a skipped sequence's rows are set to 0.  work: device memory of attn_dev_paged_work_bytes() (which takes the

@@ -1,10 +1,10 @@
-"""Edges of the attention over the paged cache and of the append: scores that are all NaN, a pool without pages, drafts
-in a stretched context.
+"""Edges of the attention over the paged cache and of the append: scores that are all NaN or infinite, a pool without pages, drafts
+in a stretched context, caches that span more than 32 bits.
 A row is NaN or it is not: what is finite has the tolerances of test_gpu_paged_attention.py."""
 import pytest
 import torch
 
-from test_gpu_paged_attention import BF16, F, NAN, case, check
+from test_gpu_paged_attention import BF16, F, INF, NAN, case, check
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,65 @@ def test_drafts_in_a_stretched_context(gpu, dtype):
     assert all(torch.equal(x, y) for x, y in zip(*results))
     want = gpu.rotary(q, positions, freqs, amplitude=amplitude)
     assert torch.equal(results[1][0], want)
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("stride", [1 << 31, (1 << 31) + (1 << 20) + 64])  # (elements between pages)
+def test_caches_past_32_bits(gpu, stride, dtype):
+    """Pages 2^31 elements apart: every entry point's offsets, in elements and in bytes, past 32 bits for each page but
+    the first.  The same bits as from a cache in one piece, from single tokens, from prompts and by the append."""
+    for new, held in (([2, 1], [30, 20]), ([40, 3], [20, 5]), ([300], [10])):  # (one to eight wavefronts)
+        args, starts = case(new, held, 4, 2, 64, 16, dtype)
+        q, K, V, tables, cached = args
+        pages, n = K.shape[0], 16 * 2 * 64
+        order = torch.randperm(pages - 1, generator=torch.Generator().manual_seed(3)).to(torch.int32) + 1
+        repeated = pages > 7  # (not more than six pages far apart: their tokens again and again)
+        if repeated:
+            tables.copy_((tables % 5 + 1).where(tables >= 0, tables))
+            K, V = K[:7].nan_to_num(1.0), V[:7].nan_to_num(1.0)
+            pages = 7
+        else:
+            K, V = K.clone(), V.clone()
+            back = torch.full((pages,), -1, dtype=torch.int32)
+            used = tables[tables >= 0].long().cpu()
+            back[used] = order[: len(used)]
+            for old, to in zip(used.tolist(), back[used].tolist()):
+                K[to], V[to] = args[1][old], args[2][old]
+            tables[tables >= 0] = back.cuda()[tables[tables >= 0].long()]
+        assert bool((tables[tables >= 0] >= 1).all())  # (no page that 32 bits would reach)
+        far = torch.empty((pages - 1) * stride + 2 * n, dtype=dtype, device="cuda")
+        K2, V2 = (torch.as_strided(far, K.shape, (stride, 128, 64, 1), i * n) for i in range(2))
+        K2.copy_(K)
+        V2.copy_(V)
+        near = gpu.paged_attention(q, K, V, tables, cached, starts)
+        assert bool(torch.isfinite(near).all())
+        assert torch.equal(gpu.paged_attention(q, K2, V2, tables, cached, starts), near)
+        if repeated:
+            continue  # (two rows must not meet in one place)
+        freqs, _ = gpu.rotary_frequencies(32)
+        k, v = (torch.randn(sum(new), 2, 64, device="cuda").to(dtype) for _ in range(2))
+        for caches in ((K, V), (K2, V2)):
+            gpu.kv_cache_append(k, v, *caches, tables, cached, starts, freqs=freqs)
+        at = tables[tables >= 0].long()
+        for x, y in ((K, K2), (V, V2)):
+            assert torch.equal(x[at].nan_to_num(9.0), y[at].nan_to_num(9.0))
+        del far, K2, V2
+
+
+@pytest.mark.parametrize("dtype", [F, BF16])
+@pytest.mark.parametrize("dim", [64, 80, 256])
+def test_keys_with_an_infinity(gpu, dim, dtype):
+    """A score of -infinity is a weight of 0, one of infinity makes its row NaN, and a row whose every score is -infinity
+    is 0: in single tokens, drafts and prompts, split over workgroups or not."""
+    for new, cached, places in ((1, 0, [0]), (1, 500, [0, 300, 499]), (5, 20000, [17, 9000]), (40, 60, [3, 61, 99]),
+                                (40, 0, [0, 1, 2])):
+        args, starts = case([new, 2], [cached, 33], 4, 2, dim, 16, dtype)
+        q, K, V, tables, held = args
+        for j in places:
+            K[int(tables[0, j // 16]), j % 16, 0, 7] = INF
+            K[int(tables[0, j // 16]), j % 16, 1, 7] = -INF
+        q[0, :, 7] = torch.tensor([-1.0, 1.0, 1.0, -1.0])
+        got = check(gpu, args, starts, dtype)
+        assert bool(torch.isfinite(got[0, [0, 2]]).all()) and bool(torch.isnan(got[0, [1, 3]]).all())
+        if cached == 0:
+            assert bool((got[0, [0, 2]] == 0).all())
