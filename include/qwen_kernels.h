@@ -622,8 +622,8 @@ int bf16_dev_lm_head_loss_grad(const lm_head_loss_args* args, void* stream);
  *
  * freqs: rot / 2 doubles on the device, radians a position (a context's scaling is
  * in them and in the amplitude).  t is made and brought into one turn in double, so that a far
- * position's angle is off by 2^-53 of itself (at 2^20 radians 2^-33); its sine and
- * cosine and the rotation are float32, and a bf16 result is rounded once.
+ * position's angle is off by up to 3 x 2^-53 of itself (at 2^20 radians 2^-31); its sine and
+ * cosine, of the angle's float32, and the rotation are float32, and a bf16 result is rounded once.
  *
  * x, out: rows x heads x dim, float32 or bf16 (dtype), head h of row r at
  * r * x_row + h * x_head elements.  out may be x with the same strides (elements from rot on are
@@ -665,7 +665,7 @@ int rope_dev_grad(const rope_dev_args* args, void* stream);
  * keys are rotated on the way as rope_dev_apply does, at positions[row], or (NULL)
  * at their place; q, if not NULL, is rotated to q_out in the same launch (of every row of a sequence
  * that is not skipped; q_out may be q with the same strides).  rot 0: keys as they are, and no q.
- * Places of one call have to be different: where two rows meet in one, each 16-byte part of it
+ * Places of one call have to be different: where two rows meet in one, each element of it
  * is from one of the two.
  *
  * dtype: of q, k, v and the cache (QWEN_F32, QWEN_BF16).  dim a multiple of 8 up
@@ -706,16 +706,19 @@ int kv_dev_append(const kv_dev_append_args* args, void* stream);
  * any number, and drafted tokens that branch have attn_dev_tree's mask.
  *
  * Scores, maxima, sums and o are float32.  With bf16 the weights w_j are rounded to bf16 as an operand of their
- * product with v, each by up to 2^-9 of itself either way, and the sum that divides takes the rounded ones, so that
+ * product with v, each by up to 2^-8 of itself either way, and the sum that divides takes the rounded ones, so that
  * equal weights leave no error.  A row whose query is NaN, or that sees a key with a NaN, is NaN; a score of infinity
  * makes its row NaN, one of -infinity is a weight of 0.  A NaN or infinity in a value shows in the rows that see it, in
  * its element.  None of these shows in any other row, and one that no row sees (a later token's, a free place's) in none.
  *
  * Rows of a skipped sequence, and rows that no sequence holds, are left as they were; with zero_rest
  * not 0 a skipped sequence's rows are set to 0.  work: device memory of attn_dev_paged_work_bytes() (which takes the
- * sizes alone, not cached or tables), 256-byte aligned, the caller's (calls that may overlap need one each).
+ * sizes alone, not cached or tables: up to 135 MB, with 256 bf16 elements from 129 rows of a sequence and key head on,
+ * on average), 256-byte aligned, the caller's (calls that may overlap need one each).
  * The same call gives the same bits; in another call they may differ in rounding, as the
- * keys are split over workgroups by the lengths of the whole call.
+ * keys are split over workgroups by the lengths of the whole call.  Kernel and tile are chosen for a call by its mean,
+ * rows (heads_q / heads_k) / n_seq: up to 16 each key is read once for 16 rows.  A long prompt among many single tokens or
+ * empty places is right there, and faster in a call of its own.
  *
  * scale above 0, a normal number of up to 1e38; dim a multiple of 8 up to 256; heads_q a multiple of heads_k,
  * rows heads_q up to 2^28; n_seq up to 2^20; mask_words up to 2^16 (mask NULL: not read).  q and out are

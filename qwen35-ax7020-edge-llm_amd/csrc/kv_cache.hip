@@ -106,8 +106,8 @@ struct Head {
 
 // ---- rotation alone -------------------------------------------------------------------
 // 16 bytes a thread and piece, both of a pair's elements by the same thread (so that out may be x): 16,384 rows of 10
-// heads of 256 bf16 elements in 27.6 us, 168 MB at 6.1 TB/s; 5,003 of 12 heads of 96 float32 ones 8.6; one row 3.8, a
-// launch's latency.
+// heads of 256 bf16 elements, 168 MB, in 36 us among other work, 4.7 TB/s (27.8 us again on the same rows, which the
+// memory-side cache holds in part); 5,003 of 12 heads of 96 float32 ones 8.7; one row 3.8, a launch's latency.
 template <class T, bool VEC, bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_kernel(rope_dev_args a, int each, int back, int units, Divisor by_units,
                                                         Divisor by_heads) {
@@ -164,8 +164,9 @@ __device__ __forceinline__ int owner_by_wave(const int32_t* starts, int rows, in
 }
 
 // A wavefront a row finds where it goes, then all threads take the rows' pieces: keys, values and queries in one
-// launch.  9,001 tokens of 24 sequences, 8 and 2 heads of 256 bf16 elements: 25.7 us, 111 MB at 4.3 TB/s (a row's bytes
-// wait for its place, three loads one after the other); one token 5.0 us.
+// launch.  9,001 tokens of 24 sequences, 8 and 2 heads of 256 bf16 elements, 111 MB: 34.8 us among other work, 3.2 TB/s
+// (a row's bytes wait for its place, three loads one after the other; 25.6 us again on the same tokens, from the
+// memory-side cache in part); one token 5.1 us.
 template <class T, bool VEC, bool INTER>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(kv_dev_append_args a, Divisor page, int each, Units n, int copy_v) {
     using H = Head<T, VEC, INTER>;

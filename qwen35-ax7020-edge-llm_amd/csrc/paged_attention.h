@@ -41,7 +41,9 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     const size_t mean = ((size_t)a.rows * p.group + std::max(a.n_seq, 1) - 1) / std::max(a.n_seq, 1);
     // Up to 16 rows: attn_step_kernel (64 sequences of 4,000 keys, 16 rows of 256 bf16 elements, 130 us, by attn_kernel
     // 135; 32 of 2,000, 128 float32 ones, 47 for 61; but 48 of 2,000 and 16 rows on average, many with more, 71 for
-    // 55).
+    // 55).  By the mean, for the lengths are on the device: a batch of few long sequences and many short ones pays for it
+    // (255 tokens on 1,000 keys each and a chunk of 512 on 30,000 in one call 1,147 us, in two 106 and 172; 32 tokens on
+    // 8,000 and one of 2,048 on 2,048 236 | 108 and 109; 1,023 empty places and a prompt of 2,048 226 | 74).
     p.few = mean <= 16;
     // More: as many rows to a tile as there are, so that its keys are read once.  Two wavefronts at least, to copy (one
     // | two: 48 sequences of 28 rows of 128 elements 70 | 62 us, 64 of 32 rows of 256 174 | 149).  Of 256 bf16 elements
@@ -56,7 +58,9 @@ inline AttnPlan attn_plan(const attn_dev_args& a) {
     p.each = a.starts || !a.n_seq ? 0 : (a.rows / a.n_seq * p.group + p.rows - 1) / p.rows;
     // (64 keys: half as many waits for the copies; four wavefronts gained nothing by it)
     p.keys = p.few || (bf16 && p.waves == 8) ? 64 : 32;
-    // as many as are at work at a time, by LDS and registers (8 wavefronts a compute unit), up to four a unit
+    // attn_kernel: as many as are at work at a time, by LDS and registers (8 wavefronts a compute unit), up to four a
+    // unit.  attn_step_kernel: two a unit, though of 256 float32 elements LDS holds one at a time (64 sequences of 4,096
+    // keys 200 us, 5.4 TB/s, for 105 and 5.1 with bf16).
     const size_t lds = (size_t)4 * p.keys * p.dim * (bf16 ? 2 : 4) + ATTN_HELD * 4 + 256;
     p.grid = 256 * (p.few ? 2 : (int)std::min<size_t>(std::min(4, 8 / p.waves), 160 * 1024 / lds));
     // A part is written and read again, 8 bytes an output: of many rows as much as several tiles of keys (one sequence of
